@@ -1,4 +1,5 @@
-// C ABI entry points (declared in include/double_attention_hip.h).
+// C ABI entry points (declared in include/double_attention_hip.h and
+// include/double_attention_int8.h).
 //
 // Each entry point validates its arguments on the host, then enqueues the
 // kernels on the caller's stream.  Nothing is allocated, freed or
@@ -12,8 +13,10 @@
 #include <string>
 
 #include "../../include/double_attention_hip.h"
+#include "../../include/double_attention_int8.h"
 #include "da_launch.h"
 #include "dict_norm.h"
+#include "int8_rows.h"
 
 namespace {
 
@@ -123,7 +126,7 @@ extern "C" {
 static_assert(DA_OUT_SPLIT == da::kOutSplit, "split-output flag");
 static_assert(DA_ROUTE_BETA_IS_LOG_SCALE == da::kRouteBetaIsLogScale, "route flag");
 
-int da_abi_version(void) { return 19; }
+int da_abi_version(void) { return 20; }
 
 const char* da_last_error(void) { return g_error.c_str(); }
 
@@ -699,6 +702,205 @@ int da_layer_norm_backward(const void* x, const void* grad, int64_t rows, int64_
   da::launch_layer_norm_backward(x, grad, rows, static_cast<int>(dim), weight, param_dtype, eps, dtype, grad_x,
                                  grad_params, reinterpret_cast<hipStream_t>(stream));
   return check_launch("layer_norm backward");
+}
+
+namespace {
+
+static_assert(DA_INT8_GROUP == da::kInt8Group, "columns per scale");
+constexpr int64_t kInt8MaxElements = 1LL << 40;
+
+int64_t element_bytes(int dtype) { return dtype == DA_F32 ? 4 : 2; }
+
+// Rows of a 16-bit or fp32 matrix.
+int validate_rows(const char* what, const char* name, const void* p, int64_t cols, int64_t ld, int dtype) {
+  if (!p) return fail(DA_ERR_INVALID_ARGUMENT, "%s: %s is null", what, name);
+  if (!aligned(p, static_cast<int>(element_bytes(dtype))))
+    return fail(DA_ERR_ALIGNMENT, "%s: %s is not aligned to its elements", what, name);
+  if (ld < cols || ld > kInt8MaxElements) return fail(DA_ERR_INVALID_ARGUMENT, "%s: %s has a pitch below its width", what, name);
+  return DA_OK;
+}
+
+// 8-bit rows and their scales.
+int validate_int8(const char* what, const char* name, const void* values, int64_t ldv, const void* scales, int64_t cols) {
+  if (!values || !scales) return fail(DA_ERR_INVALID_ARGUMENT, "%s: %s or its scales are null", what, name);
+  if (!aligned(values, 16) || ldv % 16 || !aligned(scales, 4))
+    return fail(DA_ERR_ALIGNMENT, "%s: %s must be 16-byte aligned at a pitch of a multiple of 16", what, name);
+  if (ldv < cols || ldv > kInt8MaxElements) return fail(DA_ERR_INVALID_ARGUMENT, "%s: %s has a pitch below its width", what, name);
+  return DA_OK;
+}
+
+int validate_sizes(const char* what, int64_t rows, int64_t cols, int64_t max_cols) {
+  if (rows < 0 || cols < 1) return fail(DA_ERR_INVALID_ARGUMENT, "%s: needs rows >= 0 and at least one column", what);
+  if (cols > max_cols) return fail(DA_ERR_UNSUPPORTED, "%s: rows of at most %lld columns", what, (long long)max_cols);
+  if (rows > 0x7fffffffLL || rows * ((cols + da::kInt8Group - 1) / da::kInt8Group) >= 0x7fff0000LL)
+    return fail(DA_ERR_UNSUPPORTED, "%s: too many rows", what);
+  return DA_OK;
+}
+
+constexpr int64_t kInt8MaxCols = 1 << 24;   // of rows in groups
+
+}  // namespace
+
+int da_quantize_int8(const void* x, int64_t rows, int64_t cols, int64_t ldx, int dtype, int64_t group, void* values,
+                     int64_t ldv, float* scales, da_stream_t stream) {
+  if (!any_dtype(dtype)) return fail(DA_ERR_INVALID_ARGUMENT, "quantize: bad dtype");
+  if (group != 0 && group != DA_INT8_GROUP)
+    return fail(DA_ERR_UNSUPPORTED, "quantize: a scale for each row (0) or each %d columns", DA_INT8_GROUP);
+  int rc = validate_sizes("quantize", rows, cols, group ? kInt8MaxCols : da::kRowInt8MaxCols);
+  if (rc) return rc;
+  if (rows == 0) return ok();
+  if ((rc = validate_rows("quantize", "x", x, cols, ldx, dtype))) return rc;
+  if ((rc = validate_int8("quantize", "values", values, ldv, scales, cols))) return rc;
+  int8_t* q = static_cast<int8_t*>(values);
+  if (group) {
+    da::launch_int8_save({x, ldx, rows, static_cast<int>(cols), dtype, q, ldv, scales, false, nullptr, nullptr, 0},
+                         reinterpret_cast<hipStream_t>(stream));
+  } else {
+    da::launch_row_int8({x, ldx, nullptr, 0, rows, static_cast<int>(cols), dtype, nullptr, 0, 0.f, nullptr, nullptr, q, ldv, scales},
+                        false, reinterpret_cast<hipStream_t>(stream));
+  }
+  return check_launch("quantize");
+}
+
+int da_dequantize_int8(const void* values, int64_t rows, int64_t cols, int64_t ldv, const float* scales, int64_t group,
+                       void* out, int64_t ldo, int out_dtype, da_stream_t stream) {
+  if (!any_dtype(out_dtype)) return fail(DA_ERR_INVALID_ARGUMENT, "dequantize: bad dtype");
+  if (group != 0 && group != DA_INT8_GROUP)
+    return fail(DA_ERR_UNSUPPORTED, "dequantize: a scale for each row (0) or each %d columns", DA_INT8_GROUP);
+  int rc = validate_sizes("dequantize", rows, cols, kInt8MaxCols);
+  if (rc) return rc;
+  if (rows == 0) return ok();
+  if ((rc = validate_rows("dequantize", "out", out, cols, ldo, out_dtype))) return rc;
+  if ((rc = validate_int8("dequantize", "values", values, ldv, scales, cols))) return rc;
+  da::launch_int8_restore({nullptr, 0, rows, static_cast<int>(cols), out_dtype,
+                           static_cast<int8_t*>(const_cast<void*>(values)), ldv, const_cast<float*>(scales), group == 0, out,
+                           nullptr, ldo},
+                          reinterpret_cast<hipStream_t>(stream));
+  return check_launch("dequantize");
+}
+
+int da_linear_int8(const void* x, int64_t ldx, const float* x_scales, int64_t rows, int64_t in_features,
+                   const void* weight, int64_t ldw, const float* w_scales, int64_t out_features, const void* bias,
+                   int bias_dtype, int activation, const void* residual, int64_t ldr, void* out, int dtype,
+                   da_stream_t stream) {
+  if (!half_dtype(dtype)) return fail(DA_ERR_INVALID_ARGUMENT, "linear_int8: dtype must be DA_F16 or DA_BF16");
+  if (activation != DA_ACT_NONE && activation != DA_ACT_GELU)
+    return fail(DA_ERR_INVALID_ARGUMENT, "linear_int8: unknown activation %d", activation);
+  if (bias && !any_dtype(bias_dtype)) return fail(DA_ERR_INVALID_ARGUMENT, "linear_int8: bad bias dtype");
+  if (bias && !aligned(bias, static_cast<int>(element_bytes(bias_dtype))))
+    return fail(DA_ERR_ALIGNMENT, "linear_int8: the bias is not aligned to its elements");
+  int rc = validate_sizes("linear_int8", rows, in_features, da::kRowInt8MaxCols);
+  if (rc) return rc;
+  if (out_features < 1 || out_features > (1 << 24) ||
+      ((rows + 63) / 64) * ((out_features + 63) / 64) > 0x7fff0000LL)
+    return fail(DA_ERR_UNSUPPORTED, "linear_int8: out_features must be in [1, 2^24], and the output's tiles below 2^31");
+  if (rows == 0) return ok();
+  if ((rc = validate_int8("linear_int8", "x", x, ldx, x_scales, in_features))) return rc;
+  if ((rc = validate_int8("linear_int8", "weight", weight, ldw, w_scales, in_features))) return rc;
+  if ((rc = validate_rows("linear_int8", "out", out, out_features, out_features, dtype))) return rc;
+  if (residual && (rc = validate_rows("linear_int8", "residual", residual, out_features, ldr, dtype))) return rc;
+  da::launch_linear_int8({static_cast<const int8_t*>(x), ldx, x_scales, rows, static_cast<int>(in_features),
+                          static_cast<const int8_t*>(weight), ldw, w_scales, out_features, bias, bias_dtype,
+                          activation == DA_ACT_GELU ? da::kGemmActGelu : da::kGemmActNone, residual, ldr, out, dtype},
+                         reinterpret_cast<hipStream_t>(stream));
+  return check_launch("linear_int8");
+}
+
+namespace {
+
+int validate_rms(const char* what, int64_t rows, int64_t dim, const void* weight, int param_dtype, float eps, int dtype) {
+  if (!half_dtype(dtype)) return fail(DA_ERR_INVALID_ARGUMENT, "%s: dtype must be DA_F16 or DA_BF16", what);
+  if (!any_dtype(param_dtype)) return fail(DA_ERR_INVALID_ARGUMENT, "%s: bad parameter dtype", what);
+  if (!(eps > 0.f) || !std::isfinite(eps)) return fail(DA_ERR_INVALID_ARGUMENT, "%s: eps must be positive and finite", what);
+  if (weight && !aligned(weight, static_cast<int>(element_bytes(param_dtype))))
+    return fail(DA_ERR_ALIGNMENT, "%s: the weight is not aligned to its elements", what);
+  return validate_sizes(what, rows, dim, da::kRmsNormMaxDim);
+}
+
+}  // namespace
+
+int da_add_rms_norm(const void* x, int64_t ldx, const void* residual, int64_t ldr, int64_t rows, int64_t dim,
+                    const void* weight, int param_dtype, float eps, int dtype, void* sum, void* out, void* values,
+                    int64_t ldv, float* scales, da_stream_t stream) {
+  int rc = validate_rms("add_rms_norm", rows, dim, weight, param_dtype, eps, dtype);
+  if (rc) return rc;
+  if (rows == 0) return ok();
+  if ((rc = validate_rows("add_rms_norm", "x", x, dim, ldx, dtype))) return rc;
+  if (residual && (rc = validate_rows("add_rms_norm", "residual", residual, dim, ldr, dtype))) return rc;
+  if (residual && (rc = validate_rows("add_rms_norm", "sum", sum, dim, dim, dtype))) return rc;
+  if (!out && !values) return fail(DA_ERR_INVALID_ARGUMENT, "add_rms_norm: no output asked for");
+  if (out && (rc = validate_rows("add_rms_norm", "out", out, dim, dim, dtype))) return rc;
+  if (values && (rc = validate_int8("add_rms_norm", "values", values, ldv, scales, dim))) return rc;
+  da::launch_row_int8({x, ldx, residual, ldr, rows, static_cast<int>(dim), dtype, weight, param_dtype, eps, sum, out,
+                       static_cast<int8_t*>(values), ldv, scales},
+                      true, reinterpret_cast<hipStream_t>(stream));
+  return check_launch("add_rms_norm");
+}
+
+int64_t da_add_rms_norm_backward_workspace_bytes(int64_t rows, int64_t dim) {
+  if (rows < 0 || dim < 1 || dim > da::kRmsNormMaxDim) return 0;
+  return align_up(static_cast<int64_t>(da::rms_norm_backward_blocks(rows, static_cast<int>(dim))) * dim * 4 + 16);
+}
+
+int da_add_rms_norm_backward(const void* sum, int64_t ldsum, const void* grad, int64_t ldg, const void* grad_sum,
+                             int64_t ldgs, int64_t rows, int64_t dim, const void* weight, int param_dtype, float eps,
+                             int dtype, void* grad_x, void* grad_weight, void* workspace, int64_t workspace_bytes,
+                             da_stream_t stream) {
+  int rc = validate_rms("add_rms_norm backward", rows, dim, weight, param_dtype, eps, dtype);
+  if (rc) return rc;
+  if (grad_weight) {
+    if (!aligned(grad_weight, static_cast<int>(element_bytes(param_dtype))))
+      return fail(DA_ERR_ALIGNMENT, "add_rms_norm backward: grad_weight is not aligned to its elements");
+    if (!workspace || workspace_bytes < da_add_rms_norm_backward_workspace_bytes(rows, dim))
+      return fail(DA_ERR_WORKSPACE, "add_rms_norm backward: the workspace needs %lld bytes",
+                  (long long)da_add_rms_norm_backward_workspace_bytes(rows, dim));
+    if (!aligned(workspace, 16)) return fail(DA_ERR_ALIGNMENT, "add_rms_norm backward: the workspace must be 16-byte aligned");
+  } else if (rows == 0) {
+    return ok();
+  }
+  if (rows > 0) {
+    if ((rc = validate_rows("add_rms_norm backward", "sum", sum, dim, ldsum, dtype))) return rc;
+    if ((rc = validate_rows("add_rms_norm backward", "grad", grad, dim, ldg, dtype))) return rc;
+    if (grad_sum && (rc = validate_rows("add_rms_norm backward", "grad_sum", grad_sum, dim, ldgs, dtype))) return rc;
+    if ((rc = validate_rows("add_rms_norm backward", "grad_x", grad_x, dim, dim, dtype))) return rc;
+  }
+  da::launch_rms_norm_backward({sum, ldsum, grad, ldg, grad_sum, ldgs, rows, static_cast<int>(dim), dtype, weight,
+                                param_dtype, eps, grad_x, grad_weight ? static_cast<float*>(workspace) : nullptr,
+                                grad_weight},
+                               reinterpret_cast<hipStream_t>(stream));
+  return check_launch("add_rms_norm backward");
+}
+
+int da_gelu_int8(const void* z, int64_t rows, int64_t cols, int64_t ldz, int dtype, void* out, void* values,
+                 int64_t ldv, float* scales, da_stream_t stream) {
+  if (!half_dtype(dtype)) return fail(DA_ERR_INVALID_ARGUMENT, "gelu_int8: dtype must be DA_F16 or DA_BF16");
+  int rc = validate_sizes("gelu_int8", rows, cols, kInt8MaxCols);
+  if (rc) return rc;
+  if (rows == 0) return ok();
+  if ((rc = validate_rows("gelu_int8", "z", z, cols, ldz, dtype))) return rc;
+  if ((rc = validate_rows("gelu_int8", "out", out, cols, cols, dtype))) return rc;
+  if ((rc = validate_int8("gelu_int8", "values", values, ldv, scales, cols))) return rc;
+  da::launch_gelu_int8({z, ldz, rows, static_cast<int>(cols), dtype, static_cast<int8_t*>(values), ldv, scales, false, out,
+                        nullptr, cols},
+                       reinterpret_cast<hipStream_t>(stream));
+  return check_launch("gelu_int8");
+}
+
+int da_gelu_int8_backward(const void* values, int64_t rows, int64_t cols, int64_t ldv, const float* scales,
+                          const void* grad, int64_t ldg, int dtype, void* grad_z, void* out, da_stream_t stream) {
+  if (!half_dtype(dtype)) return fail(DA_ERR_INVALID_ARGUMENT, "gelu_int8 backward: dtype must be DA_F16 or DA_BF16");
+  int rc = validate_sizes("gelu_int8 backward", rows, cols, kInt8MaxCols);
+  if (rc) return rc;
+  if (rows == 0) return ok();
+  if ((rc = validate_rows("gelu_int8 backward", "grad", grad, cols, ldg, dtype))) return rc;
+  if ((rc = validate_rows("gelu_int8 backward", "grad_z", grad_z, cols, cols, dtype))) return rc;
+  if (out && (rc = validate_rows("gelu_int8 backward", "out", out, cols, cols, dtype))) return rc;
+  if ((rc = validate_int8("gelu_int8 backward", "values", values, ldv, scales, cols))) return rc;
+  da::launch_gelu_int8_backward({grad, ldg, rows, static_cast<int>(cols), dtype,
+                                 static_cast<int8_t*>(const_cast<void*>(values)), ldv, const_cast<float*>(scales), false,
+                                 grad_z, out, cols},
+                                reinterpret_cast<hipStream_t>(stream));
+  return check_launch("gelu_int8 backward");
 }
 
 int64_t da_sda_workspace_offset(int64_t batch, int64_t length, int64_t model_dim, int64_t qk_width,

@@ -264,6 +264,96 @@ void launch_layer_norm(const void* x, int64_t rows, int dim, const void* weight,
 constexpr int kLnParamCopies = 8;
 void launch_layer_norm_backward(const void* x, const void* dy, int64_t rows, int dim, const void* weight,
                                 int param_dtype, float eps, int dtype, void* dx, float* dparams, hipStream_t stream);
+// Rows in 8 bits with a scale per 128 columns (int8_groups.hip): kept (x ->
+// values, scales), restored (values, scales -> out; row_scale: one scale a
+// row), GELU (x -> out, values, scales) and its backward (x is the gradient at
+// GELU's output, out the one at its input, again GELU's output or nullptr).
+// rows * ceil(cols / 128) < 2^31.  dtype: x, out and again (kF32 only for
+// save and restore).
+struct Int8GroupArgs {
+  const void* x;
+  int64_t ldx;
+  int64_t rows;
+  int cols;
+  int dtype;
+  int8_t* values;
+  int64_t ldv;        // a multiple of 16, at least cols
+  float* scales;      // [rows][ceil(cols / 128)], or [rows]
+  bool row_scale;
+  void* out;
+  void* again;        // at out's pitch
+  int64_t ldo;
+};
+void launch_int8_save(const Int8GroupArgs& a, hipStream_t stream);
+void launch_int8_restore(const Int8GroupArgs& a, hipStream_t stream);
+void launch_gelu_int8(const Int8GroupArgs& a, hipStream_t stream);
+void launch_gelu_int8_backward(const Int8GroupArgs& a, hipStream_t stream);
+
+// Rows with one scale each (rms_norm.hip): values, scales = int8(x), or with
+// `norm` the root-mean-square norm of s = x + residual, as out (16 bits), as
+// values and scales, or both.
+struct RowInt8Args {
+  const void* x;
+  int64_t ldx;
+  const void* residual;   // or nullptr: s is x, and sum is not written
+  int64_t ldr;
+  int64_t rows;
+  int dim;                // <= kRowInt8MaxCols, with `norm` <= kRmsNormMaxDim
+  int dtype;              // kF32 only without `norm`
+  const void* weight;     // [dim] of param_dtype, or nullptr (1)
+  int param_dtype;
+  float eps;
+  void* sum;              // [rows][dim]
+  void* out;              // [rows][dim] or nullptr
+  int8_t* values;         // or nullptr (with `norm`)
+  int64_t ldv;            // a multiple of 16, at least dim
+  float* scales;          // [rows]
+};
+constexpr int kRowInt8MaxCols = 65536;
+constexpr int kRmsNormMaxDim = 16384;
+void launch_row_int8(const RowInt8Args& a, bool norm, hipStream_t stream);
+
+struct RmsNormBackwardArgs {
+  const void* sum;
+  int64_t ldsum;
+  const void* grad;
+  int64_t ldg;
+  const void* grad_sum;   // or nullptr (0)
+  int64_t ldgs;
+  int64_t rows;
+  int dim;
+  int dtype;
+  const void* weight;     // or nullptr (1)
+  int param_dtype;        // of weight and grad_weight
+  float eps;
+  void* grad_x;           // [rows][dim]
+  float* partials;        // [rms_norm_backward_blocks][dim], or nullptr (no grad_weight)
+  void* grad_weight;      // [dim]
+};
+int rms_norm_backward_blocks(int64_t rows, int dim);
+void launch_rms_norm_backward(const RmsNormBackwardArgs& a, hipStream_t stream);
+
+// Linear layer on 8-bit rows (gemm_int8.hip).
+struct LinearInt8Args {
+  const int8_t* x;
+  int64_t ldx;            // multiples of 16, as ldw
+  const float* x_scales;  // [rows]
+  int64_t rows;
+  int K;                  // <= kRowInt8MaxCols
+  const int8_t* w;
+  int64_t ldw;
+  const float* w_scales;  // [N]
+  int64_t N;
+  const void* bias;
+  int bias_dtype;
+  int act;                // kGemmActNone or kGemmActGelu
+  const void* residual;   // or nullptr
+  int64_t ldr;
+  void* out;              // [rows][N]
+  int dtype;              // out and residual
+};
+void launch_linear_int8(const LinearInt8Args& a, hipStream_t stream);
+
 // Launch shape of the attention for a problem: value slice width, waves per
 // query tile, sub-streams, query tiles, the stream split of long key ranges (run length, 0
 // = none; runs per sequence and slice) and the bytes of partials it needs

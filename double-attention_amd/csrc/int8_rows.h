@@ -1,0 +1,165 @@
+// Device helpers of the 8-bit rows: signed integers from -127 to 127 with an
+// fp32 scale for each row, or for each 128 columns of a row.
+//
+//   scale = max(amax, 127 * 2^-126) / 127,   q = rint(x / scale)
+//
+// The floor on the scale keeps 1 / scale finite (an all-zero row has the
+// least scale and zeros).  A row (group) that holds an infinity or a NaN has
+// no such integers: its scale is NaN and its integers are 0, so that all of it
+// stands for NaN instead of for some finite numbers.
+#pragma once
+
+#include "da_common.h"
+
+namespace da {
+
+constexpr int kInt8Group = 128;             // columns that share a scale in grouped rows
+constexpr float kInt8Least = 0x1p-126f;     // the least scale
+// A multiple of 2^23 added to a float in its last place's range: x + kRoundMagic
+// rounds x to an integer (ties to even) and leaves it in the sum's low bits, in
+// two's complement.  |x| < 2^22.
+constexpr float kRoundMagic = 12582912.f;   // 1.5 * 2^23
+
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+// 16-byte and 8-byte chunks at any 2-byte (4-byte for fp32 rows) address: rows
+// of odd widths start there.  The hardware loads and stores them at full width.
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+
+__device__ __forceinline__ u32x4 load16B_any(const void* p) { return *static_cast<const u32x4_any*>(p); }
+__device__ __forceinline__ void store16B_any(void* p, u32x4 v) { *static_cast<u32x4_any*>(p) = v; }
+
+// Eight elements of a row from column c on, of which n (<= 8) exist; the
+// others are 0.
+template <typename T>
+__device__ __forceinline__ void load_chunk(const T* p, int n, float (&v)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    if (n >= 8) {
+      const u32x4 a = load16B_any(p), b = load16B_any(p + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[e] = __uint_as_float(a[e]);
+        v[e + 4] = __uint_as_float(b[e]);
+      }
+      return;
+    }
+  } else {
+    if (n >= 8) {
+      const typename Elem<T>::v8 a = __builtin_bit_cast(typename Elem<T>::v8, load16B_any(p));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = static_cast<float>(a[e]);
+      return;
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = e < n ? static_cast<float>(p[e]) : 0.f;
+}
+
+template <typename T>
+__device__ __forceinline__ void store_chunk(T* p, int n, const float (&v)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    if (n >= 8) {
+      store16B_any(p, u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])});
+      store16B_any(p + 4, u32x4{__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7])});
+      return;
+    }
+  } else {
+    if (n >= 8) {
+      typename Elem<T>::v8 o;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] = static_cast<T>(v[e]);
+      store16B_any(p, __builtin_bit_cast(u32x4, o));
+      return;
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (e < n) p[e] = static_cast<T>(v[e]);
+}
+
+// Largest magnitude as the bits of a non-negative float: unsigned integers
+// order like the floats, and infinities and NaN come out on top, so the
+// maximum does not lose them.
+__device__ __forceinline__ uint32_t magnitude_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+// All-lane reductions over the 16 lanes of a row (DPP rotations), then over
+// the wave's four rows.
+template <int R>
+__device__ __forceinline__ uint32_t row_rotate(uint32_t v) {
+  return __builtin_amdgcn_update_dpp(0, v, 0x120 + R, 0xf, 0xf, false);
+}
+__device__ __forceinline__ uint32_t row16_max(uint32_t v) {
+  v = max(v, row_rotate<8>(v));
+  v = max(v, row_rotate<4>(v));
+  v = max(v, row_rotate<2>(v));
+  return max(v, row_rotate<1>(v));
+}
+__device__ __forceinline__ float row16_sum(float v) {
+  v += __uint_as_float(row_rotate<8>(__float_as_uint(v)));
+  v += __uint_as_float(row_rotate<4>(__float_as_uint(v)));
+  v += __uint_as_float(row_rotate<2>(__float_as_uint(v)));
+  return v + __uint_as_float(row_rotate<1>(__float_as_uint(v)));
+}
+__device__ __forceinline__ uint32_t wave_max_bits(uint32_t v) {
+  v = row16_max(v);
+  const auto a = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  v = max(a[0], a[1]);
+  const auto b = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  return max(b[0], b[1]);
+}
+__device__ __forceinline__ float wave_sum_dpp(float v) { return group_sum(row16_sum(v)); }
+
+struct Int8Scale {
+  float scale;     // what a step of the integers stands for; NaN: the row has no integers
+  float inverse;   // 1 / scale, 0 where the scale is NaN
+  uint32_t keep;   // all ones, 0 where the scale is NaN
+};
+__device__ __forceinline__ Int8Scale int8_scale(uint32_t amax_bits, float factor = 1.f) {
+  const bool finite = amax_bits < 0x7f800000u;
+  const float s = fmaxf(__uint_as_float(amax_bits) * factor * (1.f / 127.f), kInt8Least);
+  return Int8Scale{finite ? s : __uint_as_float(0x7fc00000u), finite ? 1.f / s : 0.f, finite ? 0xffffffffu : 0u};
+}
+
+// Eight integers rint(v * inverse) as bytes.  |v * inverse| <= 127 (1 + 2^-22)
+// by the choice of the scale, so rounding keeps them in [-127, 127].
+__device__ __forceinline__ u32x2 pack_int8(const float (&v)[8], float inverse, uint32_t keep) {
+  uint32_t t[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) t[e] = __float_as_uint(__builtin_fmaf(v[e], inverse, kRoundMagic));
+  u32x2 r;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t lo = __builtin_amdgcn_perm(t[4 * h + 1], t[4 * h], 0x0c0c0400u);
+    const uint32_t hi = __builtin_amdgcn_perm(t[4 * h + 3], t[4 * h + 2], 0x04000c0cu);
+    r[h] = (lo | hi) & keep;
+  }
+  return r;
+}
+
+// The eight floats that stored bytes stand for.
+__device__ __forceinline__ void unpack_int8(u32x2 q, float scale, float (&v)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int b = static_cast<int>(q[e / 4] << (24 - 8 * (e % 4))) >> 24;
+    v[e] = static_cast<float>(b) * scale;
+  }
+}
+
+// Bytes of a chunk of n (<= 8) columns: whole 8-byte stores (the pitch is a
+// multiple of 16 and the columns behind the row are the storage's own).
+__device__ __forceinline__ void store_bytes(int8_t* p, u32x2 q) { *reinterpret_cast<u32x2*>(p) = q; }
+__device__ __forceinline__ u32x2 load_bytes(const int8_t* p) { return *reinterpret_cast<const u32x2*>(p); }
+
+// n / d for 0 <= n < 2^31 by a multiplication (d >= 1; Granlund and
+// Montgomery, "Division by invariant integers using multiplication", 1994).
+struct FastDiv {
+  uint32_t d, mul, shift;
+};
+inline FastDiv make_fast_div(uint32_t d) {
+  uint32_t s = 0;
+  while ((1ull << s) < d) ++s;
+  const uint64_t m = ((1ull << 32) * ((1ull << s) - d)) / d + 1;
+  return FastDiv{d, static_cast<uint32_t>(m), s};
+}
+__device__ __forceinline__ uint32_t fast_div(uint32_t n, FastDiv f) { return (__umulhi(n, f.mul) + n) >> f.shift; }
+
+}  // namespace da

@@ -1,0 +1,336 @@
+// Rows in 8 bits with one scale each, and the root-mean-square norm with the
+// residual's addition in front of it.
+//
+//   s = x + r (rounded to the activations' type: the model carries it on)
+//   n = s rstd w,  rstd = 1 / sqrt(mean(s^2) + eps)          fp32 statistics
+//   out = n (one rounding), and / or  q, scale = int8(n)     (int8_rows.h)
+//
+// One pass over memory: NT threads hold a row in registers (CH chunks of
+// eight columns each).  The scale of the integers needs no second reduction:
+// max |n| = rstd max |s w|, so the sum of squares and the largest |s w| are
+// reduced together, and q = rint(s w (rstd / scale)).
+//
+// Backward at dy = dL/dn and ds = dL/ds (the gradient that reaches s past the
+// norm), with xh = s rstd and g = dy w:
+//   dx = dr = rstd (g - xh mean(g xh)) + ds          (one rounding)
+//   dw = sum over rows of dy xh                      (fp32)
+// The weight's gradient is added up in an order fixed by the sizes alone: a
+// thread over its workgroup's rows, the workgroups' sums by a second, small
+// launch.
+#include "da_launch.h"
+#include "int8_rows.h"
+
+namespace da {
+
+// Eight parameters of type pdt from column c on, of which n exist (1 without
+// parameters, 0 behind the row).
+__device__ __forceinline__ void load_weight8(const void* p, int pdt, int64_t c, int n, float (&w)[8]) {
+  if (p == nullptr) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = 1.f;
+  } else if (pdt == kF32) {
+    load_chunk(static_cast<const float*>(p) + c, n, w);
+  } else if (pdt == kF16) {
+    load_chunk(static_cast<const _Float16*>(p) + c, n, w);
+  } else {
+    load_chunk(static_cast<const __bf16*>(p) + c, n, w);
+  }
+}
+
+// The row's sum and largest magnitude over its NT threads.
+template <int NT>
+__device__ __forceinline__ void row_reduce(float& sum, uint32_t& amax, float* lds) {
+  sum = wave_sum_dpp(sum);
+  amax = wave_max_bits(amax);
+  if constexpr (NT > 64) {
+    constexpr int W = NT / 64;
+    if (lane_id() == 0) {
+      lds[wave_id()] = sum;
+      lds[W + wave_id()] = __uint_as_float(amax);
+    }
+    __syncthreads();
+    sum = 0.f;
+    amax = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      sum += lds[w];
+      amax = max(amax, __float_as_uint(lds[W + w]));
+    }
+  }
+}
+
+template <int NT>
+constexpr int row_block() { return NT < 256 ? 256 : NT; }
+
+template <typename T, int NT, int CH, bool NORM>
+__global__ __launch_bounds__(row_block<NT>()) void row_int8_kernel(RowInt8Args a) {
+  __shared__ float lds[2 * (NT / 64)];
+  constexpr int ROWS = row_block<NT>() / NT;
+  const int t = static_cast<int>(threadIdx.x) % NT;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / NT;
+  if (row >= a.rows) return;   // whole waves of a workgroup without barriers (NT == 64)
+  const T* x = static_cast<const T*>(a.x) + row * a.ldx;
+  float v[CH][8], w[CH][8];
+#pragma unroll
+  for (int k = 0; k < CH; ++k) {
+    const int c = (k * NT + t) * 8;
+    load_chunk(x + c, a.dim - c, v[k]);
+  }
+  float sum = 0.f;
+  uint32_t amax = 0;
+  if constexpr (NORM) {
+    if (a.residual != nullptr) {
+      const T* r = static_cast<const T*>(a.residual) + row * a.ldr;
+#pragma unroll
+      for (int k = 0; k < CH; ++k) {
+        const int c = (k * NT + t) * 8;
+        load_chunk(r + c, a.dim - c, w[k]);
+      }
+#pragma unroll
+      for (int k = 0; k < CH; ++k) {
+        const int c = (k * NT + t) * 8;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[k][e] = static_cast<float>(static_cast<T>(v[k][e] + w[k][e]));
+        store_chunk(static_cast<T*>(a.sum) + row * a.dim + c, a.dim - c, v[k]);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+      const int c = (k * NT + t) * 8;
+      load_weight8(a.weight, a.param_dtype, c, a.dim - c, w[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < CH; ++k)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        sum = __builtin_fmaf(v[k][e], v[k][e], sum);
+        v[k][e] *= w[k][e];
+      }
+  }
+#pragma unroll
+  for (int k = 0; k < CH; ++k)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) amax = max(amax, magnitude_bits(v[k][e]));
+  row_reduce<NT>(sum, amax, lds);
+  float rstd = 1.f;
+  if constexpr (NORM) rstd = 1.f / sqrtf(sum / static_cast<float>(a.dim) + a.eps);
+  if constexpr (NORM) {
+    if (a.out != nullptr) {
+      T* out = static_cast<T*>(a.out) + row * a.dim;
+#pragma unroll
+      for (int k = 0; k < CH; ++k) {
+        const int c = (k * NT + t) * 8;
+        float o[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = v[k][e] * rstd;
+        store_chunk(out + c, a.dim - c, o);
+      }
+    }
+    if (a.values == nullptr) return;
+  }
+  const Int8Scale s = int8_scale(amax, rstd);
+  // A row whose scale is the floor may have an inverse beyond fp32.
+  const float inverse = NORM ? fminf(rstd * s.inverse, 3.4028234e38f) : s.inverse;
+  int8_t* q = a.values + row * a.ldv;
+#pragma unroll
+  for (int k = 0; k < CH; ++k) {
+    const int c = (k * NT + t) * 8;
+    if (c < a.dim) store_bytes(q + c, pack_int8(v[k], inverse, s.keep));
+  }
+  if (t == 0) a.scales[row] = s.scale;
+}
+
+// Rows blockIdx.x, blockIdx.x + gridDim.x, ... of ROWS each.  `partials`
+// [gridDim.x][dim]: the workgroup's share of the weight's gradient.
+template <typename T, int NT, int CH>
+__global__ __launch_bounds__(row_block<NT>()) void rms_norm_backward_kernel(RmsNormBackwardArgs a) {
+  constexpr int ROWS = row_block<NT>() / NT;
+  // Row reductions (two sets of slots), or [dim] sums of workgroups whose
+  // waves hold a row each.
+  extern __shared__ float lds[];
+  const int t = static_cast<int>(threadIdx.x) % NT;
+  float w[CH][8], gw[CH][8];
+#pragma unroll
+  for (int k = 0; k < CH; ++k) {
+    const int c = (k * NT + t) * 8;
+    load_weight8(a.weight, a.param_dtype, c, a.dim - c, w[k]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) gw[k][e] = 0.f;
+  }
+  const float inv_dim = 1.f / static_cast<float>(a.dim);
+  int turn = 0;
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / NT; row < a.rows;
+       row += static_cast<int64_t>(gridDim.x) * ROWS, turn ^= 1) {
+    float v[CH][8], g[CH][8];
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+      const int c = (k * NT + t) * 8;
+      load_chunk(static_cast<const T*>(a.sum) + row * a.ldsum + c, a.dim - c, v[k]);
+      load_chunk(static_cast<const T*>(a.grad) + row * a.ldg + c, a.dim - c, g[k]);
+    }
+    float ss = 0.f, sg = 0.f;
+#pragma unroll
+    for (int k = 0; k < CH; ++k)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        ss = __builtin_fmaf(v[k][e], v[k][e], ss);
+        sg = __builtin_fmaf(g[k][e] * w[k][e], v[k][e], sg);
+      }
+    ss = wave_sum_dpp(ss);
+    sg = wave_sum_dpp(sg);
+    if constexpr (NT > 64) {
+      // Two sets of slots, taken in turn: a wave that runs ahead writes the
+      // set that no wave is reading any more.
+      constexpr int W = NT / 64;
+      float* slot = lds + turn * 2 * W;
+      if (lane_id() == 0) {
+        slot[wave_id()] = ss;
+        slot[W + wave_id()] = sg;
+      }
+      __syncthreads();
+      ss = sg = 0.f;
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        ss += slot[i];
+        sg += slot[W + i];
+      }
+    }
+    const float rstd = 1.f / sqrtf(ss * inv_dim + a.eps);
+    const float mean = sg * inv_dim * rstd * rstd;   // mean(g xh) rstd
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+      const int c = (k * NT + t) * 8;
+      float d[8];
+      if (a.grad_sum != nullptr) {
+        load_chunk(static_cast<const T*>(a.grad_sum) + row * a.ldgs + c, a.dim - c, d);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) d[e] = 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        gw[k][e] = __builtin_fmaf(g[k][e], v[k][e] * rstd, gw[k][e]);
+        d[e] += rstd * (g[k][e] * w[k][e] - v[k][e] * mean);
+      }
+      store_chunk(static_cast<T*>(a.grad_x) + row * a.dim + c, a.dim - c, d);
+    }
+  }
+  if (a.partials == nullptr) return;
+  float* part = a.partials + static_cast<int64_t>(blockIdx.x) * a.dim;
+  if constexpr (NT > 64) {
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+      const int c = (k * NT + t) * 8;
+      store_chunk(part + c, a.dim - c, gw[k]);
+    }
+  } else {
+    // The workgroup's waves add their sums in turn.
+    for (int q = 0; q < ROWS; ++q) {
+      if (wave_id() == q) {
+#pragma unroll
+        for (int k = 0; k < CH; ++k)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int c = (k * NT + t) * 8 + e;
+            if (c < a.dim) lds[c] = q > 0 ? lds[c] + gw[k][e] : gw[k][e];
+          }
+      }
+      __syncthreads();
+    }
+    for (int c = static_cast<int>(threadIdx.x); c < a.dim; c += row_block<NT>()) part[c] = lds[c];
+  }
+}
+
+// out[c] = sum over the workgroups of partials[b][c], in their order within
+// eight interleaved runs.
+constexpr int kSumCols = 32;
+template <typename T>
+__global__ __launch_bounds__(256) void rms_norm_weight_kernel(const float* partials, int blocks, int dim, T* out) {
+  __shared__ float lds[8][kSumCols];
+  const int c = static_cast<int>(threadIdx.x) % kSumCols, r = static_cast<int>(threadIdx.x) / kSumCols;
+  const int col = static_cast<int>(blockIdx.x) * kSumCols + c;
+  float sum = 0.f;
+  if (col < dim)
+    for (int b = r; b < blocks; b += 8) sum += partials[static_cast<int64_t>(b) * dim + col];
+  lds[r][c] = sum;
+  __syncthreads();
+  if (r == 0 && col < dim) {
+    for (int i = 1; i < 8; ++i) sum += lds[i][c];
+    out[col] = static_cast<T>(sum);
+  }
+}
+
+template <typename T, int NT, int CH, bool NORM>
+static void launch_row_k(const RowInt8Args& a, hipStream_t stream) {
+  constexpr int ROWS = row_block<NT>() / NT;
+  hipLaunchKernelGGL((row_int8_kernel<T, NT, CH, NORM>), dim3(static_cast<unsigned>((a.rows + ROWS - 1) / ROWS)),
+                     dim3(row_block<NT>()), 0, stream, a);
+}
+
+template <typename T, bool NORM>
+static void launch_row_t(const RowInt8Args& a, hipStream_t stream) {
+  if (a.dim <= 512) launch_row_k<T, 64, 1, NORM>(a, stream);
+  else if (a.dim <= 1024) launch_row_k<T, 64, 2, NORM>(a, stream);
+  else if (a.dim <= 2048) launch_row_k<T, 256, 1, NORM>(a, stream);
+  else if (a.dim <= 4096) launch_row_k<T, 256, 2, NORM>(a, stream);
+  else if (a.dim <= 8192) launch_row_k<T, 256, 4, NORM>(a, stream);
+  else if (a.dim <= 16384) launch_row_k<T, 1024, 2, NORM>(a, stream);
+  else if constexpr (!NORM) {
+    if (a.dim <= 32768) launch_row_k<T, 1024, 4, NORM>(a, stream);
+    else launch_row_k<T, 1024, 8, NORM>(a, stream);
+  }
+}
+
+void launch_row_int8(const RowInt8Args& a, bool norm, hipStream_t stream) {
+  if (norm) {
+    if (a.dtype == kF16) launch_row_t<_Float16, true>(a, stream);
+    else launch_row_t<__bf16, true>(a, stream);
+  } else if (a.dtype == kF16) {
+    launch_row_t<_Float16, false>(a, stream);
+  } else if (a.dtype == kBF16) {
+    launch_row_t<__bf16, false>(a, stream);
+  } else {
+    launch_row_t<float, false>(a, stream);
+  }
+}
+
+int rms_norm_backward_blocks(int64_t rows, int dim) {
+  const int64_t per = dim <= 1024 ? 4 : 1;
+  const int64_t blocks = (rows + per - 1) / per;
+  return static_cast<int>(blocks < 512 ? blocks : 512);
+}
+
+template <typename T, int NT, int CH>
+static void launch_backward_k(const RmsNormBackwardArgs& a, hipStream_t stream) {
+  const size_t lds = NT > 64 ? 4 * (NT / 64) * sizeof(float) : (static_cast<size_t>(a.dim) + 8) * sizeof(float);
+  hipLaunchKernelGGL((rms_norm_backward_kernel<T, NT, CH>), dim3(rms_norm_backward_blocks(a.rows, a.dim)),
+                     dim3(row_block<NT>()), lds, stream, a);
+}
+
+template <typename T>
+static void launch_backward_t(const RmsNormBackwardArgs& a, hipStream_t stream) {
+  if (a.dim <= 512) launch_backward_k<T, 64, 1>(a, stream);
+  else if (a.dim <= 1024) launch_backward_k<T, 64, 2>(a, stream);
+  else if (a.dim <= 2048) launch_backward_k<T, 256, 1>(a, stream);
+  else if (a.dim <= 4096) launch_backward_k<T, 256, 2>(a, stream);
+  else if (a.dim <= 8192) launch_backward_k<T, 256, 4>(a, stream);
+  else launch_backward_k<T, 1024, 2>(a, stream);
+}
+
+void launch_rms_norm_backward(const RmsNormBackwardArgs& a, hipStream_t stream) {
+  if (a.rows == 0) {
+    // No rows: the weight's gradient is a sum over no workgroups.
+  } else if (a.dtype == kF16) launch_backward_t<_Float16>(a, stream);
+  else launch_backward_t<__bf16>(a, stream);
+  if (a.partials == nullptr) return;
+  const int blocks = rms_norm_backward_blocks(a.rows, a.dim);
+  const dim3 grid((a.dim + kSumCols - 1) / kSumCols);
+  if (a.param_dtype == kF32)
+    hipLaunchKernelGGL((rms_norm_weight_kernel<float>), grid, dim3(256), 0, stream, a.partials, blocks, a.dim, static_cast<float*>(a.grad_weight));
+  else if (a.param_dtype == kF16)
+    hipLaunchKernelGGL((rms_norm_weight_kernel<_Float16>), grid, dim3(256), 0, stream, a.partials, blocks, a.dim, static_cast<_Float16*>(a.grad_weight));
+  else
+    hipLaunchKernelGGL((rms_norm_weight_kernel<__bf16>), grid, dim3(256), 0, stream, a.partials, blocks, a.dim, static_cast<__bf16*>(a.grad_weight));
+}
+
+}  // namespace da

@@ -1,4 +1,5 @@
-"""ctypes binding of the gfx950 C ABI (``include/double_attention_hip.h``).
+"""ctypes binding of the gfx950 C ABI (``include/double_attention_hip.h`` and
+``include/double_attention_int8.h``).
 
 The library is built in-tree by ``double-attention_amd/build.py`` into
 ``double_attention/lib/libdouble_attention_hip.so``.  Loading needs no GPU
@@ -49,7 +50,8 @@ ERROR_NAMES = {
     -5: "workspace too small",
 }
 
-ABI_VERSION = 19
+ABI_VERSION = 20
+INT8_GROUP = 128
 NOALLOC_SCRATCH_BYTES = 128 << 20
 
 _vp = ctypes.c_void_p
@@ -143,7 +145,7 @@ class AttentionBackwardArgs(ctypes.Structure):
     ]
 
 
-# name -> (restype, argtypes); every function declared in the public header.
+# name -> (restype, argtypes); every function declared in include/double_attention_hip.h.
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "da_abi_version": (_i32, []),
     "da_last_error": (ctypes.c_char_p, []),
@@ -213,6 +215,32 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "da_shared_dictionary_attention_forward_noalloc": (_i32, [ctypes.POINTER(SdaForwardArgs), _vp]),
 }
 
+# The 8-bit operators, declared in include/double_attention_int8.h.
+INT8_SIGNATURES: dict[str, tuple[object, list[object]]] = {
+    "da_quantize_int8": (_i32, [_vp, _i64, _i64, _i64, _i32, _i64, _vp, _i64, _vp, _vp]),
+    "da_dequantize_int8": (_i32, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _i32, _vp]),
+    "da_linear_int8": (
+        _i32,
+        [
+            _vp, _i64, _vp, _i64, _i64,  # x, pitch, scales, rows, in_features
+            _vp, _i64, _vp, _i64,  # weight, pitch, scales, out_features
+            _vp, _i32, _i32, _vp, _i64,  # bias, bias dtype, activation, residual, its pitch
+            _vp, _i32, _vp,  # out, dtype, stream
+        ],
+    ),
+    "da_add_rms_norm": (
+        _i32,
+        [_vp, _i64, _vp, _i64, _i64, _i64, _vp, _i32, _f32, _i32, _vp, _vp, _vp, _i64, _vp, _vp],
+    ),
+    "da_add_rms_norm_backward_workspace_bytes": (_i64, [_i64, _i64]),
+    "da_add_rms_norm_backward": (
+        _i32,
+        [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _i32, _f32, _i32, _vp, _vp, _vp, _i64, _vp],
+    ),
+    "da_gelu_int8": (_i32, [_vp, _i64, _i64, _i64, _i32, _vp, _vp, _i64, _vp, _vp]),
+    "da_gelu_int8_backward": (_i32, [_vp, _i64, _i64, _i64, _vp, _vp, _i64, _i32, _vp, _vp, _vp]),
+}
+
 _lib: ctypes.CDLL | None = None
 _load_error: str | None = None
 
@@ -229,7 +257,7 @@ def _load() -> ctypes.CDLL:
             f"{path} does not exist; build it with `python double-attention_amd/build.py`"
         )
     lib = ctypes.CDLL(str(path))
-    for name, (restype, argtypes) in SIGNATURES.items():
+    for name, (restype, argtypes) in {**SIGNATURES, **INT8_SIGNATURES}.items():
         fn = getattr(lib, name)  # AttributeError if the symbol is missing
         fn.restype = restype
         fn.argtypes = argtypes

@@ -1,0 +1,417 @@
+"""8-bit operators of the blocks' feed-forward on the gfx950 kernels.
+
+Three operators around one format (``QuantizedRows``: signed integers from
+-127 to 127 with an fp32 scale for each row, or for each 128 columns of it):
+
+* ``linear_int8_hip``: the linear layer on 8-bit integers, one scale per token
+  and per output channel, with bias, GELU and residual;
+* ``add_rms_norm_int8_hip`` and ``add_rms_norm_hip``: the root-mean-square
+  norm with the residual's addition in front of it, for that linear layer in
+  8 bits, or in 16 bits with a backward pass;
+* ``gelu_int8_hip`` / ``gelu_int8_backward_hip``, and ``quantize_int8_hip`` /
+  ``dequantize_int8_hip`` in groups of 128: activations that the backward pass
+  finds in 8 bits.
+
+As in ``hip_ops``, PyTorch supplies memory and the current stream, and nothing
+falls back to another implementation: a call the kernels do not cover raises.
+The kernels run on the inputs' device, whichever is current.
+"""
+
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+from torch import Tensor
+
+from . import _lib
+from .hip_ops import _half_code, _stream, dtype_code
+
+INT8_GROUP = _lib.INT8_GROUP
+# Columns of rows with one scale each, and widths of the norm.
+MAX_ROW_COLUMNS = 65536
+MAX_NORM_WIDTH = 16384
+
+
+class QuantizedRows(NamedTuple):
+    """Rows in 8 bits.
+
+    ``values`` is int8 ``[..., columns]``, ``scales`` fp32 ``[..., G]``: G = 1
+    (``group`` None, a scale for each row) or the columns' groups of 128
+    (``group`` 128).  ``values * scale`` is what the rows stand for.  A row
+    (group) whose scale is NaN held an infinity or a NaN.  ``values`` made
+    here are views of rows padded to a multiple of 16 bytes, the pitch the
+    kernels read; others are copied into such rows in each call.
+    """
+
+    values: Tensor
+    scales: Tensor
+    group: int | None = None
+
+
+def _launch(what: str, device: torch.device, fn, *args) -> None:
+    """``fn(*args, stream)`` on ``device``, which need not be the current one."""
+
+    stream = _stream(device)
+    if device.index is None or device.index == torch._C._cuda_getDevice():
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, stream)
+    if rc:
+        _lib.check(rc, what)
+
+
+def _on_device(what: str, device: torch.device, *tensors: Tensor | None) -> None:
+    if device.type != "cuda":
+        raise ValueError(f"{what}: HIP kernels require tensors on a ROCm device")
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"{what}: all tensors must be on {device}, got one on {t.device}")
+
+
+def _no_grad(what: str, *tensors: Tensor | None) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError(f"{what} has no autograd of its own: call it under torch.no_grad(), or detach its inputs")
+
+
+def _rows(t: Tensor) -> tuple[Tensor, int]:
+    """``t`` as ``[rows, columns]`` with unit column stride, and its row pitch.
+
+    Rows at any pitch are read where they are; other orders are copied."""
+
+    columns = t.shape[-1]
+    if t.ndim != 2:
+        t = t.reshape(-1, columns) if columns else t.reshape(0, 0)
+    rows = t.shape[0]
+    if columns > 1 and t.stride(1) != 1:
+        t = t.contiguous()
+    pitch = t.stride(0) if rows > 1 else columns
+    if pitch < columns:   # expanded rows
+        t = t.contiguous()
+        pitch = columns
+    return t, pitch
+
+
+def _check_rows(what: str, t: Tensor, floating: bool = False) -> None:
+    if t.ndim < 1 or t.shape[-1] < 1:
+        raise ValueError(f"{what}: expected rows of at least one column, got shape {tuple(t.shape)}")
+    if floating:
+        dtype_code(t.dtype)
+    else:
+        _half_code(t.dtype)
+
+
+def _new_values(lead: torch.Size, columns: int, device: torch.device) -> tuple[Tensor, int]:
+    pitch = (columns + 15) // 16 * 16
+    store = torch.empty(*lead, pitch, dtype=torch.int8, device=device)
+    return (store if pitch == columns else store[..., :columns]), pitch
+
+
+def _values_rows(t: Tensor) -> tuple[Tensor, int]:
+    """8-bit rows as the kernels read them: 16-byte aligned at a pitch of a
+    multiple of 16, with the last row's last 16 bytes inside the storage."""
+
+    t, pitch = _rows(t)
+    rows, columns = t.shape
+    if rows == 1:
+        pitch = (columns + 15) // 16 * 16
+    fits = pitch % 16 == 0 and t.data_ptr() % 16 == 0
+    if fits and columns % 16 and rows:
+        last = t.storage_offset() + (rows - 1) * pitch + (columns + 15) // 16 * 16
+        fits = last <= t.untyped_storage().nbytes()
+    if not fits:
+        padded, pitch = _new_values(t.shape[:1], columns, t.device)
+        padded.copy_(t)
+        t = padded
+    return t, pitch
+
+
+def _check_quantized(what: str, rows: QuantizedRows) -> None:
+    values, scales, group = rows
+    if values.dtype != torch.int8 or scales.dtype != torch.float32:
+        raise ValueError(f"{what}: quantized rows are int8 values with fp32 scales")
+    if group not in (None, INT8_GROUP):
+        raise NotImplementedError(f"{what}: a scale for each row (group None) or each {INT8_GROUP} columns")
+    if values.ndim < 1 or values.shape[-1] < 1:
+        raise ValueError(f"{what}: expected rows of at least one column, got shape {tuple(values.shape)}")
+    groups = 1 if group is None else -(-values.shape[-1] // group)
+    if scales.shape[:-1] != values.shape[:-1] or scales.ndim != values.ndim or scales.shape[-1] != groups:
+        raise ValueError(f"{what}: scales of shape {tuple(scales.shape)} do not fit values of shape {tuple(values.shape)}")
+
+
+def quantize_int8_hip(x: Tensor, group: int | None = None) -> QuantizedRows:
+    """``x``'s rows (the last dimension; fp32, fp16 or bf16) in 8 bits.
+
+    ``scale = max(amax, 127 * 2^-126) / 127`` over each row (``group`` None, up
+    to 65536 columns: tokens and output channels of ``linear_int8_hip``) or
+    each 128 columns of it (``INT8_GROUP``: saved activations), values
+    ``rint(x / scale)``.  A row (group) with an infinity or a NaN stands for
+    NaN throughout.
+    """
+
+    _check_rows("quantize_int8_hip", x, floating=True)
+    _on_device("quantize_int8_hip", x.device)
+    if group not in (None, INT8_GROUP):
+        raise NotImplementedError(f"quantize_int8_hip: a scale for each row (group None) or each {INT8_GROUP} columns")
+    lead, columns = x.shape[:-1], x.shape[-1]
+    rows, pitch = _rows(x.detach())
+    values, ldv = _new_values(lead, columns, x.device)
+    scales = torch.empty(*lead, 1 if group is None else -(-columns // INT8_GROUP), dtype=torch.float32, device=x.device)
+    _launch("quantize_int8_hip", x.device, _lib.get().da_quantize_int8, rows.data_ptr(), rows.shape[0], columns, pitch,
+            dtype_code(x.dtype), group or 0, values.data_ptr(), ldv, scales.data_ptr())
+    return QuantizedRows(values, scales, group)
+
+
+def dequantize_int8_hip(rows: QuantizedRows, dtype: torch.dtype = torch.bfloat16) -> Tensor:
+    """What the 8-bit rows stand for: ``values * scale``, rounded once to ``dtype``."""
+
+    _check_quantized("dequantize_int8_hip", rows)
+    device = rows.values.device
+    _on_device("dequantize_int8_hip", device, rows.scales)
+    values, pitch = _values_rows(rows.values)
+    columns = values.shape[1]
+    scales = rows.scales.contiguous()
+    out = torch.empty(rows.values.shape, dtype=dtype, device=device)
+    _launch("dequantize_int8_hip", device, _lib.get().da_dequantize_int8, values.data_ptr(), values.shape[0], columns,
+            pitch, scales.data_ptr(), rows.group or 0, out.data_ptr(), columns, dtype_code(dtype))
+    return out
+
+
+def linear_int8_hip(
+    x: Tensor | QuantizedRows,
+    weight: QuantizedRows,
+    bias: Tensor | None = None,
+    *,
+    activation: str | None = None,
+    residual: Tensor | None = None,
+    dtype: torch.dtype | None = None,
+) -> Tensor:
+    """``act(x @ weight.T (+ bias)) (+ residual)`` on 8-bit integers.
+
+    ``weight``: ``quantize_int8_hip`` of the ``[out_features, in_features]``
+    matrix (a scale for each output channel), made once.  ``x``: 8-bit rows
+    with a scale for each token (``add_rms_norm_int8_hip``), or a 16-bit
+    tensor, which is quantized so here.  The products and sums are exact
+    integers; scales, bias and ``activation`` (None or ``"gelu"``) are fp32,
+    the result is rounded to ``dtype`` (default: the 16-bit input's or
+    residual's type, else bf16), then the residual is added and rounded, as by
+    ``linear_hip``.  For inference: no backward.
+    """
+
+    what = "linear_int8_hip"
+    if activation not in (None, "gelu"):
+        raise ValueError(f"unsupported activation {activation!r}")
+    _check_quantized(what, weight)
+    if weight.values.ndim != 2 or weight.group is not None:
+        raise ValueError(f"{what}: the weight is [out_features, in_features] with one scale for each output channel")
+    if isinstance(x, QuantizedRows):
+        _check_quantized(what, x)
+        if x.group is not None:
+            raise ValueError(f"{what}: x needs one scale for each token")
+        if dtype is None:
+            dtype = torch.bfloat16 if residual is None else residual.dtype
+        shape, device = x.values.shape, x.values.device
+        _on_device(what, device, x.scales)
+    else:
+        _check_rows(what, x)
+        shape, device = x.shape, x.device
+        if dtype is None:
+            dtype = x.dtype
+    code = _half_code(dtype)
+    out_features, in_features = weight.values.shape
+    if shape[-1] != in_features:
+        raise ValueError(f"{what}: rows of {shape[-1]} columns against a weight of {in_features}")
+    _on_device(what, device, weight.values, weight.scales, bias, residual)
+    if bias is not None and bias.shape != (out_features,):
+        raise ValueError(f"{what}: the bias must have shape ({out_features},)")
+    if residual is not None and (residual.shape != (*shape[:-1], out_features) or residual.dtype != dtype):
+        raise ValueError(f"{what}: the residual must match the output's shape and dtype")
+    _no_grad(what, None if isinstance(x, QuantizedRows) else x, bias, residual)
+    if not isinstance(x, QuantizedRows):
+        x = quantize_int8_hip(x)
+    rows, ldx = _values_rows(x.values)
+    w, ldw = _values_rows(weight.values)
+    x_scales, w_scales = x.scales.contiguous(), weight.scales.contiguous()
+    if bias is not None:
+        bias = bias.contiguous()
+    res, ldr = (None, 0) if residual is None else _rows(residual)
+    out = torch.empty(*shape[:-1], out_features, dtype=dtype, device=device)
+    _launch(what, device, _lib.get().da_linear_int8, rows.data_ptr(), ldx, x_scales.data_ptr(), rows.shape[0],
+            in_features, w.data_ptr(), ldw, w_scales.data_ptr(), out_features,
+            None if bias is None else bias.data_ptr(), _lib.DA_F32 if bias is None else dtype_code(bias.dtype),
+            _lib.DA_ACT_GELU if activation else _lib.DA_ACT_NONE, None if res is None else res.data_ptr(), ldr,
+            out.data_ptr(), code)
+    return out
+
+
+def _check_norm(what: str, x: Tensor, weight: Tensor | None, *others: Tensor | None) -> None:
+    _check_rows(what, x)
+    _on_device(what, x.device, weight, *others)
+    for t in others:
+        if t is not None and (t.shape != x.shape or t.dtype != x.dtype):
+            raise ValueError(f"{what}: expected shape {tuple(x.shape)} and {x.dtype}, got {tuple(t.shape)} and {t.dtype}")
+    if weight is not None:
+        dtype_code(weight.dtype)
+        if weight.shape != x.shape[-1:]:
+            raise ValueError(f"{what}: the weight must have shape ({x.shape[-1]},)")
+
+
+def _add_rms_norm(what, x, residual, weight, eps, want_out, want_int8):
+    width, device = x.shape[-1], x.device
+    rows, ldx = _rows(x)
+    res, ldr = (None, 0) if residual is None else _rows(residual)
+    w = None if weight is None else weight.contiguous()
+    total = x if residual is None else torch.empty(x.shape, dtype=x.dtype, device=device)
+    out = torch.empty(x.shape, dtype=x.dtype, device=device) if want_out else None
+    values = scales = None
+    ldv = 0
+    if want_int8:
+        values, ldv = _new_values(x.shape[:-1], width, device)
+        scales = torch.empty(*x.shape[:-1], 1, dtype=torch.float32, device=device)
+    _launch(what, device, _lib.get().da_add_rms_norm, rows.data_ptr(), ldx, None if res is None else res.data_ptr(), ldr,
+            rows.shape[0], width, None if w is None else w.data_ptr(), _lib.DA_F32 if w is None else dtype_code(w.dtype),
+            float(eps), _half_code(x.dtype), None if residual is None else total.data_ptr(),
+            None if out is None else out.data_ptr(), None if values is None else values.data_ptr(), ldv,
+            None if scales is None else scales.data_ptr())
+    return out, values, scales, total
+
+
+class _AddRmsNormFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, weight, eps):  # type: ignore[override]
+        out, _, _, total = _add_rms_norm("add_rms_norm_hip", x, residual, weight, eps, True, False)
+        ctx.save_for_backward(total, weight)
+        ctx.eps = eps
+        ctx.set_materialize_grads(False)
+        return out if residual is None else (out, total)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad, grad_sum=None):  # type: ignore[override]
+        total, weight = ctx.saved_tensors
+        wants_x = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
+        wants_weight = ctx.needs_input_grad[2]
+        if grad is None:
+            d_x, d_weight = grad_sum, None
+        else:
+            d_x, d_weight = add_rms_norm_backward_hip(total, grad, grad_sum, weight, ctx.eps, want_weight=wants_weight)
+        d_x = d_x if wants_x else None
+        return (d_x if ctx.needs_input_grad[0] else None, d_x if ctx.needs_input_grad[1] else None,
+                d_weight if wants_weight else None, None)
+
+
+def add_rms_norm_hip(
+    x: Tensor, residual: Tensor | None = None, weight: Tensor | None = None, eps: float = 1e-6
+) -> tuple[Tensor, Tensor]:
+    """``(n, s)``: the sum ``s = x + residual`` (rounded to x's 16-bit type; x
+    itself without a residual) and its root-mean-square norm
+    ``n = s / sqrt(mean(s^2) + eps) * weight`` over the last dimension (at most
+    16384 wide), statistics in fp32 and one rounding; one launch.
+    Differentiable in x, the residual and the weight, through both outputs.
+    """
+
+    _check_norm("add_rms_norm_hip", x, weight, residual)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight)):
+        got = _AddRmsNormFunction.apply(x, residual, weight, eps)
+        return (got, x) if residual is None else got
+    out, _, _, total = _add_rms_norm("add_rms_norm_hip", x, residual, weight, eps, True, False)
+    return out, total
+
+
+def add_rms_norm_int8_hip(
+    x: Tensor, residual: Tensor | None = None, weight: Tensor | None = None, eps: float = 1e-6
+) -> tuple[QuantizedRows, Tensor]:
+    """``add_rms_norm_hip`` with its norm in 8 bits, a scale for each row: the
+    fp32 norm is quantized without a rounding to 16 bits in between.  The sum
+    stays 16-bit.  For inference: no backward."""
+
+    what = "add_rms_norm_int8_hip"
+    _check_norm(what, x, weight, residual)
+    _no_grad(what, x, residual, weight)
+    _, values, scales, total = _add_rms_norm(what, x, residual, weight, eps, False, True)
+    return QuantizedRows(values, scales), total
+
+
+def add_rms_norm_backward_hip(
+    total: Tensor,
+    grad: Tensor,
+    grad_sum: Tensor | None,
+    weight: Tensor | None,
+    eps: float = 1e-6,
+    *,
+    want_weight: bool = True,
+) -> tuple[Tensor, Tensor | None]:
+    """The backward of ``add_rms_norm_hip``: ``(grad_x, grad_weight)`` from its
+    sum, the gradient at its norm and the one at its sum (None: zero).  grad_x
+    is the gradient at x and at the residual; grad_weight (None without a
+    weight, or unless wanted) is summed in fp32 in an order that the sizes
+    fix, and rounded once to the weight's type.
+    """
+
+    what = "add_rms_norm_backward_hip"
+    _check_norm(what, total, weight, grad, grad_sum)
+    width, device = total.shape[-1], total.device
+    lib = _lib.get()
+    s, lds = _rows(total.detach())
+    g, ldg = _rows(grad.detach())
+    gs, ldgs = (None, 0) if grad_sum is None else _rows(grad_sum.detach())
+    w = None if weight is None else weight.detach().contiguous()
+    grad_x = torch.empty(total.shape, dtype=total.dtype, device=device)
+    grad_weight = workspace = None
+    nbytes = 0
+    if w is not None and want_weight:
+        grad_weight = torch.empty_like(w)
+        nbytes = lib.da_add_rms_norm_backward_workspace_bytes(s.shape[0], width)
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    _launch(what, device, lib.da_add_rms_norm_backward, s.data_ptr(), lds, g.data_ptr(), ldg,
+            None if gs is None else gs.data_ptr(), ldgs, s.shape[0], width, None if w is None else w.data_ptr(),
+            _lib.DA_F32 if w is None else dtype_code(w.dtype), float(eps), _half_code(total.dtype), grad_x.data_ptr(),
+            None if grad_weight is None else grad_weight.data_ptr(),
+            None if workspace is None else workspace.data_ptr(), nbytes)
+    return grad_x, grad_weight
+
+
+def gelu_int8_hip(z: Tensor) -> tuple[Tensor, QuantizedRows]:
+    """``(gelu(z), kept)``: the exact GELU of a 16-bit tensor, and z in 8 bits
+    in groups of 128 for ``gelu_int8_backward_hip``, in one pass.  The output
+    is of z itself; only the backward sees the kept rows."""
+
+    what = "gelu_int8_hip"
+    _check_rows(what, z)
+    _on_device(what, z.device)
+    _no_grad(what, z)
+    columns, device = z.shape[-1], z.device
+    rows, pitch = _rows(z)
+    out = torch.empty(z.shape, dtype=z.dtype, device=device)
+    values, ldv = _new_values(z.shape[:-1], columns, device)
+    scales = torch.empty(*z.shape[:-1], -(-columns // INT8_GROUP), dtype=torch.float32, device=device)
+    _launch(what, device, _lib.get().da_gelu_int8, rows.data_ptr(), rows.shape[0], columns, pitch, _half_code(z.dtype),
+            out.data_ptr(), values.data_ptr(), ldv, scales.data_ptr())
+    return out, QuantizedRows(values, scales, INT8_GROUP)
+
+
+def gelu_int8_backward_hip(kept: QuantizedRows, grad: Tensor, *, want_output: bool = True) -> tuple[Tensor, Tensor | None]:
+    """``(grad_z, gelu)`` from the rows that ``gelu_int8_hip`` kept:
+    ``grad * gelu'(zt)`` and, unless not wanted, ``gelu(zt)`` again (the
+    operand of the next layer's weight gradient), with ``zt`` what the kept
+    rows stand for; fp32, one rounding to grad's 16-bit type."""
+
+    what = "gelu_int8_backward_hip"
+    _check_quantized(what, kept)
+    _check_rows(what, grad)
+    if kept.group != INT8_GROUP:
+        raise ValueError(f"{what}: rows kept in groups of {INT8_GROUP} columns")
+    if kept.values.shape != grad.shape:
+        raise ValueError(f"{what}: gradients of shape {tuple(grad.shape)} at kept rows of shape {tuple(kept.values.shape)}")
+    device = grad.device
+    _on_device(what, device, kept.values, kept.scales)
+    values, ldv = _values_rows(kept.values)
+    scales = kept.scales.contiguous()
+    g, ldg = _rows(grad.detach())
+    grad_z = torch.empty(grad.shape, dtype=grad.dtype, device=device)
+    out = torch.empty(grad.shape, dtype=grad.dtype, device=device) if want_output else None
+    _launch(what, device, _lib.get().da_gelu_int8_backward, values.data_ptr(), values.shape[0], values.shape[1], ldv,
+            scales.data_ptr(), g.data_ptr(), ldg, _half_code(grad.dtype), grad_z.data_ptr(),
+            None if out is None else out.data_ptr())
+    return grad_z, out
