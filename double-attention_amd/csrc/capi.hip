@@ -706,8 +706,9 @@ int da_layer_norm_backward(const void* x, const void* grad, int64_t rows, int64_
 
 namespace {
 
-static_assert(DA_INT8_GROUP == da::kInt8Group, "columns per scale");
+static_assert(DA_INT8_GROUP == da::kInt8Group && DA_I8 == da::kI8, "columns per scale, dtype code");
 constexpr int64_t kInt8MaxElements = 1LL << 40;
+constexpr int64_t kInt8MaxPitch = 1 << 23;   // of 8-bit rows: 256 of them span less than 2^32 bytes
 
 int64_t element_bytes(int dtype) { return dtype == DA_F32 ? 4 : 2; }
 
@@ -725,7 +726,8 @@ int validate_int8(const char* what, const char* name, const void* values, int64_
   if (!values || !scales) return fail(DA_ERR_INVALID_ARGUMENT, "%s: %s or its scales are null", what, name);
   if (!aligned(values, 16) || ldv % 16 || !aligned(scales, 4))
     return fail(DA_ERR_ALIGNMENT, "%s: %s must be 16-byte aligned at a pitch of a multiple of 16", what, name);
-  if (ldv < cols || ldv > kInt8MaxElements) return fail(DA_ERR_INVALID_ARGUMENT, "%s: %s has a pitch below its width", what, name);
+  if (ldv < cols) return fail(DA_ERR_INVALID_ARGUMENT, "%s: %s has a pitch below its width", what, name);
+  if (ldv > kInt8MaxPitch) return fail(DA_ERR_UNSUPPORTED, "%s: %s has a pitch over 2^23", what, name);
   return DA_OK;
 }
 
@@ -737,7 +739,7 @@ int validate_sizes(const char* what, int64_t rows, int64_t cols, int64_t max_col
   return DA_OK;
 }
 
-constexpr int64_t kInt8MaxCols = 1 << 24;   // of rows in groups
+constexpr int64_t kInt8MaxCols = kInt8MaxPitch;   // of rows in groups
 
 }  // namespace
 
@@ -779,11 +781,18 @@ int da_dequantize_int8(const void* values, int64_t rows, int64_t cols, int64_t l
   return check_launch("dequantize");
 }
 
-int da_linear_int8(const void* x, int64_t ldx, const float* x_scales, int64_t rows, int64_t in_features,
+int64_t da_linear_int8_workspace_bytes(int64_t rows, int64_t in_features, int x_dtype) {
+  if (x_dtype == DA_I8 || rows < 1 || in_features < 1) return 0;
+  return align_up(rows * da::round_up(in_features, 16)) + align_up(rows * 4);
+}
+
+int da_linear_int8(const void* x, int x_dtype, int64_t ldx, const float* x_scales, int64_t rows, int64_t in_features,
                    const void* weight, int64_t ldw, const float* w_scales, int64_t out_features, const void* bias,
                    int bias_dtype, int activation, const void* residual, int64_t ldr, void* out, int dtype,
-                   da_stream_t stream) {
+                   void* workspace, int64_t workspace_bytes, da_stream_t stream) {
   if (!half_dtype(dtype)) return fail(DA_ERR_INVALID_ARGUMENT, "linear_int8: dtype must be DA_F16 or DA_BF16");
+  if (x_dtype != DA_I8 && !half_dtype(x_dtype))
+    return fail(DA_ERR_INVALID_ARGUMENT, "linear_int8: x must be DA_I8, DA_F16 or DA_BF16");
   if (activation != DA_ACT_NONE && activation != DA_ACT_GELU)
     return fail(DA_ERR_INVALID_ARGUMENT, "linear_int8: unknown activation %d", activation);
   if (bias && !any_dtype(bias_dtype)) return fail(DA_ERR_INVALID_ARGUMENT, "linear_int8: bad bias dtype");
@@ -795,14 +804,36 @@ int da_linear_int8(const void* x, int64_t ldx, const float* x_scales, int64_t ro
       ((rows + 63) / 64) * ((out_features + 63) / 64) > 0x7fff0000LL)
     return fail(DA_ERR_UNSUPPORTED, "linear_int8: out_features must be in [1, 2^24], and the output's tiles below 2^31");
   if (rows == 0) return ok();
-  if ((rc = validate_int8("linear_int8", "x", x, ldx, x_scales, in_features))) return rc;
+  // 16-bit rows of x's type are quantized by the kernel of few rows; others
+  // into the workspace first.
+  const bool quantize = x_dtype != DA_I8 && !(x_dtype == dtype && da::linear_int8_quantizes(rows, in_features));
+  if (x_dtype == DA_I8) rc = validate_int8("linear_int8", "x", x, ldx, x_scales, in_features);
+  else rc = validate_rows("linear_int8", "x", x, in_features, ldx, x_dtype);
+  if (rc) return rc;
   if ((rc = validate_int8("linear_int8", "weight", weight, ldw, w_scales, in_features))) return rc;
   if ((rc = validate_rows("linear_int8", "out", out, out_features, out_features, dtype))) return rc;
   if (residual && (rc = validate_rows("linear_int8", "residual", residual, out_features, ldr, dtype))) return rc;
-  da::launch_linear_int8({static_cast<const int8_t*>(x), ldx, x_scales, rows, static_cast<int>(in_features),
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (quantize) {
+    const int64_t ldv = da::round_up(in_features, 16);
+    const int64_t need = align_up(rows * ldv) + align_up(rows * 4);
+    if (!workspace || workspace_bytes < need)
+      return fail(DA_ERR_WORKSPACE, "linear_int8: the workspace needs %lld bytes", (long long)need);
+    if (!aligned(workspace, 16)) return fail(DA_ERR_ALIGNMENT, "linear_int8: the workspace must be 16-byte aligned");
+    int8_t* values = static_cast<int8_t*>(workspace);
+    float* scales = reinterpret_cast<float*>(values + align_up(rows * ldv));
+    da::launch_row_int8({x, ldx, nullptr, 0, rows, static_cast<int>(in_features), x_dtype, nullptr, 0, 0.f, nullptr,
+                         nullptr, values, ldv, scales},
+                        false, s);
+    x = values;
+    x_dtype = DA_I8;
+    ldx = ldv;
+    x_scales = scales;
+  }
+  da::launch_linear_int8({x, x_dtype, ldx, x_scales, rows, static_cast<int>(in_features),
                           static_cast<const int8_t*>(weight), ldw, w_scales, out_features, bias, bias_dtype,
                           activation == DA_ACT_GELU ? da::kGemmActGelu : da::kGemmActNone, residual, ldr, out, dtype},
-                         reinterpret_cast<hipStream_t>(stream));
+                         s);
   return check_launch("linear_int8");
 }
 

@@ -335,9 +335,10 @@ void launch_rms_norm_backward(const RmsNormBackwardArgs& a, hipStream_t stream);
 
 // Linear layer on 8-bit rows (gemm_int8.hip).
 struct LinearInt8Args {
-  const int8_t* x;
-  int64_t ldx;            // multiples of 16, as ldw
-  const float* x_scales;  // [rows]
+  const void* x;
+  int x_dtype;            // kI8, or 16 bits (== dtype) where linear_int8_quantizes(rows, K)
+  int64_t ldx;            // a multiple of 16 for kI8, as ldw
+  const float* x_scales;  // [rows] (kI8)
   int64_t rows;
   int K;                  // <= kRowInt8MaxCols
   const int8_t* w;
@@ -352,6 +353,7 @@ struct LinearInt8Args {
   void* out;              // [rows][N]
   int dtype;              // out and residual
 };
+bool linear_int8_quantizes(int64_t rows, int64_t K);
 void launch_linear_int8(const LinearInt8Args& a, hipStream_t stream);
 
 // Launch shape of the attention for a problem: value slice width, waves per

@@ -9,12 +9,16 @@
 // and, with a residual, added and rounded again (the order of an unfused
 // x + linear(...)).
 //
-// Tiles: 128 channels x 128 tokens per workgroup, four waves of 64 x 64 in
-// 16x16x64 MFMA blocks (v_mfma_i32_16x16x64_i8), K in stages of 128 bytes
-// through a ring of two XOR-swizzled LDS buffers filled by global->LDS DMA:
-// the layout of the 16-bit GEMM at twice the k per byte.  A stage's chunks
-// behind K (the pitch is a multiple of 16, the bytes between K and the pitch
-// are anything) are cut off in W's fragments: zero times anything is zero.
+// The tile kernel takes BI channels x BJ tokens a workgroup in 16x16x64 MFMA
+// blocks (v_mfma_i32_16x16x64_i8), K in stages of 128 bytes through a ring of
+// NST XOR-swizzled LDS buffers filled by global->LDS DMA: the layout of the
+// 16-bit GEMM at twice the k per byte.  A stage is two halves of 64 bytes, and
+// the fragments of a half are read from LDS while the half before it is
+// multiplied; the workgroup's one barrier a stage falls between the halves, so
+// the matrix cores have operands on both sides of it, and the buffer that it
+// frees is loaded again at once.  A stage's chunks behind K (the pitch is a
+// multiple of 16, the bytes between K and the pitch are anything) are cut off
+// in W's fragments: zero times anything is zero.
 #include "da_erf.h"
 #include "da_launch.h"
 #include "da_tile.h"
@@ -24,9 +28,7 @@ namespace da {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kI8Tile = 128;
 constexpr int kI8Stage = 128;   // bytes of k
-typedef XorTile<kI8Tile, kI8Stage / 16, false> TileI8;
 
 // The first n of a fragment's 16 bytes, zeros behind.
 __device__ __forceinline__ i32x4 first_bytes(i32x4 v, int n) {
@@ -38,156 +40,524 @@ __device__ __forceinline__ i32x4 first_bytes(i32x4 v, int n) {
   return v;
 }
 
-template <typename T, int EPI>
-__global__ __launch_bounds__(256) void linear_int8_kernel(LinearInt8Args a, int tiles_i, int tiles_j) {
-  constexpr int STAGE = 2 * TileI8::BYTES;
-  constexpr int PER_WAVE = 2 * TileI8::LOADS / 4;
-  __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
+// lds_barrier() with waits that the compiler takes into its own accounts: it
+// then knows that the fragments read before the barrier have arrived, and
+// does not wait for the ones read behind it before using them.
+__device__ __forceinline__ void counted_barrier() {
+  __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0)
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// A workgroup's tile: BI channels x BJ tokens over NWI x NWJ waves, NST stages
+// in LDS.  AHEAD > 0: stages that the L2 is asked for AHEAD stages before they
+// are multiplied (see below).
+template <int BI, int BJ, int NWI, int NWJ, int NST, int AHEAD = 0>
+struct I8Cfg {
+  static constexpr int kAhead = AHEAD;
+  static constexpr int kBI = BI, kBJ = BJ, kNWI = NWI, kNWJ = NWJ, kNST = NST;
+  static constexpr int WAVES = NWI * NWJ;
+  static constexpr int WI = BI / NWI, WJ = BJ / NWJ;    // a wave's block
+  static constexpr int NA = WI / 16, NB = WJ / 16;      // its MFMA blocks
+  typedef XorTile<BI, kI8Stage / 16, false> TileW;
+  typedef XorTile<BJ, kI8Stage / 16, false> TileX;
+  static constexpr int STAGE = TileW::BYTES + TileX::BYTES;
+  static constexpr int LOADS = (TileW::LOADS + TileX::LOADS) / WAVES;   // a wave's, each stage
+  static_assert((TileW::LOADS + TileX::LOADS) % WAVES == 0, "every wave loads as much");
+  static constexpr int ROWB = WI * 2 + 16;              // bytes of a staged output row
+  static_assert(TileW::LOADS % WAVES == 0 && WAVES % 2 == 0, "a load of all waves is of one operand, and 16 rows or a multiple");
+  static constexpr int PARAMS = 2 * BI + BJ;            // floats that the epilogue reads
+  static_assert(16 * ROWB * WAVES + 4 * PARAMS <= NST * STAGE, "the epilogue's rows and parameters fit the stage buffers");
+  static_assert(BI <= 64 * WAVES && BJ <= 64 * WAVES, "a thread fetches one channel's and one token's parameters");
+};
+
+// Tile `t` of the launch's tiles: bands of eight channel tiles, token tiles
+// outside of channel tiles in each, so that the tiles in flight on an XCD (a
+// contiguous range of t) share both operands in its L2.
+__device__ __forceinline__ void i8_tile(int t, int tiles_i, int tiles_j, int& ti, int& tj) {
+  const int band = t / (8 * tiles_j);
+  const int wide = min(8, tiles_i - band * 8);
+  const int r = t - band * 8 * tiles_j;
+  ti = band * 8 + r % wide;
+  tj = r / wide;
+}
+
+template <typename T, int EPI, typename Cfg>
+__global__ __launch_bounds__(64 * Cfg::WAVES) void linear_int8_kernel(LinearInt8Args a, int tiles_i, int tiles_j) {
+  typedef typename Cfg::TileW TileW;
+  typedef typename Cfg::TileX TileX;
+  constexpr int NA = Cfg::NA, NB = Cfg::NB, NST = Cfg::kNST, STAGE = Cfg::STAGE, LOADS = Cfg::LOADS;
+  constexpr int AHEAD = Cfg::kAhead, EXTRA = AHEAD ? 1 : 0;
+  __shared__ __attribute__((aligned(1024))) char lds[NST * STAGE + 256 * EXTRA];
   const int tiles = tiles_i * tiles_j;
   const int w = static_cast<int>(blockIdx.x);
-  // Workgroups go to the XCDs round-robin: one XCD takes a contiguous range
-  // of tiles, whose blocks of the larger operand its L2 then fetches once.
+  // Workgroups go to the XCDs round-robin: one XCD takes a contiguous range.
   const int xcd = w % kXcds;
   const int per = tiles / kXcds, rem = tiles % kXcds;
-  const int tile = xcd * per + min(xcd, rem) + w / kXcds;
-  const bool i_fast = tiles_i <= tiles_j;
-  const int64_t i0 = static_cast<int64_t>(i_fast ? tile % tiles_i : tile / tiles_j) * kI8Tile;
-  const int64_t j0 = static_cast<int64_t>(i_fast ? tile / tiles_i : tile % tiles_j) * kI8Tile;
+  int ti, tj;
+  i8_tile(xcd * per + min(xcd, rem) + w / kXcds, tiles_i, tiles_j, ti, tj);
+  const int64_t i0 = static_cast<int64_t>(ti) * Cfg::kBI;
+  const int64_t j0 = static_cast<int64_t>(tj) * Cfg::kBJ;
   const int lane = lane_id();
   const int c = lane & 15;
   const int g = lane >> 4;
   const int wave = uniform_wave();
-  const int wi = wave & 1, wj = wave >> 1;
+  const int wi = wave % Cfg::kNWI, wj = wave / Cfg::kNWI;
   const int K = a.K;
   const int n_stages = (K + kI8Stage - 1) / kI8Stage;
   const int last_chunk = (K - 1) / 16 * 16;
 
-  const int8_t* src[PER_WAVE];
-  int kchunk[PER_WAVE], slot[PER_WAVE];
+  // The epilogue's scales and biases, one channel and one token a thread,
+  // fetched ahead of the stages and without branches: they land with the first.
+  const int tid = static_cast<int>(threadIdx.x);
+  const int64_t chan = min(i0 + min(tid, Cfg::kBI - 1), a.N - 1);
+  const float chan_scale = a.w_scales[chan];
+  const float tok_scale = a.x_scales[min(j0 + min(tid, Cfg::kBJ - 1), a.rows - 1)];
+  const bool has_bias = a.bias != nullptr;
+  const ScalarHalves bias_raw = fetch_scalar(has_bias ? a.bias : a.w_scales, has_bias ? a.bias_dtype : kF32, chan);
+
+  // A wave's loads of a stage: lane offsets from the tile's first row
+  // (its rows span less than 2^32 bytes: the host checks the pitches).
+  uint32_t off[LOADS];
+  int kchunk = 0;
 #pragma unroll
-  for (int n = 0; n < PER_WAVE; ++n) {
-    const int j = n * 4 + wave;
-    slot[n] = j * 1024;
+  for (int n = 0; n < LOADS; ++n) {
+    const int j = n * Cfg::WAVES + wave;
     int r, ck;
-    if (j < TileI8::LOADS) {
-      TileI8::slot_chunk(j * 64 + lane, r, ck);
-      src[n] = a.w + min(i0 + r, a.N - 1) * a.ldw;
+    if (j < TileW::LOADS) {
+      TileW::slot_chunk(j * 64 + lane, r, ck);
+      off[n] = static_cast<uint32_t>(min(static_cast<int64_t>(r), a.N - 1 - i0) * a.ldw);
     } else {
-      TileI8::slot_chunk((j - TileI8::LOADS) * 64 + lane, r, ck);
-      src[n] = a.x + min(j0 + r, a.rows - 1) * a.ldx;
+      TileX::slot_chunk((j - TileW::LOADS) * 64 + lane, r, ck);
+      off[n] = static_cast<uint32_t>(min(static_cast<int64_t>(r), a.rows - 1 - j0) * a.ldx);
     }
-    kchunk[n] = ck * 16;
+    kchunk = ck * 16;   // the same for all n: their rows are 8 WAVES apart, and the swizzle repeats every 16
   }
-  auto issue = [&](char* buf, int k0) {
+  const int8_t* const w0 = a.w + i0 * a.ldw;
+  const int8_t* const x0 = static_cast<const int8_t*>(a.x) + j0 * a.ldx;
+  // A stage's loads from..to: scalar bases (made anew, or the compiler keeps a
+  // 64-bit address a load) plus the lane's offset.
+  struct StageLoads {
+    const int8_t* w;
+    const int8_t* x;
+    uint32_t kc;
+    char* buf;
+  };
+  auto stage_loads = [&](int st) {
+    const int k0 = st * kI8Stage;
+    return StageLoads{uniform_ptr(w0 + k0), uniform_ptr(x0 + k0), static_cast<uint32_t>(min(kchunk, last_chunk - k0)),
+                      lds + (st % NST) * STAGE + wave * 1024};
+  };
+  auto issue = [&](const StageLoads& l, int from, int to) {
 #pragma unroll
-    for (int n = 0; n < PER_WAVE; ++n) dma16(src[n] + min(k0 + kchunk[n], last_chunk), buf + slot[n]);
+    for (int n = 0; n < LOADS; ++n)
+      if (n >= from && n < to) dma16((n * Cfg::WAVES < TileW::LOADS ? l.w : l.x) + (off[n] + l.kc), l.buf + n * Cfg::WAVES * 1024);
   };
 
-  i32x4 acc[4][4];
-#pragma unroll
-  for (int p = 0; p < 4; ++p)
-#pragma unroll
-    for (int q = 0; q < 4; ++q) acc[p][q] = i32x4{0, 0, 0, 0};
-  const int afrag[2] = {TileI8::base(wi * 64 + c, g, 0), TileI8::base(wi * 64 + c, g, 1)};
-  const int bfrag[2] = {TileI8::BYTES + TileI8::base(wj * 64 + c, g, 0), TileI8::BYTES + TileI8::base(wj * 64 + c, g, 1)};
+  // The DMA's loads of a stage wait for the L2's misses, and a CU has only so
+  // many in flight.  The tiles in flight on an XCD (8 of channels x 4 of
+  // tokens, i8_tile) share their operands 4-fold and 8-fold, so each asks the
+  // L2 for its part of a later stage's lines, a dword each, into a corner of
+  // LDS that nobody reads (8192 x 4096 x 4096: 124 -> 117 us).
+  uint32_t aoff = 0;
+  bool asks = false, asks_w = false;
+  if constexpr (AHEAD > 0) {
+    constexpr int WL = Cfg::kBI / 4 / Cfg::WAVES, XL = Cfg::kBJ / 8 / Cfg::WAVES;
+    asks_w = lane < WL;
+    asks = lane < WL + XL;
+    const int r = asks_w ? (tj % 4) * (Cfg::kBI / 4) + wave * WL + lane : (ti % 8) * (Cfg::kBJ / 8) + wave * XL + min(lane - WL, XL - 1);
+    aoff = asks_w ? static_cast<uint32_t>(min(static_cast<int64_t>(r), a.N - 1 - i0) * a.ldw)
+                  : static_cast<uint32_t>(min(static_cast<int64_t>(r), a.rows - 1 - j0) * a.ldx);
+  }
+  auto ask = [&](int st) {
+    if constexpr (AHEAD > 0) {
+      const int k0 = min(st * kI8Stage, last_chunk);
+      if (asks) __builtin_amdgcn_global_load_lds((asks_w ? w0 : x0) + k0 + aoff, (lds_void_t*)(lds + NST * STAGE), 4, 0, 0);
+    }
+  };
 
-  auto step = [&](int st, char* cur, char* nxt) {
+  i32x4 acc[NA][NB];
+#pragma unroll
+  for (int p = 0; p < NA; ++p)
+#pragma unroll
+    for (int q = 0; q < NB; ++q) acc[p][q] = i32x4{0, 0, 0, 0};
+  const int afrag[2] = {TileW::base(wi * Cfg::WI + c, g, 0), TileW::base(wi * Cfg::WI + c, g, 1)};
+  const int bfrag[2] = {TileW::BYTES + TileX::base(wj * Cfg::WJ + c, g, 0), TileW::BYTES + TileX::base(wj * Cfg::WJ + c, g, 1)};
+  i32x4 af[2][NA], bf[2][NB];
+  // Fragments from..to of half kk of stage st: NB of the tokens', then NA of
+  // the channels'.
+  auto read = [&](int st, int kk, int from, int to) {
+    const char* buf = lds + (st % NST) * STAGE;
+#pragma unroll
+    for (int f = 0; f < NA + NB; ++f) {
+      if (f < from || f >= to) continue;
+      if (f < NB) bf[kk][f] = *reinterpret_cast<const i32x4*>(buf + bfrag[kk] + f * TileX::ROW_BLOCK);
+      else af[kk][f - NB] = *reinterpret_cast<const i32x4*>(buf + afrag[kk] + (f - NB) * TileW::ROW_BLOCK);
+    }
+  };
+  auto multiply = [&](int kk, int p) {
+#pragma unroll
+    for (int q = 0; q < NB; ++q) acc[p][q] = __builtin_amdgcn_mfma_i32_16x16x64_i8(af[kk][p], bf[kk][q], acc[p][q], 0, 0, 0);
+  };
+  // The products of a half go in NA groups with the other half's fragment
+  // reads between the first of them, and a stage's loads between the last:
+  // a wave issues in order, so a run of reads or loads would keep its matrix
+  // core waiting behind them.
+  constexpr int READ_GROUPS = NA / 2, READS = (NA + NB + READ_GROUPS - 1) / READ_GROUPS;
+  constexpr int LOAD_GROUPS = NA - READ_GROUPS, LOADS_EACH = (LOADS + LOAD_GROUPS - 1) / LOAD_GROUPS;
+
+  // Stages 0 .. NST - 1 are in flight before the loop.  In the middle of
+  // stage st, the wave waits for its loads of stage st + 1 (the NST - 2 later
+  // ones may stay in flight) and its reads of stage st; behind the barrier
+  // every wave's are done, so stage st + 1 is readable and stage st + NST may
+  // be loaded into stage st's buffer.
+#pragma unroll
+  for (int st = 0; st < NST; ++st)
+    if (st < n_stages) issue(stage_loads(st), 0, LOADS);
+  if constexpr (AHEAD > 0) {
+#pragma unroll
+    for (int st = NST; st < AHEAD; ++st) ask(st);
+    if (n_stages >= NST) wait_vmem_at_most<(NST - 1) * LOADS + AHEAD - NST>();
+    else wait_vmem();
+  } else if (n_stages >= NST) {
+    wait_vmem_at_most<(NST - 1) * LOADS>();
+  } else {
     wait_vmem();
-    lds_barrier();
-    i32x4 af[2][4], bf[2][4];
+  }
+  counted_barrier();
+  read(0, 0, 0, NA + NB);
+  for (int st = 0; st + 1 < n_stages; ++st) {
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-#pragma unroll
-      for (int p = 0; p < 4; ++p) af[kk][p] = *reinterpret_cast<const i32x4*>(cur + afrag[kk] + p * TileI8::ROW_BLOCK);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) bf[kk][q] = *reinterpret_cast<const i32x4*>(cur + bfrag[kk] + q * TileI8::ROW_BLOCK);
+    for (int p = 0; p < NA; ++p) {
+      multiply(0, p);
+      __builtin_amdgcn_sched_barrier(0);
+      if (p < READ_GROUPS) read(st, 1, p * READS, (p + 1) * READS);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    if (st + 1 < n_stages) issue(nxt, (st + 1) * kI8Stage);
-    const int left = K - st * kI8Stage;
-    if (left < kI8Stage) {
+    if (st + NST - 1 < n_stages) wait_vmem_at_most<(NST - 2) * (LOADS + EXTRA) + EXTRA>();
+    else wait_vmem();
+    counted_barrier();
+    const StageLoads next = stage_loads(st + NST);
+    const bool load = st + NST < n_stages;
 #pragma unroll
-      for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-        for (int p = 0; p < 4; ++p) af[kk][p] = first_bytes(af[kk][p], left - kk * 64 - g * 16);
+    for (int p = 0; p < NA; ++p) {
+      multiply(1, p);
+      __builtin_amdgcn_sched_barrier(0);
+      if (p < READ_GROUPS) read(st + 1, 0, p * READS, (p + 1) * READS);
+      else if (load) issue(next, (p - READ_GROUPS) * LOADS_EACH, (p - READ_GROUPS + 1) * LOADS_EACH);
+      if (load && p == NA - 1) ask(st + AHEAD);
+      __builtin_amdgcn_sched_barrier(0);
     }
+  }
+  read(n_stages - 1, 1, 0, NA + NB);
+  const int left = K - (n_stages - 1) * kI8Stage;
+  if (left < kI8Stage) {
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
-      for (int p = 0; p < 4; ++p)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) acc[p][q] = __builtin_amdgcn_mfma_i32_16x16x64_i8(af[kk][p], bf[kk][q], acc[p][q], 0, 0, 0);
-  };
-  issue(lds, 0);
-  int st = 0;
-  for (; st + 1 < n_stages; st += 2) {
-    step(st, lds, lds + STAGE);
-    step(st + 1, lds + STAGE, lds);
+      for (int p = 0; p < NA; ++p) af[kk][p] = first_bytes(af[kk][p], left - kk * 64 - g * 16);
   }
-  if (st < n_stages) step(st, lds, lds + STAGE);
+#pragma unroll
+  for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+    for (int p = 0; p < NA; ++p) multiply(kk, p);
 
-  // Lane (c, g) holds rows i = 16p + 4g + r of column j = 16q + c.  Each wave
-  // stages its 64 x 64 block in LDS as [j][i] rows and writes them back in
+  // Lane (c, g) holds rows i = 16p + 4g + r of column j = 16q + c.  A wave
+  // stages 16 columns at a time in LDS as [j][i] rows and writes them back in
   // 16-byte chunks along i.
-  constexpr int ROWB = 64 * 2 + 16;
-  static_assert(64 * ROWB <= STAGE / 2, "a wave's staging block fits its quarter of the stage buffers");
+  __syncthreads();   // every wave is done reading the stage buffers
+  char* stage_w = lds + wave * (16 * Cfg::ROWB);
+  float* const chan_scales = reinterpret_cast<float*>(lds + NST * STAGE) - Cfg::PARAMS;
+  float* const chan_biases = chan_scales + Cfg::kBI;
+  float* const token_scales = chan_biases + Cfg::kBI;
+  if (tid < Cfg::kBI) {
+    chan_scales[tid] = chan_scale;
+    chan_biases[tid] = has_bias ? scalar_value(bias_raw, a.bias_dtype) : 0.f;
+  }
+  if (tid < Cfg::kBJ) token_scales[tid] = tok_scale;
   __syncthreads();
-  char* stage_w = lds + wave * (STAGE / 2);
-  float ws[4][4], bias[4][4];
+  T* out = static_cast<T*>(a.out);
 #pragma unroll
-  for (int p = 0; p < 4; ++p)
+  for (int q = 0; q < NB; ++q) {
+    const int64_t jq = j0 + wj * Cfg::WJ + q * 16;
+    const float xs = token_scales[wj * Cfg::WJ + q * 16 + c];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int64_t i = min(i0 + wi * 64 + p * 16 + 4 * g + r, a.N - 1);
-      ws[p][r] = a.w_scales[i];
-      bias[p][r] = a.bias ? load_scalar(a.bias, a.bias_dtype, i) : 0.f;
-    }
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const float xs = a.x_scales[min(j0 + wj * 64 + q * 16 + c, a.rows - 1)];
-#pragma unroll
-    for (int p = 0; p < 4; ++p) {
+    for (int p = 0; p < NA; ++p) {
+      const int at = wi * Cfg::WI + p * 16 + 4 * g;
+      const f32x4 ws = *reinterpret_cast<const f32x4*>(chan_scales + at);
+      const f32x4 bias = *reinterpret_cast<const f32x4*>(chan_biases + at);
       typename Elem<T>::v4 o;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        float v = __builtin_fmaf(static_cast<float>(acc[p][q][r]) * xs, ws[p][r], bias[p][r]);
+        float v = __builtin_fmaf(static_cast<float>(acc[p][q][r]) * xs, ws[r], bias[r]);
         if constexpr ((EPI & kGemmActGelu) != 0) v = 0.5f * v * (1.f + erf_fast(v * kSqrtHalf));
         o[r] = static_cast<T>(v);
       }
-      *reinterpret_cast<typename Elem<T>::v4*>(stage_w + (q * 16 + c) * ROWB + (p * 16 + 4 * g) * 2) = o;
+      *reinterpret_cast<typename Elem<T>::v4*>(stage_w + c * Cfg::ROWB + (p * 16 + 4 * g) * 2) = o;
     }
-  }
-  T* out = static_cast<T*>(a.out);
+    constexpr int CHUNKS = Cfg::WI / 8;             // 16-byte chunks of a staged row
+    constexpr int ROWS = 64 / CHUNKS;               // rows written at a time
 #pragma unroll
-  for (int pass = 0; pass < 8; ++pass) {
-    const int jr = pass * 8 + lane / 8;
-    const int ic = (lane % 8) * 8;
-    const int64_t j = j0 + wj * 64 + jr;
-    const int64_t i = i0 + wi * 64 + ic;
-    const u32x4 v = *reinterpret_cast<const u32x4*>(stage_w + jr * ROWB + ic * 2);
-    if (j >= a.rows || i >= a.N) continue;
-    const int n = static_cast<int>(min(a.N - i, static_cast<int64_t>(8)));
-    T* dst = out + j * a.N + i;
-    const typename Elem<T>::v8 e8 = __builtin_bit_cast(typename Elem<T>::v8, v);
-    if constexpr ((EPI & 2) != 0) {
-      float res[8];
-      load_chunk(static_cast<const T*>(a.residual) + j * a.ldr + i, n, res);
+    for (int pass = 0; pass < 16 / ROWS; ++pass) {
+      const int jr = pass * ROWS + lane / CHUNKS;
+      const int ic = (lane % CHUNKS) * 8;
+      const int64_t j = jq + jr;
+      const int64_t i = i0 + wi * Cfg::WI + ic;
+      const u32x4 v = *reinterpret_cast<const u32x4*>(stage_w + jr * Cfg::ROWB + ic * 2);
+      if (j >= a.rows || i >= a.N) continue;
+      const int n = static_cast<int>(min(a.N - i, static_cast<int64_t>(8)));
+      T* dst = out + j * a.N + i;
+      const typename Elem<T>::v8 e8 = __builtin_bit_cast(typename Elem<T>::v8, v);
+      if constexpr ((EPI & 2) != 0) {
+        float res[8];
+        load_chunk(static_cast<const T*>(a.residual) + j * a.ldr + i, n, res);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) res[e] += static_cast<float>(e8[e]);
-      store_chunk(dst, n, res);
-    } else if (n == 8) {
-      store16B_any(dst, v);
-    } else {
+        for (int e = 0; e < 8; ++e) res[e] += static_cast<float>(e8[e]);
+        store_chunk(dst, n, res);
+      } else if (n == 8) {
+        store16B_any(dst, v);
+      } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (e < n) dst[e] = e8[e];
+        for (int e = 0; e < 8; ++e)
+          if (e < n) dst[e] = e8[e];
+      }
     }
   }
 }
 
+// Few tokens (MT tiles of 16): the weights' bytes bound the call, so the work
+// is split over K inside the workgroup.  A workgroup takes 16 channels; its
+// eight waves take K's steps of 64 bytes in turn, two neighbours at a time (a
+// row's whole 128-byte line), straight from memory into MFMA fragments, eight
+// steps in flight.  Their integer sums meet in LDS (in any order: they are
+// exact).  With 16-bit tokens (XT = T, MT = 1) each workgroup quantizes them
+// itself instead of waiting for another launch: the waves' largest magnitudes
+// meet in LDS, then the integers of a step are formed where they are
+// multiplied, from the registers that hold K's one batch of steps.
+constexpr int kFewWaves = 8;
+constexpr int kFewBatch = 8;    // steps of a wave in flight
+// Calls whose tokens are quantized in the kernel: one tile of tokens, one batch.
+constexpr int kFewRows = 16, kFewCols = 64 * kFewWaves * kFewBatch;
+
+// The 16 elements of a step's chunk as they lie in memory; n of them exist, the
+// others are 0.
+template <typename T>
+struct RawStep {
+  u32x4 d[2];
+};
+template <typename T>
+__device__ __forceinline__ RawStep<T> fetch_step(const T* p, int n) {
+  RawStep<T> r{{u32x4{0, 0, 0, 0}, u32x4{0, 0, 0, 0}}};
+  if (n >= 16) {
+    r.d[0] = load16B_any(p);
+    r.d[1] = load16B_any(p + 8);
+  } else {
+    const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      if (e < n) r.d[e / 8][e / 2 % 4] |= static_cast<uint32_t>(h[e]) << (16 * (e % 2));
+  }
+  return r;
+}
+// Largest magnitudes of 16-bit floats as unsigned integers (they order alike),
+// two at a time.
+template <typename T>
+__device__ __forceinline__ uint32_t step_max(const RawStep<T>& r, uint32_t pair) {
+  u16x2 m = __builtin_bit_cast(u16x2, pair);
+#pragma unroll
+  for (int d = 0; d < 8; ++d) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, r.d[d / 4][d % 4] & 0x7fff7fffu));
+  return __builtin_bit_cast(uint32_t, m);
+}
+
+template <typename T, typename XT, int MT, int EPI>
+__global__ __launch_bounds__(64 * kFewWaves) void linear_int8_few_kernel(LinearInt8Args a) {
+  constexpr bool QUANT = sizeof(XT) == 2;
+  static_assert(!QUANT || MT == 1, "one tile of tokens is quantized here");
+  __shared__ __attribute__((aligned(16))) int part[kFewWaves][MT * 256];
+  __shared__ uint32_t largest[kFewWaves][16];
+  __shared__ float token_scale[16];
+  const int lane = lane_id();
+  const int c = lane & 15;
+  const int g = lane >> 4;
+  const int wave = uniform_wave();
+  const int K = a.K;
+  const int steps = (K + 63) / 64;
+  const int last_chunk = (K - 1) / 16 * 16;
+  const int64_t i0 = static_cast<int64_t>(blockIdx.x) * 16;
+  const int8_t* w = a.w + min(i0 + c, a.N - 1) * a.ldw;
+  const XT* x[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+    x[m] = static_cast<const XT*>(a.x) + min(static_cast<int64_t>(m * 16 + c), a.rows - 1) * a.ldx;
+  // The u-th step of this wave's batch that starts at step s0.
+  auto step_of = [&](int s0, int u) { return s0 + (u >> 1) * (2 * kFewWaves) + 2 * wave + (u & 1); };
+  constexpr int BATCH = kFewWaves * kFewBatch;   // steps of a batch, over the waves
+
+  // A batch's weights, and its tokens: raw 16-bit chunks or 8-bit fragments.
+  i32x4 wf[kFewBatch];
+  RawStep<T> raw[QUANT ? kFewBatch : 1];
+  i32x4 xf[QUANT ? 1 : kFewBatch][MT];
+  auto fetch_w = [&](int s0) {
+#pragma unroll
+    for (int u = 0; u < kFewBatch; ++u) {
+      const int s = step_of(s0, u);
+      if (s < steps) wf[u] = *reinterpret_cast<const i32x4*>(w + min(s * 64 + g * 16, last_chunk));
+    }
+  };
+  auto fetch_x = [&](int s0) {
+#pragma unroll
+    for (int u = 0; u < kFewBatch; ++u) {
+      const int s = step_of(s0, u);
+      const int k = s * 64 + g * 16;
+      if (s < steps) {
+        if constexpr (QUANT) {
+          raw[u] = fetch_step(x[0] + k, K - k);
+        } else {
+#pragma unroll
+          for (int m = 0; m < MT; ++m) xf[u][m] = *reinterpret_cast<const i32x4*>(x[m] + min(k, last_chunk));
+        }
+      }
+    }
+  };
+
+  Int8Scale xs{1.f, 1.f, 0xffffffffu};
+  fetch_x(0);
+  fetch_w(0);   // on their way while the tokens are quantized
+
+  // This thread's outputs, token e / 16 and channel e % 16 of the workgroup's,
+  // and what their epilogue reads.
+  constexpr int OUTS = (MT * 256 + 64 * kFewWaves - 1) / (64 * kFewWaves);
+  float w_scale[OUTS], x_scale[OUTS], res[OUTS];
+  ScalarHalves bias_raw[OUTS];
+  const bool has_bias = a.bias != nullptr;
+#pragma unroll
+  for (int o = 0; o < OUTS; ++o) {
+    const int e = static_cast<int>(threadIdx.x) + o * 64 * kFewWaves;
+    const int64_t j = min(static_cast<int64_t>(e / 16), a.rows - 1), i = min(i0 + e % 16, a.N - 1);
+    w_scale[o] = a.w_scales[i];
+    bias_raw[o] = fetch_scalar(has_bias ? a.bias : a.w_scales, has_bias ? a.bias_dtype : kF32, i);
+    x_scale[o] = QUANT ? 0.f : a.x_scales[j];
+    if constexpr ((EPI & 2) != 0) res[o] = static_cast<float>(static_cast<const T*>(a.residual)[j * a.ldr + i]);
+  }
+  if constexpr (QUANT) {
+    uint32_t pair = 0;
+#pragma unroll
+    for (int u = 0; u < kFewBatch; ++u)
+      if (step_of(0, u) < steps) pair = step_max(raw[u], pair);
+    const uint16_t larger = static_cast<uint16_t>(max(pair & 0xffffu, pair >> 16));
+    uint32_t amax = __float_as_uint(static_cast<float>(__builtin_bit_cast(T, larger)));
+    const auto p = __builtin_amdgcn_permlane32_swap(amax, amax, false, false);
+    amax = max(p[0], p[1]);
+    const auto r = __builtin_amdgcn_permlane16_swap(amax, amax, false, false);
+    amax = max(r[0], r[1]);
+    if (g == 0) largest[wave][c] = amax;
+    __syncthreads();
+    amax = 0;
+#pragma unroll
+    for (int v = 0; v < kFewWaves; ++v) amax = max(amax, largest[v][c]);
+    xs = int8_scale(amax);
+    if (wave == 0 && g == 0) token_scale[c] = xs.scale;
+  }
+
+  i32x4 acc[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) acc[m] = i32x4{0, 0, 0, 0};
+  for (int s0 = 0; s0 < steps; s0 += BATCH) {
+    if (s0) {
+      fetch_x(s0);
+      fetch_w(s0);
+    }
+#pragma unroll
+    for (int u = 0; u < kFewBatch; ++u) {
+      const int s = step_of(s0, u);
+      if (s >= steps) continue;
+      const int k = s * 64 + g * 16;
+      if (s * 64 + 64 > K) wf[u] = first_bytes(wf[u], K - k);
+      if constexpr (QUANT) {
+        i32x4 q;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const typename Elem<T>::v8 half = __builtin_bit_cast(typename Elem<T>::v8, raw[u].d[h]);
+          float v[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = static_cast<float>(half[e]);
+          const u32x2 packed = pack_int8(v, xs.inverse, xs.keep);
+          q[2 * h] = static_cast<int>(packed[0]);
+          q[2 * h + 1] = static_cast<int>(packed[1]);
+        }
+        acc[0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[u], q, acc[0], 0, 0, 0);
+      } else {
+#pragma unroll
+        for (int m = 0; m < MT; ++m) acc[m] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[u], xf[u][m], acc[m], 0, 0, 0);
+      }
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < MT; ++m) *reinterpret_cast<i32x4*>(&part[wave][m * 256 + c * 16 + 4 * g]) = acc[m];
+  __syncthreads();
+  T* out = static_cast<T*>(a.out);
+#pragma unroll
+  for (int o = 0; o < OUTS; ++o) {
+    const int e = static_cast<int>(threadIdx.x) + o * 64 * kFewWaves;
+    const int64_t j = e / 16, i = i0 + e % 16;
+    if (e >= MT * 256 || j >= a.rows || i >= a.N) continue;
+    int sum = 0;
+#pragma unroll
+    for (int v = 0; v < kFewWaves; ++v) sum += part[v][e];
+    const float bias = has_bias ? scalar_value(bias_raw[o], a.bias_dtype) : 0.f;
+    float y = __builtin_fmaf(static_cast<float>(sum) * (QUANT ? token_scale[j] : x_scale[o]), w_scale[o], bias);
+    if constexpr ((EPI & kGemmActGelu) != 0) y = 0.5f * y * (1.f + erf_fast(y * kSqrtHalf));
+    T t = static_cast<T>(y);
+    if constexpr ((EPI & 2) != 0) t = static_cast<T>(static_cast<float>(t) + res[o]);
+    out[j * a.N + i] = t;
+  }
+}
+
+typedef I8Cfg<256, 256, 2, 4, 2, 3> Tile256;   // one workgroup a CU (128 KiB of LDS)
+typedef I8Cfg<128, 128, 2, 4, 2> Tile128;      // two a CU
+typedef I8Cfg<128, 128, 2, 4, 3> Tile128Deep;  // one a CU, two stages ahead
+typedef I8Cfg<128, 64, 2, 2, 2> Tile128x64;    // three a CU
+typedef I8Cfg<64, 64, 2, 2, 4> Tile64;         // two a CU, three stages ahead
+
+template <typename T, int EPI, typename Cfg>
+static void launch_tiles(const LinearInt8Args& a, hipStream_t stream) {
+  const int ti = static_cast<int>((a.N + Cfg::kBI - 1) / Cfg::kBI), tj = static_cast<int>((a.rows + Cfg::kBJ - 1) / Cfg::kBJ);
+  hipLaunchKernelGGL((linear_int8_kernel<T, EPI, Cfg>), dim3(ti * tj), dim3(64 * Cfg::WAVES), 0, stream, a, ti, tj);
+}
+
+template <typename T, typename XT, int MT, int EPI>
+static void launch_few(const LinearInt8Args& a, hipStream_t stream) {
+  hipLaunchKernelGGL((linear_int8_few_kernel<T, XT, MT, EPI>), dim3(static_cast<unsigned>((a.N + 15) / 16)),
+                     dim3(64 * kFewWaves), 0, stream, a);
+}
+
 template <typename T, int EPI>
 static void launch_linear_int8_k(const LinearInt8Args& a, hipStream_t stream) {
-  const int ti = static_cast<int>((a.N + kI8Tile - 1) / kI8Tile), tj = static_cast<int>((a.rows + kI8Tile - 1) / kI8Tile);
-  hipLaunchKernelGGL((linear_int8_kernel<T, EPI>), dim3(ti * tj), dim3(256), 0, stream, a, ti, tj);
+  if (a.x_dtype != kI8) return launch_few<T, T, 1, EPI>(a, stream);   // at most kFewRows rows
+  // (32 x 4096 -> 4096: 8.5 us against 11.0 of the 64-tiles; 64 rows: 12.9 against 11.0.)
+  if (a.rows <= 16) return launch_few<T, int8_t, 1, EPI>(a, stream);
+  if (a.rows <= 32) return launch_few<T, int8_t, 2, EPI>(a, stream);
+  // Tile by how the output fills the 256 CUs (measured in us, bf16 without
+  // GELU unless said; rows x K -> N):
+  //   256-tiles cost 1.22 times less for the same products than 128-tiles, but
+  //     come in rounds of 256 (8192 x 4096 -> 4096: 117 against 147; 2048 x
+  //     4096 -> 6144, 192 tiles: 48 against 55; 16384 x 512 -> 512: 14 against 10);
+  //   up to 384 128-tiles leave a third of the slots of their one round empty,
+  //     halves of them fill three a CU (4096 x 512 -> 1536: 8.9 against 9.1, with
+  //     GELU 11.3 against 12.6; 16384 x 512 -> 512, 512 tiles: 12.0 against 9.9);
+  //   with at most one a CU a third stage buffer is free (2048^3: 12.4 against
+  //     14.3);
+  //   few of them leave CUs idle that 64-tiles use (512 x 4096 -> 4096, 128
+  //     tiles: 15.6 against 18.2; 4096 x 1536 -> 512: 8.6 against 9.6; at 256
+  //     tiles 17.3 against 12.4).
+  const auto tiles = [&](int bi, int bj) { return ((a.N + bi - 1) / bi) * ((a.rows + bj - 1) / bj); };
+  const int64_t t256 = tiles(256, 256), t128 = tiles(128, 128);
+  if ((t256 + 255) / 256 * 100 <= (t128 + 511) / 512 * 61) launch_tiles<T, EPI, Tile256>(a, stream);
+  else if (t128 > 384) launch_tiles<T, EPI, Tile128>(a, stream);
+  else if (t128 > 256) launch_tiles<T, EPI, Tile128x64>(a, stream);
+  else if (t128 > 144) launch_tiles<T, EPI, Tile128Deep>(a, stream);
+  else launch_tiles<T, EPI, Tile64>(a, stream);
 }
 
 template <typename T>
@@ -199,6 +569,8 @@ static void launch_linear_int8_t(const LinearInt8Args& a, hipStream_t stream) {
     default: launch_linear_int8_k<T, kGemmActGelu | 2>(a, stream); break;
   }
 }
+
+bool linear_int8_quantizes(int64_t rows, int64_t K) { return rows <= kFewRows && K <= kFewCols; }
 
 void launch_linear_int8(const LinearInt8Args& a, hipStream_t stream) {
   if (a.dtype == kF16) launch_linear_int8_t<_Float16>(a, stream);

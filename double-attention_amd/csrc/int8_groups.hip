@@ -22,40 +22,6 @@ namespace da {
 
 enum : int { kOpSave = 0, kOpRestore = 1, kOpGelu = 2, kOpGeluBackward = 3 };
 
-// Raw loads of a chunk, kept apart from their use so that all chunks of a
-// thread are in flight before the first is waited for.
-template <typename T>
-struct RawChunk {
-  u32x4 lo, hi;
-};
-
-template <typename T>
-__device__ __forceinline__ RawChunk<T> fetch_chunk(const T* p, int n) {
-  RawChunk<T> r{u32x4{0, 0, 0, 0}, u32x4{0, 0, 0, 0}};
-  if (n >= 8) {
-    r.lo = load16B_any(p);
-    if constexpr (sizeof(T) == 4) r.hi = load16B_any(p + 4);
-  }
-  return r;
-}
-
-// The chunk's floats; a row's last, partial chunk is read here.
-template <typename T>
-__device__ __forceinline__ void chunk_floats(const RawChunk<T>& r, const T* p, int n, float (&v)[8]) {
-  if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      v[e] = __uint_as_float(r.lo[e]);
-      v[e + 4] = __uint_as_float(r.hi[e]);
-    }
-  } else {
-    const typename Elem<T>::v8 a = __builtin_bit_cast(typename Elem<T>::v8, r.lo);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = static_cast<float>(a[e]);
-  }
-  if (n > 0 && n < 8) load_chunk(p, n, v);
-}
-
 __device__ __forceinline__ uint32_t group_amax(const float (&v)[8]) {
   uint32_t m = 0;
 #pragma unroll

@@ -13,6 +13,7 @@
 
 namespace da {
 
+constexpr int kI8 = 3;                      // dtype code of 8-bit rows
 constexpr int kInt8Group = 128;             // columns that share a scale in grouped rows
 constexpr float kInt8Least = 0x1p-126f;     // the least scale
 // A multiple of 2^23 added to a float in its last place's range: x + kRoundMagic
@@ -52,6 +53,40 @@ __device__ __forceinline__ void load_chunk(const T* p, int n, float (&v)[8]) {
   }
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] = e < n ? static_cast<float>(p[e]) : 0.f;
+}
+
+// Raw loads of a chunk, kept apart from their use so that all of a thread's are
+// in flight before the first is waited for.
+template <typename T>
+struct RawChunk {
+  u32x4 lo, hi;
+};
+
+template <typename T>
+__device__ __forceinline__ RawChunk<T> fetch_chunk(const T* p, int n) {
+  RawChunk<T> r{u32x4{0, 0, 0, 0}, u32x4{0, 0, 0, 0}};
+  if (n >= 8) {
+    r.lo = load16B_any(p);
+    if constexpr (sizeof(T) == 4) r.hi = load16B_any(p + 4);
+  }
+  return r;
+}
+
+// The chunk's floats; a row's last, partial chunk is read here.
+template <typename T>
+__device__ __forceinline__ void chunk_floats(const RawChunk<T>& r, const T* p, int n, float (&v)[8]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[e] = __uint_as_float(r.lo[e]);
+      v[e + 4] = __uint_as_float(r.hi[e]);
+    }
+  } else {
+    const typename Elem<T>::v8 a = __builtin_bit_cast(typename Elem<T>::v8, r.lo);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = static_cast<float>(a[e]);
+  }
+  if (n > 0 && n < 8) load_chunk(p, n, v);
 }
 
 template <typename T>

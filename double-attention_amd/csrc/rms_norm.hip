@@ -158,16 +158,44 @@ __global__ __launch_bounds__(row_block<NT>()) void rms_norm_backward_kernel(RmsN
     for (int e = 0; e < 8; ++e) gw[k][e] = 0.f;
   }
   const float inv_dim = 1.f / static_cast<float>(a.dim);
-  int turn = 0;
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / NT; row < a.rows;
-       row += static_cast<int64_t>(gridDim.x) * ROWS, turn ^= 1) {
-    float v[CH][8], g[CH][8];
+  const int64_t step = static_cast<int64_t>(gridDim.x) * ROWS;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / NT;
+  const T* const sum = static_cast<const T*>(a.sum);
+  const T* const grad = static_cast<const T*>(a.grad);
+  const T* const grad_sum = static_cast<const T*>(a.grad_sum);
+  // A row's loads are issued while the row before it is reduced (the widest
+  // rows take the registers for that themselves).
+  constexpr bool EARLY = NT < 512;
+  RawChunk<T> rv[CH], rg[CH], rs[CH];
+  auto fetch_row = [&](int64_t r) {
+    if (r >= a.rows) return;
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
       const int c = (k * NT + t) * 8;
-      load_chunk(static_cast<const T*>(a.sum) + row * a.ldsum + c, a.dim - c, v[k]);
-      load_chunk(static_cast<const T*>(a.grad) + row * a.ldg + c, a.dim - c, g[k]);
+      rv[k] = fetch_chunk(sum + r * a.ldsum + c, a.dim - c);
+      rg[k] = fetch_chunk(grad + r * a.ldg + c, a.dim - c);
+      if (grad_sum != nullptr) rs[k] = fetch_chunk(grad_sum + r * a.ldgs + c, a.dim - c);
     }
+  };
+  if constexpr (EARLY) fetch_row(row);
+  int turn = 0;
+  for (; row < a.rows; row += step, turn ^= 1) {
+    if constexpr (!EARLY) fetch_row(row);
+    float v[CH][8], g[CH][8], d[CH][8];
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+      const int c = (k * NT + t) * 8;
+      chunk_floats(rv[k], sum + row * a.ldsum + c, a.dim - c, v[k]);
+      chunk_floats(rg[k], grad + row * a.ldg + c, a.dim - c, g[k]);
+      if (grad_sum != nullptr) {
+        chunk_floats(rs[k], grad_sum + row * a.ldgs + c, a.dim - c, d[k]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) d[k][e] = 0.f;
+      }
+    }
+    if constexpr (EARLY) fetch_row(row + step);
+    __builtin_amdgcn_sched_barrier(0);
     float ss = 0.f, sg = 0.f;
 #pragma unroll
     for (int k = 0; k < CH; ++k)
@@ -200,19 +228,12 @@ __global__ __launch_bounds__(row_block<NT>()) void rms_norm_backward_kernel(RmsN
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
       const int c = (k * NT + t) * 8;
-      float d[8];
-      if (a.grad_sum != nullptr) {
-        load_chunk(static_cast<const T*>(a.grad_sum) + row * a.ldgs + c, a.dim - c, d);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) d[e] = 0.f;
-      }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         gw[k][e] = __builtin_fmaf(g[k][e], v[k][e] * rstd, gw[k][e]);
-        d[e] += rstd * (g[k][e] * w[k][e] - v[k][e] * mean);
+        d[k][e] += rstd * (g[k][e] * w[k][e] - v[k][e] * mean);
       }
-      store_chunk(static_cast<T*>(a.grad_x) + row * a.dim + c, a.dim - c, d);
+      store_chunk(static_cast<T*>(a.grad_x) + row * a.dim + c, a.dim - c, d[k]);
     }
   }
   if (a.partials == nullptr) return;
@@ -241,21 +262,31 @@ __global__ __launch_bounds__(row_block<NT>()) void rms_norm_backward_kernel(RmsN
   }
 }
 
-// out[c] = sum over the workgroups of partials[b][c], in their order within
-// eight interleaved runs.
-constexpr int kSumCols = 32;
+// out[c] = sum over the workgroups b of partials[b][c].  A workgroup takes 16
+// columns, 64 threads each: thread r adds workgroups r, r + 64, ... in order,
+// the sums meet four to a wave and then wave by wave.
+constexpr int kSumCols = 16, kSumRuns = 64;
 template <typename T>
-__global__ __launch_bounds__(256) void rms_norm_weight_kernel(const float* partials, int blocks, int dim, T* out) {
-  __shared__ float lds[8][kSumCols];
+__global__ __launch_bounds__(kSumCols * kSumRuns) void rms_norm_weight_kernel(const float* partials, int blocks, int dim, T* out) {
+  __shared__ float lds[kSumRuns / 4][kSumCols];
   const int c = static_cast<int>(threadIdx.x) % kSumCols, r = static_cast<int>(threadIdx.x) / kSumCols;
   const int col = static_cast<int>(blockIdx.x) * kSumCols + c;
+  const float* p = partials + min(col, dim - 1);
   float sum = 0.f;
-  if (col < dim)
-    for (int b = r; b < blocks; b += 8) sum += partials[static_cast<int64_t>(b) * dim + col];
-  lds[r][c] = sum;
+  for (int b0 = r; b0 < blocks; b0 += 8 * kSumRuns) {
+    float v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = p[static_cast<int64_t>(min(b0 + u * kSumRuns, blocks - 1)) * dim];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) sum += b0 + u * kSumRuns < blocks ? v[u] : 0.f;
+  }
+  sum = group_sum(sum);   // the wave's four threads of this column
+  if (lane_id() < kSumCols) lds[wave_id()][c] = sum;
   __syncthreads();
   if (r == 0 && col < dim) {
-    for (int i = 1; i < 8; ++i) sum += lds[i][c];
+    sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < kSumRuns / 4; ++i) sum += lds[i][c];
     out[col] = static_cast<T>(sum);
   }
 }
@@ -314,7 +345,7 @@ static void launch_backward_t(const RmsNormBackwardArgs& a, hipStream_t stream) 
   else if (a.dim <= 2048) launch_backward_k<T, 256, 1>(a, stream);
   else if (a.dim <= 4096) launch_backward_k<T, 256, 2>(a, stream);
   else if (a.dim <= 8192) launch_backward_k<T, 256, 4>(a, stream);
-  else launch_backward_k<T, 1024, 2>(a, stream);
+  else launch_backward_k<T, 512, 4>(a, stream);
 }
 
 void launch_rms_norm_backward(const RmsNormBackwardArgs& a, hipStream_t stream) {
@@ -326,11 +357,11 @@ void launch_rms_norm_backward(const RmsNormBackwardArgs& a, hipStream_t stream) 
   const int blocks = rms_norm_backward_blocks(a.rows, a.dim);
   const dim3 grid((a.dim + kSumCols - 1) / kSumCols);
   if (a.param_dtype == kF32)
-    hipLaunchKernelGGL((rms_norm_weight_kernel<float>), grid, dim3(256), 0, stream, a.partials, blocks, a.dim, static_cast<float*>(a.grad_weight));
+    hipLaunchKernelGGL((rms_norm_weight_kernel<float>), grid, dim3(kSumCols * kSumRuns), 0, stream, a.partials, blocks, a.dim, static_cast<float*>(a.grad_weight));
   else if (a.param_dtype == kF16)
-    hipLaunchKernelGGL((rms_norm_weight_kernel<_Float16>), grid, dim3(256), 0, stream, a.partials, blocks, a.dim, static_cast<_Float16*>(a.grad_weight));
+    hipLaunchKernelGGL((rms_norm_weight_kernel<_Float16>), grid, dim3(kSumCols * kSumRuns), 0, stream, a.partials, blocks, a.dim, static_cast<_Float16*>(a.grad_weight));
   else
-    hipLaunchKernelGGL((rms_norm_weight_kernel<__bf16>), grid, dim3(256), 0, stream, a.partials, blocks, a.dim, static_cast<__bf16*>(a.grad_weight));
+    hipLaunchKernelGGL((rms_norm_weight_kernel<__bf16>), grid, dim3(kSumCols * kSumRuns), 0, stream, a.partials, blocks, a.dim, static_cast<__bf16*>(a.grad_weight));
 }
 
 }  // namespace da

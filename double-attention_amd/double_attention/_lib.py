@@ -17,6 +17,7 @@ from pathlib import Path
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libdouble_attention_hip.so"
 
 DA_F32, DA_F16, DA_BF16 = 0, 1, 2
+DA_I8 = 3   # 8-bit rows (linear_int8)
 DA_OUT_SPLIT = 0x100
 
 DA_ROUTE_NORMALIZE_INPUT = 1
@@ -219,13 +220,14 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
 INT8_SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "da_quantize_int8": (_i32, [_vp, _i64, _i64, _i64, _i32, _i64, _vp, _i64, _vp, _vp]),
     "da_dequantize_int8": (_i32, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _i32, _vp]),
+    "da_linear_int8_workspace_bytes": (_i64, [_i64, _i64, _i32]),
     "da_linear_int8": (
         _i32,
         [
-            _vp, _i64, _vp, _i64, _i64,  # x, pitch, scales, rows, in_features
+            _vp, _i32, _i64, _vp, _i64, _i64,  # x, dtype, pitch, scales, rows, in_features
             _vp, _i64, _vp, _i64,  # weight, pitch, scales, out_features
             _vp, _i32, _i32, _vp, _i64,  # bias, bias dtype, activation, residual, its pitch
-            _vp, _i32, _vp,  # out, dtype, stream
+            _vp, _i32, _vp, _i64, _vp,  # out, dtype, workspace, its bytes, stream
         ],
     ),
     "da_add_rms_norm": (

@@ -25,12 +25,15 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from .hip_ops import _half_code, _stream, dtype_code
+from .hip_ops import _stream, dtype_code
 
 INT8_GROUP = _lib.INT8_GROUP
 # Columns of rows with one scale each, and widths of the norm.
 MAX_ROW_COLUMNS = 65536
 MAX_NORM_WIDTH = 16384
+# Up to so many 16-bit tokens of so many columns the linear layer's kernel
+# quantizes itself (da_linear_int8 needs no workspace then).
+QUANTIZED_IN_KERNEL = (16, 4096)
 
 
 class QuantizedRows(NamedTuple):
@@ -49,30 +52,62 @@ class QuantizedRows(NamedTuple):
     group: int | None = None
 
 
+_current_device = torch._C._cuda_getDevice
+_CODES = {torch.float32: _lib.DA_F32, torch.float16: _lib.DA_F16, torch.bfloat16: _lib.DA_BF16}
+_HALF_CODES = {torch.float16: _lib.DA_F16, torch.bfloat16: _lib.DA_BF16}
+
+
 def _launch(what: str, device: torch.device, fn, *args) -> None:
     """``fn(*args, stream)`` on ``device``, which need not be the current one."""
 
-    stream = _stream(device)
-    if device.index is None or device.index == torch._C._cuda_getDevice():
-        rc = fn(*args, stream)
+    if device.index == _current_device():
+        rc = fn(*args, _stream(device))
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, stream)
+            rc = fn(*args, _stream(device))
     if rc:
         _lib.check(rc, what)
 
 
-def _on_device(what: str, device: torch.device, *tensors: Tensor | None) -> None:
-    if device.type != "cuda":
+def _check_input(what: str, x: Tensor, codes: dict = _HALF_CODES) -> int:
+    """The dtype code of ``x``: rows of at least one column on a device."""
+
+    code = codes.get(x.dtype)
+    if code is None:
+        names = " or ".join(str(t).removeprefix("torch.") for t in codes)
+        raise ValueError(f"{what}: HIP kernels require {names} tensors, got {x.dtype}")
+    shape = x.shape
+    if not shape or shape[-1] < 1:
+        raise ValueError(f"{what}: expected rows of at least one column, got shape {tuple(shape)}")
+    if not x.is_cuda:
         raise ValueError(f"{what}: HIP kernels require tensors on a ROCm device")
-    for t in tensors:
-        if t is not None and t.device != device:
-            raise ValueError(f"{what}: all tensors must be on {device}, got one on {t.device}")
+    return code
+
+
+def _check_on(what: str, device: torch.device, t: Tensor) -> None:
+    if t.device != device:
+        raise ValueError(f"{what}: all tensors must be on {device}, got one on {t.device}")
+
+
+def _check_like(what: str, x: Tensor, t: Tensor) -> None:
+    if t.shape != x.shape or t.dtype != x.dtype:
+        raise ValueError(f"{what}: expected shape {tuple(x.shape)} and {x.dtype}, got {tuple(t.shape)} and {t.dtype}")
+    _check_on(what, x.device, t)
+
+
+def _check_param(what: str, device: torch.device, t: Tensor, size: int) -> int:
+    code = _CODES.get(t.dtype)
+    if code is None or t.ndim != 1 or t.shape[0] != size:
+        raise ValueError(f"{what}: expected a floating parameter of shape ({size},), got {t.dtype} {tuple(t.shape)}")
+    _check_on(what, device, t)
+    return code
 
 
 def _no_grad(what: str, *tensors: Tensor | None) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError(f"{what} has no autograd of its own: call it under torch.no_grad(), or detach its inputs")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{what} has no autograd of its own: call it under torch.no_grad(), or detach its inputs")
 
 
 def _rows(t: Tensor) -> tuple[Tensor, int]:
@@ -82,7 +117,9 @@ def _rows(t: Tensor) -> tuple[Tensor, int]:
 
     columns = t.shape[-1]
     if t.ndim != 2:
-        t = t.reshape(-1, columns) if columns else t.reshape(0, 0)
+        t = t.reshape(-1, columns)
+    if t.is_contiguous():
+        return t, columns
     rows = t.shape[0]
     if columns > 1 and t.stride(1) != 1:
         t = t.contiguous()
@@ -91,15 +128,6 @@ def _rows(t: Tensor) -> tuple[Tensor, int]:
         t = t.contiguous()
         pitch = columns
     return t, pitch
-
-
-def _check_rows(what: str, t: Tensor, floating: bool = False) -> None:
-    if t.ndim < 1 or t.shape[-1] < 1:
-        raise ValueError(f"{what}: expected rows of at least one column, got shape {tuple(t.shape)}")
-    if floating:
-        dtype_code(t.dtype)
-    else:
-        _half_code(t.dtype)
 
 
 def _new_values(lead: torch.Size, columns: int, device: torch.device) -> tuple[Tensor, int]:
@@ -114,6 +142,8 @@ def _values_rows(t: Tensor) -> tuple[Tensor, int]:
 
     t, pitch = _rows(t)
     rows, columns = t.shape
+    if pitch == columns and columns % 16 == 0 and t.data_ptr() % 16 == 0:
+        return t, pitch
     if rows == 1:
         pitch = (columns + 15) // 16 * 16
     fits = pitch % 16 == 0 and t.data_ptr() % 16 == 0
@@ -127,17 +157,24 @@ def _values_rows(t: Tensor) -> tuple[Tensor, int]:
     return t, pitch
 
 
-def _check_quantized(what: str, rows: QuantizedRows) -> None:
+def _check_quantized(what: str, rows: QuantizedRows, device: torch.device | None = None) -> None:
     values, scales, group = rows
-    if values.dtype != torch.int8 or scales.dtype != torch.float32:
+    if values.dtype is not torch.int8 or scales.dtype is not torch.float32:
         raise ValueError(f"{what}: quantized rows are int8 values with fp32 scales")
-    if group not in (None, INT8_GROUP):
+    if group is not None and group != INT8_GROUP:
         raise NotImplementedError(f"{what}: a scale for each row (group None) or each {INT8_GROUP} columns")
-    if values.ndim < 1 or values.shape[-1] < 1:
-        raise ValueError(f"{what}: expected rows of at least one column, got shape {tuple(values.shape)}")
-    groups = 1 if group is None else -(-values.shape[-1] // group)
-    if scales.shape[:-1] != values.shape[:-1] or scales.ndim != values.ndim or scales.shape[-1] != groups:
-        raise ValueError(f"{what}: scales of shape {tuple(scales.shape)} do not fit values of shape {tuple(values.shape)}")
+    shape = values.shape
+    if not shape or shape[-1] < 1:
+        raise ValueError(f"{what}: expected rows of at least one column, got shape {tuple(shape)}")
+    if scales.shape != (*shape[:-1], 1 if group is None else -(-shape[-1] // group)):
+        raise ValueError(f"{what}: scales of shape {tuple(scales.shape)} do not fit values of shape {tuple(shape)}")
+    if not values.is_cuda:
+        raise ValueError(f"{what}: HIP kernels require tensors on a ROCm device")
+    if device is None:
+        device = values.device
+    else:
+        _check_on(what, device, values)
+    _check_on(what, device, scales)
 
 
 def quantize_int8_hip(x: Tensor, group: int | None = None) -> QuantizedRows:
@@ -150,31 +187,35 @@ def quantize_int8_hip(x: Tensor, group: int | None = None) -> QuantizedRows:
     NaN throughout.
     """
 
-    _check_rows("quantize_int8_hip", x, floating=True)
-    _on_device("quantize_int8_hip", x.device)
-    if group not in (None, INT8_GROUP):
-        raise NotImplementedError(f"quantize_int8_hip: a scale for each row (group None) or each {INT8_GROUP} columns")
+    what = "quantize_int8_hip"
+    code = _check_input(what, x, _CODES)
+    if group is not None and group != INT8_GROUP:
+        raise NotImplementedError(f"{what}: a scale for each row (group None) or each {INT8_GROUP} columns")
+    device = x.device
     lead, columns = x.shape[:-1], x.shape[-1]
-    rows, pitch = _rows(x.detach())
-    values, ldv = _new_values(lead, columns, x.device)
-    scales = torch.empty(*lead, 1 if group is None else -(-columns // INT8_GROUP), dtype=torch.float32, device=x.device)
-    _launch("quantize_int8_hip", x.device, _lib.get().da_quantize_int8, rows.data_ptr(), rows.shape[0], columns, pitch,
-            dtype_code(x.dtype), group or 0, values.data_ptr(), ldv, scales.data_ptr())
+    rows, pitch = _rows(x)
+    values, ldv = _new_values(lead, columns, device)
+    groups = 1 if group is None else -(-columns // INT8_GROUP)
+    scales = torch.empty(*lead, groups, dtype=torch.float32, device=device)
+    _launch(what, device, _lib.get().da_quantize_int8, rows.data_ptr(), rows.shape[0], columns, pitch, code, group or 0,
+            values.data_ptr(), ldv, scales.data_ptr())
     return QuantizedRows(values, scales, group)
 
 
 def dequantize_int8_hip(rows: QuantizedRows, dtype: torch.dtype = torch.bfloat16) -> Tensor:
     """What the 8-bit rows stand for: ``values * scale``, rounded once to ``dtype``."""
 
-    _check_quantized("dequantize_int8_hip", rows)
-    device = rows.values.device
-    _on_device("dequantize_int8_hip", device, rows.scales)
-    values, pitch = _values_rows(rows.values)
+    what = "dequantize_int8_hip"
+    _check_quantized(what, rows)
+    values, scales, group = rows
+    code = dtype_code(dtype)
+    device = values.device
+    out = torch.empty(values.shape, dtype=dtype, device=device)
+    values, pitch = _values_rows(values)
+    scales = scales.contiguous()
     columns = values.shape[1]
-    scales = rows.scales.contiguous()
-    out = torch.empty(rows.values.shape, dtype=dtype, device=device)
-    _launch("dequantize_int8_hip", device, _lib.get().da_dequantize_int8, values.data_ptr(), values.shape[0], columns,
-            pitch, scales.data_ptr(), rows.group or 0, out.data_ptr(), columns, dtype_code(dtype))
+    _launch(what, device, _lib.get().da_dequantize_int8, values.data_ptr(), values.shape[0], columns, pitch,
+            scales.data_ptr(), group or 0, out.data_ptr(), columns, code)
     return out
 
 
@@ -200,80 +241,95 @@ def linear_int8_hip(
     """
 
     what = "linear_int8_hip"
-    if activation not in (None, "gelu"):
+    if activation is not None and activation != "gelu":
         raise ValueError(f"unsupported activation {activation!r}")
-    _check_quantized(what, weight)
-    if weight.values.ndim != 2 or weight.group is not None:
-        raise ValueError(f"{what}: the weight is [out_features, in_features] with one scale for each output channel")
     if isinstance(x, QuantizedRows):
         _check_quantized(what, x)
-        if x.group is not None:
+        x, x_scales, group = x
+        if group is not None:
             raise ValueError(f"{what}: x needs one scale for each token")
+        x_code = _lib.DA_I8
         if dtype is None:
             dtype = torch.bfloat16 if residual is None else residual.dtype
-        shape, device = x.values.shape, x.values.device
-        _on_device(what, device, x.scales)
     else:
-        _check_rows(what, x)
-        shape, device = x.shape, x.device
+        x_scales = None
+        x_code = _check_input(what, x)
         if dtype is None:
             dtype = x.dtype
-    code = _half_code(dtype)
-    out_features, in_features = weight.values.shape
+    shape, device = x.shape, x.device
+    _check_quantized(what, weight, device)
+    w, w_scales, group = weight
+    if w.ndim != 2 or group is not None:
+        raise ValueError(f"{what}: the weight is [out_features, in_features] with one scale for each output channel")
+    code = _HALF_CODES.get(dtype)
+    if code is None:
+        raise ValueError(f"{what}: the output must be fp16 or bf16, not {dtype}")
+    out_features, in_features = w.shape
     if shape[-1] != in_features:
         raise ValueError(f"{what}: rows of {shape[-1]} columns against a weight of {in_features}")
-    _on_device(what, device, weight.values, weight.scales, bias, residual)
-    if bias is not None and bias.shape != (out_features,):
-        raise ValueError(f"{what}: the bias must have shape ({out_features},)")
-    if residual is not None and (residual.shape != (*shape[:-1], out_features) or residual.dtype != dtype):
-        raise ValueError(f"{what}: the residual must match the output's shape and dtype")
-    _no_grad(what, None if isinstance(x, QuantizedRows) else x, bias, residual)
-    if not isinstance(x, QuantizedRows):
-        x = quantize_int8_hip(x)
-    rows, ldx = _values_rows(x.values)
-    w, ldw = _values_rows(weight.values)
-    x_scales, w_scales = x.scales.contiguous(), weight.scales.contiguous()
+    out_shape = (*shape[:-1], out_features)
+    _no_grad(what, x, bias, residual)
+    bias_ptr, bias_code = None, _lib.DA_F32
     if bias is not None:
+        bias_code = _check_param(what, device, bias, out_features)
         bias = bias.contiguous()
-    res, ldr = (None, 0) if residual is None else _rows(residual)
-    out = torch.empty(*shape[:-1], out_features, dtype=dtype, device=device)
-    _launch(what, device, _lib.get().da_linear_int8, rows.data_ptr(), ldx, x_scales.data_ptr(), rows.shape[0],
-            in_features, w.data_ptr(), ldw, w_scales.data_ptr(), out_features,
-            None if bias is None else bias.data_ptr(), _lib.DA_F32 if bias is None else dtype_code(bias.dtype),
-            _lib.DA_ACT_GELU if activation else _lib.DA_ACT_NONE, None if res is None else res.data_ptr(), ldr,
-            out.data_ptr(), code)
+        bias_ptr = bias.data_ptr()
+    res_ptr, ldr = None, 0
+    if residual is not None:
+        if residual.shape != out_shape or residual.dtype != dtype:
+            raise ValueError(f"{what}: the residual must match the output's shape and dtype")
+        _check_on(what, device, residual)
+        residual, ldr = _rows(residual)
+        res_ptr = residual.data_ptr()
+    lib = _lib.get()
+    w, ldw = _values_rows(w)
+    w_scales = w_scales.contiguous()
+    scales_ptr, workspace_ptr, nbytes = None, None, 0
+    if x_scales is None:
+        rows, ldx = _rows(x)
+        if rows.shape[0] > QUANTIZED_IN_KERNEL[0] or in_features > QUANTIZED_IN_KERNEL[1] or dtype != x.dtype:
+            nbytes = lib.da_linear_int8_workspace_bytes(rows.shape[0], in_features, x_code)
+            workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            workspace_ptr = workspace.data_ptr()
+    else:
+        rows, ldx = _values_rows(x)
+        x_scales = x_scales.contiguous()
+        scales_ptr = x_scales.data_ptr()
+    out = torch.empty(out_shape, dtype=dtype, device=device)
+    _launch(what, device, lib.da_linear_int8, rows.data_ptr(), x_code, ldx, scales_ptr, rows.shape[0], in_features,
+            w.data_ptr(), ldw, w_scales.data_ptr(), out_features, bias_ptr, bias_code,
+            _lib.DA_ACT_GELU if activation else _lib.DA_ACT_NONE, res_ptr, ldr, out.data_ptr(), code, workspace_ptr, nbytes)
     return out
 
 
-def _check_norm(what: str, x: Tensor, weight: Tensor | None, *others: Tensor | None) -> None:
-    _check_rows(what, x)
-    _on_device(what, x.device, weight, *others)
-    for t in others:
-        if t is not None and (t.shape != x.shape or t.dtype != x.dtype):
-            raise ValueError(f"{what}: expected shape {tuple(x.shape)} and {x.dtype}, got {tuple(t.shape)} and {t.dtype}")
-    if weight is not None:
-        dtype_code(weight.dtype)
-        if weight.shape != x.shape[-1:]:
-            raise ValueError(f"{what}: the weight must have shape ({x.shape[-1]},)")
-
-
 def _add_rms_norm(what, x, residual, weight, eps, want_out, want_int8):
-    width, device = x.shape[-1], x.device
+    code = _check_input(what, x)
+    shape, device, dtype = x.shape, x.device, x.dtype
+    width = shape[-1]
     rows, ldx = _rows(x)
-    res, ldr = (None, 0) if residual is None else _rows(residual)
-    w = None if weight is None else weight.contiguous()
-    total = x if residual is None else torch.empty(x.shape, dtype=x.dtype, device=device)
-    out = torch.empty(x.shape, dtype=x.dtype, device=device) if want_out else None
-    values = scales = None
+    total, res_ptr, ldr, total_ptr = x, None, 0, None
+    if residual is not None:
+        _check_like(what, x, residual)
+        residual, ldr = _rows(residual)
+        res_ptr = residual.data_ptr()
+        total = torch.empty(shape, dtype=dtype, device=device)
+        total_ptr = total.data_ptr()
+    weight_ptr, weight_code = None, _lib.DA_F32
+    if weight is not None:
+        weight_code = _check_param(what, device, weight, width)
+        weight = weight.contiguous()
+        weight_ptr = weight.data_ptr()
+    out = values = scales = out_ptr = values_ptr = scales_ptr = None
     ldv = 0
+    if want_out:
+        out = torch.empty(shape, dtype=dtype, device=device)
+        out_ptr = out.data_ptr()
     if want_int8:
-        values, ldv = _new_values(x.shape[:-1], width, device)
-        scales = torch.empty(*x.shape[:-1], 1, dtype=torch.float32, device=device)
-    _launch(what, device, _lib.get().da_add_rms_norm, rows.data_ptr(), ldx, None if res is None else res.data_ptr(), ldr,
-            rows.shape[0], width, None if w is None else w.data_ptr(), _lib.DA_F32 if w is None else dtype_code(w.dtype),
-            float(eps), _half_code(x.dtype), None if residual is None else total.data_ptr(),
-            None if out is None else out.data_ptr(), None if values is None else values.data_ptr(), ldv,
-            None if scales is None else scales.data_ptr())
+        values, ldv = _new_values(shape[:-1], width, device)
+        scales = torch.empty(*shape[:-1], 1, dtype=torch.float32, device=device)
+        values_ptr, scales_ptr = values.data_ptr(), scales.data_ptr()
+    _launch(what, device, _lib.get().da_add_rms_norm, rows.data_ptr(), ldx, res_ptr, ldr, rows.shape[0], width, weight_ptr,
+            weight_code, float(eps), code, total_ptr, out_ptr, values_ptr, ldv, scales_ptr)
     return out, values, scales, total
 
 
@@ -311,7 +367,6 @@ def add_rms_norm_hip(
     Differentiable in x, the residual and the weight, through both outputs.
     """
 
-    _check_norm("add_rms_norm_hip", x, weight, residual)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight)):
         got = _AddRmsNormFunction.apply(x, residual, weight, eps)
         return (got, x) if residual is None else got
@@ -327,7 +382,6 @@ def add_rms_norm_int8_hip(
     stays 16-bit.  For inference: no backward."""
 
     what = "add_rms_norm_int8_hip"
-    _check_norm(what, x, weight, residual)
     _no_grad(what, x, residual, weight)
     _, values, scales, total = _add_rms_norm(what, x, residual, weight, eps, False, True)
     return QuantizedRows(values, scales), total
@@ -350,25 +404,34 @@ def add_rms_norm_backward_hip(
     """
 
     what = "add_rms_norm_backward_hip"
-    _check_norm(what, total, weight, grad, grad_sum)
-    width, device = total.shape[-1], total.device
+    code = _check_input(what, total)
+    _check_like(what, total, grad)
+    shape, device = total.shape, total.device
+    width = shape[-1]
     lib = _lib.get()
-    s, lds = _rows(total.detach())
-    g, ldg = _rows(grad.detach())
-    gs, ldgs = (None, 0) if grad_sum is None else _rows(grad_sum.detach())
-    w = None if weight is None else weight.detach().contiguous()
-    grad_x = torch.empty(total.shape, dtype=total.dtype, device=device)
-    grad_weight = workspace = None
+    s, lds = _rows(total)
+    g, ldg = _rows(grad)
+    gs_ptr, ldgs = None, 0
+    if grad_sum is not None:
+        _check_like(what, total, grad_sum)
+        grad_sum, ldgs = _rows(grad_sum)
+        gs_ptr = grad_sum.data_ptr()
+    grad_x = torch.empty(shape, dtype=total.dtype, device=device)
+    weight_ptr, weight_code = None, _lib.DA_F32
+    grad_weight = grad_weight_ptr = workspace_ptr = None
     nbytes = 0
-    if w is not None and want_weight:
-        grad_weight = torch.empty_like(w)
-        nbytes = lib.da_add_rms_norm_backward_workspace_bytes(s.shape[0], width)
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    _launch(what, device, lib.da_add_rms_norm_backward, s.data_ptr(), lds, g.data_ptr(), ldg,
-            None if gs is None else gs.data_ptr(), ldgs, s.shape[0], width, None if w is None else w.data_ptr(),
-            _lib.DA_F32 if w is None else dtype_code(w.dtype), float(eps), _half_code(total.dtype), grad_x.data_ptr(),
-            None if grad_weight is None else grad_weight.data_ptr(),
-            None if workspace is None else workspace.data_ptr(), nbytes)
+    if weight is not None:
+        weight_code = _check_param(what, device, weight, width)
+        weight = weight.contiguous()
+        weight_ptr = weight.data_ptr()
+        if want_weight:
+            grad_weight = torch.empty(width, dtype=weight.dtype, device=device)
+            grad_weight_ptr = grad_weight.data_ptr()
+            nbytes = lib.da_add_rms_norm_backward_workspace_bytes(s.shape[0], width)
+            workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            workspace_ptr = workspace.data_ptr()
+    _launch(what, device, lib.da_add_rms_norm_backward, s.data_ptr(), lds, g.data_ptr(), ldg, gs_ptr, ldgs, s.shape[0],
+            width, weight_ptr, weight_code, float(eps), code, grad_x.data_ptr(), grad_weight_ptr, workspace_ptr, nbytes)
     return grad_x, grad_weight
 
 
@@ -378,16 +441,16 @@ def gelu_int8_hip(z: Tensor) -> tuple[Tensor, QuantizedRows]:
     is of z itself; only the backward sees the kept rows."""
 
     what = "gelu_int8_hip"
-    _check_rows(what, z)
-    _on_device(what, z.device)
+    code = _check_input(what, z)
     _no_grad(what, z)
-    columns, device = z.shape[-1], z.device
+    shape, device = z.shape, z.device
+    columns = shape[-1]
     rows, pitch = _rows(z)
-    out = torch.empty(z.shape, dtype=z.dtype, device=device)
-    values, ldv = _new_values(z.shape[:-1], columns, device)
-    scales = torch.empty(*z.shape[:-1], -(-columns // INT8_GROUP), dtype=torch.float32, device=device)
-    _launch(what, device, _lib.get().da_gelu_int8, rows.data_ptr(), rows.shape[0], columns, pitch, _half_code(z.dtype),
-            out.data_ptr(), values.data_ptr(), ldv, scales.data_ptr())
+    out = torch.empty(shape, dtype=z.dtype, device=device)
+    values, ldv = _new_values(shape[:-1], columns, device)
+    scales = torch.empty(*shape[:-1], -(-columns // INT8_GROUP), dtype=torch.float32, device=device)
+    _launch(what, device, _lib.get().da_gelu_int8, rows.data_ptr(), rows.shape[0], columns, pitch, code, out.data_ptr(),
+            values.data_ptr(), ldv, scales.data_ptr())
     return out, QuantizedRows(values, scales, INT8_GROUP)
 
 
@@ -398,20 +461,19 @@ def gelu_int8_backward_hip(kept: QuantizedRows, grad: Tensor, *, want_output: bo
     rows stand for; fp32, one rounding to grad's 16-bit type."""
 
     what = "gelu_int8_backward_hip"
-    _check_quantized(what, kept)
-    _check_rows(what, grad)
-    if kept.group != INT8_GROUP:
+    code = _check_input(what, grad)
+    shape, device = grad.shape, grad.device
+    _check_quantized(what, kept, device)
+    values, scales, group = kept
+    if group is None:
         raise ValueError(f"{what}: rows kept in groups of {INT8_GROUP} columns")
-    if kept.values.shape != grad.shape:
-        raise ValueError(f"{what}: gradients of shape {tuple(grad.shape)} at kept rows of shape {tuple(kept.values.shape)}")
-    device = grad.device
-    _on_device(what, device, kept.values, kept.scales)
-    values, ldv = _values_rows(kept.values)
-    scales = kept.scales.contiguous()
-    g, ldg = _rows(grad.detach())
-    grad_z = torch.empty(grad.shape, dtype=grad.dtype, device=device)
-    out = torch.empty(grad.shape, dtype=grad.dtype, device=device) if want_output else None
+    if values.shape != shape:
+        raise ValueError(f"{what}: gradients of shape {tuple(shape)} at kept rows of shape {tuple(values.shape)}")
+    values, ldv = _values_rows(values)
+    scales = scales.contiguous()
+    g, ldg = _rows(grad)
+    grad_z = torch.empty(shape, dtype=grad.dtype, device=device)
+    out = torch.empty(shape, dtype=grad.dtype, device=device) if want_output else None
     _launch(what, device, _lib.get().da_gelu_int8_backward, values.data_ptr(), values.shape[0], values.shape[1], ldv,
-            scales.data_ptr(), g.data_ptr(), ldg, _half_code(grad.dtype), grad_z.data_ptr(),
-            None if out is None else out.data_ptr())
+            scales.data_ptr(), g.data_ptr(), ldg, code, grad_z.data_ptr(), None if out is None else out.data_ptr())
     return grad_z, out

@@ -32,6 +32,7 @@ extern "C" {
  * outside of the rows it is given.
  */
 #define DA_INT8_GROUP 128
+#define DA_I8 3 /* dtype code of 8-bit rows with one scale each */
 
 /* values, scales = int8(x); x of any dtype.  group 0: cols <= 65536. */
 int da_quantize_int8(const void* x, int64_t rows, int64_t cols, int64_t ldx, int dtype, int64_t group, void* values,
@@ -47,15 +48,20 @@ int da_dequantize_int8(const void* values, int64_t rows, int64_t cols, int64_t l
  * the sum in 32-bit integers (exact), the rest in fp32, rounded to dtype
  * (DA_F16 or DA_BF16), then + residual (NULL or [rows, out_features] of dtype
  * at pitch ldr; added to the rounded result and rounded again, as the unfused
- * `x + linear(...)` does).  x: [rows, in_features] at pitch ldx, weight:
- * [out_features, in_features] at pitch ldw (multiples of 16, 16-byte aligned
- * rows of any integers, -128 too; the bytes behind in_features are not used).
- * in_features <= 65536.  out: contiguous [rows, out_features].
+ * `x + linear(...)` does).  x: [rows, in_features] at pitch ldx, of x_dtype
+ * DA_I8 with x_scales, or 16-bit rows (x_scales is not read) that are quantized
+ * as by da_quantize_int8, into the workspace (16-byte aligned, as many bytes
+ * as da_linear_int8_workspace_bytes returns; up to 16 rows of up to 4096
+ * columns of the output's type need none) or inside the kernel.  weight: [out_features, in_features]
+ * at pitch ldw.  8-bit rows may hold any integers, -128 too; the bytes behind
+ * in_features are not used.  in_features <= 65536, pitches of 8-bit rows at
+ * most 2^23.  out: contiguous [rows, out_features].
  */
-int da_linear_int8(const void* x, int64_t ldx, const float* x_scales, int64_t rows, int64_t in_features,
+int64_t da_linear_int8_workspace_bytes(int64_t rows, int64_t in_features, int x_dtype);
+int da_linear_int8(const void* x, int x_dtype, int64_t ldx, const float* x_scales, int64_t rows, int64_t in_features,
                    const void* weight, int64_t ldw, const float* w_scales, int64_t out_features, const void* bias,
                    int bias_dtype, int activation, const void* residual, int64_t ldr, void* out, int dtype,
-                   da_stream_t stream);
+                   void* workspace, int64_t workspace_bytes, da_stream_t stream);
 
 /*
  * Root-mean-square norm with the residual's addition in front of it:

@@ -187,7 +187,7 @@ def check_linear(got, kept_x, kept_w, bias, gelu, residual, dtype):
     (1, 512, 1536), (1, 1, 1), (2, 16, 4), (3, 17, 9), (5, 127, 33), (16, 128, 130), (17, 129, 128), (31, 1000, 65),
     (33, 64, 257), (64, 1536, 512), (65, 100, 64), (127, 255, 127), (128, 256, 128), (129, 384, 129),
     (300, 1000, 1111), (513, 512, 1536), (1, 4096, 4096), (16, 4096, 1000), (48, 2048, 640), (4, 65536, 24),
-    (700, 700, 3), (2000, 15, 300),
+    (700, 700, 3), (2000, 15, 300), (2100, 200, 1500), (1500, 130, 1900), (3000, 64, 2000), (4100, 333, 2500), (5000, 700, 4500),
 ])
 def test_linear(rows, inner, outer, dtype) -> None:
     x = _randn(rows, inner, seed=rows, dtype=dtype)
@@ -203,6 +203,8 @@ def test_linear(rows, inner, outer, dtype) -> None:
         check_linear(got, kept, w, b, gelu, res, dtype)
         again = da.linear_int8_hip(kept, w, b, dtype=dtype, **options)
         assert torch.equal(got, again), "16-bit rows and the same rows quantized before"
+    other = torch.float16 if dtype == torch.bfloat16 else torch.bfloat16
+    check_linear(da.linear_int8_hip(x, w, dtype=other), kept, w, None, False, None, other)
 
 
 @pytest.mark.gpu
@@ -343,8 +345,8 @@ def test_add_rms_norm_backward(width, dtype) -> None:
                 assert grad_weight is None
                 continue
             assert grad_weight.dtype == w.dtype
-            # A thread's rows, 64 runs, 8 parts: at most rows + 8 additions.
-            bound = dw_size * ((rows + 8) * F32 + NORM_F32 + 2 * F32)
+            # A thread's rows, then the workgroups' sums: at most rows + 32 additions.
+            bound = dw_size * ((rows + 32) * F32 + NORM_F32 + 2 * F32)
             close(grad_weight, dw, dw.abs() * half_step(w.dtype) + bound + least(w.dtype))
             again = da.add_rms_norm_backward_hip(s, g, extra, w, 1e-5)
             assert torch.equal(grad_x, again[0]) and torch.equal(grad_weight, again[1])
@@ -544,7 +546,7 @@ def test_refusals_on_the_host() -> None:
             call()
     with pytest.raises(ValueError, match="at least one column"):
         da.quantize_int8_hip(torch.zeros(3, 0))
-    with pytest.raises(ValueError, match="dtype"):
+    with pytest.raises(ValueError, match="float64"):
         da.quantize_int8_hip(torch.zeros(3, 4, dtype=torch.float64))
     for bad in (da.QuantizedRows(kept.values.float(), kept.scales), da.QuantizedRows(kept.values, kept.scales.half()),
                 da.QuantizedRows(kept.values, kept.scales[:3]), da.QuantizedRows(kept.values, kept.scales[:, 0]),
@@ -555,7 +557,7 @@ def test_refusals_on_the_host() -> None:
         da.dequantize_int8_hip(da.QuantizedRows(kept.values, kept.scales, 64))
     with pytest.raises(ValueError, match="activation"):
         da.linear_int8_hip(x, kept, activation="relu")
-    with pytest.raises(ValueError, match="fp16 or bf16"):
+    with pytest.raises(ValueError, match="float16 or bfloat16"):
         da.gelu_int8_hip(torch.zeros(2, 2))
 
 
@@ -613,7 +615,8 @@ def test_refusals_of_the_c_abi() -> None:
     assert lib.da_quantize_int8(p, 1 << 31, 8, 8, F16C, 128, p, 16, p, None) == -2
     assert lib.da_dequantize_int8(p, 2, 8, 16, None, 0, p, 8, F32C, None) == -1
     assert lib.da_dequantize_int8(p, 2, 8, 16, p, 32, p, 8, F32C, None) == -2
-    linear = [p, 16, p, 2, 8, p, 16, p, 6, None, F32C, 0, None, 0, p, F16C, None]
+    I8C = _lib.DA_I8
+    linear = [p, I8C, 16, p, 2, 8, p, 16, p, 6, None, F32C, 0, None, 0, p, F16C, None, 0, None]
 
     def linear_with(**changes):
         args = list(linear)
@@ -621,11 +624,18 @@ def test_refusals_of_the_c_abi() -> None:
             args[int(i[1:])] = v
         return lib.da_linear_int8(*args)
 
-    assert linear_with(_15=F32C) == -1 and linear_with(_11=2) == -1 and linear_with(_8=0) == -2
-    assert linear_with(_4=65537, _1=65552, _6=65552) == -2 and linear_with(_1=8) == -3 and linear_with(_6=24) == -3
-    assert linear_with(_0=None) == -1 and linear_with(_7=None) == -1 and linear_with(_14=None) == -1
-    assert linear_with(_9=p, _10=9) == -1 and linear_with(_9=p + 2) == -3 and linear_with(_12=p, _13=5) == -1
-    assert linear_with(_3=1 << 31) == -2 and linear_with(_3=1 << 22, _8=1 << 24) == -2
+    assert linear_with(_16=F32C) == -1 and linear_with(_12=2) == -1 and linear_with(_9=0) == -2
+    assert linear_with(_5=65537, _2=65552, _7=65552) == -2 and linear_with(_2=8) == -3 and linear_with(_7=24) == -3
+    assert linear_with(_0=None) == -1 and linear_with(_8=None) == -1 and linear_with(_15=None) == -1
+    assert linear_with(_3=None) == -1 and linear_with(_1=F32C) == -1 and linear_with(_7=(1 << 23) + 16) == -2
+    assert linear_with(_10=p, _11=9) == -1 and linear_with(_10=p + 2) == -3 and linear_with(_13=p, _14=5) == -1
+    assert linear_with(_4=1 << 31) == -2 and linear_with(_4=1 << 22, _9=1 << 24) == -2
+    # 16-bit rows that need a workspace: too many, or of another type than the output.
+    need = lib.da_linear_int8_workspace_bytes(100, 8, F16C)
+    assert need > 0 and lib.da_linear_int8_workspace_bytes(100, 8, I8C) == 0
+    assert linear_with(_1=F16C, _2=8, _4=100) == -5 and linear_with(_1=F16C, _2=8, _4=100, _17=p, _18=need - 1) == -5
+    assert linear_with(_1=F16C, _2=8, _4=100, _17=p + 8, _18=need) == -3
+    assert linear_with(_1=_lib.DA_BF16, _2=8) == -5
     assert lib.da_add_rms_norm(p, 8, None, 0, 2, 8, None, F32C, 0.0, F16C, None, p, None, 0, None, None) == -1
     assert lib.da_add_rms_norm(p, 8, None, 0, 2, 8, None, F32C, 1e-6, F16C, None, None, None, 0, None, None) == -1
     assert lib.da_add_rms_norm(p, 8, p, 8, 2, 8, None, F32C, 1e-6, F16C, None, p, None, 0, None, None) == -1
@@ -640,7 +650,7 @@ def test_refusals_of_the_c_abi() -> None:
     assert lib.da_gelu_int8_backward(p, 2, 8, 16, p, p, 8, F16C, None, None, None) == -1
     # No rows: nothing to do, whatever the pointers are.
     assert lib.da_quantize_int8(None, 0, 8, 8, F16C, 0, None, 16, None, None) == 0
-    assert lib.da_linear_int8(*[None if v == p else v for v in linear][:3], 0, *[None if v == p else v for v in linear][4:]) == 0
+    assert linear_with(_0=None, _3=None, _4=0, _6=None, _15=None) == 0
 
 
 def test_fast_division_is_exact() -> None:
