@@ -291,7 +291,7 @@ __global__ __launch_bounds__(64 * Cfg::WAVES) void linear_int8_kernel(LinearInt8
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         float v = __builtin_fmaf(static_cast<float>(acc[p][q][r]) * xs, ws[r], bias[r]);
-        if constexpr ((EPI & kGemmActGelu) != 0) v = 0.5f * v * (1.f + erf_fast(v * kSqrtHalf));
+        if constexpr ((EPI & kGemmActGelu) != 0) v = gelu(v);
         o[r] = static_cast<T>(v);
       }
       *reinterpret_cast<typename Elem<T>::v4*>(stage_w + c * Cfg::ROWB + (p * 16 + 4 * g) * 2) = o;
@@ -360,16 +360,6 @@ __device__ __forceinline__ RawStep<T> fetch_step(const T* p, int n) {
   }
   return r;
 }
-// Largest magnitudes of 16-bit floats as unsigned integers (they order alike),
-// two at a time.
-template <typename T>
-__device__ __forceinline__ uint32_t step_max(const RawStep<T>& r, uint32_t pair) {
-  u16x2 m = __builtin_bit_cast(u16x2, pair);
-#pragma unroll
-  for (int d = 0; d < 8; ++d) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, r.d[d / 4][d % 4] & 0x7fff7fffu));
-  return __builtin_bit_cast(uint32_t, m);
-}
-
 template <typename T, typename XT, int MT, int EPI>
 __global__ __launch_bounds__(64 * kFewWaves) void linear_int8_few_kernel(LinearInt8Args a) {
   constexpr bool QUANT = sizeof(XT) == 2;
@@ -444,9 +434,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_int8_few_kernel(LinearI
     uint32_t pair = 0;
 #pragma unroll
     for (int u = 0; u < kFewBatch; ++u)
-      if (step_of(0, u) < steps) pair = step_max(raw[u], pair);
-    const uint16_t larger = static_cast<uint16_t>(max(pair & 0xffffu, pair >> 16));
-    uint32_t amax = __float_as_uint(static_cast<float>(__builtin_bit_cast(T, larger)));
+      if (step_of(0, u) < steps) pair = max_pairs(raw[u].d[1], max_pairs(raw[u].d[0], pair));
+    uint32_t amax = magnitude_bits(half_value<T>(max(pair & 0xffffu, pair >> 16)));
     const auto p = __builtin_amdgcn_permlane32_swap(amax, amax, false, false);
     amax = max(p[0], p[1]);
     const auto r = __builtin_amdgcn_permlane16_swap(amax, amax, false, false);
@@ -507,7 +496,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_int8_few_kernel(LinearI
     for (int v = 0; v < kFewWaves; ++v) sum += part[v][e];
     const float bias = has_bias ? scalar_value(bias_raw[o], a.bias_dtype) : 0.f;
     float y = __builtin_fmaf(static_cast<float>(sum) * (QUANT ? token_scale[j] : x_scale[o]), w_scale[o], bias);
-    if constexpr ((EPI & kGemmActGelu) != 0) y = 0.5f * y * (1.f + erf_fast(y * kSqrtHalf));
+    if constexpr ((EPI & kGemmActGelu) != 0) y = gelu(y);
     T t = static_cast<T>(y);
     if constexpr ((EPI & 2) != 0) t = static_cast<T>(static_cast<float>(t) + res[o]);
     out[j * a.N + i] = t;

@@ -116,6 +116,21 @@ __device__ __forceinline__ void store_chunk(T* p, int n, const float (&v)[8]) {
 // maximum does not lose them.
 __device__ __forceinline__ uint32_t magnitude_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
+// Largest magnitudes of the 16-bit floats in d, as pairs of 16-bit integers.
+__device__ __forceinline__ uint32_t max_pairs(u32x4 d, uint32_t pair) {
+  u16x2 m = __builtin_bit_cast(u16x2, pair);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, d[i] & 0x7fff7fffu));
+  return __builtin_bit_cast(uint32_t, m);
+}
+
+// The float of a 16-bit float's bits.
+template <typename T>
+__device__ __forceinline__ float half_value(uint32_t bits) {
+  if constexpr (sizeof(T) == 2) return static_cast<float>(__builtin_bit_cast(T, static_cast<uint16_t>(bits)));
+  else return 0.f;
+}
+
 // All-lane reductions over the 16 lanes of a row (DPP rotations), then over
 // the wave's four rows.
 template <int R>

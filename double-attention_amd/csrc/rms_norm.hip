@@ -145,9 +145,8 @@ __global__ __launch_bounds__(row_block<NT>()) void row_int8_kernel(RowInt8Args a
 template <typename T, int NT, int CH>
 __global__ __launch_bounds__(row_block<NT>()) void rms_norm_backward_kernel(RmsNormBackwardArgs a) {
   constexpr int ROWS = row_block<NT>() / NT;
-  // Row reductions (two sets of slots), or [dim] sums of workgroups whose
-  // waves hold a row each.
-  extern __shared__ float lds[];
+  // Row reductions (two sets of slots), or the sums of waves that hold a row each.
+  extern __shared__ __attribute__((aligned(16))) float lds[];
   const int t = static_cast<int>(threadIdx.x) % NT;
   float w[CH][8], gw[CH][8];
 #pragma unroll
@@ -245,20 +244,20 @@ __global__ __launch_bounds__(row_block<NT>()) void rms_norm_backward_kernel(RmsN
       store_chunk(part + c, a.dim - c, gw[k]);
     }
   } else {
-    // The workgroup's waves add their sums in turn.
-    for (int q = 0; q < ROWS; ++q) {
-      if (wave_id() == q) {
+    // The waves' sums side by side in LDS, then added in the waves' order.
 #pragma unroll
-        for (int k = 0; k < CH; ++k)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int c = (k * NT + t) * 8 + e;
-            if (c < a.dim) lds[c] = q > 0 ? lds[c] + gw[k][e] : gw[k][e];
-          }
-      }
-      __syncthreads();
+    for (int k = 0; k < CH; ++k) {
+      float* at = lds + (wave_id() * CH + k) * 512 + t * 8;
+      *reinterpret_cast<f32x4*>(at) = f32x4{gw[k][0], gw[k][1], gw[k][2], gw[k][3]};
+      *reinterpret_cast<f32x4*>(at + 4) = f32x4{gw[k][4], gw[k][5], gw[k][6], gw[k][7]};
     }
-    for (int c = static_cast<int>(threadIdx.x); c < a.dim; c += row_block<NT>()) part[c] = lds[c];
+    __syncthreads();
+    for (int c = static_cast<int>(threadIdx.x); c < a.dim; c += row_block<NT>()) {
+      float sum = lds[c];
+#pragma unroll
+      for (int q = 1; q < ROWS; ++q) sum += lds[q * CH * 512 + c];
+      part[c] = sum;
+    }
   }
 }
 
@@ -325,6 +324,9 @@ void launch_row_int8(const RowInt8Args& a, bool norm, hipStream_t stream) {
   }
 }
 
+// Two workgroups a CU: with half of them the rows' loads do not fill the
+// memory's queues (16384 x 2048 49 us against 65), with twice as many the
+// partial sums cost more than that gains (55 us).
 int rms_norm_backward_blocks(int64_t rows, int dim) {
   const int64_t per = dim <= 1024 ? 4 : 1;
   const int64_t blocks = (rows + per - 1) / per;
@@ -333,7 +335,7 @@ int rms_norm_backward_blocks(int64_t rows, int dim) {
 
 template <typename T, int NT, int CH>
 static void launch_backward_k(const RmsNormBackwardArgs& a, hipStream_t stream) {
-  const size_t lds = NT > 64 ? 4 * (NT / 64) * sizeof(float) : (static_cast<size_t>(a.dim) + 8) * sizeof(float);
+  const size_t lds = NT > 64 ? 4 * (NT / 64) * sizeof(float) : 4 * CH * 512 * sizeof(float);
   hipLaunchKernelGGL((rms_norm_backward_kernel<T, NT, CH>), dim3(rms_norm_backward_blocks(a.rows, a.dim)),
                      dim3(row_block<NT>()), lds, stream, a);
 }

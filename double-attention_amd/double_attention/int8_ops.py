@@ -53,6 +53,7 @@ class QuantizedRows(NamedTuple):
 
 
 _current_device = torch._C._cuda_getDevice
+_INT8, _FLOAT32 = torch.int8, torch.float32
 _CODES = {torch.float32: _lib.DA_F32, torch.float16: _lib.DA_F16, torch.bfloat16: _lib.DA_BF16}
 _HALF_CODES = {torch.float16: _lib.DA_F16, torch.bfloat16: _lib.DA_BF16}
 
@@ -85,19 +86,20 @@ def _check_input(what: str, x: Tensor, codes: dict = _HALF_CODES) -> int:
 
 
 def _check_on(what: str, device: torch.device, t: Tensor) -> None:
-    if t.device != device:
+    if t.get_device() != device.index:
         raise ValueError(f"{what}: all tensors must be on {device}, got one on {t.device}")
 
 
 def _check_like(what: str, x: Tensor, t: Tensor) -> None:
-    if t.shape != x.shape or t.dtype != x.dtype:
+    if t.shape != x.shape or t.dtype is not x.dtype:
         raise ValueError(f"{what}: expected shape {tuple(x.shape)} and {x.dtype}, got {tuple(t.shape)} and {t.dtype}")
-    _check_on(what, x.device, t)
+    if t.get_device() != x.get_device():
+        raise ValueError(f"{what}: all tensors must be on {x.device}, got one on {t.device}")
 
 
 def _check_param(what: str, device: torch.device, t: Tensor, size: int) -> int:
     code = _CODES.get(t.dtype)
-    if code is None or t.ndim != 1 or t.shape[0] != size:
+    if code is None or t.shape != (size,):
         raise ValueError(f"{what}: expected a floating parameter of shape ({size},), got {t.dtype} {tuple(t.shape)}")
     _check_on(what, device, t)
     return code
@@ -115,8 +117,9 @@ def _rows(t: Tensor) -> tuple[Tensor, int]:
 
     Rows at any pitch are read where they are; other orders are copied."""
 
-    columns = t.shape[-1]
-    if t.ndim != 2:
+    shape = t.shape
+    columns = shape[-1]
+    if len(shape) != 2:
         t = t.reshape(-1, columns)
     if t.is_contiguous():
         return t, columns
@@ -130,8 +133,8 @@ def _rows(t: Tensor) -> tuple[Tensor, int]:
     return t, pitch
 
 
-def _new_values(lead: torch.Size, columns: int, device: torch.device) -> tuple[Tensor, int]:
-    pitch = (columns + 15) // 16 * 16
+def _new_values(lead: tuple[int, ...], columns: int, device: torch.device) -> tuple[Tensor, int]:
+    pitch = (columns + 15) & ~15
     store = torch.empty(*lead, pitch, dtype=torch.int8, device=device)
     return (store if pitch == columns else store[..., :columns]), pitch
 
@@ -142,7 +145,7 @@ def _values_rows(t: Tensor) -> tuple[Tensor, int]:
 
     t, pitch = _rows(t)
     rows, columns = t.shape
-    if pitch == columns and columns % 16 == 0 and t.data_ptr() % 16 == 0:
+    if pitch == columns and not (columns | t.data_ptr()) & 15:
         return t, pitch
     if rows == 1:
         pitch = (columns + 15) // 16 * 16
@@ -159,22 +162,21 @@ def _values_rows(t: Tensor) -> tuple[Tensor, int]:
 
 def _check_quantized(what: str, rows: QuantizedRows, device: torch.device | None = None) -> None:
     values, scales, group = rows
-    if values.dtype is not torch.int8 or scales.dtype is not torch.float32:
+    if values.dtype is not _INT8 or scales.dtype is not _FLOAT32:
         raise ValueError(f"{what}: quantized rows are int8 values with fp32 scales")
     if group is not None and group != INT8_GROUP:
         raise NotImplementedError(f"{what}: a scale for each row (group None) or each {INT8_GROUP} columns")
     shape = values.shape
     if not shape or shape[-1] < 1:
         raise ValueError(f"{what}: expected rows of at least one column, got shape {tuple(shape)}")
-    if scales.shape != (*shape[:-1], 1 if group is None else -(-shape[-1] // group)):
+    *lead, columns = shape
+    if scales.shape != (*lead, 1 if group is None else -(-columns // group)):
         raise ValueError(f"{what}: scales of shape {tuple(scales.shape)} do not fit values of shape {tuple(shape)}")
     if not values.is_cuda:
         raise ValueError(f"{what}: HIP kernels require tensors on a ROCm device")
-    if device is None:
-        device = values.device
-    else:
-        _check_on(what, device, values)
-    _check_on(what, device, scales)
+    index = values.get_device() if device is None else device.index
+    if scales.get_device() != index or values.get_device() != index:
+        raise ValueError(f"{what}: all tensors must be on one device")
 
 
 def quantize_int8_hip(x: Tensor, group: int | None = None) -> QuantizedRows:
@@ -192,11 +194,11 @@ def quantize_int8_hip(x: Tensor, group: int | None = None) -> QuantizedRows:
     if group is not None and group != INT8_GROUP:
         raise NotImplementedError(f"{what}: a scale for each row (group None) or each {INT8_GROUP} columns")
     device = x.device
-    lead, columns = x.shape[:-1], x.shape[-1]
+    *lead, columns = x.shape
     rows, pitch = _rows(x)
     values, ldv = _new_values(lead, columns, device)
     groups = 1 if group is None else -(-columns // INT8_GROUP)
-    scales = torch.empty(*lead, groups, dtype=torch.float32, device=device)
+    scales = torch.empty(*lead, groups, dtype=_FLOAT32, device=device)
     _launch(what, device, _lib.get().da_quantize_int8, rows.data_ptr(), rows.shape[0], columns, pitch, code, group or 0,
             values.data_ptr(), ldv, scales.data_ptr())
     return QuantizedRows(values, scales, group)
@@ -259,7 +261,7 @@ def linear_int8_hip(
     shape, device = x.shape, x.device
     _check_quantized(what, weight, device)
     w, w_scales, group = weight
-    if w.ndim != 2 or group is not None:
+    if group is not None or w.ndim != 2:
         raise ValueError(f"{what}: the weight is [out_features, in_features] with one scale for each output channel")
     code = _HALF_CODES.get(dtype)
     if code is None:
@@ -267,7 +269,8 @@ def linear_int8_hip(
     out_features, in_features = w.shape
     if shape[-1] != in_features:
         raise ValueError(f"{what}: rows of {shape[-1]} columns against a weight of {in_features}")
-    out_shape = (*shape[:-1], out_features)
+    *lead, _ = shape
+    out_shape = (*lead, out_features)
     _no_grad(what, x, bias, residual)
     bias_ptr, bias_code = None, _lib.DA_F32
     if bias is not None:
@@ -276,7 +279,7 @@ def linear_int8_hip(
         bias_ptr = bias.data_ptr()
     res_ptr, ldr = None, 0
     if residual is not None:
-        if residual.shape != out_shape or residual.dtype != dtype:
+        if residual.shape != out_shape or residual.dtype is not dtype:
             raise ValueError(f"{what}: the residual must match the output's shape and dtype")
         _check_on(what, device, residual)
         residual, ldr = _rows(residual)
@@ -305,7 +308,7 @@ def linear_int8_hip(
 def _add_rms_norm(what, x, residual, weight, eps, want_out, want_int8):
     code = _check_input(what, x)
     shape, device, dtype = x.shape, x.device, x.dtype
-    width = shape[-1]
+    *lead, width = shape
     rows, ldx = _rows(x)
     total, res_ptr, ldr, total_ptr = x, None, 0, None
     if residual is not None:
@@ -325,8 +328,8 @@ def _add_rms_norm(what, x, residual, weight, eps, want_out, want_int8):
         out = torch.empty(shape, dtype=dtype, device=device)
         out_ptr = out.data_ptr()
     if want_int8:
-        values, ldv = _new_values(shape[:-1], width, device)
-        scales = torch.empty(*shape[:-1], 1, dtype=torch.float32, device=device)
+        values, ldv = _new_values(lead, width, device)
+        scales = torch.empty(*lead, 1, dtype=_FLOAT32, device=device)
         values_ptr, scales_ptr = values.data_ptr(), scales.data_ptr()
     _launch(what, device, _lib.get().da_add_rms_norm, rows.data_ptr(), ldx, res_ptr, ldr, rows.shape[0], width, weight_ptr,
             weight_code, float(eps), code, total_ptr, out_ptr, values_ptr, ldv, scales_ptr)
@@ -444,11 +447,11 @@ def gelu_int8_hip(z: Tensor) -> tuple[Tensor, QuantizedRows]:
     code = _check_input(what, z)
     _no_grad(what, z)
     shape, device = z.shape, z.device
-    columns = shape[-1]
+    *lead, columns = shape
     rows, pitch = _rows(z)
     out = torch.empty(shape, dtype=z.dtype, device=device)
-    values, ldv = _new_values(shape[:-1], columns, device)
-    scales = torch.empty(*shape[:-1], -(-columns // INT8_GROUP), dtype=torch.float32, device=device)
+    values, ldv = _new_values(lead, columns, device)
+    scales = torch.empty(*lead, -(-columns // INT8_GROUP), dtype=_FLOAT32, device=device)
     _launch(what, device, _lib.get().da_gelu_int8, rows.data_ptr(), rows.shape[0], columns, pitch, code, out.data_ptr(),
             values.data_ptr(), ldv, scales.data_ptr())
     return out, QuantizedRows(values, scales, INT8_GROUP)
