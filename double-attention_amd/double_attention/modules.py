@@ -747,10 +747,51 @@ def _hip_layer_norm_applies(norm: nn.Module, x: Tensor, backend: str) -> bool:
     return resolve_backend(backend, (_Spec(True, x.dtype),)) == "hip"  # type: ignore[arg-type]
 
 
-def _layer_norm(norm: nn.LayerNorm, x: Tensor, backend: str) -> Tensor:
+def _layer_norm(norm: nn.Module, x: Tensor, backend: str) -> Tensor:
     if _hip_layer_norm_applies(norm, x, backend):
         return _HipLayerNormFunction.apply(x, norm.weight, norm.bias, norm.eps)
+    if _hip_rms_norm_applies(norm, x, backend):
+        return _hip_norm(norm, x)
     return norm(x)
+
+
+def _make_norm(kind: str, width: int) -> nn.Module:
+    """The blocks' and the LM's norm: ``"layer"`` (the reference's
+    ``nn.LayerNorm``) or ``"rms"`` (``nn.RMSNorm`` with eps 1e-6)."""
+
+    if kind == "layer":
+        return nn.LayerNorm(width)
+    if kind == "rms":
+        return nn.RMSNorm(width, eps=1e-6)
+    raise ValueError(f"unsupported norm {kind!r}: 'layer' or 'rms'")
+
+
+def _hip_rms_norm_applies(norm: nn.Module, x: Tensor, backend: str) -> bool:
+    """Whether ``norm`` (an ``nn.RMSNorm`` over one dimension) runs on the
+    library's norm kernels (``add_rms_norm_hip``, any width up to 16384) on x:
+    a 16-bit CUDA input whose backend resolves to HIP."""
+
+    from .int8_ops import MAX_NORM_WIDTH
+
+    if backend == "torch" or not isinstance(norm, nn.RMSNorm) or len(norm.normalized_shape) != 1:
+        return False
+    if x.dtype not in (torch.float16, torch.bfloat16) or not x.is_cuda or torch.is_autocast_enabled("cuda"):
+        return False
+    if norm.eps is None or norm.eps <= 0 or norm.normalized_shape[0] > MAX_NORM_WIDTH:
+        return False
+    return resolve_backend(backend, (_Spec(True, x.dtype),)) == "hip"  # type: ignore[arg-type]
+
+
+def _hip_norm(norm: nn.Module, x: Tensor) -> Tensor:
+    """A block's norm on the library's kernels."""
+
+    if isinstance(norm, nn.RMSNorm):
+        from .int8_ops import add_rms_norm_hip
+
+        return add_rms_norm_hip(x, None, norm.weight, norm.eps)[0]
+    from . import hip_ops
+
+    return hip_ops.layer_norm_hip(x, norm.weight, norm.bias, norm.eps)
 
 
 class _HipFeedForwardFunction(torch.autograd.Function):
@@ -800,8 +841,72 @@ class _HipFeedForwardFunction(torch.autograd.Function):
         return dx, dh, d_w1, d_b1, d_w2, d_b2
 
 
+class _HipFeedForwardInt8Function(torch.autograd.Function):
+    """``_HipFeedForwardFunction`` with its saved activations in 8 bits.
+
+    The forward computes the same values; it keeps h and z in groups of 128
+    columns (one byte an element and 3% of scales, where the 16-bit function
+    keeps h, z and u: with a feed-forward three times as wide as the model, 4.1
+    bytes instead of 14 for each model feature of a token).  The backward takes
+    GELU's slope and u from the kept z, and the first weight's gradient from
+    the kept h, each formed once in one pass.
+    """
+
+    @staticmethod
+    def forward(ctx, x, h, w1, b1, w2, b2):  # type: ignore[override]
+        from . import hip_ops, int8_ops
+
+        dtype = x.dtype
+        cast = lambda t: t if t is None or t.dtype == dtype else t.to(dtype)  # noqa: E731
+        z = hip_ops.linear_hip(h, cast(w1.detach()), b1.detach() if b1 is not None else None)
+        u, kept_z = int8_ops.gelu_int8_hip(z)
+        y = hip_ops.linear_hip(u, cast(w2.detach()), b2.detach() if b2 is not None else None, residual=x.detach())
+        # h is kept for the first weight's gradient alone.
+        kept_h = int8_ops.quantize_int8_hip(h, int8_ops.INT8_GROUP) if ctx.needs_input_grad[2] else None
+        ctx.save_for_backward(kept_z.values, kept_z.scales, *(kept_h[:2] if kept_h is not None else (None, None)), w1, w2)
+        ctx.has_bias = (b1 is not None, b2 is not None)
+        ctx.bias_dtypes = (b1.dtype if b1 is not None else None, b2.dtype if b2 is not None else None)
+        ctx.dtype = dtype
+        ctx.h_shape = h.shape
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):  # type: ignore[override]
+        from . import hip_ops, int8_ops
+
+        z_values, z_scales, h_values, h_scales, w1, w2 = ctx.saved_tensors
+        dtype = ctx.dtype
+        wants = ctx.needs_input_grad
+        dy = grad.reshape(-1, grad.shape[-1]).to(dtype)
+        du = torch.mm(dy, w2.detach().to(dtype))
+
+        def rows_of(values: Tensor, scales: Tensor) -> int8_ops.QuantizedRows:
+            return int8_ops.QuantizedRows(values.reshape(-1, values.shape[-1]), scales.reshape(-1, scales.shape[-1]),
+                                          int8_ops.INT8_GROUP)
+
+        kept = rows_of(z_values, z_scales)
+        dz, u = int8_ops.gelu_int8_backward_hip(kept, du, want_output=wants[4])
+        d_w2 = hip_ops._mm_tn_f32(dy, u, w2.dtype) if wants[4] else None
+        d_b2 = hip_ops.column_sums(dy, ctx.bias_dtypes[1]) if ctx.has_bias[1] and wants[5] else None
+        d_w1 = None
+        if wants[2]:
+            d_w1 = hip_ops._mm_tn_f32(dz, int8_ops.dequantize_int8_hip(rows_of(h_values, h_scales), dtype), w1.dtype)
+        d_b1 = hip_ops.column_sums(dz, ctx.bias_dtypes[0]) if ctx.has_bias[0] and wants[3] else None
+        dh = torch.mm(dz, w1.detach().to(dtype)).view(ctx.h_shape) if wants[1] else None
+        return grad if wants[0] else None, dh, d_w1, d_b1, d_w2, d_b2
+
+
 class DoubleAttentionBlock(nn.Module):
-    """Pre-norm transformer block around ``SharedDictionaryAttention`` (``modules.py:294-356``)."""
+    """Pre-norm transformer block around ``SharedDictionaryAttention`` (``modules.py:294-356``).
+
+    Beyond the reference's arguments: ``norm="rms"`` takes root-mean-square
+    norms instead of LayerNorms; ``activation_checkpoint="int8"`` keeps the
+    feed-forward's activations for the backward pass in 8 bits where it runs on
+    the HIP kernels (elsewhere they are kept as they are).
+    ``quantize_feedforward()`` lets inference on the HIP kernels run the
+    feed-forward on 8-bit integers.
+    """
 
     def __init__(
         self,
@@ -809,17 +914,24 @@ class DoubleAttentionBlock(nn.Module):
         *,
         feedforward_dim: int | None = None,
         dropout: float = 0.0,
+        norm: str = "layer",
+        activation_checkpoint: str | None = None,
     ) -> None:
         super().__init__()
+        if activation_checkpoint not in (None, "int8"):
+            raise ValueError(f"unsupported activation_checkpoint {activation_checkpoint!r}: None or 'int8'")
+        if activation_checkpoint is not None and config.q_dictionary_feedforward:
+            raise ValueError("activation_checkpoint='int8' does not cover the Q-dictionary FFN")
+        self.activation_checkpoint = activation_checkpoint
         feedforward_dim = feedforward_dim or 3 * config.model_dim
         if config.q_dictionary_feedforward:
             if config.qk_branches != 1:
                 raise ValueError("Q-dictionary FFN requires exactly one Q branch")
             if feedforward_dim != config.dictionary_size:
                 raise ValueError("Q-dictionary FFN requires feedforward_dim == dictionary_size")
-        self.attention_norm = nn.LayerNorm(config.model_dim)
+        self.attention_norm = _make_norm(norm, config.model_dim)
         self.attention = SharedDictionaryAttention(config, create_bank=False)
-        self.feedforward_norm = nn.LayerNorm(config.model_dim)
+        self.feedforward_norm = _make_norm(norm, config.model_dim)
         # The Q-dictionary FFN keeps the standard FFN's module indices; only
         # feedforward[0] (the expansion) is replaced by Dk^T Q (modules.py:314-323).
         first = nn.Identity() if config.q_dictionary_feedforward else nn.Linear(config.model_dim, feedforward_dim)
@@ -829,6 +941,57 @@ class DoubleAttentionBlock(nn.Module):
             nn.Linear(feedforward_dim, config.model_dim),
             nn.Dropout(dropout),
         )
+        # Set by quantize_feedforward: the two weights in 8 bits and the
+        # versions of the parameters that they were made from.
+        self._int8_feedforward: tuple | None = None
+
+    def quantize_feedforward(self, enabled: bool = True) -> None:
+        """Run the feed-forward on 8-bit integers in inference on the HIP kernels.
+
+        Both linears' weights are quantized now, a scale for each output channel
+        (``quantize_int8_hip``); activations are quantized for each token in
+        every forward.  Call it again after the weights change (a forward that
+        finds them changed in place raises ``RuntimeError``); ``enabled=False``
+        drops the 8-bit weights.  Forwards that autograd records, and those
+        that do not run on the HIP kernels, use the full weights as before.
+        """
+
+        if not enabled:
+            self._int8_feedforward = None
+            return
+        first, second = self.feedforward[0], self.feedforward[2]
+        if not isinstance(first, nn.Linear):
+            raise NotImplementedError("the Q-dictionary FFN has no 8-bit form")
+        from .hip_ops import _version_of
+        from .int8_ops import quantize_int8_hip
+
+        with torch.no_grad():
+            self._int8_feedforward = (
+                quantize_int8_hip(first.weight), quantize_int8_hip(second.weight),
+                (_version_of(first.weight), _version_of(second.weight)),
+            )
+
+    def _int8_weights(self) -> tuple | None:
+        """The 8-bit weights, if the feed-forward runs on them."""
+
+        if self._int8_feedforward is None:
+            return None
+        from .hip_ops import _version_of
+
+        w1, w2, versions = self._int8_feedforward
+        first, second = self.feedforward[0].weight, self.feedforward[2].weight
+        if (_version_of(first), _version_of(second)) != versions or w1.values.device != first.device:
+            raise RuntimeError("the feed-forward's weights changed after quantize_feedforward(); call it again")
+        return w1, w2
+
+    def _feedforward_int8(self, x: Tensor, normalized, weights: tuple) -> Tensor:
+        """``x + FFN`` on 8-bit integers; ``normalized`` a 16-bit tensor or 8-bit rows."""
+
+        from .int8_ops import linear_int8_hip
+
+        first, second = self.feedforward[0], self.feedforward[2]
+        expanded = linear_int8_hip(normalized, weights[0], first.bias, activation="gelu", dtype=x.dtype)
+        return linear_int8_hip(expanded, weights[1], second.bias, residual=x)
 
     def _hip_block(
         self,
@@ -838,7 +1001,7 @@ class DoubleAttentionBlock(nn.Module):
     ) -> Tensor | None:
         """The block on the HIP kernels, without autograd, or None.
 
-        LayerNorms run as the library's LayerNorm kernel; the residual adds
+        Norms run as the library's LayerNorm (or RMS norm) kernel; the residual adds
         ride in the epilogues of the attention's output projection and of the
         FFN's second linear; the FFN's GELU rides in its first linear.  The
         Q-dictionary FFN expands on the library's GEMM against the normalized
@@ -855,13 +1018,24 @@ class DoubleAttentionBlock(nn.Module):
             return None
         if normalized_dictionary is not None and any(t.requires_grad for t in normalized_dictionary):
             return None
+        for norm in (self.attention_norm, self.feedforward_norm):
+            if isinstance(norm, nn.RMSNorm) and not _hip_rms_norm_applies(norm, x, attention.config.backend):
+                return None
         hip_ops.check_module_supported(attention.config)
         x = x.contiguous()
-        norm1 = self.attention_norm
-        hidden = hip_ops.layer_norm_hip(x, norm1.weight, norm1.bias, norm1.eps)
+        hidden = _hip_norm(self.attention_norm, x)
         x = attention._hip_call(hidden, bank, normalized_dictionary, dtype, residual=x, want_routed=False).output
         norm2 = self.feedforward_norm
-        normalized_x = hip_ops.layer_norm_hip(x, norm2.weight, norm2.bias, norm2.eps)
+        weights = self._int8_weights()
+        if weights is not None:
+            if isinstance(norm2, nn.RMSNorm):
+                from .int8_ops import add_rms_norm_int8_hip
+
+                normalized, _ = add_rms_norm_int8_hip(x, None, norm2.weight, norm2.eps)
+            else:
+                normalized = _hip_norm(norm2, x)
+            return self._feedforward_int8(x, normalized, weights)
+        normalized_x = _hip_norm(norm2, x)
         if attention.config.q_dictionary_feedforward:
             return self._q_dictionary_feedforward_hip(x, normalized_x, bank, normalized_dictionary, dtype)
         first, second = self.feedforward[0], self.feedforward[2]
@@ -920,15 +1094,29 @@ class DoubleAttentionBlock(nn.Module):
         if fused is not None:
             return fused
         backend = self.attention.config.backend
-        x = x + self.attention(
+        attended = self.attention(
             _layer_norm(self.attention_norm, x, backend), bank=bank, normalized_dictionary=normalized_dictionary
         )
-        normalized_x = _layer_norm(self.feedforward_norm, x, backend)
+        norm2 = self.feedforward_norm
+        if attended.dtype == x.dtype and _hip_rms_norm_applies(norm2, x, backend):
+            # The residual's addition and the norm in one launch.
+            from .int8_ops import add_rms_norm_hip
+
+            normalized_x, x = add_rms_norm_hip(attended, x, norm2.weight, norm2.eps)
+        else:
+            x = x + attended
+            normalized_x = _layer_norm(norm2, x, backend)
         if not self.attention.config.q_dictionary_feedforward:
             if self._hip_feedforward_applies(x, normalized_x):
                 first, second = self.feedforward[0], self.feedforward[2]
-                return _HipFeedForwardFunction.apply(x, normalized_x, first.weight, first.bias, second.weight,
-                                                     second.bias)
+                tensors = (x, normalized_x, first.weight, first.bias, second.weight, second.bias)
+                if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in tensors):
+                    weights = self._int8_weights()
+                    if weights is not None:
+                        return self._feedforward_int8(x, normalized_x, weights)
+                if self.activation_checkpoint == "int8":
+                    return _HipFeedForwardInt8Function.apply(*tensors)
+                return _HipFeedForwardFunction.apply(*tensors)
             return x + self.feedforward(normalized_x)
         return self._q_dictionary_feedforward(x, normalized_x, bank, normalized_dictionary)
 
@@ -967,6 +1155,8 @@ class DoubleAttentionStack(nn.Module):
         dictionary_group_size: int | None = None,
         feedforward_dim: int | None = None,
         dropout: float = 0.0,
+        norm: str = "layer",
+        activation_checkpoint: str | None = None,
     ) -> None:
         super().__init__()
         if num_layers <= 0:
@@ -982,9 +1172,16 @@ class DoubleAttentionStack(nn.Module):
             for _ in range(math.ceil(num_layers / group_size))
         )
         self.blocks = nn.ModuleList(
-            DoubleAttentionBlock(config, feedforward_dim=feedforward_dim, dropout=dropout)
+            DoubleAttentionBlock(config, feedforward_dim=feedforward_dim, dropout=dropout, norm=norm,
+                                 activation_checkpoint=activation_checkpoint)
             for _ in range(num_layers)
         )
+
+    def quantize_feedforward(self, enabled: bool = True) -> None:
+        """``DoubleAttentionBlock.quantize_feedforward`` of every block."""
+
+        for block in self.blocks:
+            block.quantize_feedforward(enabled)
 
     def _normalize_banks(self, x: Tensor) -> tuple[tuple[Tensor, Tensor], ...]:
         # Each bank is normalized once per forward and reused by every block
@@ -1023,6 +1220,8 @@ class DoubleAttentionLM(nn.Module):
         dictionary_group_size: int | None = None,
         feedforward_dim: int | None = None,
         dropout: float = 0.0,
+        norm: str = "layer",
+        activation_checkpoint: str | None = None,
     ) -> None:
         super().__init__()
         self.max_sequence_length = max_sequence_length
@@ -1034,21 +1233,28 @@ class DoubleAttentionLM(nn.Module):
             dictionary_group_size=dictionary_group_size,
             feedforward_dim=feedforward_dim,
             dropout=dropout,
+            norm=norm,
+            activation_checkpoint=activation_checkpoint,
         )
-        self.final_norm = nn.LayerNorm(config.model_dim)
+        self.final_norm = _make_norm(norm, config.model_dim)
         # Built (consuming its init draws) and then tied to the embedding.
         self.lm_head = nn.Linear(config.model_dim, vocab_size, bias=False)
         self.lm_head.weight = self.token_embedding.weight
 
+    def quantize_feedforward(self, enabled: bool = True) -> None:
+        """``DoubleAttentionBlock.quantize_feedforward`` of every block."""
+
+        self.stack.quantize_feedforward(enabled)
+
     def _final_norm(self, hidden: Tensor) -> Tensor:
-        # On the HIP path the final LayerNorm is the library's kernel (with
+        # On the HIP path the final norm is the library's kernel (with
         # its native backward when training).
         attention = self.stack.blocks[0].attention
         needs_grad = torch.is_grad_enabled() and any(p.requires_grad for p in self.final_norm.parameters())
-        if not needs_grad and attention._hip_inference_dtype(hidden, self.stack.banks[0]) == hidden.dtype:
-            from . import hip_ops
-
-            return hip_ops.layer_norm_hip(hidden, self.final_norm.weight, self.final_norm.bias, self.final_norm.eps)
+        norm = self.final_norm
+        covered = not isinstance(norm, nn.RMSNorm) or _hip_rms_norm_applies(norm, hidden, attention.config.backend)
+        if not needs_grad and covered and attention._hip_inference_dtype(hidden, self.stack.banks[0]) == hidden.dtype:
+            return _hip_norm(self.final_norm, hidden)
         return _layer_norm(self.final_norm, hidden, attention.config.backend)
 
     def forward(self, token_ids: Tensor, targets: Tensor | None = None) -> tuple[Tensor, Tensor | None]:
