@@ -781,8 +781,9 @@ int da_dequantize_int8(const void* values, int64_t rows, int64_t cols, int64_t l
   return check_launch("dequantize");
 }
 
-int64_t da_linear_int8_workspace_bytes(int64_t rows, int64_t in_features, int x_dtype) {
-  if (x_dtype == DA_I8 || rows < 1 || in_features < 1) return 0;
+int64_t da_linear_int8_workspace_bytes(int64_t rows, int64_t in_features, int64_t out_features, int x_dtype, int dtype) {
+  if (x_dtype == DA_I8 || rows < 1 || in_features < 1 || out_features < 1) return 0;
+  if (x_dtype == dtype && da::linear_int8_quantizes(rows, in_features, out_features)) return 0;
   return align_up(rows * da::round_up(in_features, 16)) + align_up(rows * 4);
 }
 
@@ -804,9 +805,8 @@ int da_linear_int8(const void* x, int x_dtype, int64_t ldx, const float* x_scale
       ((rows + 63) / 64) * ((out_features + 63) / 64) > 0x7fff0000LL)
     return fail(DA_ERR_UNSUPPORTED, "linear_int8: out_features must be in [1, 2^24], and the output's tiles below 2^31");
   if (rows == 0) return ok();
-  // 16-bit rows of x's type are quantized by the kernel of few rows; others
-  // into the workspace first.
-  const bool quantize = x_dtype != DA_I8 && !(x_dtype == dtype && da::linear_int8_quantizes(rows, in_features));
+  // 16-bit rows are quantized where they are multiplied, or into the workspace.
+  const int64_t need = da_linear_int8_workspace_bytes(rows, in_features, out_features, x_dtype, dtype);
   if (x_dtype == DA_I8) rc = validate_int8("linear_int8", "x", x, ldx, x_scales, in_features);
   else rc = validate_rows("linear_int8", "x", x, in_features, ldx, x_dtype);
   if (rc) return rc;
@@ -814,9 +814,8 @@ int da_linear_int8(const void* x, int x_dtype, int64_t ldx, const float* x_scale
   if ((rc = validate_rows("linear_int8", "out", out, out_features, out_features, dtype))) return rc;
   if (residual && (rc = validate_rows("linear_int8", "residual", residual, out_features, ldr, dtype))) return rc;
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  if (quantize) {
+  if (need > 0) {
     const int64_t ldv = da::round_up(in_features, 16);
-    const int64_t need = align_up(rows * ldv) + align_up(rows * 4);
     if (!workspace || workspace_bytes < need)
       return fail(DA_ERR_WORKSPACE, "linear_int8: the workspace needs %lld bytes", (long long)need);
     if (!aligned(workspace, 16)) return fail(DA_ERR_ALIGNMENT, "linear_int8: the workspace must be 16-byte aligned");

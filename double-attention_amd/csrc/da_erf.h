@@ -31,8 +31,10 @@ __device__ __forceinline__ float erf_fast(float x) {
 // forms on the way: with x = |v| / sqrt(2), Phi(-|v|) = (1 - erf(x)) / 2 =
 // (a1 t + ... + a5 t^5) / 2 e^(-x^2), at most 7.5e-8 off.  The factors 1 / 2
 // and 1 / sqrt(2) sit in the constants: GELU is v Phi(v), and its slope
-// Phi(v) + v e^(-v^2 / 2) / sqrt(2 pi).
+// Phi(v) + v e^(-v^2 / 2) / sqrt(2 pi).  No contraction beyond the FMAs that are
+// written, so that every kernel rounds alike.
 __device__ __forceinline__ float normal_cdf(float v, float& density) {
+#pragma clang fp contract(off)
   const float a = fabsf(v);
   const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f * kSqrtHalf, a, 1.f));
   float poly = __builtin_fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);
@@ -45,6 +47,7 @@ __device__ __forceinline__ float normal_cdf(float v, float& density) {
   return v < 0.f ? tail : 1.f - tail;
 }
 __device__ __forceinline__ float gelu(float v) {
+#pragma clang fp contract(off)
   float density;
   return v * normal_cdf(v, density);
 }

@@ -336,7 +336,7 @@ void launch_rms_norm_backward(const RmsNormBackwardArgs& a, hipStream_t stream);
 // Linear layer on 8-bit rows (gemm_int8.hip).
 struct LinearInt8Args {
   const void* x;
-  int x_dtype;            // kI8, or 16 bits (== dtype) where linear_int8_quantizes(rows, K)
+  int x_dtype;            // kI8, or 16 bits (== dtype) where linear_int8_quantizes(rows, K, N)
   int64_t ldx;            // a multiple of 16 for kI8, as ldw
   const float* x_scales;  // [rows] (kI8)
   int64_t rows;
@@ -353,7 +353,7 @@ struct LinearInt8Args {
   void* out;              // [rows][N]
   int dtype;              // out and residual
 };
-bool linear_int8_quantizes(int64_t rows, int64_t K);
+bool linear_int8_quantizes(int64_t rows, int64_t K, int64_t N);
 void launch_linear_int8(const LinearInt8Args& a, hipStream_t stream);
 
 // Launch shape of the attention for a problem: value slice width, waves per

@@ -30,6 +30,19 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kI8Stage = 128;   // bytes of k
 
+// The layer's result in fp32, the same bits in every kernel: two roundings
+// (the scaled sum, the sum with the bias), then GELU's.  The empty statement
+// keeps the compiler from folding the last of them into a conversion to 16
+// bits (v_fma_mixlo_f16 rounds once where v_fma_f32 and v_cvt_f16_f32 round
+// twice), which it would do in one kernel and not in another.
+template <int EPI>
+__device__ __forceinline__ float linear_result(int sum, float x_scale, float w_scale, float bias) {
+  float y = __builtin_fmaf(static_cast<float>(sum) * x_scale, w_scale, bias);
+  if constexpr ((EPI & kGemmActGelu) != 0) y = gelu(y);
+  asm("" : "+v"(y));
+  return y;
+}
+
 // The first n of a fragment's 16 bytes, zeros behind.
 __device__ __forceinline__ i32x4 first_bytes(i32x4 v, int n) {
 #pragma unroll
@@ -52,19 +65,25 @@ __device__ __forceinline__ void counted_barrier() {
 
 // A workgroup's tile: BI channels x BJ tokens over NWI x NWJ waves, NST stages
 // in LDS.  AHEAD > 0: stages that the L2 is asked for AHEAD stages before they
-// are multiplied (see below).
-template <int BI, int BJ, int NWI, int NWJ, int NST, int AHEAD = 0>
+// are multiplied (see below).  XS > 0: the tokens are 16-bit rows of up to XS
+// stages, quantized into LDS by the workgroup, and only W goes through the ring.
+template <int BI, int BJ, int NWI, int NWJ, int NST, int AHEAD = 0, int XS = 0>
 struct I8Cfg {
-  static constexpr int kAhead = AHEAD;
+  static constexpr int kAhead = AHEAD, kXS = XS;
   static constexpr int kBI = BI, kBJ = BJ, kNWI = NWI, kNWJ = NWJ, kNST = NST;
   static constexpr int WAVES = NWI * NWJ;
   static constexpr int WI = BI / NWI, WJ = BJ / NWJ;    // a wave's block
   static constexpr int NA = WI / 16, NB = WJ / 16;      // its MFMA blocks
   typedef XorTile<BI, kI8Stage / 16, false> TileW;
   typedef XorTile<BJ, kI8Stage / 16, false> TileX;
-  static constexpr int STAGE = TileW::BYTES + TileX::BYTES;
-  static constexpr int LOADS = (TileW::LOADS + TileX::LOADS) / WAVES;   // a wave's, each stage
-  static_assert((TileW::LOADS + TileX::LOADS) % WAVES == 0, "every wave loads as much");
+  static constexpr int STAGE = TileW::BYTES + (XS ? 0 : TileX::BYTES);
+  static constexpr int STAGE_LOADS = TileW::LOADS + (XS ? 0 : TileX::LOADS);
+  static constexpr int LOADS = STAGE_LOADS / WAVES;     // a wave's, each stage
+  static_assert(STAGE_LOADS % WAVES == 0, "every wave loads as much");
+  // Behind the ring: the corner that the L2's asking writes, the quantized
+  // tokens and their scales.
+  static constexpr int X_AT = NST * STAGE + (AHEAD ? 256 : 0);
+  static constexpr int LDS = X_AT + XS * TileX::BYTES + (XS ? 4 * BJ : 0);
   static constexpr int ROWB = WI * 2 + 16;              // bytes of a staged output row
   static_assert(TileW::LOADS % WAVES == 0 && WAVES % 2 == 0, "a load of all waves is of one operand, and 16 rows or a multiple");
   static constexpr int PARAMS = 2 * BI + BJ;            // floats that the epilogue reads
@@ -83,13 +102,63 @@ __device__ __forceinline__ void i8_tile(int t, int tiles_i, int tiles_j, int& ti
   tj = r / wide;
 }
 
+// The tokens' 8-bit rows in LDS, in the layout of their stages (XS > 0; zeros
+// behind K), and their scales.  A wave takes every WAVES-th row, its lanes eight
+// columns each of 512 at a time; W's first stages (`first_loads`) are asked for
+// behind the tokens' and arrive while these are quantized.
+template <typename T, typename Cfg, typename F>
+__device__ __forceinline__ void quantize_tokens(const LinearInt8Args& a, int64_t j0, int n_stages, char* lds, F first_loads) {
+  if constexpr (Cfg::kXS == 0) {
+    first_loads();
+  } else {
+    typedef typename Cfg::TileX TileX;
+    constexpr int ROWS = Cfg::kBJ / Cfg::WAVES, PASSES = (Cfg::kXS * kI8Stage + 511) / 512;
+    char* const values = lds + Cfg::X_AT;
+    float* const scales = reinterpret_cast<float*>(values + Cfg::kXS * TileX::BYTES);
+    const int lane = lane_id(), wave = uniform_wave();
+    u32x4 raw[ROWS][PASSES];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      const T* x = static_cast<const T*>(a.x) + min(j0 + wave + r * Cfg::WAVES, a.rows - 1) * a.ldx;
+#pragma unroll
+      for (int p = 0; p < PASSES; ++p) {
+        const int k = p * 512 + lane * 8;
+        raw[r][p] = fetch_bits(x + k, a.K - k);
+      }
+    }
+    first_loads();
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      uint32_t pair = 0;
+#pragma unroll
+      for (int p = 0; p < PASSES; ++p) pair = max_pairs(raw[r][p], pair);
+      const uint32_t largest = wave_max_bits(max(pair & 0xffffu, pair >> 16));
+      const Int8Scale s = int8_scale(magnitude_bits(half_value<T>(largest)));
+      const int row = wave + r * Cfg::WAVES;
+#pragma unroll
+      for (int p = 0; p < PASSES; ++p) {
+        const int k = p * 512 + lane * 8;
+        const typename Elem<T>::v8 h = __builtin_bit_cast(typename Elem<T>::v8, raw[r][p]);
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = static_cast<float>(h[e]);
+        const u32x2 q = pack_int8(v, s.inverse, s.keep);
+        const int st = k / kI8Stage;
+        if (st < n_stages)
+          *reinterpret_cast<u32x2*>(values + st * TileX::BYTES + TileX::offset(row, k % kI8Stage / 16) + k % 16) = q;
+      }
+      if (lane == 0) scales[row] = s.scale;
+    }
+  }
+}
+
 template <typename T, int EPI, typename Cfg>
 __global__ __launch_bounds__(64 * Cfg::WAVES) void linear_int8_kernel(LinearInt8Args a, int tiles_i, int tiles_j) {
   typedef typename Cfg::TileW TileW;
   typedef typename Cfg::TileX TileX;
   constexpr int NA = Cfg::NA, NB = Cfg::NB, NST = Cfg::kNST, STAGE = Cfg::STAGE, LOADS = Cfg::LOADS;
-  constexpr int AHEAD = Cfg::kAhead, EXTRA = AHEAD ? 1 : 0;
-  __shared__ __attribute__((aligned(1024))) char lds[NST * STAGE + 256 * EXTRA];
+  constexpr int AHEAD = Cfg::kAhead, EXTRA = AHEAD ? 1 : 0, XS = Cfg::kXS;
+  __shared__ __attribute__((aligned(1024))) char lds[Cfg::LDS];
   const int tiles = tiles_i * tiles_j;
   const int w = static_cast<int>(blockIdx.x);
   // Workgroups go to the XCDs round-robin: one XCD takes a contiguous range.
@@ -113,7 +182,7 @@ __global__ __launch_bounds__(64 * Cfg::WAVES) void linear_int8_kernel(LinearInt8
   const int tid = static_cast<int>(threadIdx.x);
   const int64_t chan = min(i0 + min(tid, Cfg::kBI - 1), a.N - 1);
   const float chan_scale = a.w_scales[chan];
-  const float tok_scale = a.x_scales[min(j0 + min(tid, Cfg::kBJ - 1), a.rows - 1)];
+  const float tok_scale = XS ? 0.f : a.x_scales[min(j0 + min(tid, Cfg::kBJ - 1), a.rows - 1)];
   const bool has_bias = a.bias != nullptr;
   const ScalarHalves bias_raw = fetch_scalar(has_bias ? a.bias : a.w_scales, has_bias ? a.bias_dtype : kF32, chan);
 
@@ -183,16 +252,17 @@ __global__ __launch_bounds__(64 * Cfg::WAVES) void linear_int8_kernel(LinearInt8
 #pragma unroll
     for (int q = 0; q < NB; ++q) acc[p][q] = i32x4{0, 0, 0, 0};
   const int afrag[2] = {TileW::base(wi * Cfg::WI + c, g, 0), TileW::base(wi * Cfg::WI + c, g, 1)};
-  const int bfrag[2] = {TileW::BYTES + TileX::base(wj * Cfg::WJ + c, g, 0), TileW::BYTES + TileX::base(wj * Cfg::WJ + c, g, 1)};
+  const int bfrag[2] = {TileX::base(wj * Cfg::WJ + c, g, 0), TileX::base(wj * Cfg::WJ + c, g, 1)};
   i32x4 af[2][NA], bf[2][NB];
   // Fragments from..to of half kk of stage st: NB of the tokens', then NA of
   // the channels'.
   auto read = [&](int st, int kk, int from, int to) {
     const char* buf = lds + (st % NST) * STAGE;
+    const char* xbuf = XS ? lds + Cfg::X_AT + st * TileX::BYTES : buf + TileW::BYTES;
 #pragma unroll
     for (int f = 0; f < NA + NB; ++f) {
       if (f < from || f >= to) continue;
-      if (f < NB) bf[kk][f] = *reinterpret_cast<const i32x4*>(buf + bfrag[kk] + f * TileX::ROW_BLOCK);
+      if (f < NB) bf[kk][f] = *reinterpret_cast<const i32x4*>(xbuf + bfrag[kk] + f * TileX::ROW_BLOCK);
       else af[kk][f - NB] = *reinterpret_cast<const i32x4*>(buf + afrag[kk] + (f - NB) * TileW::ROW_BLOCK);
     }
   };
@@ -212,9 +282,11 @@ __global__ __launch_bounds__(64 * Cfg::WAVES) void linear_int8_kernel(LinearInt8
   // ones may stay in flight) and its reads of stage st; behind the barrier
   // every wave's are done, so stage st + 1 is readable and stage st + NST may
   // be loaded into stage st's buffer.
+  quantize_tokens<T, Cfg>(a, j0, n_stages, lds, [&] {
 #pragma unroll
-  for (int st = 0; st < NST; ++st)
-    if (st < n_stages) issue(stage_loads(st), 0, LOADS);
+    for (int st = 0; st < NST; ++st)
+      if (st < n_stages) issue(stage_loads(st), 0, LOADS);
+  });
   if constexpr (AHEAD > 0) {
 #pragma unroll
     for (int st = NST; st < AHEAD; ++st) ask(st);
@@ -275,9 +347,27 @@ __global__ __launch_bounds__(64 * Cfg::WAVES) void linear_int8_kernel(LinearInt8
     chan_scales[tid] = chan_scale;
     chan_biases[tid] = has_bias ? scalar_value(bias_raw, a.bias_dtype) : 0.f;
   }
-  if (tid < Cfg::kBJ) token_scales[tid] = tok_scale;
+  if (tid < Cfg::kBJ)
+    token_scales[tid] = XS ? reinterpret_cast<const float*>(lds + Cfg::X_AT + XS * TileX::BYTES)[tid] : tok_scale;
   __syncthreads();
   T* out = static_cast<T*>(a.out);
+  constexpr int CHUNKS = Cfg::WI / 8;             // 16-byte chunks of a staged row
+  constexpr int ROWS = 64 / CHUNKS;               // rows written at a time
+  constexpr int PASSES = 16 / ROWS;
+  const int ic = (lane % CHUNKS) * 8;
+  const int64_t i = i0 + wi * Cfg::WI + ic;
+  const int n = static_cast<int>(min(a.N - i, static_cast<int64_t>(8)));   // channels of this lane's chunks
+  // All of a wave's residual chunks, before the stores that could be theirs.
+  RawChunk<T> res[(EPI & 2) ? NB : 1][(EPI & 2) ? PASSES : 1];
+  if constexpr ((EPI & 2) != 0) {
+#pragma unroll
+    for (int q = 0; q < NB; ++q)
+#pragma unroll
+      for (int pass = 0; pass < PASSES; ++pass) {
+        const int64_t j = j0 + wj * Cfg::WJ + q * 16 + pass * ROWS + lane / CHUNKS;
+        if (j < a.rows) res[q][pass] = fetch_chunk(static_cast<const T*>(a.residual) + j * a.ldr + i, n);
+      }
+  }
 #pragma unroll
   for (int q = 0; q < NB; ++q) {
     const int64_t jq = j0 + wj * Cfg::WJ + q * 16;
@@ -289,32 +379,23 @@ __global__ __launch_bounds__(64 * Cfg::WAVES) void linear_int8_kernel(LinearInt8
       const f32x4 bias = *reinterpret_cast<const f32x4*>(chan_biases + at);
       typename Elem<T>::v4 o;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float v = __builtin_fmaf(static_cast<float>(acc[p][q][r]) * xs, ws[r], bias[r]);
-        if constexpr ((EPI & kGemmActGelu) != 0) v = gelu(v);
-        o[r] = static_cast<T>(v);
-      }
+      for (int r = 0; r < 4; ++r) o[r] = static_cast<T>(linear_result<EPI>(acc[p][q][r], xs, ws[r], bias[r]));
       *reinterpret_cast<typename Elem<T>::v4*>(stage_w + c * Cfg::ROWB + (p * 16 + 4 * g) * 2) = o;
     }
-    constexpr int CHUNKS = Cfg::WI / 8;             // 16-byte chunks of a staged row
-    constexpr int ROWS = 64 / CHUNKS;               // rows written at a time
 #pragma unroll
-    for (int pass = 0; pass < 16 / ROWS; ++pass) {
+    for (int pass = 0; pass < PASSES; ++pass) {
       const int jr = pass * ROWS + lane / CHUNKS;
-      const int ic = (lane % CHUNKS) * 8;
       const int64_t j = jq + jr;
-      const int64_t i = i0 + wi * Cfg::WI + ic;
       const u32x4 v = *reinterpret_cast<const u32x4*>(stage_w + jr * Cfg::ROWB + ic * 2);
-      if (j >= a.rows || i >= a.N) continue;
-      const int n = static_cast<int>(min(a.N - i, static_cast<int64_t>(8)));
+      if (j >= a.rows || n <= 0) continue;
       T* dst = out + j * a.N + i;
       const typename Elem<T>::v8 e8 = __builtin_bit_cast(typename Elem<T>::v8, v);
       if constexpr ((EPI & 2) != 0) {
-        float res[8];
-        load_chunk(static_cast<const T*>(a.residual) + j * a.ldr + i, n, res);
+        float r[8];
+        chunk_floats(res[q][pass], static_cast<const T*>(a.residual) + j * a.ldr + i, n, r);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) res[e] += static_cast<float>(e8[e]);
-        store_chunk(dst, n, res);
+        for (int e = 0; e < 8; ++e) r[e] += static_cast<float>(e8[e]);
+        store_chunk(dst, n, r);
       } else if (n == 8) {
         store16B_any(dst, v);
       } else {
@@ -340,26 +421,12 @@ constexpr int kFewBatch = 8;    // steps of a wave in flight
 // Calls whose tokens are quantized in the kernel: one tile of tokens, one batch.
 constexpr int kFewRows = 16, kFewCols = 64 * kFewWaves * kFewBatch;
 
-// The 16 elements of a step's chunk as they lie in memory; n of them exist, the
-// others are 0.
+// The 16 elements of a step's chunk as they lie in memory.
 template <typename T>
 struct RawStep {
   u32x4 d[2];
 };
-template <typename T>
-__device__ __forceinline__ RawStep<T> fetch_step(const T* p, int n) {
-  RawStep<T> r{{u32x4{0, 0, 0, 0}, u32x4{0, 0, 0, 0}}};
-  if (n >= 16) {
-    r.d[0] = load16B_any(p);
-    r.d[1] = load16B_any(p + 8);
-  } else {
-    const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
-#pragma unroll
-    for (int e = 0; e < 16; ++e)
-      if (e < n) r.d[e / 8][e / 2 % 4] |= static_cast<uint32_t>(h[e]) << (16 * (e % 2));
-  }
-  return r;
-}
+
 template <typename T, typename XT, int MT, int EPI>
 __global__ __launch_bounds__(64 * kFewWaves) void linear_int8_few_kernel(LinearInt8Args a) {
   constexpr bool QUANT = sizeof(XT) == 2;
@@ -402,7 +469,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_int8_few_kernel(LinearI
       const int k = s * 64 + g * 16;
       if (s < steps) {
         if constexpr (QUANT) {
-          raw[u] = fetch_step(x[0] + k, K - k);
+          raw[u].d[0] = fetch_bits(x[0] + k, K - k);
+          raw[u].d[1] = fetch_bits(x[0] + k + 8, K - k - 8);
         } else {
 #pragma unroll
           for (int m = 0; m < MT; ++m) xf[u][m] = *reinterpret_cast<const i32x4*>(x[m] + min(k, last_chunk));
@@ -495,9 +563,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_int8_few_kernel(LinearI
 #pragma unroll
     for (int v = 0; v < kFewWaves; ++v) sum += part[v][e];
     const float bias = has_bias ? scalar_value(bias_raw[o], a.bias_dtype) : 0.f;
-    float y = __builtin_fmaf(static_cast<float>(sum) * (QUANT ? token_scale[j] : x_scale[o]), w_scale[o], bias);
-    if constexpr ((EPI & kGemmActGelu) != 0) y = gelu(y);
-    T t = static_cast<T>(y);
+    T t = static_cast<T>(linear_result<EPI>(sum, QUANT ? token_scale[j] : x_scale[o], w_scale[o], bias));
     if constexpr ((EPI & 2) != 0) t = static_cast<T>(static_cast<float>(t) + res[o]);
     out[j * a.N + i] = t;
   }
@@ -521,14 +587,28 @@ static void launch_few(const LinearInt8Args& a, hipStream_t stream) {
                      dim3(64 * kFewWaves), 0, stream, a);
 }
 
-template <typename T, int EPI>
-static void launch_linear_int8_k(const LinearInt8Args& a, hipStream_t stream) {
-  if (a.x_dtype != kI8) return launch_few<T, T, 1, EPI>(a, stream);   // at most kFewRows rows
-  // (32 x 4096 -> 4096: 8.5 us against 11.0 of the 64-tiles; 64 rows: 12.9 against 11.0.)
-  if (a.rows <= 16) return launch_few<T, int8_t, 1, EPI>(a, stream);
-  if (a.rows <= 32) return launch_few<T, int8_t, 2, EPI>(a, stream);
-  // Tile by how the output fills the 256 CUs (measured in us, bf16 without
-  // GELU unless said; rows x K -> N):
+typedef I8Cfg<128, 64, 4, 2, 2, 0, 4> Token128;      // 64 KiB of LDS: two a CU
+typedef I8Cfg<64, 64, 2, 4, 4, 0, 4> Token64;        // 64 KiB
+typedef I8Cfg<64, 64, 2, 4, 4, 0, 8> Token64x1024;   // 96 KiB: one a CU
+
+// How a call runs.  Measured in us, bf16 without GELU unless said; rows x K -> N.
+enum class I8Plan { kFew, kFew32, kToken64, kToken64x1024, kToken128, k256, k128, k128x64, k128Deep, k64 };
+static int64_t tiles_of(int64_t rows, int64_t N, int bi, int bj) { return ((N + bi - 1) / bi) * ((rows + bj - 1) / bj); }
+static I8Plan plan_linear_int8(int64_t rows, int64_t K, int64_t N, bool quantize) {
+  // (32 x 4096 -> 4096: 8.5 of the split K against 11.0 of the 64-tiles; 64 rows: 12.9 against 11.0.)
+  if (rows <= kFewRows && (!quantize || K <= kFewCols)) return I8Plan::kFew;
+  if (rows <= 32 && !quantize) return I8Plan::kFew32;
+  // 16-bit tokens are quantized again by every workgroup that multiplies them:
+  // as fast as a launch of its own for that, or nearly, while the workgroups
+  // are one round (4096 x 512 -> 512 7.6 against 8.6, 1024 x 512 -> 1536 7.4
+  // against 7.6, 64 x 512 -> 1536 6.3 against 6.3, 777 x 1000 -> 1111 10.5 against
+  // 9.2), and the call has one launch less, 3 us of the host's time.  Beyond, it is
+  // not (4096 x 512 -> 1536 16.3 against 14.2, 4096 x 1024 -> 1024 19 against 14).
+  // Between the two tiles: 64 x 512 -> 1536, 24 64-tiles, 6.3 against 6.8; 1024 x
+  // 512 -> 1536, 384 of them, 9.2 against 7.4.
+  if (quantize && K <= 1024 && tiles_of(rows, N, 64, 64) <= 256) return K <= 512 ? I8Plan::kToken64 : I8Plan::kToken64x1024;
+  if (quantize && K <= 512 && tiles_of(rows, N, 128, 64) <= 512) return I8Plan::kToken128;
+  // Tiles by how the output fills the 256 CUs:
   //   256-tiles cost 1.22 times less for the same products than 128-tiles, but
   //     come in rounds of 256 (8192 x 4096 -> 4096: 117 against 147; 2048 x
   //     4096 -> 6144, 192 tiles: 48 against 55; 16384 x 512 -> 512: 14 against 10);
@@ -540,13 +620,31 @@ static void launch_linear_int8_k(const LinearInt8Args& a, hipStream_t stream) {
   //   few of them leave CUs idle that 64-tiles use (512 x 4096 -> 4096, 128
   //     tiles: 15.6 against 18.2; 4096 x 1536 -> 512: 8.6 against 9.6; at 256
   //     tiles 17.3 against 12.4).
-  const auto tiles = [&](int bi, int bj) { return ((a.N + bi - 1) / bi) * ((a.rows + bj - 1) / bj); };
-  const int64_t t256 = tiles(256, 256), t128 = tiles(128, 128);
-  if ((t256 + 255) / 256 * 100 <= (t128 + 511) / 512 * 61) launch_tiles<T, EPI, Tile256>(a, stream);
-  else if (t128 > 384) launch_tiles<T, EPI, Tile128>(a, stream);
-  else if (t128 > 256) launch_tiles<T, EPI, Tile128x64>(a, stream);
-  else if (t128 > 144) launch_tiles<T, EPI, Tile128Deep>(a, stream);
-  else launch_tiles<T, EPI, Tile64>(a, stream);
+  const int64_t t256 = tiles_of(rows, N, 256, 256), t128 = tiles_of(rows, N, 128, 128);
+  if ((t256 + 255) / 256 * 100 <= (t128 + 511) / 512 * 61) return I8Plan::k256;
+  if (t128 > 384) return I8Plan::k128;
+  if (t128 > 256) return I8Plan::k128x64;
+  return t128 > 144 ? I8Plan::k128Deep : I8Plan::k64;
+}
+
+template <typename T, int EPI>
+static void launch_linear_int8_k(const LinearInt8Args& a, hipStream_t stream) {
+  const bool quantize = a.x_dtype != kI8;
+  switch (plan_linear_int8(a.rows, a.K, a.N, quantize)) {
+    case I8Plan::kFew:
+      if (quantize) launch_few<T, T, 1, EPI>(a, stream);
+      else launch_few<T, int8_t, 1, EPI>(a, stream);
+      break;
+    case I8Plan::kFew32: launch_few<T, int8_t, 2, EPI>(a, stream); break;
+    case I8Plan::kToken64: launch_tiles<T, EPI, Token64>(a, stream); break;
+    case I8Plan::kToken64x1024: launch_tiles<T, EPI, Token64x1024>(a, stream); break;
+    case I8Plan::kToken128: launch_tiles<T, EPI, Token128>(a, stream); break;
+    case I8Plan::k256: launch_tiles<T, EPI, Tile256>(a, stream); break;
+    case I8Plan::k128: launch_tiles<T, EPI, Tile128>(a, stream); break;
+    case I8Plan::k128x64: launch_tiles<T, EPI, Tile128x64>(a, stream); break;
+    case I8Plan::k128Deep: launch_tiles<T, EPI, Tile128Deep>(a, stream); break;
+    case I8Plan::k64: launch_tiles<T, EPI, Tile64>(a, stream); break;
+  }
 }
 
 template <typename T>
@@ -559,7 +657,10 @@ static void launch_linear_int8_t(const LinearInt8Args& a, hipStream_t stream) {
   }
 }
 
-bool linear_int8_quantizes(int64_t rows, int64_t K) { return rows <= kFewRows && K <= kFewCols; }
+bool linear_int8_quantizes(int64_t rows, int64_t K, int64_t N) {
+  const I8Plan plan = plan_linear_int8(rows, K, N, true);
+  return plan == I8Plan::kFew || plan == I8Plan::kToken64 || plan == I8Plan::kToken64x1024 || plan == I8Plan::kToken128;
+}
 
 void launch_linear_int8(const LinearInt8Args& a, hipStream_t stream) {
   if (a.dtype == kF16) launch_linear_int8_t<_Float16>(a, stream);

@@ -116,6 +116,22 @@ __device__ __forceinline__ void store_chunk(T* p, int n, const float (&v)[8]) {
 // maximum does not lose them.
 __device__ __forceinline__ uint32_t magnitude_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
+// A chunk of eight 16-bit elements as they lie in memory; n of them exist (the
+// others are 0).
+template <typename T>
+__device__ __forceinline__ u32x4 fetch_bits(const T* p, int n) {
+  u32x4 d{0, 0, 0, 0};
+  if (n >= 8) {
+    d = load16B_any(p);
+  } else {
+    const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) d[e / 2] |= static_cast<uint32_t>(h[e]) << (16 * (e % 2));
+  }
+  return d;
+}
+
 // Largest magnitudes of the 16-bit floats in d, as pairs of 16-bit integers.
 __device__ __forceinline__ uint32_t max_pairs(u32x4 d, uint32_t pair) {
   u16x2 m = __builtin_bit_cast(u16x2, pair);

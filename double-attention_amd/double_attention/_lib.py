@@ -220,7 +220,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
 INT8_SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "da_quantize_int8": (_i32, [_vp, _i64, _i64, _i64, _i32, _i64, _vp, _i64, _vp, _vp]),
     "da_dequantize_int8": (_i32, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _i32, _vp]),
-    "da_linear_int8_workspace_bytes": (_i64, [_i64, _i64, _i32]),
+    "da_linear_int8_workspace_bytes": (_i64, [_i64, _i64, _i64, _i32, _i32]),
     "da_linear_int8": (
         _i32,
         [

@@ -31,9 +31,6 @@ INT8_GROUP = _lib.INT8_GROUP
 # Columns of rows with one scale each, and widths of the norm.
 MAX_ROW_COLUMNS = 65536
 MAX_NORM_WIDTH = 16384
-# Up to so many 16-bit tokens of so many columns the linear layer's kernel
-# quantizes itself (da_linear_int8 needs no workspace then).
-QUANTIZED_IN_KERNEL = (16, 4096)
 
 
 class QuantizedRows(NamedTuple):
@@ -290,8 +287,8 @@ def linear_int8_hip(
     scales_ptr, workspace_ptr, nbytes = None, None, 0
     if x_scales is None:
         rows, ldx = _rows(x)
-        if rows.shape[0] > QUANTIZED_IN_KERNEL[0] or in_features > QUANTIZED_IN_KERNEL[1] or dtype != x.dtype:
-            nbytes = lib.da_linear_int8_workspace_bytes(rows.shape[0], in_features, x_code)
+        nbytes = lib.da_linear_int8_workspace_bytes(rows.shape[0], in_features, out_features, x_code, code)
+        if nbytes:
             workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
             workspace_ptr = workspace.data_ptr()
     else:

@@ -50,14 +50,14 @@ int da_dequantize_int8(const void* values, int64_t rows, int64_t cols, int64_t l
  * at pitch ldr; added to the rounded result and rounded again, as the unfused
  * `x + linear(...)` does).  x: [rows, in_features] at pitch ldx, of x_dtype
  * DA_I8 with x_scales, or 16-bit rows (x_scales is not read) that are quantized
- * as by da_quantize_int8, into the workspace (16-byte aligned, as many bytes
- * as da_linear_int8_workspace_bytes returns; up to 16 rows of up to 4096
- * columns of the output's type need none) or inside the kernel.  weight: [out_features, in_features]
- * at pitch ldw.  8-bit rows may hold any integers, -128 too; the bytes behind
- * in_features are not used.  in_features <= 65536, pitches of 8-bit rows at
- * most 2^23.  out: contiguous [rows, out_features].
+ * as by da_quantize_int8, where they are multiplied or into the workspace
+ * (16-byte aligned, as many bytes as da_linear_int8_workspace_bytes returns;
+ * with 0 it may be NULL).  weight: [out_features, in_features] at pitch ldw.
+ * 8-bit rows may hold any integers, -128 too; the bytes behind in_features are
+ * not used.  in_features <= 65536, pitches of 8-bit rows at most 2^23.  out:
+ * contiguous [rows, out_features].
  */
-int64_t da_linear_int8_workspace_bytes(int64_t rows, int64_t in_features, int x_dtype);
+int64_t da_linear_int8_workspace_bytes(int64_t rows, int64_t in_features, int64_t out_features, int x_dtype, int dtype);
 int da_linear_int8(const void* x, int x_dtype, int64_t ldx, const float* x_scales, int64_t rows, int64_t in_features,
                    const void* weight, int64_t ldw, const float* w_scales, int64_t out_features, const void* bias,
                    int bias_dtype, int activation, const void* residual, int64_t ldr, void* out, int dtype,

@@ -188,6 +188,7 @@ def check_linear(got, kept_x, kept_w, bias, gelu, residual, dtype):
     (33, 64, 257), (64, 1536, 512), (65, 100, 64), (127, 255, 127), (128, 256, 128), (129, 384, 129),
     (300, 1000, 1111), (513, 512, 1536), (1, 4096, 4096), (16, 4096, 1000), (48, 2048, 640), (4, 65536, 24),
     (700, 700, 3), (2000, 15, 300), (2100, 200, 1500), (1500, 130, 1900), (3000, 64, 2000), (4100, 333, 2500), (5000, 700, 4500),
+    (200, 512, 200), (130, 513, 70), (66, 1024, 65), (700, 900, 1500), (90, 1025, 64), (40, 1537, 40), (1100, 500, 1500), (4000, 33, 500),
 ])
 def test_linear(rows, inner, outer, dtype) -> None:
     x = _randn(rows, inner, seed=rows, dtype=dtype)
@@ -630,11 +631,12 @@ def test_refusals_of_the_c_abi() -> None:
     assert linear_with(_3=None) == -1 and linear_with(_1=F32C) == -1 and linear_with(_7=(1 << 23) + 16) == -2
     assert linear_with(_10=p, _11=9) == -1 and linear_with(_10=p + 2) == -3 and linear_with(_13=p, _14=5) == -1
     assert linear_with(_4=1 << 31) == -2 and linear_with(_4=1 << 22, _9=1 << 24) == -2
-    # 16-bit rows that need a workspace: too many, or of another type than the output.
-    need = lib.da_linear_int8_workspace_bytes(100, 8, F16C)
-    assert need > 0 and lib.da_linear_int8_workspace_bytes(100, 8, I8C) == 0
-    assert linear_with(_1=F16C, _2=8, _4=100) == -5 and linear_with(_1=F16C, _2=8, _4=100, _17=p, _18=need - 1) == -5
-    assert linear_with(_1=F16C, _2=8, _4=100, _17=p + 8, _18=need) == -3
+    # 16-bit rows that need a workspace: too many columns, or of another type than the output.
+    need = lib.da_linear_int8_workspace_bytes(100, 5000, 6, F16C, F16C)
+    assert need > 0 and lib.da_linear_int8_workspace_bytes(100, 5000, 6, I8C, F16C) == 0
+    wide = {"_1": F16C, "_2": 5000, "_4": 100, "_5": 5000, "_7": 5008}
+    assert linear_with(**wide) == -5 and linear_with(**wide, _17=p, _18=need - 1) == -5
+    assert linear_with(**wide, _17=p + 8, _18=need) == -3
     assert linear_with(_1=_lib.DA_BF16, _2=8) == -5
     assert lib.da_add_rms_norm(p, 8, None, 0, 2, 8, None, F32C, 0.0, F16C, None, p, None, 0, None, None) == -1
     assert lib.da_add_rms_norm(p, 8, None, 0, 2, 8, None, F32C, 1e-6, F16C, None, None, None, 0, None, None) == -1
