@@ -731,11 +731,13 @@ int validate_int8(const char* what, const char* name, const void* values, int64_
   return DA_OK;
 }
 
-int validate_sizes(const char* what, int64_t rows, int64_t cols, int64_t max_cols) {
+// A launch has fewer than 2^32 threads: rows in groups take 16 a group, rows
+// held whole up to 1024 (rms_norm.hip).
+int validate_sizes(const char* what, int64_t rows, int64_t cols, int64_t max_cols, bool grouped) {
   if (rows < 0 || cols < 1) return fail(DA_ERR_INVALID_ARGUMENT, "%s: needs rows >= 0 and at least one column", what);
   if (cols > max_cols) return fail(DA_ERR_UNSUPPORTED, "%s: rows of at most %lld columns", what, (long long)max_cols);
-  if (rows > 0x7fffffffLL || rows * ((cols + da::kInt8Group - 1) / da::kInt8Group) >= 0x7fff0000LL)
-    return fail(DA_ERR_UNSUPPORTED, "%s: too many rows", what);
+  const int64_t threads = grouped ? 16 * ((cols + da::kInt8Group - 1) / da::kInt8Group) : cols <= 1024 ? 64 : cols <= 8192 ? 256 : 1024;
+  if (rows > (0xffff0000LL - 1024) / threads) return fail(DA_ERR_UNSUPPORTED, "%s: too many rows", what);
   return DA_OK;
 }
 
@@ -748,7 +750,7 @@ int da_quantize_int8(const void* x, int64_t rows, int64_t cols, int64_t ldx, int
   if (!any_dtype(dtype)) return fail(DA_ERR_INVALID_ARGUMENT, "quantize: bad dtype");
   if (group != 0 && group != DA_INT8_GROUP)
     return fail(DA_ERR_UNSUPPORTED, "quantize: a scale for each row (0) or each %d columns", DA_INT8_GROUP);
-  int rc = validate_sizes("quantize", rows, cols, group ? kInt8MaxCols : da::kRowInt8MaxCols);
+  int rc = validate_sizes("quantize", rows, cols, group ? kInt8MaxCols : da::kRowInt8MaxCols, group != 0);
   if (rc) return rc;
   if (rows == 0) return ok();
   if ((rc = validate_rows("quantize", "x", x, cols, ldx, dtype))) return rc;
@@ -769,7 +771,7 @@ int da_dequantize_int8(const void* values, int64_t rows, int64_t cols, int64_t l
   if (!any_dtype(out_dtype)) return fail(DA_ERR_INVALID_ARGUMENT, "dequantize: bad dtype");
   if (group != 0 && group != DA_INT8_GROUP)
     return fail(DA_ERR_UNSUPPORTED, "dequantize: a scale for each row (0) or each %d columns", DA_INT8_GROUP);
-  int rc = validate_sizes("dequantize", rows, cols, kInt8MaxCols);
+  int rc = validate_sizes("dequantize", rows, cols, kInt8MaxCols, true);
   if (rc) return rc;
   if (rows == 0) return ok();
   if ((rc = validate_rows("dequantize", "out", out, cols, ldo, out_dtype))) return rc;
@@ -799,11 +801,11 @@ int da_linear_int8(const void* x, int x_dtype, int64_t ldx, const float* x_scale
   if (bias && !any_dtype(bias_dtype)) return fail(DA_ERR_INVALID_ARGUMENT, "linear_int8: bad bias dtype");
   if (bias && !aligned(bias, static_cast<int>(element_bytes(bias_dtype))))
     return fail(DA_ERR_ALIGNMENT, "linear_int8: the bias is not aligned to its elements");
-  int rc = validate_sizes("linear_int8", rows, in_features, da::kRowInt8MaxCols);
+  int rc = validate_sizes("linear_int8", rows, in_features, da::kRowInt8MaxCols, false);
   if (rc) return rc;
   if (out_features < 1 || out_features > (1 << 24) ||
-      ((rows + 63) / 64) * ((out_features + 63) / 64) > 0x7fff0000LL)
-    return fail(DA_ERR_UNSUPPORTED, "linear_int8: out_features must be in [1, 2^24], and the output's tiles below 2^31");
+      ((rows + 63) / 64) * ((out_features + 63) / 64) >= 1 << 23)
+    return fail(DA_ERR_UNSUPPORTED, "linear_int8: out_features must be in [1, 2^24], and the output's 64 x 64 tiles below 2^23");
   if (rows == 0) return ok();
   // 16-bit rows are quantized where they are multiplied, or into the workspace.
   const int64_t need = da_linear_int8_workspace_bytes(rows, in_features, out_features, x_dtype, dtype);
@@ -844,7 +846,7 @@ int validate_rms(const char* what, int64_t rows, int64_t dim, const void* weight
   if (!(eps > 0.f) || !std::isfinite(eps)) return fail(DA_ERR_INVALID_ARGUMENT, "%s: eps must be positive and finite", what);
   if (weight && !aligned(weight, static_cast<int>(element_bytes(param_dtype))))
     return fail(DA_ERR_ALIGNMENT, "%s: the weight is not aligned to its elements", what);
-  return validate_sizes(what, rows, dim, da::kRmsNormMaxDim);
+  return validate_sizes(what, rows, dim, da::kRmsNormMaxDim, false);
 }
 
 }  // namespace
@@ -904,7 +906,7 @@ int da_add_rms_norm_backward(const void* sum, int64_t ldsum, const void* grad, i
 int da_gelu_int8(const void* z, int64_t rows, int64_t cols, int64_t ldz, int dtype, void* out, void* values,
                  int64_t ldv, float* scales, da_stream_t stream) {
   if (!half_dtype(dtype)) return fail(DA_ERR_INVALID_ARGUMENT, "gelu_int8: dtype must be DA_F16 or DA_BF16");
-  int rc = validate_sizes("gelu_int8", rows, cols, kInt8MaxCols);
+  int rc = validate_sizes("gelu_int8", rows, cols, kInt8MaxCols, true);
   if (rc) return rc;
   if (rows == 0) return ok();
   if ((rc = validate_rows("gelu_int8", "z", z, cols, ldz, dtype))) return rc;
@@ -919,7 +921,7 @@ int da_gelu_int8(const void* z, int64_t rows, int64_t cols, int64_t ldz, int dty
 int da_gelu_int8_backward(const void* values, int64_t rows, int64_t cols, int64_t ldv, const float* scales,
                           const void* grad, int64_t ldg, int dtype, void* grad_z, void* out, da_stream_t stream) {
   if (!half_dtype(dtype)) return fail(DA_ERR_INVALID_ARGUMENT, "gelu_int8 backward: dtype must be DA_F16 or DA_BF16");
-  int rc = validate_sizes("gelu_int8 backward", rows, cols, kInt8MaxCols);
+  int rc = validate_sizes("gelu_int8 backward", rows, cols, kInt8MaxCols, true);
   if (rc) return rc;
   if (rows == 0) return ok();
   if ((rc = validate_rows("gelu_int8 backward", "grad", grad, cols, ldg, dtype))) return rc;

@@ -29,7 +29,9 @@ extern "C" {
  *
  * The 16-bit (and fp32) tensors of these operators are rows of any width at
  * any pitch >= that width, aligned to their elements.  No call reads or writes
- * outside of the rows it is given.
+ * outside of the rows it is given.  A launch takes fewer than 2^32 threads, 16
+ * for each group of a row, or 64, 256 or 1024 for a row held whole (up to 1024,
+ * 8192 and more columns); calls with more rows are refused (DA_ERR_UNSUPPORTED).
  */
 #define DA_INT8_GROUP 128
 #define DA_I8 3 /* dtype code of 8-bit rows with one scale each */
@@ -67,6 +69,7 @@ int da_linear_int8(const void* x, int x_dtype, int64_t ldx, const float* x_scale
  * Root-mean-square norm with the residual's addition in front of it:
  *   s = x + residual (rounded to dtype; residual NULL: s is x),
  *   n = s / sqrt(mean(s^2) + eps) * weight   over the last dimension, in fp32,
+ * (rows whose squares exceed fp32, |s| above about 1e19, have none),
  * n as out (rounded to dtype), as 8-bit rows with one scale each (values, ldv,
  * scales), or as both (out or values may be NULL, not both).  sum receives s
  * ([rows, dim] contiguous; required with a residual, not written without).

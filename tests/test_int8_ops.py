@@ -188,7 +188,8 @@ def check_linear(got, kept_x, kept_w, bias, gelu, residual, dtype):
     (33, 64, 257), (64, 1536, 512), (65, 100, 64), (127, 255, 127), (128, 256, 128), (129, 384, 129),
     (300, 1000, 1111), (513, 512, 1536), (1, 4096, 4096), (16, 4096, 1000), (48, 2048, 640), (4, 65536, 24),
     (700, 700, 3), (2000, 15, 300), (2100, 200, 1500), (1500, 130, 1900), (3000, 64, 2000), (4100, 333, 2500), (5000, 700, 4500),
-    (200, 512, 200), (130, 513, 70), (66, 1024, 65), (700, 900, 1500), (90, 1025, 64), (40, 1537, 40), (1100, 500, 1500), (4000, 33, 500),
+    (200, 512, 200), (130, 513, 70), (66, 1024, 65), (700, 900, 1500), (4000, 100, 4000), (4000, 200, 4000), (4000, 300, 4000), (3300, 50, 2100), (2000, 100, 1300), (2000, 200, 1300),
+    (90, 1025, 64), (40, 1537, 40), (1100, 500, 1500), (4000, 33, 500),
 ])
 def test_linear(rows, inner, outer, dtype) -> None:
     x = _randn(rows, inner, seed=rows, dtype=dtype)
@@ -533,6 +534,71 @@ def test_capture_other_streams_and_repeats() -> None:
         torch.cuda.synchronize()
 
 
+@pytest.mark.gpu
+def test_offsets_past_32_bits() -> None:
+    """Rows behind 2^32 elements (and bytes): the last ones of a long tensor."""
+
+    device = _device()
+    rows, width = 66000, 65536
+    x = torch.zeros(rows, width, dtype=torch.bfloat16, device=device)
+    tail = _randn(40, width, seed=1, dtype=torch.bfloat16)
+    x[-40:] = tail
+    for group in (None, 128):
+        kept = da.quantize_int8_hip(x, group)
+        want = da.quantize_int8_hip(tail, group)
+        assert torch.equal(kept.values[-40:], want.values) and torch.equal(kept.scales[-40:], want.scales)
+        assert not kept.values[:-40].any()
+        back = da.dequantize_int8_hip(kept)
+        assert torch.equal(back[-40:], da.dequantize_int8_hip(want)) and not back[:-40].any()
+        del back
+    x = x.view(-1, 16384)
+    n = x.shape[0]
+    out, total = da.add_rms_norm_hip(x, x)
+    assert n * 16384 > 1 << 32 and torch.equal(out[-160:], da.add_rms_norm_hip(x[-160:], x[-160:])[0])
+    dx, _ = da.add_rms_norm_backward_hip(total, x, None, None)
+    assert torch.equal(dx[-160:], da.add_rms_norm_backward_hip(total[-160:], x[-160:], None, None)[0])
+    del out, total, dx
+    u, kept = da.gelu_int8_hip(x)
+    assert torch.equal(u[-160:], da.gelu_int8_hip(x[-160:])[0])
+    dz, _ = da.gelu_int8_backward_hip(kept, x, want_output=False)
+    want_dz = da.gelu_int8_backward_hip(da.gelu_int8_hip(x[-160:])[1], x[-160:])[0]
+    assert torch.equal(dz[-160:], want_dz)
+    del u, kept, dz
+    # A linear layer whose output and tokens lie behind 2^32, from both sides.
+    wide = x.view(-1, 8192)[:, :64]
+    w = da.quantize_int8_hip(_randn(9000, 64, seed=2))
+    got = da.linear_int8_hip(wide, w)
+    assert got.numel() > 1 << 32
+    assert torch.equal(got[-300:], da.linear_int8_hip(wide[-300:], w)) and not got[:1000].any()
+
+
+def test_launch_on_another_device(monkeypatch) -> None:
+    """A launch switches to its tensors' device where another one is current."""
+
+    seen = []
+
+    class Switch:
+        def __init__(self, device):
+            self.device = device
+
+        def __enter__(self):
+            seen.append(("enter", self.device))
+
+        def __exit__(self, *_):
+            seen.append(("exit", self.device))
+
+    monkeypatch.setattr(int8_ops, "_current_device", lambda: 0)
+    monkeypatch.setattr(int8_ops, "_stream", lambda device: ("stream", device.index))
+    monkeypatch.setattr(torch.cuda, "device", Switch)
+    call = lambda *args: seen.append(args) or 0  # noqa: E731
+    int8_ops._launch("test", torch.device("cuda", 0), call, 1, 2)
+    assert seen == [(1, 2, ("stream", 0))]
+    seen.clear()
+    other = torch.device("cuda", 1)
+    int8_ops._launch("test", other, call, 3)
+    assert seen == [("enter", other), (3, ("stream", 1)), ("exit", other)]
+
+
 # ---- refusals ------------------------------------------------------------
 
 
@@ -613,7 +679,14 @@ def test_refusals_of_the_c_abi() -> None:
     assert lib.da_quantize_int8(p, 2, 8, 8, F16C, 0, p, 8, p, None) == -3
     assert lib.da_quantize_int8(p, 2, 24, 24, F16C, 0, p, 16, p, None) == -1
     assert lib.da_quantize_int8(p, 2, 8, 8, F16C, 0, p + 8, 16, p, None) == -3
-    assert lib.da_quantize_int8(p, 1 << 31, 8, 8, F16C, 128, p, 16, p, None) == -2
+    # Launches of 2^32 threads and more: 16 a group, 64 to 1024 a row.
+    assert lib.da_quantize_int8(p, 1 << 28, 8, 8, F16C, 128, p, 16, p, None) == -2
+    assert lib.da_quantize_int8(p, 1 << 26, 8, 8, F16C, 0, p, 16, p, None) == -2
+    assert lib.da_quantize_int8(p, 1 << 24, 2000, 2000, F16C, 0, p, 2000, p, None) == -2
+    assert lib.da_quantize_int8(p, 1 << 22, 20000, 20000, F16C, 0, p, 20000, p, None) == -2
+    assert lib.da_dequantize_int8(p, 1 << 27, 256, 256, p, 128, p, 256, F16C, None) == -2
+    assert lib.da_gelu_int8(p, 1 << 28, 8, 8, F16C, p, p, 16, p, None) == -2
+    assert lib.da_add_rms_norm(p, 8, None, 0, 1 << 26, 8, None, F32C, 1e-6, F16C, None, p, None, 0, None, None) == -2
     assert lib.da_dequantize_int8(p, 2, 8, 16, None, 0, p, 8, F32C, None) == -1
     assert lib.da_dequantize_int8(p, 2, 8, 16, p, 32, p, 8, F32C, None) == -2
     I8C = _lib.DA_I8
@@ -630,7 +703,7 @@ def test_refusals_of_the_c_abi() -> None:
     assert linear_with(_0=None) == -1 and linear_with(_8=None) == -1 and linear_with(_15=None) == -1
     assert linear_with(_3=None) == -1 and linear_with(_1=F32C) == -1 and linear_with(_7=(1 << 23) + 16) == -2
     assert linear_with(_10=p, _11=9) == -1 and linear_with(_10=p + 2) == -3 and linear_with(_13=p, _14=5) == -1
-    assert linear_with(_4=1 << 31) == -2 and linear_with(_4=1 << 22, _9=1 << 24) == -2
+    assert linear_with(_4=1 << 31) == -2 and linear_with(_4=1 << 18, _9=1 << 17) == -2
     # 16-bit rows that need a workspace: too many columns, or of another type than the output.
     need = lib.da_linear_int8_workspace_bytes(100, 5000, 6, F16C, F16C)
     assert need > 0 and lib.da_linear_int8_workspace_bytes(100, 5000, 6, I8C, F16C) == 0
