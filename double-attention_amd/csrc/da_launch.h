@@ -268,7 +268,7 @@ void launch_layer_norm_backward(const void* x, const void* dy, int64_t rows, int
 // values, scales), restored (values, scales -> out; row_scale: one scale a
 // row), GELU (x -> out, values, scales) and its backward (x is the gradient at
 // GELU's output, out the one at its input, again GELU's output or nullptr).
-// rows * ceil(cols / 128) < 2^31.  dtype: x, out and again (kF32 only for
+// rows * ceil(cols / 128) < 2^28.  dtype: x, out and again (kF32 only for
 // save and restore).
 struct Int8GroupArgs {
   const void* x;

@@ -95,7 +95,7 @@ __global__ __launch_bounds__(kGroupThreads) void int8_group_kernel(Int8GroupArgs
 template <typename T, int OP>
 static void launch_group(const Int8GroupArgs& a, hipStream_t stream) {
   const uint32_t groups = static_cast<uint32_t>((a.cols + kInt8Group - 1) / kInt8Group);
-  const uint32_t total = static_cast<uint32_t>(a.rows * groups);   // < 2^31 (checked by the caller)
+  const uint32_t total = static_cast<uint32_t>(a.rows * groups);   // < 2^28 (checked by the caller)
   constexpr uint32_t per = kGroupThreads / 16;
   hipLaunchKernelGGL((int8_group_kernel<T, OP>), dim3((total + per - 1) / per), dim3(kGroupThreads), 0, stream, a,
                      make_fast_div(groups), total);

@@ -22,8 +22,8 @@ constexpr float kInt8Least = 0x1p-126f;     // the least scale
 constexpr float kRoundMagic = 12582912.f;   // 1.5 * 2^23
 
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-// 16-byte and 8-byte chunks at any 2-byte (4-byte for fp32 rows) address: rows
-// of odd widths start there.  The hardware loads and stores them at full width.
+// 16-byte accesses at any 2-byte (4-byte for fp32 rows) address: rows of odd
+// widths start there, and the hardware takes such accesses whole.
 typedef u32x4 u32x4_any __attribute__((aligned(2)));
 
 __device__ __forceinline__ u32x4 load16B_any(const void* p) { return *static_cast<const u32x4_any*>(p); }
@@ -210,8 +210,8 @@ __device__ __forceinline__ void unpack_int8(u32x2 q, float scale, float (&v)[8])
   }
 }
 
-// Bytes of a chunk of n (<= 8) columns: whole 8-byte stores (the pitch is a
-// multiple of 16 and the columns behind the row are the storage's own).
+// A chunk's bytes, whole also where the row ends inside it: the pitch is a
+// multiple of 16, and the columns behind the row are the storage's own.
 __device__ __forceinline__ void store_bytes(int8_t* p, u32x2 q) { *reinterpret_cast<u32x2*>(p) = q; }
 __device__ __forceinline__ u32x2 load_bytes(const int8_t* p) { return *reinterpret_cast<const u32x2*>(p); }
 

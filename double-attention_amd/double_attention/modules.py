@@ -950,9 +950,10 @@ class DoubleAttentionBlock(nn.Module):
 
         Both linears' weights are quantized now, a scale for each output channel
         (``quantize_int8_hip``); activations are quantized for each token in
-        every forward.  Call it again after the weights change (a forward that
-        finds them changed in place raises ``RuntimeError``); ``enabled=False``
-        drops the 8-bit weights.  Forwards that autograd records, and those
+        every forward.  Call it again after the weights change: a forward that
+        finds them changed in place raises ``RuntimeError`` (writes through
+        ``.data`` and into a captured graph's weights are not seen);
+        ``enabled=False`` drops the 8-bit weights.  Forwards that autograd records, and those
         that do not run on the HIP kernels, use the full weights as before.
         """
 
@@ -983,6 +984,19 @@ class DoubleAttentionBlock(nn.Module):
         if (_version_of(first), _version_of(second)) != versions or w1.values.device != first.device:
             raise RuntimeError("the feed-forward's weights changed after quantize_feedforward(); call it again")
         return w1, w2
+
+    def _int8_inference(self, x: Tensor, attended: Tensor) -> tuple | None:
+        """The 8-bit weights, where a forward that does not run as one fused
+        block takes them: no autograd, and a feed-forward on the HIP kernels."""
+
+        if self._int8_feedforward is None or not self._hip_feedforward_applies(x, attended):
+            return None
+        if torch.is_grad_enabled() and any(
+            t.requires_grad
+            for t in (x, attended, *self.feedforward.parameters(), *self.feedforward_norm.parameters())
+        ):
+            return None
+        return self._int8_weights()
 
     def _feedforward_int8(self, x: Tensor, normalized, weights: tuple) -> Tensor:
         """``x + FFN`` on 8-bit integers; ``normalized`` a 16-bit tensor or 8-bit rows."""
@@ -1098,22 +1112,22 @@ class DoubleAttentionBlock(nn.Module):
             _layer_norm(self.attention_norm, x, backend), bank=bank, normalized_dictionary=normalized_dictionary
         )
         norm2 = self.feedforward_norm
+        weights = self._int8_inference(x, attended)
         if attended.dtype == x.dtype and _hip_rms_norm_applies(norm2, x, backend):
             # The residual's addition and the norm in one launch.
-            from .int8_ops import add_rms_norm_hip
+            from .int8_ops import add_rms_norm_hip, add_rms_norm_int8_hip
 
-            normalized_x, x = add_rms_norm_hip(attended, x, norm2.weight, norm2.eps)
+            add_norm = add_rms_norm_hip if weights is None else add_rms_norm_int8_hip
+            normalized_x, x = add_norm(attended, x, norm2.weight, norm2.eps)
         else:
             x = x + attended
             normalized_x = _layer_norm(norm2, x, backend)
+        if weights is not None:
+            return self._feedforward_int8(x, normalized_x, weights)
         if not self.attention.config.q_dictionary_feedforward:
             if self._hip_feedforward_applies(x, normalized_x):
                 first, second = self.feedforward[0], self.feedforward[2]
                 tensors = (x, normalized_x, first.weight, first.bias, second.weight, second.bias)
-                if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in tensors):
-                    weights = self._int8_weights()
-                    if weights is not None:
-                        return self._feedforward_int8(x, normalized_x, weights)
                 if self.activation_checkpoint == "int8":
                     return _HipFeedForwardInt8Function.apply(*tensors)
                 return _HipFeedForwardFunction.apply(*tensors)

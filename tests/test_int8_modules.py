@@ -183,6 +183,17 @@ def test_quantized_feedforward_without_output_projection() -> None:
         block.quantize_feedforward()
         got = block(x, bank)
         assert not torch.equal(got, full) and rel(got, full) < 4e-2
+        # The residual's addition, the norm and its integers in one call.
+        n1, n2 = block.attention_norm, block.feedforward_norm
+        attended = block.attention(da.add_rms_norm_hip(x, None, n1.weight, n1.eps)[0], bank=bank)
+        kept, s = da.add_rms_norm_int8_hip(attended, x, n2.weight, n2.eps)
+        first, second = block.feedforward[0], block.feedforward[2]
+        w1, w2 = da.quantize_int8_hip(first.weight), da.quantize_int8_hip(second.weight)
+        u = da.linear_int8_hip(kept, w1, first.bias, activation="gelu", dtype=torch.bfloat16)
+        assert torch.equal(got, da.linear_int8_hip(u, w2, second.bias, residual=s))
+    # Autograd takes the full weights there, too.
+    y = block(x, bank)
+    assert y.requires_grad and rel(y, full) < 2 * torch.finfo(torch.bfloat16).eps
 
 
 @pytest.mark.gpu

@@ -21,7 +21,7 @@ from double_attention import _lib, int8_ops
 
 HALF = [torch.bfloat16, torch.float16]
 F32 = 2.0 ** -24   # half a step of fp32
-WIDTHS = [1, 7, 8, 9, 127, 128, 129, 135, 512, 1001, 1536, 2049]
+WIDTHS = [1, 7, 8, 9, 127, 128, 129, 135, 505, 512, 1001, 1536, 2049]
 
 
 def _device() -> torch.device:
@@ -274,7 +274,7 @@ def norm64(s, w, eps):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", HALF)
-@pytest.mark.parametrize("width", [*WIDTHS, 1024, 4096, 8191, 16384])
+@pytest.mark.parametrize("width", [*WIDTHS, 1018, 1024, 4096, 8191, 16377, 16383, 16384])
 def test_add_rms_norm(width, dtype) -> None:
     for rows in (1, 6, 131):
         x = _randn(rows, width, seed=width, dtype=dtype)
@@ -330,7 +330,7 @@ def backward64(s, g, gs, w, eps):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", HALF)
-@pytest.mark.parametrize("width", [*WIDTHS, 1024, 4096, 8191, 16384])
+@pytest.mark.parametrize("width", [*WIDTHS, 1018, 1024, 4096, 8191, 16377, 16383, 16384])
 def test_add_rms_norm_backward(width, dtype) -> None:
     for rows in (1, 6, 700):
         s = _randn(rows, width, seed=width, dtype=dtype)
