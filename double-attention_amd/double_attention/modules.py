@@ -941,8 +941,8 @@ class DoubleAttentionBlock(nn.Module):
             nn.Linear(feedforward_dim, config.model_dim),
             nn.Dropout(dropout),
         )
-        # Set by quantize_feedforward: the two weights in 8 bits and the
-        # versions of the parameters that they were made from.
+        # Set by quantize_feedforward: the two weights in 8 bits, the
+        # parameters that they were made from and those parameters' versions.
         self._int8_feedforward: tuple | None = None
 
     def quantize_feedforward(self, enabled: bool = True) -> None:
@@ -951,10 +951,11 @@ class DoubleAttentionBlock(nn.Module):
         Both linears' weights are quantized now, a scale for each output channel
         (``quantize_int8_hip``); activations are quantized for each token in
         every forward.  Call it again after the weights change: a forward that
-        finds them changed in place raises ``RuntimeError`` (writes through
-        ``.data`` and into a captured graph's weights are not seen);
-        ``enabled=False`` drops the 8-bit weights.  Forwards that autograd records, and those
-        that do not run on the HIP kernels, use the full weights as before.
+        finds them replaced or changed in place raises ``RuntimeError`` (writes
+        through ``.data`` and into a captured graph's weights are not seen);
+        ``enabled=False`` drops the 8-bit weights.  Forwards that autograd
+        records, and those that do not run on the HIP kernels, use the full
+        weights as before.
         """
 
         if not enabled:
@@ -969,6 +970,7 @@ class DoubleAttentionBlock(nn.Module):
         with torch.no_grad():
             self._int8_feedforward = (
                 quantize_int8_hip(first.weight), quantize_int8_hip(second.weight),
+                (first.weight, second.weight),
                 (_version_of(first.weight), _version_of(second.weight)),
             )
 
@@ -979,9 +981,14 @@ class DoubleAttentionBlock(nn.Module):
             return None
         from .hip_ops import _version_of
 
-        w1, w2, versions = self._int8_feedforward
+        w1, w2, made_from, versions = self._int8_feedforward
         first, second = self.feedforward[0].weight, self.feedforward[2].weight
-        if (_version_of(first), _version_of(second)) != versions or w1.values.device != first.device:
+        if (
+            first is not made_from[0]
+            or second is not made_from[1]
+            or (_version_of(first), _version_of(second)) != versions
+            or w1.values.device != first.device
+        ):
             raise RuntimeError("the feed-forward's weights changed after quantize_feedforward(); call it again")
         return w1, w2
 

@@ -173,6 +173,28 @@ def test_quantized_feedforward(norm, dtype) -> None:
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("which", [0, 2])
+def test_quantized_feedforward_of_replaced_weights(which) -> None:
+    """A parameter put in a weight's place has the weight's version, not its values."""
+
+    block, bank = _block(torch.bfloat16)
+    x = _randn(2, 5, 128, seed=1, dtype=torch.bfloat16)
+    with torch.no_grad():
+        block.quantize_feedforward()
+        block(x, bank)
+        linear = block.feedforward[which]
+        kept = linear.weight
+        linear.weight = nn.Parameter(-kept)
+        while linear.weight._version < kept._version:
+            linear.weight.mul_(1.0)
+        assert linear.weight._version == kept._version
+        with pytest.raises(RuntimeError, match="quantize_feedforward"):
+            block(x, bank)
+        linear.weight = kept
+        block(x, bank)
+
+
+@pytest.mark.gpu
 def test_quantized_feedforward_without_output_projection() -> None:
     """The block that does not run as one fused forward takes the 8-bit weights, too."""
 
