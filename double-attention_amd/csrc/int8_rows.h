@@ -1,10 +1,11 @@
 // Device helpers of the 8-bit rows: signed integers from -127 to 127 with an
 // fp32 scale for each row, or for each 128 columns of a row.
 //
-//   scale = max(amax, 127 * 2^-126) / 127,   q = rint(x / scale)
+//   scale = max(amax, 127 * 2^-126) / 127,   q = round(x / scale)
 //
 // The floor on the scale keeps 1 / scale finite (an all-zero row has the
-// least scale and zeros).  A row (group) that holds an infinity or a NaN has
+// least scale and zeros).  Rows of 16-bit floats above that floor get the
+// integers nearest to 127 x / amax itself, halves away from zero.  A row (group) that holds an infinity or a NaN has
 // no such integers: its scale is NaN and its integers are 0, so that all of it
 // stands for NaN instead of for some finite numbers.
 #pragma once
@@ -174,18 +175,26 @@ __device__ __forceinline__ uint32_t wave_max_bits(uint32_t v) {
 }
 __device__ __forceinline__ float wave_sum_dpp(float v) { return group_sum(row16_sum(v)); }
 
+// 16-bit rows hold exact halves of their amax, 63.5 steps, and with the nearest
+// float to 1 / scale about half of the amax would round them down, half up.
+// Two units above it, a relative 2^-22 to 2^-21, cover the rounding of the
+// scale (1.5 * 2^-24 at most, 1 / 127 included) and of its inverse, so that every
+// half of a step rounds away from zero; no other quotient of two 16-bit floats is
+// within 2^-19 of a half: |254 x - (2 k + 1) amax| is at least a unit of x's
+// place, 2^-11 of x for fp16.
 struct Int8Scale {
   float scale;     // what a step of the integers stands for; NaN: the row has no integers
-  float inverse;   // 1 / scale, 0 where the scale is NaN
+  float inverse;   // 1 / scale and two units more, 0 where the scale is NaN
   uint32_t keep;   // all ones, 0 where the scale is NaN
 };
 __device__ __forceinline__ Int8Scale int8_scale(uint32_t amax_bits, float factor = 1.f) {
   const bool finite = amax_bits < 0x7f800000u;
   const float s = fmaxf(__uint_as_float(amax_bits) * factor * (1.f / 127.f), kInt8Least);
-  return Int8Scale{finite ? s : __uint_as_float(0x7fc00000u), finite ? 1.f / s : 0.f, finite ? 0xffffffffu : 0u};
+  const float inverse = __uint_as_float(__float_as_uint(1.f / s) + 2);
+  return Int8Scale{finite ? s : __uint_as_float(0x7fc00000u), finite ? inverse : 0.f, finite ? 0xffffffffu : 0u};
 }
 
-// Eight integers rint(v * inverse) as bytes.  |v * inverse| <= 127 (1 + 2^-22)
+// Eight integers rint(v * inverse) as bytes.  |v * inverse| <= 127 (1 + 2^-20)
 // by the choice of the scale, so rounding keeps them in [-127, 127].
 __device__ __forceinline__ u32x2 pack_int8(const float (&v)[8], float inverse, uint32_t keep) {
   uint32_t t[8];

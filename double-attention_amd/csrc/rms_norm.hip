@@ -8,7 +8,7 @@
 // One pass over memory: NT threads hold a row in registers (CH chunks of
 // eight columns each).  The scale of the integers needs no second reduction:
 // max |n| = rstd max |s w|, so the sum of squares and the largest |s w| are
-// reduced together, and q = rint(s w (rstd / scale)).
+// reduced together, and q = round(s w (rstd / scale)).
 //
 // Backward at dy = dL/dn and ds = dL/ds (the gradient that reaches s past the
 // norm), with xh = s rstd and g = dy w:

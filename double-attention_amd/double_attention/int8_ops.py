@@ -182,8 +182,8 @@ def quantize_int8_hip(x: Tensor, group: int | None = None) -> QuantizedRows:
     ``scale = max(amax, 127 * 2^-126) / 127`` over each row (``group`` None, up
     to 65536 columns: tokens and output channels of ``linear_int8_hip``) or
     each 128 columns of it (``INT8_GROUP``: saved activations), values
-    ``rint(x / scale)``.  A row (group) with an infinity or a NaN stands for
-    NaN throughout.
+    ``round(x / scale)``, halves away from zero.  A row (group) with an
+    infinity or a NaN stands for NaN throughout.
     """
 
     what = "quantize_int8_hip"

@@ -156,6 +156,48 @@ def test_quantize_values_out_of_the_ordinary(dtype, group) -> None:
     assert (back[0] == 0).all() and (back[6] == 0).all()
 
 
+def halves(rows, width, dtype):
+    """Rows with both halves of their largest magnitude, 63.5 steps but for the scale's rounding."""
+
+    x = _randn(rows, width, seed=5, dtype=dtype)
+    x[:, ::16] = x[:, 1::16] = 0
+    amax = x.abs().amax(-1, keepdim=True)
+    x[:, :1], x[:, 16::16], x[:, 1::16] = amax, amax / 2, -amax / 2
+    return x
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [*HALF, torch.float32])
+def test_quantize_rounds_to_the_nearest_step(dtype) -> None:
+    """16-bit rows get the integers nearest to 127 x / amax, halves away from zero."""
+
+    x = halves(300, 320, dtype)
+    x[200:] *= 2.0 ** -8
+    kinds = [da.quantize_int8_hip(x), da.quantize_int8_hip(x, 128)]
+    if dtype != torch.float32:
+        kinds.append(da.gelu_int8_hip(x)[1])
+    for kept in kinds:
+        values = kept.values.cpu().double()
+        parts = groups_of(x.cpu().double(), kept.group)
+        amax = parts.abs().amax(-1, keepdim=True)
+        # Sums and products of few bits: exact, and so is a quotient that is whole.
+        nearest = parts.sign() * torch.floor((254 * parts.abs() + amax) / (2 * amax))
+        nearest = nearest.flatten(-2)[:, :320]
+        if dtype == torch.float32:
+            # Other quotients may be as near to a half as fp32 resolves.
+            first = slice(16, 320 if kept.group is None else 128, 16)
+            assert torch.equal(values[:, first], nearest[:, first])
+            assert (values - nearest).abs().max().item() <= 1
+        else:
+            assert torch.equal(values, nearest)
+    if dtype != torch.float32:
+        # Tokens that are quantized where they are multiplied: few, and in tiles.
+        w = da.quantize_int8_hip(_randn(300, 320, seed=6))
+        for rows in (1, 16, 300):
+            kept = da.quantize_int8_hip(x[:rows])
+            assert torch.equal(da.linear_int8_hip(x[:rows], w), da.linear_int8_hip(kept, w, dtype=dtype))
+
+
 def linear64(kept_x, kept_w, bias, gelu):
     """The layer's result before its rounding, and the fp32 error bound."""
 
