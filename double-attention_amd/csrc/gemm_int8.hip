@@ -127,13 +127,23 @@ __device__ __forceinline__ void quantize_tokens(const LinearInt8Args& a, int64_t
       }
     }
     first_loads();
+    // Lane r forms row r's scale: a chain of some 40 instructions, once.
+    uint32_t mine = 0;
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
       uint32_t pair = 0;
 #pragma unroll
       for (int p = 0; p < PASSES; ++p) pair = max_pairs(raw[r][p], pair);
       const uint32_t largest = wave_max_bits(max(pair & 0xffffu, pair >> 16));
-      const Int8Scale s = int8_scale(magnitude_bits(half_value<T>(largest)));
+      mine = lane == r ? largest : mine;
+    }
+    const Int8Scale rows = int8_scale<T>(magnitude_bits(half_value<T>(mine)));
+    const uint64_t divide = __builtin_amdgcn_ballot_w64(rows.divide);
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      const auto of_row = [&](uint32_t v) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(v, r)); };
+      const Int8Scale s{__uint_as_float(of_row(__float_as_uint(rows.scale))), __uint_as_float(of_row(__float_as_uint(rows.inverse))),
+                        of_row(rows.keep), (divide >> r & 1) != 0};
       const int row = wave + r * Cfg::WAVES;
 #pragma unroll
       for (int p = 0; p < PASSES; ++p) {
@@ -142,13 +152,13 @@ __device__ __forceinline__ void quantize_tokens(const LinearInt8Args& a, int64_t
         float v[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = static_cast<float>(h[e]);
-        const u32x2 q = pack_int8(v, s.inverse, s.keep);
+        const u32x2 q = pack_int8<T>(v, s);
         const int st = k / kI8Stage;
         if (st < n_stages)
           *reinterpret_cast<u32x2*>(values + st * TileX::BYTES + TileX::offset(row, k % kI8Stage / 16) + k % 16) = q;
       }
-      if (lane == 0) scales[row] = s.scale;
     }
+    if (lane < ROWS) scales[wave + lane * Cfg::WAVES] = rows.scale;
   }
 }
 
@@ -513,7 +523,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_int8_few_kernel(LinearI
     amax = 0;
 #pragma unroll
     for (int v = 0; v < kFewWaves; ++v) amax = max(amax, largest[v][c]);
-    xs = int8_scale(amax);
+    xs = int8_scale<T>(amax);
     if (wave == 0 && g == 0) token_scale[c] = xs.scale;
   }
 
@@ -539,7 +549,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_int8_few_kernel(LinearI
           float v[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[e] = static_cast<float>(half[e]);
-          const u32x2 packed = pack_int8(v, xs.inverse, xs.keep);
+          const u32x2 packed = pack_int8<T>(v, xs);
           q[2 * h] = static_cast<int>(packed[0]);
           q[2 * h + 1] = static_cast<int>(packed[1]);
         }

@@ -58,9 +58,9 @@ __global__ __launch_bounds__(kGroupThreads) void int8_group_kernel(Int8GroupArgs
   if constexpr (OP == kOpSave || OP == kOpGelu) {
     const RawChunk<T> raw = fetch_chunk(x, n);
     chunk_floats(raw, x, n, v);
-    const Int8Scale s = int8_scale(group_amax(raw, n, v));
+    const Int8Scale s = int8_scale<T>(group_amax(raw, n, v));
     if (n > 0) {
-      store_bytes(values, pack_int8(v, s.inverse, s.keep));
+      store_bytes(values, pack_int8<T>(v, s));
       if (lane16 == 0) *scale = s.scale;
     }
     if constexpr (OP == kOpGelu) {

@@ -1,11 +1,10 @@
 // Device helpers of the 8-bit rows: signed integers from -127 to 127 with an
 // fp32 scale for each row, or for each 128 columns of a row.
 //
-//   scale = max(amax, 127 * 2^-126) / 127,   q = round(x / scale)
+//   scale = max(amax, 127 * 2^-126) / 127,   q = rint(x / scale)
 //
 // The floor on the scale keeps 1 / scale finite (an all-zero row has the
-// least scale and zeros).  Rows of 16-bit floats above that floor get the
-// integers nearest to 127 x / amax itself, halves away from zero.  A row (group) that holds an infinity or a NaN has
+// least scale and zeros).  A row (group) that holds an infinity or a NaN has
 // no such integers: its scale is NaN and its integers are 0, so that all of it
 // stands for NaN instead of for some finite numbers.
 #pragma once
@@ -175,31 +174,54 @@ __device__ __forceinline__ uint32_t wave_max_bits(uint32_t v) {
 }
 __device__ __forceinline__ float wave_sum_dpp(float v) { return group_sum(row16_sum(v)); }
 
-// 16-bit rows hold exact halves of their amax, 63.5 steps, and with the nearest
-// float to 1 / scale about half of the amax would round them down, half up.
-// Two units above it, a relative 2^-22 to 2^-21, cover the rounding of the
-// scale (1.5 * 2^-24 at most, 1 / 127 included) and of its inverse, so that every
-// half of a step rounds away from zero; no other quotient of two 16-bit floats is
-// within 2^-19 of a half: |254 x - (2 k + 1) amax| is at least a unit of x's
-// place, 2^-11 of x for fp16.
+// The integers are those of a plain fp32 division, rint(x / scale) with ties to
+// even, at the price of a multiplication.  x * inverse would do but for the
+// halves of a step, which roundings of the scale and of its inverse push either
+// way.  In a row of 16-bit floats (p = 8 or 11 bits) a quotient 127 x / amax is
+// such a half or at least 2^-19 of itself from one (|254 x - (2 k + 1) amax| is
+// a unit of x's place or more), so any inverse within some 2^-21 of 1 / scale
+// gives the others.  The halves are
+//   * amax / 2, 63.5 steps, in all rows: the inverse is set two units, more
+//     than both roundings together, to the side on which the division falls;
+//   * odd multiples of amax / 254 where 127 divides amax's p bits, so that
+//     the scale is exact: 254 for bf16, a power of two as a scale, where
+//     x * inverse is exact too; 127 j, j < 16, for fp16, where seven rows of
+//     1024 take the division's steps (fp32 rows take them all).
+// Checked against fp32 division for every pair of values up to 2^-11 of each
+// other.
+template <typename T> inline constexpr bool kInt8Divides = true;        // all of fp32's rows
+template <> inline constexpr bool kInt8Divides<__bf16> = false;
 struct Int8Scale {
   float scale;     // what a step of the integers stands for; NaN: the row has no integers
-  float inverse;   // 1 / scale and two units more, 0 where the scale is NaN
+  float inverse;   // 1 / scale, or two units beside it; 0 where the scale is NaN
   uint32_t keep;   // all ones, 0 where the scale is NaN
+  bool divide;     // the integers need the rounded quotient
 };
-__device__ __forceinline__ Int8Scale int8_scale(uint32_t amax_bits, float factor = 1.f) {
-  const bool finite = amax_bits < 0x7f800000u;
-  const float s = fmaxf(__uint_as_float(amax_bits) * factor * (1.f / 127.f), kInt8Least);
-  const float inverse = __uint_as_float(__float_as_uint(1.f / s) + 2);
-  return Int8Scale{finite ? s : __uint_as_float(0x7fc00000u), finite ? inverse : 0.f, finite ? 0xffffffffu : 0u};
+
+// v / scale as fp32 rounds it: one step of Newton's iteration on the product with
+// the rounded inverse (Markstein, "Computation of elementary functions on the
+// IBM RISC System/6000 processor", 1990).  The residual is exact in an FMA.
+__device__ __forceinline__ float quotient(float v, float scale, float inverse) {
+#pragma clang fp contract(off)
+  const float t = v * inverse;
+  return __builtin_fmaf(__builtin_fmaf(-t, scale, v), inverse, t);
 }
 
-// Eight integers rint(v * inverse) as bytes.  |v * inverse| <= 127 (1 + 2^-20)
-// by the choice of the scale, so rounding keeps them in [-127, 127].
-__device__ __forceinline__ u32x2 pack_int8(const float (&v)[8], float inverse, uint32_t keep) {
-  uint32_t t[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) t[e] = __float_as_uint(__builtin_fmaf(v[e], inverse, kRoundMagic));
+template <typename T>
+__device__ __forceinline__ Int8Scale int8_scale(uint32_t amax_bits, float factor = 1.f) {
+  const bool finite = amax_bits < 0x7f800000u;
+  const float amax = __uint_as_float(amax_bits) * factor;
+  const float s = fmaxf(amax * (1.f / 127.f), kInt8Least);
+  float inverse = 1.f / s;
+  const uint32_t mantissa = __float_as_uint(s) & 0x7fffffu;
+  const bool divide = kInt8Divides<T> && (sizeof(T) == 4 || (mantissa != 0 && (mantissa & 0xfffffu) == 0));
+  if (!divide && mantissa != 0)
+    inverse = __uint_as_float(__float_as_uint(inverse) + (quotient(0.5f * amax, s, inverse) >= 63.5f ? 2u : -2u));
+  return Int8Scale{finite ? s : __uint_as_float(0x7fc00000u), finite ? inverse : 0.f, finite ? 0xffffffffu : 0u, divide};
+}
+
+// Eight bytes of sums with kRoundMagic.
+__device__ __forceinline__ u32x2 pack_rounded(const uint32_t (&t)[8], uint32_t keep) {
   u32x2 r;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -208,6 +230,27 @@ __device__ __forceinline__ u32x2 pack_int8(const float (&v)[8], float inverse, u
     r[h] = (lo | hi) & keep;
   }
   return r;
+}
+
+// Eight integers rint(v * inverse) as bytes.  |v * inverse| <= 127 (1 + 2^-21)
+// by the choice of the scale, so rounding keeps them in [-127, 127].
+__device__ __forceinline__ u32x2 pack_int8(const float (&v)[8], float inverse, uint32_t keep) {
+  uint32_t t[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) t[e] = __float_as_uint(__builtin_fmaf(v[e], inverse, kRoundMagic));
+  return pack_rounded(t, keep);
+}
+
+// Eight elements of a row of T's in their row's scale.
+template <typename T>
+__device__ __forceinline__ u32x2 pack_int8(const float (&v)[8], const Int8Scale& s) {
+  if (kInt8Divides<T> && s.divide) {
+    uint32_t t[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) t[e] = __float_as_uint(quotient(v[e], s.scale, s.inverse) + kRoundMagic);
+    return pack_rounded(t, s.keep);
+  }
+  return pack_int8(v, s.inverse, s.keep);
 }
 
 // The eight floats that stored bytes stand for.

@@ -8,7 +8,7 @@
 // One pass over memory: NT threads hold a row in registers (CH chunks of
 // eight columns each).  The scale of the integers needs no second reduction:
 // max |n| = rstd max |s w|, so the sum of squares and the largest |s w| are
-// reduced together, and q = round(s w (rstd / scale)).
+// reduced together, and q = rint(s w (rstd / scale)).
 //
 // Backward at dy = dL/dn and ds = dL/ds (the gradient that reaches s past the
 // norm), with xh = s rstd and g = dy w:
@@ -128,14 +128,15 @@ __global__ __launch_bounds__(row_block<NT>()) void row_int8_kernel(RowInt8Args a
     }
     if (a.values == nullptr) return;
   }
-  const Int8Scale s = int8_scale(amax, rstd);
+  // The norm's values are no 16-bit floats: one rounding of x * inverse.
+  const Int8Scale s = NORM ? int8_scale<float>(amax, rstd) : int8_scale<T>(amax);
   // A row whose scale is the floor may have an inverse beyond fp32.
-  const float inverse = NORM ? fminf(rstd * s.inverse, 3.4028234e38f) : s.inverse;
+  const float inverse = fminf(rstd * s.inverse, 3.4028234e38f);
   int8_t* q = a.values + row * a.ldv;
 #pragma unroll
   for (int k = 0; k < CH; ++k) {
     const int c = (k * NT + t) * 8;
-    if (c < a.dim) store_bytes(q + c, pack_int8(v[k], inverse, s.keep));
+    if (c < a.dim) store_bytes(q + c, NORM ? pack_int8(v[k], inverse, s.keep) : pack_int8<T>(v[k], s));
   }
   if (t == 0) a.scales[row] = s.scale;
 }

@@ -182,8 +182,9 @@ def quantize_int8_hip(x: Tensor, group: int | None = None) -> QuantizedRows:
     ``scale = max(amax, 127 * 2^-126) / 127`` over each row (``group`` None, up
     to 65536 columns: tokens and output channels of ``linear_int8_hip``) or
     each 128 columns of it (``INT8_GROUP``: saved activations), values
-    ``round(x / scale)``, halves away from zero.  A row (group) with an
-    infinity or a NaN stands for NaN throughout.
+    ``round(x / scale)`` with fp32's division (the scale is amax times the fp32
+    number nearest to 1 / 127).  A row (group) with an infinity or a NaN stands
+    for NaN throughout.
     """
 
     what = "quantize_int8_hip"

@@ -20,9 +20,8 @@ extern "C" {
  * Rows in 8 bits.  A row of `cols` numbers is kept as signed integers with an
  * fp32 scale for the whole row (group 0) or for each 128 columns of it (group
  * 128, DA_INT8_GROUP; the last group may be shorter):
- *   scale = max(amax, 127 * 2^-126) / 127,  q = round(x / scale) in [-127, 127]
- * A half of a step rounds away from zero; for rows of 16-bit floats q is exactly
- * that rounding of 127 x / amax (fp32 rows: up to fp32's own roundings).
+ *   scale = max(amax, 127 * 2^-126) / 127,  q = rint(x / scale) in [-127, 127]
+ * with fp32's division and ties to even; scale is amax times fp32's 1 / 127.
  * A row (group) that holds an infinity or a NaN gets the scale NaN and zeros:
  * all of it then stands for NaN.  values: [rows] rows at a pitch ldv that is a
  * multiple of 16 (>= cols), 16-byte aligned; the bytes of a row's last chunk

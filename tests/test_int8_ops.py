@@ -168,28 +168,24 @@ def halves(rows, width, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [*HALF, torch.float32])
-def test_quantize_rounds_to_the_nearest_step(dtype) -> None:
-    """16-bit rows get the integers nearest to 127 x / amax, halves away from zero."""
+def test_quantize_rounds_the_quotient(dtype) -> None:
+    """The integers are those of fp32's division, ties to even, whatever forms them."""
 
     x = halves(300, 320, dtype)
     x[200:] *= 2.0 ** -8
+    # Scales without a rounding: every odd multiple of amax / 254 is half a step.
+    exact = torch.arange(-127, 128, dtype=torch.float64) / 127
+    for row, j in enumerate([1, 2, 3, 5, 7, 8, 9, 11, 13, 15] if dtype == torch.float16 else [1, 2]):
+        x[row] = 0
+        x[row, :255] = (127 * j * exact).to(dtype)
+        x[row, 256:290] = torch.arange(34, dtype=dtype) * (j / 2)
+        x[row, 290] = -127 * j
     kinds = [da.quantize_int8_hip(x), da.quantize_int8_hip(x, 128)]
     if dtype != torch.float32:
         kinds.append(da.gelu_int8_hip(x)[1])
     for kept in kinds:
-        values = kept.values.cpu().double()
-        parts = groups_of(x.cpu().double(), kept.group)
-        amax = parts.abs().amax(-1, keepdim=True)
-        # Sums and products of few bits: exact, and so is a quotient that is whole.
-        nearest = parts.sign() * torch.floor((254 * parts.abs() + amax) / (2 * amax))
-        nearest = nearest.flatten(-2)[:, :320]
-        if dtype == torch.float32:
-            # Other quotients may be as near to a half as fp32 resolves.
-            first = slice(16, 320 if kept.group is None else 128, 16)
-            assert torch.equal(values[:, first], nearest[:, first])
-            assert (values - nearest).abs().max().item() <= 1
-        else:
-            assert torch.equal(values, nearest)
+        scales = kept.scales.cpu().repeat_interleave(128 if kept.group else 320, 1)[:, :320]
+        assert torch.equal(kept.values.cpu().float(), torch.round(x.cpu().float() / scales))
     if dtype != torch.float32:
         # Tokens that are quantized where they are multiplied: few, and in tiles.
         w = da.quantize_int8_hip(_randn(300, 320, seed=6))
