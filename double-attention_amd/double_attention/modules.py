@@ -6,7 +6,8 @@ unchanged, and a seeded construction consumes the RNG in the same order, so
 default-initialized weights are identical.  The HIP forward
 (``SharedDictionaryAttention._hip_forward``) replaces the projection,
 route, outer attention and map combine with one C call into the gfx950
-library; LayerNorm, FFN, embeddings and the LM head stay PyTorch ops.
+library; in the blocks the norms and the feed-forward run on its kernels too
+(optionally on 8-bit integers), and embeddings and the LM head stay PyTorch ops.
 """
 
 from __future__ import annotations
