@@ -102,6 +102,32 @@ __device__ __forceinline__ void i8_tile(int t, int tiles_i, int tiles_j, int& ti
   tj = r / wide;
 }
 
+// The scales of a wave's rows, lane r's of row r: a chain of some 40
+// instructions, formed once instead of for each row.  `largest`: 16-bit
+// magnitudes.
+template <typename T>
+struct LaneScales {
+  Int8Scale own;
+  uint64_t divide;
+  __device__ __forceinline__ explicit LaneScales(uint32_t largest)
+      : own(int8_scale<T>(magnitude_bits(half_value<T>(largest)))), divide(__builtin_amdgcn_ballot_w64(own.divide)) {}
+  __device__ __forceinline__ Int8Scale of(int r) const {
+    const auto lane_r = [&](uint32_t v) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(v, r)); };
+    return Int8Scale{__uint_as_float(lane_r(__float_as_uint(own.scale))), __uint_as_float(lane_r(__float_as_uint(own.inverse))),
+                     lane_r(own.keep), (divide >> r & 1) != 0};
+  }
+};
+
+// Eight 16-bit floats as they were loaded, in their row's scale.
+template <typename T>
+__device__ __forceinline__ u32x2 pack_bits(u32x4 bits, const Int8Scale& s) {
+  const typename Elem<T>::v8 h = __builtin_bit_cast(typename Elem<T>::v8, bits);
+  float v[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = static_cast<float>(h[e]);
+  return pack_int8<T>(v, s);
+}
+
 // The tokens' 8-bit rows in LDS, in the layout of their stages (XS > 0; zeros
 // behind K), and their scales.  A wave takes every WAVES-th row, its lanes eight
 // columns each of 512 at a time; W's first stages (`first_loads`) are asked for
@@ -127,7 +153,6 @@ __device__ __forceinline__ void quantize_tokens(const LinearInt8Args& a, int64_t
       }
     }
     first_loads();
-    // Lane r forms row r's scale: a chain of some 40 instructions, once.
     uint32_t mine = 0;
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
@@ -137,28 +162,20 @@ __device__ __forceinline__ void quantize_tokens(const LinearInt8Args& a, int64_t
       const uint32_t largest = wave_max_bits(max(pair & 0xffffu, pair >> 16));
       mine = lane == r ? largest : mine;
     }
-    const Int8Scale rows = int8_scale<T>(magnitude_bits(half_value<T>(mine)));
-    const uint64_t divide = __builtin_amdgcn_ballot_w64(rows.divide);
+    const LaneScales<T> rows(mine);
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
-      const auto of_row = [&](uint32_t v) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(v, r)); };
-      const Int8Scale s{__uint_as_float(of_row(__float_as_uint(rows.scale))), __uint_as_float(of_row(__float_as_uint(rows.inverse))),
-                        of_row(rows.keep), (divide >> r & 1) != 0};
+      const Int8Scale s = rows.of(r);
       const int row = wave + r * Cfg::WAVES;
 #pragma unroll
       for (int p = 0; p < PASSES; ++p) {
-        const int k = p * 512 + lane * 8;
-        const typename Elem<T>::v8 h = __builtin_bit_cast(typename Elem<T>::v8, raw[r][p]);
-        float v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = static_cast<float>(h[e]);
-        const u32x2 q = pack_int8<T>(v, s);
-        const int st = k / kI8Stage;
+        const int k = p * 512 + lane * 8, st = k / kI8Stage;
+        const u32x2 q = pack_bits<T>(raw[r][p], s);
         if (st < n_stages)
           *reinterpret_cast<u32x2*>(values + st * TileX::BYTES + TileX::offset(row, k % kI8Stage / 16) + k % 16) = q;
       }
     }
-    if (lane < ROWS) scales[wave + lane * Cfg::WAVES] = rows.scale;
+    if (lane < ROWS) scales[wave + lane * Cfg::WAVES] = rows.own.scale;
   }
 }
 
@@ -423,27 +440,25 @@ __global__ __launch_bounds__(64 * Cfg::WAVES) void linear_int8_kernel(LinearInt8
 // row's whole 128-byte line), straight from memory into MFMA fragments, eight
 // steps in flight.  Their integer sums meet in LDS (in any order: they are
 // exact).  With 16-bit tokens (XT = T, MT = 1) each workgroup quantizes them
-// itself instead of waiting for another launch: the waves' largest magnitudes
-// meet in LDS, then the integers of a step are formed where they are
-// multiplied, from the registers that hold K's one batch of steps.
+// itself instead of waiting for another launch: a wave takes two tokens whole,
+// in loads of 1 KiB, and leaves their integers in LDS (16 x 4096 -> 4096 9.2 us, 1
+// x 4096 -> 16384 16.3; 10.6 and 26.6 where each wave read the tokens' fragments
+// and quantized all 16 rows of its steps; 6.9 and 15 for 8-bit tokens).
 constexpr int kFewWaves = 8;
 constexpr int kFewBatch = 8;    // steps of a wave in flight
-// Calls whose tokens are quantized in the kernel: one tile of tokens, one batch.
+// Calls whose tokens are quantized in the kernel: one tile of tokens, 64 KiB of LDS.
 constexpr int kFewRows = 16, kFewCols = 64 * kFewWaves * kFewBatch;
-
-// The 16 elements of a step's chunk as they lie in memory.
-template <typename T>
-struct RawStep {
-  u32x4 d[2];
-};
 
 template <typename T, typename XT, int MT, int EPI>
 __global__ __launch_bounds__(64 * kFewWaves) void linear_int8_few_kernel(LinearInt8Args a) {
   constexpr bool QUANT = sizeof(XT) == 2;
   static_assert(!QUANT || MT == 1, "one tile of tokens is quantized here");
   __shared__ __attribute__((aligned(16))) int part[kFewWaves][MT * 256];
-  __shared__ uint32_t largest[kFewWaves][16];
-  __shared__ float token_scale[16];
+  // The tokens' integers, at a pitch that puts a step's 16 rows into 16 different
+  // groups of banks.
+  constexpr int PITCH = kFewCols + 16, TOKENS = kFewRows / kFewWaves, PASSES = kFewCols / 512;
+  __shared__ __attribute__((aligned(16))) char integers[QUANT ? kFewRows * PITCH : 16];
+  __shared__ float token_scale[kFewRows];
   const int lane = lane_id();
   const int c = lane & 15;
   const int g = lane >> 4;
@@ -457,13 +472,15 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_int8_few_kernel(LinearI
 #pragma unroll
   for (int m = 0; m < MT; ++m)
     x[m] = static_cast<const XT*>(a.x) + min(static_cast<int64_t>(m * 16 + c), a.rows - 1) * a.ldx;
+  // This wave's 16-bit tokens.
+  u32x4 raw[TOKENS][PASSES];
+  auto token_of = [&](int r) { return wave + r * kFewWaves; };
   // The u-th step of this wave's batch that starts at step s0.
   auto step_of = [&](int s0, int u) { return s0 + (u >> 1) * (2 * kFewWaves) + 2 * wave + (u & 1); };
   constexpr int BATCH = kFewWaves * kFewBatch;   // steps of a batch, over the waves
 
-  // A batch's weights, and its tokens: raw 16-bit chunks or 8-bit fragments.
+  // A batch's weights and 8-bit tokens.
   i32x4 wf[kFewBatch];
-  RawStep<T> raw[QUANT ? kFewBatch : 1];
   i32x4 xf[QUANT ? 1 : kFewBatch][MT];
   auto fetch_w = [&](int s0) {
 #pragma unroll
@@ -473,23 +490,28 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_int8_few_kernel(LinearI
     }
   };
   auto fetch_x = [&](int s0) {
+    if constexpr (QUANT) {
 #pragma unroll
-    for (int u = 0; u < kFewBatch; ++u) {
-      const int s = step_of(s0, u);
-      const int k = s * 64 + g * 16;
-      if (s < steps) {
-        if constexpr (QUANT) {
-          raw[u].d[0] = fetch_bits(x[0] + k, K - k);
-          raw[u].d[1] = fetch_bits(x[0] + k + 8, K - k - 8);
-        } else {
+      for (int r = 0; r < TOKENS; ++r) {
+        if (token_of(r) >= a.rows) continue;
+        const T* token = static_cast<const T*>(a.x) + token_of(r) * a.ldx;
 #pragma unroll
-          for (int m = 0; m < MT; ++m) xf[u][m] = *reinterpret_cast<const i32x4*>(x[m] + min(k, last_chunk));
+        for (int p = 0; p < PASSES; ++p) {
+          const int k = p * 512 + lane * 8;
+          if (p * 512 < K) raw[r][p] = fetch_bits(token + k, K - k);
         }
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < kFewBatch; ++u) {
+        const int s = step_of(s0, u);
+        if (s >= steps) continue;
+#pragma unroll
+        for (int m = 0; m < MT; ++m) xf[u][m] = *reinterpret_cast<const i32x4*>(x[m] + min(s * 64 + g * 16, last_chunk));
       }
     }
   };
 
-  Int8Scale xs{1.f, 1.f, 0xffffffffu};
   fetch_x(0);
   fetch_w(0);   // on their way while the tokens are quantized
 
@@ -509,22 +531,36 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_int8_few_kernel(LinearI
     if constexpr ((EPI & 2) != 0) res[o] = static_cast<float>(static_cast<const T*>(a.residual)[j * a.ldr + i]);
   }
   if constexpr (QUANT) {
-    uint32_t pair = 0;
+    const int tokens = wave >= a.rows ? 0 : wave + kFewWaves < a.rows ? 2 : 1;
+    static_assert(TOKENS == 2, "two tokens a wave");
+    uint32_t mine = 0;
 #pragma unroll
-    for (int u = 0; u < kFewBatch; ++u)
-      if (step_of(0, u) < steps) pair = max_pairs(raw[u].d[1], max_pairs(raw[u].d[0], pair));
-    uint32_t amax = magnitude_bits(half_value<T>(max(pair & 0xffffu, pair >> 16)));
-    const auto p = __builtin_amdgcn_permlane32_swap(amax, amax, false, false);
-    amax = max(p[0], p[1]);
-    const auto r = __builtin_amdgcn_permlane16_swap(amax, amax, false, false);
-    amax = max(r[0], r[1]);
-    if (g == 0) largest[wave][c] = amax;
+    for (int r = 0; r < TOKENS; ++r) {
+      if (r >= tokens) continue;
+      uint32_t pair = 0;
+#pragma unroll
+      for (int p = 0; p < PASSES; ++p)
+        if (p * 512 < K) pair = max_pairs(raw[r][p], pair);
+      const uint32_t largest = wave_max_bits(max(pair & 0xffffu, pair >> 16));
+      mine = lane == r ? largest : mine;
+    }
+    if (tokens > 0) {
+      const LaneScales<T> scales(mine);
+#pragma unroll
+      for (int r = 0; r < TOKENS; ++r) {
+        if (r >= tokens) continue;
+        const Int8Scale s = scales.of(r);
+        char* const row = integers + token_of(r) * PITCH;
+#pragma unroll
+        for (int p = 0; p < PASSES; ++p) {
+          const int k = p * 512 + lane * 8;
+          if (p * 512 >= K) continue;   // the whole wave: a shorter loop
+          if (k < K) *reinterpret_cast<u32x2*>(row + k) = pack_bits<T>(raw[r][p], s);
+        }
+      }
+      if (lane < tokens) token_scale[token_of(lane)] = scales.own.scale;
+    }
     __syncthreads();
-    amax = 0;
-#pragma unroll
-    for (int v = 0; v < kFewWaves; ++v) amax = max(amax, largest[v][c]);
-    xs = int8_scale<T>(amax);
-    if (wave == 0 && g == 0) token_scale[c] = xs.scale;
   }
 
   i32x4 acc[MT];
@@ -542,17 +578,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_int8_few_kernel(LinearI
       const int k = s * 64 + g * 16;
       if (s * 64 + 64 > K) wf[u] = first_bytes(wf[u], K - k);
       if constexpr (QUANT) {
-        i32x4 q;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const typename Elem<T>::v8 half = __builtin_bit_cast(typename Elem<T>::v8, raw[u].d[h]);
-          float v[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = static_cast<float>(half[e]);
-          const u32x2 packed = pack_int8<T>(v, xs);
-          q[2 * h] = static_cast<int>(packed[0]);
-          q[2 * h + 1] = static_cast<int>(packed[1]);
-        }
+        const i32x4 q = *reinterpret_cast<const i32x4*>(integers + c * PITCH + k);
         acc[0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[u], q, acc[0], 0, 0, 0);
       } else {
 #pragma unroll
