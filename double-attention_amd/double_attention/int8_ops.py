@@ -110,16 +110,18 @@ def _no_grad(what: str, *tensors: Tensor | None) -> None:
 
 
 def _rows(t: Tensor) -> tuple[Tensor, int]:
-    """``t`` as ``[rows, columns]`` with unit column stride, and its row pitch.
+    """``t``'s rows in memory, with unit column stride, and their pitch.
 
-    Rows at any pitch are read where they are; other orders are copied."""
+    Rows at any pitch are read where they are (as ``[rows, columns]``; a
+    contiguous tensor keeps its shape); other orders are copied."""
 
-    shape = t.shape
-    columns = shape[-1]
-    if len(shape) != 2:
-        t = t.reshape(-1, columns)
+    columns = t.shape[-1]
     if t.is_contiguous():
         return t, columns
+    if t.ndim != 2:
+        t = t.reshape(-1, columns)
+        if t.is_contiguous():
+            return t, columns
     rows = t.shape[0]
     if columns > 1 and t.stride(1) != 1:
         t = t.contiguous()
@@ -140,10 +142,11 @@ def _values_rows(t: Tensor) -> tuple[Tensor, int]:
     """8-bit rows as the kernels read them: 16-byte aligned at a pitch of a
     multiple of 16, with the last row's last 16 bytes inside the storage."""
 
+    columns = t.shape[-1]
+    if not (columns | t.data_ptr()) & 15 and t.is_contiguous():
+        return t, columns
+    rows = t.numel() // columns
     t, pitch = _rows(t)
-    rows, columns = t.shape
-    if pitch == columns and not (columns | t.data_ptr()) & 15:
-        return t, pitch
     if rows == 1:
         pitch = (columns + 15) // 16 * 16
     fits = pitch % 16 == 0 and t.data_ptr() % 16 == 0
@@ -151,8 +154,8 @@ def _values_rows(t: Tensor) -> tuple[Tensor, int]:
         last = t.storage_offset() + (rows - 1) * pitch + (columns + 15) // 16 * 16
         fits = last <= t.untyped_storage().nbytes()
     if not fits:
-        padded, pitch = _new_values(t.shape[:1], columns, t.device)
-        padded.copy_(t)
+        padded, pitch = _new_values((rows,), columns, t.device)
+        padded.copy_(t.reshape(rows, columns))
         t = padded
     return t, pitch
 
@@ -197,7 +200,7 @@ def quantize_int8_hip(x: Tensor, group: int | None = None) -> QuantizedRows:
     values, ldv = _new_values(lead, columns, device)
     groups = 1 if group is None else -(-columns // INT8_GROUP)
     scales = torch.empty(*lead, groups, dtype=_FLOAT32, device=device)
-    _launch(what, device, _lib.get().da_quantize_int8, rows.data_ptr(), rows.shape[0], columns, pitch, code, group or 0,
+    _launch(what, device, _lib.get().da_quantize_int8, rows.data_ptr(), x.numel() // columns, columns, pitch, code, group or 0,
             values.data_ptr(), ldv, scales.data_ptr())
     return QuantizedRows(values, scales, group)
 
@@ -210,11 +213,11 @@ def dequantize_int8_hip(rows: QuantizedRows, dtype: torch.dtype = torch.bfloat16
     values, scales, group = rows
     code = dtype_code(dtype)
     device = values.device
-    out = torch.empty(values.shape, dtype=dtype, device=device)
+    out = torch.empty(*values.shape, dtype=dtype, device=device)
     values, pitch = _values_rows(values)
     scales = scales.contiguous()
-    columns = values.shape[1]
-    _launch(what, device, _lib.get().da_dequantize_int8, values.data_ptr(), values.shape[0], columns, pitch,
+    columns = values.shape[-1]
+    _launch(what, device, _lib.get().da_dequantize_int8, values.data_ptr(), values.numel() // columns, columns, pitch,
             scales.data_ptr(), group or 0, out.data_ptr(), columns, code)
     return out
 
@@ -286,9 +289,10 @@ def linear_int8_hip(
     w, ldw = _values_rows(w)
     w_scales = w_scales.contiguous()
     scales_ptr, workspace_ptr, nbytes = None, None, 0
+    tokens = x.numel() // in_features
     if x_scales is None:
         rows, ldx = _rows(x)
-        nbytes = lib.da_linear_int8_workspace_bytes(rows.shape[0], in_features, out_features, x_code, code)
+        nbytes = lib.da_linear_int8_workspace_bytes(tokens, in_features, out_features, x_code, code)
         if nbytes:
             workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
             workspace_ptr = workspace.data_ptr()
@@ -296,8 +300,8 @@ def linear_int8_hip(
         rows, ldx = _values_rows(x)
         x_scales = x_scales.contiguous()
         scales_ptr = x_scales.data_ptr()
-    out = torch.empty(out_shape, dtype=dtype, device=device)
-    _launch(what, device, lib.da_linear_int8, rows.data_ptr(), x_code, ldx, scales_ptr, rows.shape[0], in_features,
+    out = torch.empty(*out_shape, dtype=dtype, device=device)
+    _launch(what, device, lib.da_linear_int8, rows.data_ptr(), x_code, ldx, scales_ptr, tokens, in_features,
             w.data_ptr(), ldw, w_scales.data_ptr(), out_features, bias_ptr, bias_code,
             _lib.DA_ACT_GELU if activation else _lib.DA_ACT_NONE, res_ptr, ldr, out.data_ptr(), code, workspace_ptr, nbytes)
     return out
@@ -313,7 +317,7 @@ def _add_rms_norm(what, x, residual, weight, eps, want_out, want_int8):
         _check_like(what, x, residual)
         residual, ldr = _rows(residual)
         res_ptr = residual.data_ptr()
-        total = torch.empty(shape, dtype=dtype, device=device)
+        total = torch.empty(*shape, dtype=dtype, device=device)
         total_ptr = total.data_ptr()
     weight_ptr, weight_code = None, _lib.DA_F32
     if weight is not None:
@@ -323,13 +327,13 @@ def _add_rms_norm(what, x, residual, weight, eps, want_out, want_int8):
     out = values = scales = out_ptr = values_ptr = scales_ptr = None
     ldv = 0
     if want_out:
-        out = torch.empty(shape, dtype=dtype, device=device)
+        out = torch.empty(*shape, dtype=dtype, device=device)
         out_ptr = out.data_ptr()
     if want_int8:
         values, ldv = _new_values(lead, width, device)
         scales = torch.empty(*lead, 1, dtype=_FLOAT32, device=device)
         values_ptr, scales_ptr = values.data_ptr(), scales.data_ptr()
-    _launch(what, device, _lib.get().da_add_rms_norm, rows.data_ptr(), ldx, res_ptr, ldr, rows.shape[0], width, weight_ptr,
+    _launch(what, device, _lib.get().da_add_rms_norm, rows.data_ptr(), ldx, res_ptr, ldr, x.numel() // width, width, weight_ptr,
             weight_code, float(eps), code, total_ptr, out_ptr, values_ptr, ldv, scales_ptr)
     return out, values, scales, total
 
@@ -409,6 +413,7 @@ def add_rms_norm_backward_hip(
     _check_like(what, total, grad)
     shape, device = total.shape, total.device
     width = shape[-1]
+    count = total.numel() // width
     lib = _lib.get()
     s, lds = _rows(total)
     g, ldg = _rows(grad)
@@ -417,7 +422,7 @@ def add_rms_norm_backward_hip(
         _check_like(what, total, grad_sum)
         grad_sum, ldgs = _rows(grad_sum)
         gs_ptr = grad_sum.data_ptr()
-    grad_x = torch.empty(shape, dtype=total.dtype, device=device)
+    grad_x = torch.empty(*shape, dtype=total.dtype, device=device)
     weight_ptr, weight_code = None, _lib.DA_F32
     grad_weight = grad_weight_ptr = workspace_ptr = None
     nbytes = 0
@@ -428,10 +433,10 @@ def add_rms_norm_backward_hip(
         if want_weight:
             grad_weight = torch.empty(width, dtype=weight.dtype, device=device)
             grad_weight_ptr = grad_weight.data_ptr()
-            nbytes = lib.da_add_rms_norm_backward_workspace_bytes(s.shape[0], width)
+            nbytes = lib.da_add_rms_norm_backward_workspace_bytes(count, width)
             workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
             workspace_ptr = workspace.data_ptr()
-    _launch(what, device, lib.da_add_rms_norm_backward, s.data_ptr(), lds, g.data_ptr(), ldg, gs_ptr, ldgs, s.shape[0],
+    _launch(what, device, lib.da_add_rms_norm_backward, s.data_ptr(), lds, g.data_ptr(), ldg, gs_ptr, ldgs, count,
             width, weight_ptr, weight_code, float(eps), code, grad_x.data_ptr(), grad_weight_ptr, workspace_ptr, nbytes)
     return grad_x, grad_weight
 
@@ -447,10 +452,10 @@ def gelu_int8_hip(z: Tensor) -> tuple[Tensor, QuantizedRows]:
     shape, device = z.shape, z.device
     *lead, columns = shape
     rows, pitch = _rows(z)
-    out = torch.empty(shape, dtype=z.dtype, device=device)
+    out = torch.empty(*shape, dtype=z.dtype, device=device)
     values, ldv = _new_values(lead, columns, device)
     scales = torch.empty(*lead, -(-columns // INT8_GROUP), dtype=_FLOAT32, device=device)
-    _launch(what, device, _lib.get().da_gelu_int8, rows.data_ptr(), rows.shape[0], columns, pitch, code, out.data_ptr(),
+    _launch(what, device, _lib.get().da_gelu_int8, rows.data_ptr(), z.numel() // columns, columns, pitch, code, out.data_ptr(),
             values.data_ptr(), ldv, scales.data_ptr())
     return out, QuantizedRows(values, scales, INT8_GROUP)
 
@@ -473,8 +478,9 @@ def gelu_int8_backward_hip(kept: QuantizedRows, grad: Tensor, *, want_output: bo
     values, ldv = _values_rows(values)
     scales = scales.contiguous()
     g, ldg = _rows(grad)
-    grad_z = torch.empty(shape, dtype=grad.dtype, device=device)
-    out = torch.empty(shape, dtype=grad.dtype, device=device) if want_output else None
-    _launch(what, device, _lib.get().da_gelu_int8_backward, values.data_ptr(), values.shape[0], values.shape[1], ldv,
+    grad_z = torch.empty(*shape, dtype=grad.dtype, device=device)
+    out = torch.empty(*shape, dtype=grad.dtype, device=device) if want_output else None
+    columns = shape[-1]
+    _launch(what, device, _lib.get().da_gelu_int8_backward, values.data_ptr(), values.numel() // columns, columns, ldv,
             scales.data_ptr(), g.data_ptr(), ldg, code, grad_z.data_ptr(), None if out is None else out.data_ptr())
     return grad_z, out
