@@ -248,6 +248,51 @@ def test_linear(rows, inner, outer, dtype) -> None:
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("inner", [8, 511, 513, 1024, 2047, 2049, 3583, 4095])
+@pytest.mark.parametrize("rows", [1, 7, 8, 9, 15, 16])
+def test_linear_few_tokens_of_any_width(rows, inner, dtype) -> None:
+    """One or two tokens a wave, whole and partial passes over them."""
+
+    x = _randn(rows + 3, inner + 5, seed=inner + rows, dtype=dtype)[2:-1, 3:-2]
+    w = da.quantize_int8_hip(_randn(37, inner, seed=1, spread=inner ** -0.5))
+    kept = da.quantize_int8_hip(x)
+    got = da.linear_int8_hip(x, w)
+    check_linear(got, kept, w, None, False, None, dtype)
+    assert torch.equal(got, da.linear_int8_hip(kept, w, dtype=dtype))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("width", [70, 96, 200])
+def test_rows_of_three_dimensions(width) -> None:
+    """The rows of [a, b, width] tensors are those of [a b, width] ones."""
+
+    x = _randn(3, 5, width, seed=1, dtype=torch.bfloat16)
+    flat = x.view(15, width)
+    weight = _randn(width, seed=2, dtype=torch.bfloat16)
+    w = da.quantize_int8_hip(_randn(24, width, seed=3))
+    for group in (None, 128):
+        kept, same = da.quantize_int8_hip(x, group), da.quantize_int8_hip(flat, group)
+        assert torch.equal(kept.values.flatten(0, 1), same.values) and torch.equal(kept.scales.flatten(0, 1), same.scales)
+        assert torch.equal(da.dequantize_int8_hip(kept).flatten(0, 1), da.dequantize_int8_hip(same))
+        turned = da.QuantizedRows(kept.values.transpose(0, 1), kept.scales.transpose(0, 1), group)
+        assert torch.equal(da.dequantize_int8_hip(turned), da.dequantize_int8_hip(kept).transpose(0, 1))
+        if group is None:
+            assert torch.equal(da.linear_int8_hip(kept, w).flatten(0, 1), da.linear_int8_hip(same, w))
+            assert torch.equal(da.linear_int8_hip(turned, w), da.linear_int8_hip(kept, w).transpose(0, 1))
+        else:
+            for a, b in zip(da.gelu_int8_backward_hip(kept, x), da.gelu_int8_backward_hip(same, flat)):
+                assert torch.equal(a.flatten(0, 1), b)
+    for a, b in zip(da.add_rms_norm_hip(x, x, weight), da.add_rms_norm_hip(flat, flat, weight)):
+        assert torch.equal(a.flatten(0, 1), b)
+    a, b = (da.add_rms_norm_backward_hip(t, t, t, weight) for t in (x, flat))
+    assert torch.equal(a[0].flatten(0, 1), b[0]) and torch.equal(a[1], b[1])
+    a, b = da.add_rms_norm_backward_hip(x.transpose(0, 1), x.transpose(0, 1), None, weight), da.add_rms_norm_backward_hip(
+        x.transpose(0, 1).contiguous(), x.transpose(0, 1).contiguous(), None, weight)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize(("rows", "inner", "outer"), [(1, 70, 90), (40, 70, 90), (200, 200, 300), (2100, 1100, 1300)])
 def test_linear_any_bytes(rows, inner, outer) -> None:
     """Integers of the whole range, -128 too, and anything behind the rows' columns."""
