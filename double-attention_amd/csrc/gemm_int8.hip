@@ -392,7 +392,7 @@ __global__ __launch_bounds__(64 * Cfg::WAVES) void linear_int8_kernel(LinearInt8
 #pragma unroll
       for (int pass = 0; pass < PASSES; ++pass) {
         const int64_t j = j0 + wj * Cfg::WJ + q * 16 + pass * ROWS + lane / CHUNKS;
-        if (j < a.rows) res[q][pass] = fetch_chunk(static_cast<const T*>(a.residual) + j * a.ldr + i, n);
+        if (j < a.rows) res[q][pass] = fetch_chunk(static_cast<const T*>(a.residual) + j * a.ldr + i, n, a.N >= 8);
       }
   }
 #pragma unroll
@@ -419,7 +419,7 @@ __global__ __launch_bounds__(64 * Cfg::WAVES) void linear_int8_kernel(LinearInt8
       const typename Elem<T>::v8 e8 = __builtin_bit_cast(typename Elem<T>::v8, v);
       if constexpr ((EPI & 2) != 0) {
         float r[8];
-        chunk_floats(res[q][pass], static_cast<const T*>(a.residual) + j * a.ldr + i, n, r);
+        chunk_floats(res[q][pass], static_cast<const T*>(a.residual) + j * a.ldr + i, n, a.N >= 8, r);
 #pragma unroll
         for (int e = 0; e < 8; ++e) r[e] += static_cast<float>(e8[e]);
         store_chunk(dst, n, r);

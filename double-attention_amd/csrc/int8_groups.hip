@@ -50,14 +50,15 @@ __global__ __launch_bounds__(kGroupThreads) void int8_group_kernel(Int8GroupArgs
   const uint32_t g = id - static_cast<uint32_t>(row) * groups.d;
   const int col = static_cast<int>(g) * kInt8Group + lane16 * 8;
   const int n = id < total ? min(a.cols - col, 8) : 0;   // columns of this chunk
+  const bool wide = a.cols >= 8;
   const T* x = static_cast<const T*>(a.x) + row * a.ldx + col;
   T* out = static_cast<T*>(a.out) + row * a.ldo + col;
   int8_t* values = a.values + row * a.ldv + col;
   float* scale = a.scales + (a.row_scale ? row : row * groups.d + g);
   float v[8], o[8];
   if constexpr (OP == kOpSave || OP == kOpGelu) {
-    const RawChunk<T> raw = fetch_chunk(x, n);
-    chunk_floats(raw, x, n, v);
+    const RawChunk<T> raw = fetch_chunk(x, n, wide);
+    chunk_floats(raw, x, n, wide, v);
     const Int8Scale s = int8_scale<T>(group_amax(raw, n, v));
     if (n > 0) {
       store_bytes(values, pack_int8<T>(v, s));
@@ -77,7 +78,7 @@ __global__ __launch_bounds__(kGroupThreads) void int8_group_kernel(Int8GroupArgs
       store_chunk(out, n, o);
     } else {
       float d[8];
-      chunk_floats(fetch_chunk(x, n), x, n, d);
+      chunk_floats(fetch_chunk(x, n, wide), x, n, wide, d);
       unpack_int8(bytes, step, v);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {

@@ -56,37 +56,56 @@ __device__ __forceinline__ void load_chunk(const T* p, int n, float (&v)[8]) {
 }
 
 // Raw loads of a chunk, kept apart from their use so that all of a thread's are
-// in flight before the first is waited for.
+// in flight before the first is waited for.  A row's last, partial chunk is read
+// as the row's last eight elements (`wide`: rows of eight columns or more) and
+// moved into place when it is used: no load waits for another, or for a branch.
 template <typename T>
 struct RawChunk {
   u32x4 lo, hi;
 };
 
 template <typename T>
-__device__ __forceinline__ RawChunk<T> fetch_chunk(const T* p, int n) {
+__device__ __forceinline__ RawChunk<T> fetch_chunk(const T* p, int n, bool wide) {
   RawChunk<T> r{u32x4{0, 0, 0, 0}, u32x4{0, 0, 0, 0}};
-  if (n >= 8) {
+  if (n > (wide ? 0 : 7)) {
+    p += min(n - 8, 0);
     r.lo = load16B_any(p);
     if constexpr (sizeof(T) == 4) r.hi = load16B_any(p + 4);
   }
   return r;
 }
 
-// The chunk's floats; a row's last, partial chunk is read here.
+// The chunk's floats.
 template <typename T>
-__device__ __forceinline__ void chunk_floats(const RawChunk<T>& r, const T* p, int n, float (&v)[8]) {
+__device__ __forceinline__ void chunk_floats(const RawChunk<T>& r, const T* p, int n, bool wide, float (&v)[8]) {
   if constexpr (sizeof(T) == 4) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       v[e] = __uint_as_float(r.lo[e]);
       v[e + 4] = __uint_as_float(r.hi[e]);
     }
+    if (wide && n > 0 && n < 8) {
+#pragma unroll
+      for (int step = 4; step; step /= 2)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = (8 - n) & step ? (e + step < 8 ? v[e + step] : 0.f) : v[e];
+    }
   } else {
-    const typename Elem<T>::v8 a = __builtin_bit_cast(typename Elem<T>::v8, r.lo);
+    u32x4 d = r.lo;
+    if (wide && n > 0 && n < 8) {
+      // Elements 8 - n and up, moved down: a shift of 128 bits.
+      const uint64_t lo = static_cast<uint64_t>(d[1]) << 32 | d[0], hi = static_cast<uint64_t>(d[3]) << 32 | d[2];
+      const int shift = 16 * (8 - n);   // 16 to 112
+      const uint64_t top = hi >> (shift & 63);
+      const uint64_t low = shift >= 64 ? top : lo >> (shift & 63) | hi << (-shift & 63);
+      const uint64_t high = shift >= 64 ? 0 : top;
+      d = u32x4{static_cast<uint32_t>(low), static_cast<uint32_t>(low >> 32), static_cast<uint32_t>(high), static_cast<uint32_t>(high >> 32)};
+    }
+    const typename Elem<T>::v8 a = __builtin_bit_cast(typename Elem<T>::v8, d);
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = static_cast<float>(a[e]);
   }
-  if (n > 0 && n < 8) load_chunk(p, n, v);
+  if (!wide && n > 0 && n < 8) load_chunk(p, n, v);
 }
 
 template <typename T>

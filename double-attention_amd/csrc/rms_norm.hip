@@ -23,18 +23,32 @@
 namespace da {
 
 // Eight parameters of type pdt from column c on, of which n exist (1 without
-// parameters, 0 behind the row).
-__device__ __forceinline__ void load_weight8(const void* p, int pdt, int64_t c, int n, float (&w)[8]) {
+// parameters, 0 behind the row), fetched and used as a chunk of a row is.
+__device__ __forceinline__ RawChunk<float> fetch_weight(const void* p, int pdt, int64_t c, int n, bool wide) {
+  if (p == nullptr) return RawChunk<float>{u32x4{0, 0, 0, 0}, u32x4{0, 0, 0, 0}};
+  if (pdt == kF32) return fetch_chunk(static_cast<const float*>(p) + c, n, wide);
+  return RawChunk<float>{fetch_chunk(static_cast<const _Float16*>(p) + c, n, wide).lo, u32x4{0, 0, 0, 0}};
+}
+__device__ __forceinline__ void weight_floats(const RawChunk<float>& r, const void* p, int pdt, int64_t c, int n, bool wide,
+                                              float (&w)[8]) {
   if (p == nullptr) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) w[e] = 1.f;
   } else if (pdt == kF32) {
-    load_chunk(static_cast<const float*>(p) + c, n, w);
+    chunk_floats(r, static_cast<const float*>(p) + c, n, wide, w);
   } else if (pdt == kF16) {
-    load_chunk(static_cast<const _Float16*>(p) + c, n, w);
+    chunk_floats(RawChunk<_Float16>{r.lo, r.hi}, static_cast<const _Float16*>(p) + c, n, wide, w);
   } else {
-    load_chunk(static_cast<const __bf16*>(p) + c, n, w);
+    chunk_floats(RawChunk<__bf16>{r.lo, r.hi}, static_cast<const __bf16*>(p) + c, n, wide, w);
   }
+}
+
+// Elements of a row from column c on, of which a chunk takes at most 8.  Rows of
+// whole chunks (TAIL false) have kernels without the code for partial ones (4096 x
+// 8192: forward 43 us against 52, backward 49 against 58).
+template <bool TAIL>
+__device__ __forceinline__ int row_left(int dim, int c) {
+  return TAIL ? dim - c : c < dim ? 8 : 0;
 }
 
 // The row's sum and largest magnitude over its NT threads.
@@ -62,7 +76,7 @@ __device__ __forceinline__ void row_reduce(float& sum, uint32_t& amax, float* ld
 template <int NT>
 constexpr int row_block() { return NT < 256 ? 256 : NT; }
 
-template <typename T, int NT, int CH, bool NORM>
+template <typename T, int NT, int CH, bool NORM, bool TAIL>
 __global__ __launch_bounds__(row_block<NT>()) void row_int8_kernel(RowInt8Args a) {
   __shared__ float lds[2 * (NT / 64)];
   constexpr int ROWS = row_block<NT>() / NT;
@@ -70,34 +84,44 @@ __global__ __launch_bounds__(row_block<NT>()) void row_int8_kernel(RowInt8Args a
   const int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / NT;
   if (row >= a.rows) return;   // whole waves of a workgroup without barriers (NT == 64)
   const T* x = static_cast<const T*>(a.x) + row * a.ldx;
+  const T* r = static_cast<const T*>(a.residual) + row * a.ldr;
+  const bool wide = !TAIL || a.dim >= 8;
+  auto left = [&](int c) { return row_left<TAIL>(a.dim, c); };
+  RawChunk<T> rx[CH], rr[CH];
+  RawChunk<float> rw[CH];
+#pragma unroll
+  for (int k = 0; k < CH; ++k) rx[k] = fetch_chunk(x + (k * NT + t) * 8, left((k * NT + t) * 8), wide);
+  if constexpr (NORM) {
+    if (a.residual != nullptr) {
+#pragma unroll
+      for (int k = 0; k < CH; ++k) rr[k] = fetch_chunk(r + (k * NT + t) * 8, left((k * NT + t) * 8), wide);
+    }
+#pragma unroll
+    for (int k = 0; k < CH; ++k) rw[k] = fetch_weight(a.weight, a.param_dtype, (k * NT + t) * 8, left((k * NT + t) * 8), wide);
+  }
   float v[CH][8], w[CH][8];
 #pragma unroll
   for (int k = 0; k < CH; ++k) {
     const int c = (k * NT + t) * 8;
-    load_chunk(x + c, a.dim - c, v[k]);
+    chunk_floats(rx[k], x + c, left(c), wide, v[k]);
   }
   float sum = 0.f;
   uint32_t amax = 0;
   if constexpr (NORM) {
     if (a.residual != nullptr) {
-      const T* r = static_cast<const T*>(a.residual) + row * a.ldr;
 #pragma unroll
       for (int k = 0; k < CH; ++k) {
         const int c = (k * NT + t) * 8;
-        load_chunk(r + c, a.dim - c, w[k]);
-      }
-#pragma unroll
-      for (int k = 0; k < CH; ++k) {
-        const int c = (k * NT + t) * 8;
+        chunk_floats(rr[k], r + c, left(c), wide, w[k]);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[k][e] = static_cast<float>(static_cast<T>(v[k][e] + w[k][e]));
-        store_chunk(static_cast<T*>(a.sum) + row * a.dim + c, a.dim - c, v[k]);
+        store_chunk(static_cast<T*>(a.sum) + row * a.dim + c, left(c), v[k]);
       }
     }
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
       const int c = (k * NT + t) * 8;
-      load_weight8(a.weight, a.param_dtype, c, a.dim - c, w[k]);
+      weight_floats(rw[k], a.weight, a.param_dtype, c, left(c), wide, w[k]);
     }
 #pragma unroll
     for (int k = 0; k < CH; ++k)
@@ -123,7 +147,7 @@ __global__ __launch_bounds__(row_block<NT>()) void row_int8_kernel(RowInt8Args a
         float o[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) o[e] = v[k][e] * rstd;
-        store_chunk(out + c, a.dim - c, o);
+        store_chunk(out + c, left(c), o);
       }
     }
     if (a.values == nullptr) return;
@@ -143,17 +167,26 @@ __global__ __launch_bounds__(row_block<NT>()) void row_int8_kernel(RowInt8Args a
 
 // Rows blockIdx.x, blockIdx.x + gridDim.x, ... of ROWS each.  `partials`
 // [gridDim.x][dim]: the workgroup's share of the weight's gradient.
-template <typename T, int NT, int CH>
-__global__ __launch_bounds__(row_block<NT>()) void rms_norm_backward_kernel(RmsNormBackwardArgs a) {
-  constexpr int ROWS = row_block<NT>() / NT;
+template <int NT>
+constexpr int backward_block() { return NT == 64 ? 512 : NT; }
+
+template <typename T, int NT, int CH, bool TAIL>
+__global__ __launch_bounds__(backward_block<NT>()) void rms_norm_backward_kernel(RmsNormBackwardArgs a) {
+  constexpr int ROWS = backward_block<NT>() / NT;
   // Row reductions (two sets of slots), or the sums of waves that hold a row each.
   extern __shared__ __attribute__((aligned(16))) float lds[];
   const int t = static_cast<int>(threadIdx.x) % NT;
+  // A row's loads are issued while the row before it is reduced (the widest
+  // rows take the registers for that, and for moving a partial chunk, themselves).
+  constexpr bool EARLY = NT * CH <= 1024;
+  const bool wide = EARLY && (!TAIL || a.dim >= 8);
+  auto left = [&](int c) { return row_left<TAIL>(a.dim, c); };
+  RawChunk<float> rw[CH];
   float w[CH][8], gw[CH][8];
 #pragma unroll
   for (int k = 0; k < CH; ++k) {
     const int c = (k * NT + t) * 8;
-    load_weight8(a.weight, a.param_dtype, c, a.dim - c, w[k]);
+    rw[k] = fetch_weight(a.weight, a.param_dtype, c, left(c), wide);
 #pragma unroll
     for (int e = 0; e < 8; ++e) gw[k][e] = 0.f;
   }
@@ -163,32 +196,39 @@ __global__ __launch_bounds__(row_block<NT>()) void rms_norm_backward_kernel(RmsN
   const T* const sum = static_cast<const T*>(a.sum);
   const T* const grad = static_cast<const T*>(a.grad);
   const T* const grad_sum = static_cast<const T*>(a.grad_sum);
-  // A row's loads are issued while the row before it is reduced (the widest
-  // rows take the registers for that themselves).
-  constexpr bool EARLY = NT < 512;
   RawChunk<T> rv[CH], rg[CH], rs[CH];
   auto fetch_row = [&](int64_t r) {
     if (r >= a.rows) return;
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
       const int c = (k * NT + t) * 8;
-      rv[k] = fetch_chunk(sum + r * a.ldsum + c, a.dim - c);
-      rg[k] = fetch_chunk(grad + r * a.ldg + c, a.dim - c);
-      if (grad_sum != nullptr) rs[k] = fetch_chunk(grad_sum + r * a.ldgs + c, a.dim - c);
+      rv[k] = fetch_chunk(sum + r * a.ldsum + c, left(c), wide);
+      rg[k] = fetch_chunk(grad + r * a.ldg + c, left(c), wide);
+      if (grad_sum != nullptr) rs[k] = fetch_chunk(grad_sum + r * a.ldgs + c, left(c), wide);
     }
   };
   if constexpr (EARLY) fetch_row(row);
+#pragma unroll
+  for (int k = 0; k < CH; ++k) {
+    const int c = (k * NT + t) * 8;
+    weight_floats(rw[k], a.weight, a.param_dtype, c, left(c), wide, w[k]);
+  }
   int turn = 0;
   for (; row < a.rows; row += step, turn ^= 1) {
     if constexpr (!EARLY) fetch_row(row);
+    // The masks of a wide row's last, partial chunk are formed again for each row:
+    // kept over the loop they take more registers than there are.
+    int dim = a.dim;
+    if constexpr (TAIL && EARLY && NT >= 512) asm volatile("" : "+s"(dim));
+    auto left_here = [&](int c) { return row_left<TAIL>(dim, c); };
     float v[CH][8], g[CH][8], d[CH][8];
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
       const int c = (k * NT + t) * 8;
-      chunk_floats(rv[k], sum + row * a.ldsum + c, a.dim - c, v[k]);
-      chunk_floats(rg[k], grad + row * a.ldg + c, a.dim - c, g[k]);
+      chunk_floats(rv[k], sum + row * a.ldsum + c, left_here(c), wide, v[k]);
+      chunk_floats(rg[k], grad + row * a.ldg + c, left_here(c), wide, g[k]);
       if (grad_sum != nullptr) {
-        chunk_floats(rs[k], grad_sum + row * a.ldgs + c, a.dim - c, d[k]);
+        chunk_floats(rs[k], grad_sum + row * a.ldgs + c, left_here(c), wide, d[k]);
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e) d[k][e] = 0.f;
@@ -233,7 +273,7 @@ __global__ __launch_bounds__(row_block<NT>()) void rms_norm_backward_kernel(RmsN
         gw[k][e] = __builtin_fmaf(g[k][e], v[k][e] * rstd, gw[k][e]);
         d[k][e] += rstd * (g[k][e] * w[k][e] - v[k][e] * mean);
       }
-      store_chunk(static_cast<T*>(a.grad_x) + row * a.dim + c, a.dim - c, d[k]);
+      store_chunk(static_cast<T*>(a.grad_x) + row * a.dim + c, left_here(c), d[k]);
     }
   }
   if (a.partials == nullptr) return;
@@ -242,7 +282,7 @@ __global__ __launch_bounds__(row_block<NT>()) void rms_norm_backward_kernel(RmsN
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
       const int c = (k * NT + t) * 8;
-      store_chunk(part + c, a.dim - c, gw[k]);
+      store_chunk(part + c, left(c), gw[k]);
     }
   } else {
     // The waves' sums side by side in LDS, then added in the waves' order.
@@ -253,7 +293,7 @@ __global__ __launch_bounds__(row_block<NT>()) void rms_norm_backward_kernel(RmsN
       *reinterpret_cast<f32x4*>(at + 4) = f32x4{gw[k][4], gw[k][5], gw[k][6], gw[k][7]};
     }
     __syncthreads();
-    for (int c = static_cast<int>(threadIdx.x); c < a.dim; c += row_block<NT>()) {
+    for (int c = static_cast<int>(threadIdx.x); c < a.dim; c += backward_block<NT>()) {
       float sum = lds[c];
 #pragma unroll
       for (int q = 1; q < ROWS; ++q) sum += lds[q * CH * 512 + c];
@@ -294,8 +334,9 @@ __global__ __launch_bounds__(kSumCols * kSumRuns) void rms_norm_weight_kernel(co
 template <typename T, int NT, int CH, bool NORM>
 static void launch_row_k(const RowInt8Args& a, hipStream_t stream) {
   constexpr int ROWS = row_block<NT>() / NT;
-  hipLaunchKernelGGL((row_int8_kernel<T, NT, CH, NORM>), dim3(static_cast<unsigned>((a.rows + ROWS - 1) / ROWS)),
-                     dim3(row_block<NT>()), 0, stream, a);
+  const dim3 grid(static_cast<unsigned>((a.rows + ROWS - 1) / ROWS)), block(row_block<NT>());
+  if (a.dim % 8) hipLaunchKernelGGL((row_int8_kernel<T, NT, CH, NORM, true>), grid, block, 0, stream, a);
+  else hipLaunchKernelGGL((row_int8_kernel<T, NT, CH, NORM, false>), grid, block, 0, stream, a);
 }
 
 template <typename T, bool NORM>
@@ -325,20 +366,23 @@ void launch_row_int8(const RowInt8Args& a, bool norm, hipStream_t stream) {
   }
 }
 
-// Two workgroups a CU: with half of them the rows' loads do not fill the
-// memory's queues (16384 x 2048 49 us against 65), with twice as many the
-// partial sums cost more than that gains (55 us).
+// Eight waves a CU, in one workgroup where a wave holds a row (half the partial
+// sums of two workgroups: 3885 x 1001 11.2 us and 2.8 for the sums against 11.7
+// and 3.9), else in two of four (or of eight, over 4096 columns).  16384 x 2048 with
+// two took 49 us, with one 65 (the rows' loads do not fill the memory's queues),
+// with four 55 (the partial sums).
 int rms_norm_backward_blocks(int64_t rows, int dim) {
-  const int64_t per = dim <= 1024 ? 4 : 1;
+  const int64_t per = dim <= 1024 ? 8 : 1, most = dim <= 1024 ? 256 : 512;
   const int64_t blocks = (rows + per - 1) / per;
-  return static_cast<int>(blocks < 512 ? blocks : 512);
+  return static_cast<int>(blocks < most ? blocks : most);
 }
 
 template <typename T, int NT, int CH>
 static void launch_backward_k(const RmsNormBackwardArgs& a, hipStream_t stream) {
-  const size_t lds = NT > 64 ? 4 * (NT / 64) * sizeof(float) : 4 * CH * 512 * sizeof(float);
-  hipLaunchKernelGGL((rms_norm_backward_kernel<T, NT, CH>), dim3(rms_norm_backward_blocks(a.rows, a.dim)),
-                     dim3(row_block<NT>()), lds, stream, a);
+  const size_t lds = NT > 64 ? 4 * (NT / 64) * sizeof(float) : backward_block<NT>() / NT * CH * 512 * sizeof(float);
+  const dim3 grid(rms_norm_backward_blocks(a.rows, a.dim)), block(backward_block<NT>());
+  if (a.dim % 8) hipLaunchKernelGGL((rms_norm_backward_kernel<T, NT, CH, true>), grid, block, lds, stream, a);
+  else hipLaunchKernelGGL((rms_norm_backward_kernel<T, NT, CH, false>), grid, block, lds, stream, a);
 }
 
 template <typename T>
@@ -347,7 +391,7 @@ static void launch_backward_t(const RmsNormBackwardArgs& a, hipStream_t stream) 
   else if (a.dim <= 1024) launch_backward_k<T, 64, 2>(a, stream);
   else if (a.dim <= 2048) launch_backward_k<T, 256, 1>(a, stream);
   else if (a.dim <= 4096) launch_backward_k<T, 256, 2>(a, stream);
-  else if (a.dim <= 8192) launch_backward_k<T, 256, 4>(a, stream);
+  else if (a.dim <= 8192) launch_backward_k<T, 512, 2>(a, stream);
   else launch_backward_k<T, 512, 4>(a, stream);
 }
 
