@@ -143,16 +143,23 @@ __device__ __forceinline__ void quantize_tokens(const LinearInt8Args& a, int64_t
     float* const scales = reinterpret_cast<float*>(values + Cfg::kXS * TileX::BYTES);
     const int lane = lane_id(), wave = uniform_wave();
     u32x4 raw[ROWS][PASSES];
+    const bool wide = a.K >= 8;
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
       const T* x = static_cast<const T*>(a.x) + min(j0 + wave + r * Cfg::WAVES, a.rows - 1) * a.ldx;
 #pragma unroll
       for (int p = 0; p < PASSES; ++p) {
         const int k = p * 512 + lane * 8;
-        raw[r][p] = fetch_bits(x + k, a.K - k);
+        raw[r][p] = fetch_bits(x + k, a.K - k, wide);
       }
     }
     first_loads();
+    if (a.K % 8) {
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+        for (int p = 0; p < PASSES; ++p) raw[r][p] = chunk_bits(raw[r][p], a.K - p * 512 - lane * 8, wide);
+    }
     uint32_t mine = 0;
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
@@ -498,7 +505,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_int8_few_kernel(LinearI
 #pragma unroll
         for (int p = 0; p < PASSES; ++p) {
           const int k = p * 512 + lane * 8;
-          if (p * 512 < K) raw[r][p] = fetch_bits(token + k, K - k);
+          if (p * 512 < K) raw[r][p] = fetch_bits(token + k, K - k, K >= 8);
         }
       }
     } else {
@@ -537,6 +544,10 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_int8_few_kernel(LinearI
 #pragma unroll
     for (int r = 0; r < TOKENS; ++r) {
       if (r >= tokens) continue;
+      if (K % 8) {
+#pragma unroll
+        for (int p = 0; p < PASSES; ++p) raw[r][p] = chunk_bits(raw[r][p], K - p * 512 - lane * 8, K >= 8);
+      }
       uint32_t pair = 0;
 #pragma unroll
       for (int p = 0; p < PASSES; ++p)
@@ -637,7 +648,7 @@ static I8Plan plan_linear_int8(int64_t rows, int64_t K, int64_t N, bool quantize
   // 16-bit tokens are quantized again by every workgroup that multiplies them:
   // as fast as a launch of its own for that, or nearly, while the workgroups
   // are one round (4096 x 512 -> 512 7.6 against 8.6, 1024 x 512 -> 1536 7.4
-  // against 7.6, 64 x 512 -> 1536 6.3 against 6.3, 777 x 1000 -> 1111 10.5 against
+  // against 7.6, 64 x 512 -> 1536 6.3 against 6.3, 777 x 1000 -> 1111 9.8 against
   // 9.2), and the call has one launch less, 3 us of the host's time.  Beyond, it is
   // not (4096 x 512 -> 1536 16.3 against 14.2, 4096 x 1024 -> 1024 19 against 14).
   // Between the two tiles: 64 x 512 -> 1536, 24 64-tiles, 6.3 against 6.8; 1024 x

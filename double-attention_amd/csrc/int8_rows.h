@@ -75,6 +75,17 @@ __device__ __forceinline__ RawChunk<T> fetch_chunk(const T* p, int n, bool wide)
   return r;
 }
 
+// A row's last eight 16-bit elements as its last n (1 to 7), and zeros: a shift of
+// 128 bits.
+__device__ __forceinline__ u32x4 moved_down(u32x4 d, int n) {
+  const uint64_t lo = static_cast<uint64_t>(d[1]) << 32 | d[0], hi = static_cast<uint64_t>(d[3]) << 32 | d[2];
+  const int shift = 16 * (8 - n);   // 16 to 112
+  const uint64_t top = hi >> (shift & 63);
+  const uint64_t low = shift >= 64 ? top : lo >> (shift & 63) | hi << (-shift & 63);
+  const uint64_t high = shift >= 64 ? 0 : top;
+  return u32x4{static_cast<uint32_t>(low), static_cast<uint32_t>(low >> 32), static_cast<uint32_t>(high), static_cast<uint32_t>(high >> 32)};
+}
+
 // The chunk's floats.
 template <typename T>
 __device__ __forceinline__ void chunk_floats(const RawChunk<T>& r, const T* p, int n, bool wide, float (&v)[8]) {
@@ -92,15 +103,7 @@ __device__ __forceinline__ void chunk_floats(const RawChunk<T>& r, const T* p, i
     }
   } else {
     u32x4 d = r.lo;
-    if (wide && n > 0 && n < 8) {
-      // Elements 8 - n and up, moved down: a shift of 128 bits.
-      const uint64_t lo = static_cast<uint64_t>(d[1]) << 32 | d[0], hi = static_cast<uint64_t>(d[3]) << 32 | d[2];
-      const int shift = 16 * (8 - n);   // 16 to 112
-      const uint64_t top = hi >> (shift & 63);
-      const uint64_t low = shift >= 64 ? top : lo >> (shift & 63) | hi << (-shift & 63);
-      const uint64_t high = shift >= 64 ? 0 : top;
-      d = u32x4{static_cast<uint32_t>(low), static_cast<uint32_t>(low >> 32), static_cast<uint32_t>(high), static_cast<uint32_t>(high >> 32)};
-    }
+    if (wide && n > 0 && n < 8) d = moved_down(d, n);
     const typename Elem<T>::v8 a = __builtin_bit_cast(typename Elem<T>::v8, d);
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = static_cast<float>(a[e]);
@@ -136,20 +139,19 @@ __device__ __forceinline__ void store_chunk(T* p, int n, const float (&v)[8]) {
 __device__ __forceinline__ uint32_t magnitude_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
 // A chunk of eight 16-bit elements as they lie in memory; n of them exist (the
-// others are 0).
+// others are 0).  Fetched like a RawChunk, and put in place by chunk_bits.
 template <typename T>
-__device__ __forceinline__ u32x4 fetch_bits(const T* p, int n) {
-  u32x4 d{0, 0, 0, 0};
-  if (n >= 8) {
-    d = load16B_any(p);
-  } else {
+__device__ __forceinline__ u32x4 fetch_bits(const T* p, int n, bool wide) {
+  u32x4 d = fetch_chunk(p, n, wide).lo;
+  if (!wide && n > 0) {
     const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
+    for (int e = 0; e < 7; ++e)
       if (e < n) d[e / 2] |= static_cast<uint32_t>(h[e]) << (16 * (e % 2));
   }
   return d;
 }
+__device__ __forceinline__ u32x4 chunk_bits(u32x4 d, int n, bool wide) { return wide && n > 0 && n < 8 ? moved_down(d, n) : d; }
 
 // Largest magnitudes of the 16-bit floats in d, as pairs of 16-bit integers.
 __device__ __forceinline__ uint32_t max_pairs(u32x4 d, uint32_t pair) {
