@@ -205,16 +205,16 @@ __device__ __forceinline__ float wave_sum_dpp(float v) { return group_sum(row16_
 //   * amax / 2, 63.5 steps, in all rows: the inverse is set two units, more
 //     than both roundings together, to the side on which the division falls;
 //   * odd multiples of amax / 254 where 127 divides amax's p bits, so that
-//     the scale is exact: 254 for bf16, a power of two as a scale, where
-//     x * inverse is exact too; 127 j, j < 16, for fp16, where seven rows of
-//     1024 take the division's steps (fp32 rows take them all).
+//     the scale is exact, amax = 127 scale: 254 for bf16, a power of two as a
+//     scale, where x * inverse is exact too; 127 j, j <= 16, for fp16, where
+//     eight rows of 1024 take the division's steps (fp32 rows take them all).
 // Checked against fp32 division for every pair of values up to 2^-11 of each
 // other.
 template <typename T> inline constexpr bool kInt8Divides = true;        // all of fp32's rows
 template <> inline constexpr bool kInt8Divides<__bf16> = false;
 struct Int8Scale {
   float scale;     // what a step of the integers stands for; NaN: the row has no integers
-  float inverse;   // 1 / scale, or two units beside it; 0 where the scale is NaN
+  float inverse;   // 1 / scale, or two units beside it
   uint32_t keep;   // all ones, 0 where the scale is NaN
   bool divide;     // the integers need the rounded quotient
 };
@@ -233,12 +233,24 @@ __device__ __forceinline__ Int8Scale int8_scale(uint32_t amax_bits, float factor
   const bool finite = amax_bits < 0x7f800000u;
   const float amax = __uint_as_float(amax_bits) * factor;
   const float s = fmaxf(amax * (1.f / 127.f), kInt8Least);
-  float inverse = 1.f / s;
-  const uint32_t mantissa = __float_as_uint(s) & 0x7fffffu;
-  const bool divide = kInt8Divides<T> && (sizeof(T) == 4 || (mantissa != 0 && (mantissa & 0xfffffu) == 0));
-  if (!divide && mantissa != 0)
-    inverse = __uint_as_float(__float_as_uint(inverse) + (quotient(0.5f * amax, s, inverse) >= 63.5f ? 2u : -2u));
-  return Int8Scale{finite ? s : __uint_as_float(0x7fc00000u), finite ? inverse : 0.f, finite ? 0xffffffffu : 0u, divide};
+  float inverse;
+  bool divide = true;
+  if constexpr (sizeof(T) == 4) {
+    inverse = 1.f / s;
+  } else {
+    // The hardware's reciprocal (one unit off at most) and a step of Newton's
+    // iteration: a hair over half a unit, and rounded like a division for the
+    // scales j 2^k of the rows that divide.
+    inverse = __builtin_amdgcn_rcpf(s);
+    inverse = __builtin_fmaf(__builtin_fmaf(-s, inverse, 1.f), inverse, inverse);
+    // amax / 2 over the scale rounds to 63.5 or more from 63.5 - 2^-19 on; the
+    // difference is exact.
+    const float beyond = __builtin_fmaf(-127.f, s, amax);
+    const float beside = __uint_as_float(__float_as_uint(inverse) + (__builtin_fmaf(0x1p-18f, s, beyond) >= 0.f ? 2u : -2u));
+    divide = kInt8Divides<T> && beyond == 0.f;
+    if (kInt8Divides<T> ? !divide : (__float_as_uint(s) & 0x7fffffu) != 0) inverse = beside;
+  }
+  return Int8Scale{finite ? s : __uint_as_float(0x7fc00000u), inverse, finite ? 0xffffffffu : 0u, divide};
 }
 
 // Eight bytes of sums with kRoundMagic.
