@@ -102,7 +102,7 @@ __device__ __forceinline__ void i8_tile(int t, int tiles_i, int tiles_j, int& ti
   tj = r / wide;
 }
 
-// The scales of a wave's rows, lane r's of row r: a chain of some 40
+// The scales of a wave's rows, lane r's of row r: a chain of some 25
 // instructions, formed once instead of for each row.  `largest`: 16-bit
 // magnitudes.
 template <typename T>
