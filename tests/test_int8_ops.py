@@ -263,6 +263,21 @@ def test_linear_few_tokens_of_any_width(rows, inner, dtype) -> None:
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("inner", [1, 3, 5, 7, 9, 1023])
+@pytest.mark.parametrize(("rows", "outer"), [(13, 7), (100, 64), (3900, 500), (5000, 2100)])
+def test_linear_narrow_and_odd_tokens(rows, outer, inner, dtype) -> None:
+    """Tokens of less than a chunk, and of one that ends inside a chunk."""
+
+    x = _randn(rows + 1, inner + 3, seed=inner, dtype=dtype)[:-1, 1:-2]
+    w = da.quantize_int8_hip(_randn(outer, inner, seed=1, spread=inner ** -0.5))
+    kept = da.quantize_int8_hip(x)
+    got = da.linear_int8_hip(x, w)
+    check_linear(got, kept, w, None, False, None, dtype)
+    assert torch.equal(got, da.linear_int8_hip(kept, w, dtype=dtype))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("width", [70, 96, 200])
 def test_rows_of_three_dimensions(width) -> None:
     """The rows of [a, b, width] tensors are those of [a b, width] ones."""
