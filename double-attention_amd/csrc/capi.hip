@@ -9,6 +9,7 @@
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
+#include <initializer_list>
 #include <mutex>
 #include <string>
 
@@ -731,6 +732,23 @@ int validate_int8(const char* what, const char* name, const void* values, int64_
   return DA_OK;
 }
 
+// The memory of rows, from the first element to the last.
+struct Rows {
+  const void* p;
+  int64_t rows, cols, ld, bytes;
+};
+
+// A kernel reads a row's last columns in loads that begin before them, while
+// other threads may have written there: outputs stay off the inputs.
+int validate_apart(const char* what, const Rows& out, std::initializer_list<Rows> inputs) {
+  const auto first = [](const Rows& r) { return static_cast<__int128>(reinterpret_cast<uintptr_t>(r.p)); };
+  const auto last = [&](const Rows& r) { return first(r) + (static_cast<__int128>(r.rows - 1) * r.ld + r.cols) * r.bytes; };
+  for (const Rows& in : inputs)
+    if (out.p && in.p && first(out) < last(in) && first(in) < last(out))
+      return fail(DA_ERR_INVALID_ARGUMENT, "%s: an output overlaps an input or another output", what);
+  return DA_OK;
+}
+
 // A launch has fewer than 2^32 threads: rows in groups take 16 a group, rows
 // held whole up to 1024 (rms_norm.hip).
 int validate_sizes(const char* what, int64_t rows, int64_t cols, int64_t max_cols, bool grouped) {
@@ -815,12 +833,19 @@ int da_linear_int8(const void* x, int x_dtype, int64_t ldx, const float* x_scale
   if ((rc = validate_int8("linear_int8", "weight", weight, ldw, w_scales, in_features))) return rc;
   if ((rc = validate_rows("linear_int8", "out", out, out_features, out_features, dtype))) return rc;
   if (residual && (rc = validate_rows("linear_int8", "residual", residual, out_features, ldr, dtype))) return rc;
-  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (need > 0) {
-    const int64_t ldv = da::round_up(in_features, 16);
     if (!workspace || workspace_bytes < need)
       return fail(DA_ERR_WORKSPACE, "linear_int8: the workspace needs %lld bytes", (long long)need);
     if (!aligned(workspace, 16)) return fail(DA_ERR_ALIGNMENT, "linear_int8: the workspace must be 16-byte aligned");
+  }
+  if ((rc = validate_apart("linear_int8", {out, rows, out_features, out_features, 2},
+                           {{x, rows, in_features, ldx, x_dtype == DA_I8 ? 1 : 2},
+                            {weight, out_features, in_features, ldw, 1},
+                            {residual, rows, out_features, ldr, 2}})))
+    return rc;
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (need > 0) {
+    const int64_t ldv = da::round_up(in_features, 16);
     int8_t* values = static_cast<int8_t*>(workspace);
     float* scales = reinterpret_cast<float*>(values + align_up(rows * ldv));
     da::launch_row_int8({x, ldx, nullptr, 0, rows, static_cast<int>(in_features), x_dtype, nullptr, 0, 0.f, nullptr,
@@ -863,6 +888,9 @@ int da_add_rms_norm(const void* x, int64_t ldx, const void* residual, int64_t ld
   if (!out && !values) return fail(DA_ERR_INVALID_ARGUMENT, "add_rms_norm: no output asked for");
   if (out && (rc = validate_rows("add_rms_norm", "out", out, dim, dim, dtype))) return rc;
   if (values && (rc = validate_int8("add_rms_norm", "values", values, ldv, scales, dim))) return rc;
+  const Rows in{x, rows, dim, ldx, 2}, in2{residual, rows, dim, ldr, 2}, total{residual ? sum : nullptr, rows, dim, dim, 2};
+  if ((rc = validate_apart("add_rms_norm", total, {in, in2}))) return rc;
+  if ((rc = validate_apart("add_rms_norm", {out, rows, dim, dim, 2}, {in, in2, total}))) return rc;
   da::launch_row_int8({x, ldx, residual, ldr, rows, static_cast<int>(dim), dtype, weight, param_dtype, eps, sum, out,
                        static_cast<int8_t*>(values), ldv, scales},
                       true, reinterpret_cast<hipStream_t>(stream));
@@ -895,6 +923,9 @@ int da_add_rms_norm_backward(const void* sum, int64_t ldsum, const void* grad, i
     if ((rc = validate_rows("add_rms_norm backward", "grad", grad, dim, ldg, dtype))) return rc;
     if (grad_sum && (rc = validate_rows("add_rms_norm backward", "grad_sum", grad_sum, dim, ldgs, dtype))) return rc;
     if ((rc = validate_rows("add_rms_norm backward", "grad_x", grad_x, dim, dim, dtype))) return rc;
+    if ((rc = validate_apart("add_rms_norm backward", {grad_x, rows, dim, dim, 2},
+                             {{sum, rows, dim, ldsum, 2}, {grad, rows, dim, ldg, 2}, {grad_sum, rows, dim, ldgs, 2}})))
+      return rc;
   }
   da::launch_rms_norm_backward({sum, ldsum, grad, ldg, grad_sum, ldgs, rows, static_cast<int>(dim), dtype, weight,
                                 param_dtype, eps, grad_x, grad_weight ? static_cast<float*>(workspace) : nullptr,
@@ -912,6 +943,7 @@ int da_gelu_int8(const void* z, int64_t rows, int64_t cols, int64_t ldz, int dty
   if ((rc = validate_rows("gelu_int8", "z", z, cols, ldz, dtype))) return rc;
   if ((rc = validate_rows("gelu_int8", "out", out, cols, cols, dtype))) return rc;
   if ((rc = validate_int8("gelu_int8", "values", values, ldv, scales, cols))) return rc;
+  if ((rc = validate_apart("gelu_int8", {out, rows, cols, cols, 2}, {{z, rows, cols, ldz, 2}}))) return rc;
   da::launch_gelu_int8({z, ldz, rows, static_cast<int>(cols), dtype, static_cast<int8_t*>(values), ldv, scales, false, out,
                         nullptr, cols},
                        reinterpret_cast<hipStream_t>(stream));
@@ -928,6 +960,9 @@ int da_gelu_int8_backward(const void* values, int64_t rows, int64_t cols, int64_
   if ((rc = validate_rows("gelu_int8 backward", "grad_z", grad_z, cols, cols, dtype))) return rc;
   if (out && (rc = validate_rows("gelu_int8 backward", "out", out, cols, cols, dtype))) return rc;
   if ((rc = validate_int8("gelu_int8 backward", "values", values, ldv, scales, cols))) return rc;
+  const Rows given{grad, rows, cols, ldg, 2}, slope{grad_z, rows, cols, cols, 2};
+  if ((rc = validate_apart("gelu_int8 backward", slope, {given}))) return rc;
+  if ((rc = validate_apart("gelu_int8 backward", {out, rows, cols, cols, 2}, {given, slope}))) return rc;
   da::launch_gelu_int8_backward({grad, ldg, rows, static_cast<int>(cols), dtype,
                                  static_cast<int8_t*>(const_cast<void*>(values)), ldv, const_cast<float*>(scales), false,
                                  grad_z, out, cols},

@@ -826,6 +826,39 @@ def test_refusals_of_the_c_abi() -> None:
     assert linear_with(_0=None, _3=None, _4=0, _6=None, _15=None) == 0
 
 
+def test_overlapping_outputs_are_refused_by_the_c_abi() -> None:
+    if not da.HIP_AVAILABLE:
+        pytest.skip("library not built")
+    lib = _lib.get()
+    F16C, F32C, I8C = _lib.DA_F16, _lib.DA_F32, _lib.DA_I8
+    a, b, c, d = (4096 * (1 + 16 * i) for i in range(4))   # no call reaches them
+    # [4, 100] 16-bit rows at a pitch of 104: 824 bytes and 12 behind.
+    end = a + 2 * (3 * 104 + 100)
+
+    def norm(x=a, residual=b, total=c, out=d):
+        return lib.da_add_rms_norm(x, 104, residual, 104, 4, 100, None, F32C, 1e-6, F16C, total, out, None, 0, None, None)
+
+    for total in (a, a - 798, end - 2, b):
+        assert norm(total=total) == -1
+    assert norm(out=a) == -1 and norm(out=b) == -1 and norm(out=c) == -1 and norm(out=c + 798) == -1
+    assert "overlaps" in _lib.get().da_last_error().decode()
+
+    def back(total=a, grad=b, grad_sum=c, grad_x=d):
+        return lib.da_add_rms_norm_backward(total, 100, grad, 100, grad_sum, 100, 4, 100, None, F32C, 1e-6, F16C, grad_x, None,
+                                            None, 0, None)
+
+    assert back(grad_x=a) == -1 and back(grad_x=b + 6) == -1 and back(grad_x=c - 6) == -1
+
+    def linear(x=a, weight=b, residual=c, out=d):
+        return lib.da_linear_int8(x, I8C, 112, d + 4096, 4, 100, weight, 112, d + 8192, 100, None, F32C, 0, residual, 100, out,
+                                  F16C, None, 0, None)
+
+    assert linear(out=a) == -1 and linear(out=b) == -1 and linear(out=c) == -1 and linear(out=c + 798) == -1
+    assert lib.da_gelu_int8(a, 4, 100, 104, F16C, end - 2, b, 112, c, None) == -1
+    assert lib.da_gelu_int8_backward(a, 4, 100, 112, b, c, 100, F16C, c, None, None) == -1
+    assert lib.da_gelu_int8_backward(a, 4, 100, 112, b, c, 100, F16C, d, d, None) == -1
+
+
 def test_fast_division_is_exact() -> None:
     """The kernels' division by multiplication, as the host sets it up."""
 
