@@ -649,8 +649,11 @@ static I8Plan plan_linear_int8(int64_t rows, int64_t K, int64_t N, bool quantize
   // as fast as a launch of its own for that, or nearly, while the workgroups
   // are one round (4096 x 512 -> 512 7.6 against 8.6, 1024 x 512 -> 1536 7.4
   // against 7.6, 64 x 512 -> 1536 6.3 against 6.3, 777 x 1000 -> 1111 9.8 against
-  // 9.2), and the call has one launch less, 3 us of the host's time.  Beyond, it is
-  // not (4096 x 512 -> 1536 16.3 against 14.2, 4096 x 1024 -> 1024 19 against 14).
+  // 9.2), and the call has one launch less, 3 us of the host's time.  Beyond, whole
+  // calls differ little either way (4096 x 512 -> 1536 16.0 against 15.8, 8192 x 512
+  // -> 1024 16.6 against 15.5, 32768 x 512 -> 512 29.9 against 26.5, but 16384 x 512
+  // -> 640 20.1 against 23.1), and with the larger rows' tiles it loses (4096 x 1024
+  // -> 1024 19 against 14).
   // Between the two tiles: 64 x 512 -> 1536, 24 64-tiles, 6.3 against 6.8; 1024 x
   // 512 -> 1536, 384 of them, 9.2 against 7.4.
   if (quantize && K <= 1024 && tiles_of(rows, N, 64, 64) <= 256) return K <= 512 ? I8Plan::kToken64 : I8Plan::kToken64x1024;
