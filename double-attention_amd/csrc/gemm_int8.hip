@@ -652,7 +652,7 @@ static I8Plan plan_linear_int8(int64_t rows, int64_t K, int64_t N, bool quantize
   // 9.2), and the call has one launch less, 3 us of the host's time.  Beyond, whole
   // calls differ little either way (4096 x 512 -> 1536 16.0 against 15.8, 8192 x 512
   // -> 1024 16.6 against 15.5, 32768 x 512 -> 512 29.9 against 26.5, but 16384 x 512
-  // -> 640 20.1 against 23.1), and with the larger rows' tiles it loses (4096 x 1024
+  // -> 640 20.1 against 23.1), and with K over 512 it loses (4096 x 1024
   // -> 1024 19 against 14).
   // Between the two tiles: 64 x 512 -> 1536, 24 64-tiles, 6.3 against 6.8; 1024 x
   // 512 -> 1536, 384 of them, 9.2 against 7.4.
