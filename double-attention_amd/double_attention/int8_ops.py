@@ -49,7 +49,8 @@ class QuantizedRows(NamedTuple):
     group: int | None = None
 
 
-_current_device = torch._C._cuda_getDevice
+# The private call skips torch.cuda's own checks; a torch without device support has none.
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 _INT8, _FLOAT32 = torch.int8, torch.float32
 _CODES = {torch.float32: _lib.DA_F32, torch.float16: _lib.DA_F16, torch.bfloat16: _lib.DA_BF16}
 _HALF_CODES = {torch.float16: _lib.DA_F16, torch.bfloat16: _lib.DA_BF16}
