@@ -732,20 +732,57 @@ int validate_int8(const char* what, const char* name, const void* values, int64_
   return DA_OK;
 }
 
-// The memory of rows, from the first element to the last.
+// The memory of a tensor: `rows` spans of `cols` elements, `ld` elements apart.
 struct Rows {
   const void* p;
   int64_t rows, cols, ld, bytes;
 };
+Rows flat(const void* p, int64_t count, int64_t bytes) { return {p, 1, count, count, bytes}; }
+// 8-bit rows that a call writes: with the rest of the last chunk of 16.
+Rows written_int8(const void* p, int64_t rows, int64_t cols, int64_t ldv) { return {p, rows, da::round_up(cols, 16), ldv, 1}; }
 
-// A kernel reads a row's last columns in loads that begin before them, while
-// other threads may have written there: outputs stay off the inputs.
-int validate_apart(const char* what, const Rows& out, std::initializer_list<Rows> inputs) {
-  const auto first = [](const Rows& r) { return static_cast<__int128>(reinterpret_cast<uintptr_t>(r.p)); };
-  const auto last = [&](const Rows& r) { return first(r) + (static_cast<__int128>(r.rows - 1) * r.ld + r.cols) * r.bytes; };
-  for (const Rows& in : inputs)
-    if (out.p && in.p && first(out) < last(in) && first(in) < last(out))
-      return fail(DA_ERR_INVALID_ARGUMENT, "%s: an output overlaps an input or another output", what);
+// Whether two tensors share a byte.  Rows of a between rows of b (columns of one
+// wider matrix) do not; where both have gaps and their pitches differ, their
+// ranges decide.
+bool overlap(const Rows& a, const Rows& b) {
+  typedef __int128 wide;
+  struct Spans {
+    wide first, count, length, pitch;
+  };
+  const auto spans = [](const Rows& r) {
+    Spans s{static_cast<wide>(reinterpret_cast<uintptr_t>(r.p)), r.rows, static_cast<wide>(r.cols) * r.bytes,
+            static_cast<wide>(r.ld) * r.bytes};
+    if (s.pitch == s.length) {
+      s.length *= s.count;
+      s.count = 1;
+    }
+    return s;
+  };
+  Spans x = spans(a), y = spans(b);
+  if (!a.p || !b.p || x.count < 1 || y.count < 1) return false;
+  if (x.first + (x.count - 1) * x.pitch + x.length <= y.first || y.first + (y.count - 1) * y.pitch + y.length <= x.first) return false;
+  // A single span has whichever pitch suits.
+  if (x.count == 1) x.pitch = y.pitch;
+  if (y.count == 1) y.pitch = x.pitch;
+  if (x.count == 1 && y.count == 1) return true;
+  if (x.pitch != y.pitch) return true;
+  // Spans i of x and j of y meet where -y.length < apart + k pitch < x.length with k = j - i.
+  const auto floor_div = [](wide n, wide d) { return n / d - (n % d != 0 && n < 0 ? 1 : 0); };
+  const wide apart = y.first - x.first, pitch = x.pitch;
+  const wide least = floor_div(-y.length - apart, pitch) + 1, most = -floor_div(apart - x.length, pitch) - 1;
+  return (least > -(x.count - 1) ? least : -(x.count - 1)) <= (most < y.count - 1 ? most : y.count - 1);
+}
+
+// Workgroups read rows that others write without an order between them, and a
+// row's last columns in loads that begin before them: what a call writes stays
+// off what it reads, and off what else it writes.
+int validate_apart(const char* what, std::initializer_list<Rows> outputs, std::initializer_list<Rows> inputs) {
+  for (const Rows* out = outputs.begin(); out != outputs.end(); ++out) {
+    for (const Rows& in : inputs)
+      if (overlap(*out, in)) return fail(DA_ERR_INVALID_ARGUMENT, "%s: an output overlaps an input", what);
+    for (const Rows* other = out + 1; other != outputs.end(); ++other)
+      if (overlap(*out, *other)) return fail(DA_ERR_INVALID_ARGUMENT, "%s: an output overlaps another output", what);
+  }
   return DA_OK;
 }
 
@@ -761,6 +798,9 @@ int validate_sizes(const char* what, int64_t rows, int64_t cols, int64_t max_col
 
 constexpr int64_t kInt8MaxCols = kInt8MaxPitch;   // of rows in groups
 
+// Scales of rows in groups (0: one a row).
+int64_t scale_count(int64_t rows, int64_t cols, int64_t group) { return group ? rows * ((cols + group - 1) / group) : rows; }
+
 }  // namespace
 
 int da_quantize_int8(const void* x, int64_t rows, int64_t cols, int64_t ldx, int dtype, int64_t group, void* values,
@@ -773,6 +813,9 @@ int da_quantize_int8(const void* x, int64_t rows, int64_t cols, int64_t ldx, int
   if (rows == 0) return ok();
   if ((rc = validate_rows("quantize", "x", x, cols, ldx, dtype))) return rc;
   if ((rc = validate_int8("quantize", "values", values, ldv, scales, cols))) return rc;
+  if ((rc = validate_apart("quantize", {written_int8(values, rows, cols, ldv), flat(scales, scale_count(rows, cols, group), 4)},
+                           {{x, rows, cols, ldx, element_bytes(dtype)}})))
+    return rc;
   int8_t* q = static_cast<int8_t*>(values);
   if (group) {
     da::launch_int8_save({x, ldx, rows, static_cast<int>(cols), dtype, q, ldv, scales, false, nullptr, nullptr, 0},
@@ -794,6 +837,9 @@ int da_dequantize_int8(const void* values, int64_t rows, int64_t cols, int64_t l
   if (rows == 0) return ok();
   if ((rc = validate_rows("dequantize", "out", out, cols, ldo, out_dtype))) return rc;
   if ((rc = validate_int8("dequantize", "values", values, ldv, scales, cols))) return rc;
+  if ((rc = validate_apart("dequantize", {{out, rows, cols, ldo, element_bytes(out_dtype)}},
+                           {{values, rows, cols, ldv, 1}, flat(scales, scale_count(rows, cols, group), 4)})))
+    return rc;
   da::launch_int8_restore({nullptr, 0, rows, static_cast<int>(cols), out_dtype,
                            static_cast<int8_t*>(const_cast<void*>(values)), ldv, const_cast<float*>(scales), group == 0, out,
                            nullptr, ldo},
@@ -838,10 +884,12 @@ int da_linear_int8(const void* x, int x_dtype, int64_t ldx, const float* x_scale
       return fail(DA_ERR_WORKSPACE, "linear_int8: the workspace needs %lld bytes", (long long)need);
     if (!aligned(workspace, 16)) return fail(DA_ERR_ALIGNMENT, "linear_int8: the workspace must be 16-byte aligned");
   }
-  if ((rc = validate_apart("linear_int8", {out, rows, out_features, out_features, 2},
-                           {{x, rows, in_features, ldx, x_dtype == DA_I8 ? 1 : 2},
-                            {weight, out_features, in_features, ldw, 1},
-                            {residual, rows, out_features, ldr, 2}})))
+  const bool kept = x_dtype == DA_I8;
+  if ((rc = validate_apart("linear_int8",
+                           {{out, rows, out_features, out_features, 2}, flat(need > 0 ? workspace : nullptr, need, 1)},
+                           {{x, rows, in_features, ldx, kept ? 1 : 2}, flat(kept ? x_scales : nullptr, rows, 4),
+                            {weight, out_features, in_features, ldw, 1}, flat(w_scales, out_features, 4),
+                            flat(bias, out_features, element_bytes(bias_dtype)), {residual, rows, out_features, ldr, 2}})))
     return rc;
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (need > 0) {
@@ -888,9 +936,11 @@ int da_add_rms_norm(const void* x, int64_t ldx, const void* residual, int64_t ld
   if (!out && !values) return fail(DA_ERR_INVALID_ARGUMENT, "add_rms_norm: no output asked for");
   if (out && (rc = validate_rows("add_rms_norm", "out", out, dim, dim, dtype))) return rc;
   if (values && (rc = validate_int8("add_rms_norm", "values", values, ldv, scales, dim))) return rc;
-  const Rows in{x, rows, dim, ldx, 2}, in2{residual, rows, dim, ldr, 2}, total{residual ? sum : nullptr, rows, dim, dim, 2};
-  if ((rc = validate_apart("add_rms_norm", total, {in, in2}))) return rc;
-  if ((rc = validate_apart("add_rms_norm", {out, rows, dim, dim, 2}, {in, in2, total}))) return rc;
+  if ((rc = validate_apart("add_rms_norm",
+                           {{residual ? sum : nullptr, rows, dim, dim, 2}, {out, rows, dim, dim, 2},
+                            written_int8(values, rows, dim, ldv), flat(values ? scales : nullptr, rows, 4)},
+                           {{x, rows, dim, ldx, 2}, {residual, rows, dim, ldr, 2}, flat(weight, dim, element_bytes(param_dtype))})))
+    return rc;
   da::launch_row_int8({x, ldx, residual, ldr, rows, static_cast<int>(dim), dtype, weight, param_dtype, eps, sum, out,
                        static_cast<int8_t*>(values), ldv, scales},
                       true, reinterpret_cast<hipStream_t>(stream));
@@ -923,10 +973,13 @@ int da_add_rms_norm_backward(const void* sum, int64_t ldsum, const void* grad, i
     if ((rc = validate_rows("add_rms_norm backward", "grad", grad, dim, ldg, dtype))) return rc;
     if (grad_sum && (rc = validate_rows("add_rms_norm backward", "grad_sum", grad_sum, dim, ldgs, dtype))) return rc;
     if ((rc = validate_rows("add_rms_norm backward", "grad_x", grad_x, dim, dim, dtype))) return rc;
-    if ((rc = validate_apart("add_rms_norm backward", {grad_x, rows, dim, dim, 2},
-                             {{sum, rows, dim, ldsum, 2}, {grad, rows, dim, ldg, 2}, {grad_sum, rows, dim, ldgs, 2}})))
-      return rc;
   }
+  if ((rc = validate_apart("add_rms_norm backward",
+                           {{grad_x, rows, dim, dim, 2}, flat(grad_weight, dim, element_bytes(param_dtype)),
+                            flat(grad_weight ? workspace : nullptr, da_add_rms_norm_backward_workspace_bytes(rows, dim), 1)},
+                           {{sum, rows, dim, ldsum, 2}, {grad, rows, dim, ldg, 2}, {grad_sum, rows, dim, ldgs, 2},
+                            flat(weight, dim, element_bytes(param_dtype))})))
+    return rc;
   da::launch_rms_norm_backward({sum, ldsum, grad, ldg, grad_sum, ldgs, rows, static_cast<int>(dim), dtype, weight,
                                 param_dtype, eps, grad_x, grad_weight ? static_cast<float*>(workspace) : nullptr,
                                 grad_weight},
@@ -943,7 +996,11 @@ int da_gelu_int8(const void* z, int64_t rows, int64_t cols, int64_t ldz, int dty
   if ((rc = validate_rows("gelu_int8", "z", z, cols, ldz, dtype))) return rc;
   if ((rc = validate_rows("gelu_int8", "out", out, cols, cols, dtype))) return rc;
   if ((rc = validate_int8("gelu_int8", "values", values, ldv, scales, cols))) return rc;
-  if ((rc = validate_apart("gelu_int8", {out, rows, cols, cols, 2}, {{z, rows, cols, ldz, 2}}))) return rc;
+  if ((rc = validate_apart("gelu_int8",
+                           {{out, rows, cols, cols, 2}, written_int8(values, rows, cols, ldv),
+                            flat(scales, scale_count(rows, cols, DA_INT8_GROUP), 4)},
+                           {{z, rows, cols, ldz, 2}})))
+    return rc;
   da::launch_gelu_int8({z, ldz, rows, static_cast<int>(cols), dtype, static_cast<int8_t*>(values), ldv, scales, false, out,
                         nullptr, cols},
                        reinterpret_cast<hipStream_t>(stream));
@@ -960,9 +1017,10 @@ int da_gelu_int8_backward(const void* values, int64_t rows, int64_t cols, int64_
   if ((rc = validate_rows("gelu_int8 backward", "grad_z", grad_z, cols, cols, dtype))) return rc;
   if (out && (rc = validate_rows("gelu_int8 backward", "out", out, cols, cols, dtype))) return rc;
   if ((rc = validate_int8("gelu_int8 backward", "values", values, ldv, scales, cols))) return rc;
-  const Rows given{grad, rows, cols, ldg, 2}, slope{grad_z, rows, cols, cols, 2};
-  if ((rc = validate_apart("gelu_int8 backward", slope, {given}))) return rc;
-  if ((rc = validate_apart("gelu_int8 backward", {out, rows, cols, cols, 2}, {given, slope}))) return rc;
+  if ((rc = validate_apart("gelu_int8 backward", {{grad_z, rows, cols, cols, 2}, {out, rows, cols, cols, 2}},
+                           {{grad, rows, cols, ldg, 2}, {values, rows, cols, ldv, 1},
+                            flat(scales, scale_count(rows, cols, DA_INT8_GROUP), 4)})))
+    return rc;
   da::launch_gelu_int8_backward({grad, ldg, rows, static_cast<int>(cols), dtype,
                                  static_cast<int8_t*>(const_cast<void*>(values)), ldv, const_cast<float*>(scales), false,
                                  grad_z, out, cols},

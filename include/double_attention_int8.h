@@ -31,7 +31,10 @@ extern "C" {
  * The 16-bit (and fp32) tensors of these operators are rows of any width at
  * any pitch >= that width, aligned to their elements.  No call reads or writes
  * outside of the rows it is given.  No output may overlap an input or another
- * output (16-bit outputs that do are refused, DA_ERR_INVALID_ARGUMENT).  A launch takes fewer than 2^32 threads, 16
+ * output, values, scales, parameters and the workspace among them: such calls
+ * are refused (DA_ERR_INVALID_ARGUMENT).  Rows of one pitch may lie in each
+ * other's gaps, and a contiguous tensor in one gap; rows of two pitches whose
+ * ranges meet count as overlapping.  A launch takes fewer than 2^32 threads, 16
  * for each group of a row, or 64, 256 or 1024 for a row held whole (up to 1024,
  * 8192 and more columns); calls with more rows are refused (DA_ERR_UNSUPPORTED).
  */

@@ -2,11 +2,26 @@
 
 from __future__ import annotations
 
+import random
 import subprocess
 import sys
 from pathlib import Path
 
+import pytest
+import torch
+
 import double_attention as da
+from double_attention import _lib
+from test_int8_ops import _device, _randn
+
+F32C, F16C, I8C = _lib.DA_F32, _lib.DA_F16, _lib.DA_I8
+REFUSED = -1   # DA_ERR_INVALID_ARGUMENT
+
+
+def _library():
+    if not da.HIP_AVAILABLE:
+        pytest.skip("library not built")
+    return _lib.get()
 
 
 def test_import_without_device_support() -> None:
@@ -28,3 +43,129 @@ assert model(torch.zeros(1, 5, dtype=torch.int64))[0].shape == (1, 5, 50)
     package = Path(da.__file__).resolve().parents[1]
     done = subprocess.run([sys.executable, "-c", code, str(package)], capture_output=True, text=True, timeout=300)
     assert done.returncode == 0, done.stderr[-2000:]
+
+
+# Buffers of the C calls below, far apart; no refused call follows them.
+X, RESIDUAL, WEIGHT, SUM, OUT, VALUES, SCALES, BIAS, SPACE, MORE = (1 << 20 | i << 24 for i in range(1, 11))
+
+
+def _calls(lib):
+    """Each entry point as ``(call(**buffers), buffers written, buffers read)``,
+    100 columns of 16-bit rows at a pitch of 104 (inputs) and 6 or 100 rows."""
+
+    def quantize(group):
+        def call(x=X, values=VALUES, scales=SCALES):
+            return lib.da_quantize_int8(x, 6, 100, 104, F16C, group, values, 112, scales, None)
+        return call, {"values": VALUES, "scales": SCALES}, {"x": X}
+
+    def dequantize(out=OUT, values=VALUES, scales=SCALES):
+        return lib.da_dequantize_int8(values, 6, 100, 112, scales, 128, out, 104, F16C, None)
+
+    def linear(x=X, x_scales=MORE, weight=WEIGHT, w_scales=SCALES, bias=BIAS, residual=RESIDUAL, out=OUT):
+        return lib.da_linear_int8(x, I8C, 112, x_scales, 6, 100, weight, 112, w_scales, 60, bias, F32C, 0, residual, 64, out, F16C,
+                                  None, 0, None)
+
+    need = lib.da_linear_int8_workspace_bytes(100, 5000, 60, F16C, F16C)
+
+    def linear16(x=X, weight=WEIGHT, w_scales=SCALES, bias=BIAS, residual=RESIDUAL, out=OUT, workspace=SPACE):
+        return lib.da_linear_int8(x, F16C, 5004, None, 100, 5000, weight, 5008, w_scales, 60, bias, F32C, 0, residual, 64, out, F16C,
+                                  workspace, need, None)
+
+    def norm(x=X, residual=RESIDUAL, weight=WEIGHT, total=SUM, out=OUT, values=VALUES, scales=SCALES):
+        return lib.da_add_rms_norm(x, 104, residual, 104, 6, 100, weight, F32C, 1e-6, F16C, total, out, values, 112, scales, None)
+
+    space = lib.da_add_rms_norm_backward_workspace_bytes(6, 100)
+
+    def norm_backward(total=X, grad=OUT, grad_sum=RESIDUAL, weight=WEIGHT, grad_x=SUM, grad_weight=BIAS, workspace=SPACE):
+        return lib.da_add_rms_norm_backward(total, 104, grad, 104, grad_sum, 104, 6, 100, weight, F32C, 1e-6, F16C, grad_x,
+                                            grad_weight, workspace, space, None)
+
+    def gelu(z=X, out=OUT, values=VALUES, scales=SCALES):
+        return lib.da_gelu_int8(z, 6, 100, 104, F16C, out, values, 112, scales, None)
+
+    def gelu_backward(values=VALUES, scales=SCALES, grad=X, grad_z=OUT, out=SUM):
+        return lib.da_gelu_int8_backward(values, 6, 100, 112, scales, grad, 104, F16C, grad_z, out, None)
+
+    return {
+        "quantize": quantize(0),
+        "quantize in groups": quantize(128),
+        "dequantize": (dequantize, {"out": OUT}, {"values": VALUES, "scales": SCALES}),
+        "linear": (linear, {"out": OUT}, {"x": X, "x_scales": MORE, "weight": WEIGHT, "w_scales": SCALES, "bias": BIAS,
+                                          "residual": RESIDUAL}),
+        "linear of 16-bit rows": (linear16, {"out": OUT, "workspace": SPACE},
+                                  {"x": X, "weight": WEIGHT, "w_scales": SCALES, "bias": BIAS, "residual": RESIDUAL}),
+        "norm": (norm, {"total": SUM, "out": OUT, "values": VALUES, "scales": SCALES},
+                 {"x": X, "residual": RESIDUAL, "weight": WEIGHT}),
+        "norm backward": (norm_backward, {"grad_x": SUM, "grad_weight": BIAS, "workspace": SPACE},
+                          {"total": X, "grad": OUT, "grad_sum": RESIDUAL, "weight": WEIGHT}),
+        "gelu": (gelu, {"out": OUT, "values": VALUES, "scales": SCALES}, {"z": X}),
+        "gelu backward": (gelu_backward, {"grad_z": OUT, "out": SUM}, {"values": VALUES, "scales": SCALES, "grad": X}),
+    }
+
+
+def test_overlapping_buffers_are_refused_by_the_c_abi() -> None:
+    """Every buffer that a call writes, on every other buffer of the call."""
+
+    lib = _library()
+    if torch.cuda.is_available():
+        pytest.skip("a call that is not refused would run on addresses that are none")
+    for name, (call, written, read) in _calls(lib).items():
+        assert call() != REFUSED, name   # apart: as far as the launch, which fails without a device
+        every = {**written, **read}
+        for mine in written:
+            for other in every:
+                if other == mine:
+                    continue
+                # At its start, and inside its first row (16: the 8-bit rows' alignment).
+                assert call(**{mine: every[other]}) == REFUSED, (name, mine, other)
+                assert call(**{other: every[mine] + 16}) == REFUSED, (name, mine, other)
+                assert "overlaps" in lib.da_last_error().decode()
+    # The rest of the last 16 bytes of 8-bit rows is written, too: [6, 100] at a pitch of 112.
+    calls = _calls(lib)
+    assert calls["quantize"][0](x=VALUES + 6 * 112 - 2) == REFUSED and calls["quantize"][0](x=VALUES + 6 * 112) != REFUSED
+    # Without a residual the sum is not written, and without a weight's gradient no workspace.
+    assert calls["norm"][0](residual=None, total=X) != REFUSED
+    assert calls["norm backward"][0](grad_weight=None, workspace=X) != REFUSED
+
+
+def test_rows_in_each_others_gaps_are_no_overlap() -> None:
+    """Against sets of bytes: only rows of two pitches, both with gaps, go by their ranges."""
+
+    lib = _library()
+    if torch.cuda.is_available():
+        pytest.skip("a call that is not refused would run on addresses that are none")
+    rng = random.Random(0)
+    seen = set()
+    for _ in range(4000):
+        rows, cols = rng.randint(1, 5), rng.randint(1, 40)
+        ldv = -(-cols // 16) * 16 + 16 * rng.randint(0, 4)
+        ldo = (ldv // 2 if rng.random() < 0.5 and ldv // 2 >= cols else cols) + rng.choice((0, 0, rng.randint(0, 40)))
+        values = 1 << 20
+        out = values + 2 * rng.randint(-rows * ldo - 20, rows * ldv // 2 + 20)
+        read = {values + r * ldv + c for r in range(rows) for c in range(cols)}
+        wrote = {out + 2 * r * ldo + c for r in range(rows) for c in range(2 * cols)}
+        meet = bool(read & wrote)
+        if not meet and rows > 1 and ldv > cols and ldo > cols and ldv != 2 * ldo:
+            meet = min(read) <= max(wrote) and min(wrote) <= max(read)
+        got = lib.da_dequantize_int8(values, rows, cols, ldv, 1 << 28, 0, out, ldo, F16C, None)
+        assert (got == REFUSED) == meet, (rows, cols, ldv, ldo, out - values)
+        seen.add((meet, max(read) >= min(wrote) and max(wrote) >= min(read)))
+    assert seen == {(True, True), (False, True), (False, False)}
+
+
+@pytest.mark.gpu
+def test_rows_in_each_others_gaps() -> None:
+    """Rows, their integers and what these stand for as columns of one buffer."""
+
+    lib = _library()
+    store = torch.zeros(37, 1024, dtype=torch.uint8, device=_device())
+    data = _randn(37, 150, seed=1, dtype=torch.float16)
+    store[:, :300] = data.view(torch.uint8)
+    scales = torch.zeros(37, 2, device=_device())
+    at, stream = store.data_ptr(), torch.cuda.current_stream().cuda_stream
+    assert lib.da_quantize_int8(at, 37, 150, 512, F16C, 128, at + 304, 1024, scales.data_ptr(), stream) == 0
+    assert lib.da_dequantize_int8(at + 304, 37, 150, 1024, scales.data_ptr(), 128, at + 464, 512, F16C, stream) == 0
+    kept = da.quantize_int8_hip(data, 128)
+    assert torch.equal(scales, kept.scales) and torch.equal(store[:, 304:454].view(torch.int8), kept.values)
+    assert torch.equal(store[:, 464:764].contiguous().view(torch.float16), da.dequantize_int8_hip(kept, torch.float16))
+    assert torch.equal(store[:, :300].contiguous().view(torch.float16), data) and not store[:, 764:].any()
