@@ -898,6 +898,42 @@ class _HipFeedForwardInt8Function(torch.autograd.Function):
         return grad if wants[0] else None, dh, d_w1, d_b1, d_w2, d_b2
 
 
+class _Int8FeedForward:
+    """A feed-forward's two weights in 8 bits, and what tells whether they still
+    stand for the parameters that they were made from."""
+
+    def __init__(self, weights: tuple[Tensor, Tensor]) -> None:
+        from .int8_ops import quantize_int8_hip
+
+        with torch.no_grad():
+            self.rows = tuple(quantize_int8_hip(w) for w in weights)
+        self.made_from = weights
+        self._read_versions()
+
+    def _read_versions(self) -> None:
+        from .hip_ops import _version_of
+
+        self.versions: tuple | None = tuple(_version_of(w) for w in self.made_from)
+
+    def unchanged(self) -> bool:
+        """Whether the parameters have not been written in place since."""
+
+        from .hip_ops import _version_of
+
+        return tuple(_version_of(w) for w in self.made_from) == self.versions
+
+    # A copied or loaded parameter counts its versions anew: what is kept of them
+    # is whether they were the current ones.
+    def __getstate__(self) -> dict:
+        return {"rows": self.rows, "made_from": self.made_from, "unchanged": self.unchanged()}
+
+    def __setstate__(self, state: dict) -> None:
+        self.rows, self.made_from = state["rows"], state["made_from"]
+        self.versions = None
+        if state["unchanged"]:
+            self._read_versions()
+
+
 class DoubleAttentionBlock(nn.Module):
     """Pre-norm transformer block around ``SharedDictionaryAttention`` (``modules.py:294-356``).
 
@@ -942,9 +978,8 @@ class DoubleAttentionBlock(nn.Module):
             nn.Linear(feedforward_dim, config.model_dim),
             nn.Dropout(dropout),
         )
-        # Set by quantize_feedforward: the two weights in 8 bits, the
-        # parameters that they were made from and those parameters' versions.
-        self._int8_feedforward: tuple | None = None
+        # Set by quantize_feedforward.
+        self._int8_feedforward: _Int8FeedForward | None = None
 
     def quantize_feedforward(self, enabled: bool = True) -> None:
         """Run the feed-forward on 8-bit integers in inference on the HIP kernels.
@@ -965,33 +1000,23 @@ class DoubleAttentionBlock(nn.Module):
         first, second = self.feedforward[0], self.feedforward[2]
         if not isinstance(first, nn.Linear):
             raise NotImplementedError("the Q-dictionary FFN has no 8-bit form")
-        from .hip_ops import _version_of
-        from .int8_ops import quantize_int8_hip
-
-        with torch.no_grad():
-            self._int8_feedforward = (
-                quantize_int8_hip(first.weight), quantize_int8_hip(second.weight),
-                (first.weight, second.weight),
-                (_version_of(first.weight), _version_of(second.weight)),
-            )
+        self._int8_feedforward = _Int8FeedForward((first.weight, second.weight))
 
     def _int8_weights(self) -> tuple | None:
         """The 8-bit weights, if the feed-forward runs on them."""
 
-        if self._int8_feedforward is None:
+        kept = self._int8_feedforward
+        if kept is None:
             return None
-        from .hip_ops import _version_of
-
-        w1, w2, made_from, versions = self._int8_feedforward
         first, second = self.feedforward[0].weight, self.feedforward[2].weight
         if (
-            first is not made_from[0]
-            or second is not made_from[1]
-            or (_version_of(first), _version_of(second)) != versions
-            or w1.values.device != first.device
+            first is not kept.made_from[0]
+            or second is not kept.made_from[1]
+            or not kept.unchanged()
+            or kept.rows[0].values.device != first.device
         ):
             raise RuntimeError("the feed-forward's weights changed after quantize_feedforward(); call it again")
-        return w1, w2
+        return kept.rows
 
     def _int8_inference(self, x: Tensor, attended: Tensor) -> tuple | None:
         """The 8-bit weights, where a forward that does not run as one fused

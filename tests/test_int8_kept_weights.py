@@ -1,0 +1,85 @@
+"""The feed-forward's 8-bit weights when the block around them is copied, saved,
+changed or captured."""
+
+from __future__ import annotations
+
+import copy
+import io
+
+import pytest
+import torch
+
+import double_attention as da
+from double_attention import int8_ops
+from test_int8_modules import _block
+from test_int8_ops import _randn
+
+
+def _stand_in(x, group=None):
+    """``quantize_int8_hip`` of weights, on the host."""
+
+    assert group is None and not torch.is_grad_enabled()
+    scales = x.detach().float().abs().amax(-1, keepdim=True) / 127
+    return da.QuantizedRows(torch.round(x.detach().float() / scales).to(torch.int8), scales)
+
+
+def _host_block(monkeypatch, **options):
+    """A block on the host, its weights written in place as by a checkpoint."""
+
+    monkeypatch.setattr(int8_ops, "quantize_int8_hip", _stand_in)
+    config = da.experiment_config("a1", backend="torch", model_dim=32, routing_dim=8, dictionary_size=16)
+    torch.manual_seed(0)
+    block = da.DoubleAttentionBlock(config, feedforward_dim=48, **options)
+    block.load_state_dict({n: p + 0.01 for n, p in block.state_dict().items()})
+    return block
+
+
+def _copies(block):
+    file = io.BytesIO()
+    torch.save(block, file)
+    file.seek(0)
+    return copy.deepcopy(block), copy.copy(block), torch.load(file, weights_only=False), copy.deepcopy(copy.deepcopy(block))
+
+
+def test_copies_of_a_quantized_block(monkeypatch) -> None:
+    """A copy has the 8-bit weights of its own parameters, and sees these change."""
+
+    block = _host_block(monkeypatch)
+    block.quantize_feedforward()
+    want = block._int8_weights()
+    for other in _copies(block):
+        for got, expected in zip(other._int8_weights(), want):
+            assert torch.equal(got.values, expected.values) and torch.equal(got.scales, expected.scales)
+    deep = copy.deepcopy(block)
+    assert deep._int8_weights()[0].values.data_ptr() != want[0].values.data_ptr()
+    with torch.no_grad():
+        deep.feedforward[2].weight.mul_(2.0)
+    with pytest.raises(RuntimeError, match="quantize_feedforward"):
+        deep._int8_weights()
+    assert block._int8_weights() is want
+    deep.quantize_feedforward()
+    assert torch.equal(deep._int8_weights()[1].scales, 2 * want[1].scales)
+
+
+def test_copies_of_a_block_whose_weights_changed(monkeypatch) -> None:
+    """They know no more about their 8-bit weights than the block itself."""
+
+    block = _host_block(monkeypatch)
+    block.quantize_feedforward()
+    with torch.no_grad():
+        block.feedforward[0].weight.add_(1.0)
+    for other in (block, *_copies(block)):
+        with pytest.raises(RuntimeError, match="quantize_feedforward"):
+            other._int8_weights()
+
+
+@pytest.mark.gpu
+def test_forward_of_a_copied_quantized_block() -> None:
+    block, bank = _block(torch.bfloat16, norm="rms")
+    x = _randn(2, 33, 128, seed=1, dtype=torch.bfloat16)
+    block.load_state_dict({n: p * 1.0 for n, p in block.state_dict().items()})
+    with torch.no_grad():
+        block.quantize_feedforward()
+        want = block(x, bank)
+        for other in _copies(block):
+            assert torch.equal(other(x, bank), want)
