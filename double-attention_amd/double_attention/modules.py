@@ -920,7 +920,8 @@ class _Int8FeedForward:
 
         from .hip_ops import _version_of
 
-        return tuple(_version_of(w) for w in self.made_from) == self.versions
+        versions = tuple(_version_of(w) for w in self.made_from)
+        return None not in versions and versions == self.versions
 
     # A copied or loaded parameter counts its versions anew: what is kept of them
     # is whether they were the current ones.
@@ -988,8 +989,9 @@ class DoubleAttentionBlock(nn.Module):
         (``quantize_int8_hip``); activations are quantized for each token in
         every forward.  Call it again after the weights change: a forward that
         finds them replaced or changed in place raises ``RuntimeError`` (writes
-        through ``.data`` and into a captured graph's weights are not seen);
-        ``enabled=False`` drops the 8-bit weights.  Forwards that autograd
+        through ``.data`` and into a captured graph's weights are not seen;
+        weights made under ``torch.inference_mode`` have nothing that would show
+        a change, and are refused); ``enabled=False`` drops the 8-bit weights.  Forwards that autograd
         records, and those that do not run on the HIP kernels, use the full
         weights as before.
         """
@@ -1000,6 +1002,9 @@ class DoubleAttentionBlock(nn.Module):
         first, second = self.feedforward[0], self.feedforward[2]
         if not isinstance(first, nn.Linear):
             raise NotImplementedError("the Q-dictionary FFN has no 8-bit form")
+        if first.weight.is_inference() or second.weight.is_inference():
+            raise ValueError("quantize_feedforward: changes of inference tensors are not seen; make the model outside of "
+                             "torch.inference_mode()")
         self._int8_feedforward = _Int8FeedForward((first.weight, second.weight))
 
     def _int8_weights(self) -> tuple | None:

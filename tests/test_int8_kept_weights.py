@@ -73,6 +73,25 @@ def test_copies_of_a_block_whose_weights_changed(monkeypatch) -> None:
             other._int8_weights()
 
 
+def test_inference_tensors_as_weights(monkeypatch) -> None:
+    """Nothing tells when they are written: no 8-bit weights are kept of them."""
+
+    with torch.inference_mode():
+        block = _host_block(monkeypatch)
+        with pytest.raises(ValueError, match="inference_mode"):
+            block.quantize_feedforward()
+        assert block._int8_weights() is None
+    # Copies made there are such tensors, too, whatever the block's own are.
+    block = _host_block(monkeypatch)
+    with torch.inference_mode():
+        block.quantize_feedforward()
+        assert block._int8_weights() is not None
+        other = copy.deepcopy(block)
+        assert other.feedforward[0].weight.is_inference()
+        with pytest.raises(RuntimeError, match="quantize_feedforward"):
+            other._int8_weights()
+
+
 @pytest.mark.gpu
 def test_forward_of_a_copied_quantized_block() -> None:
     block, bank = _block(torch.bfloat16, norm="rms")
