@@ -20,6 +20,8 @@ from typing import Any, Callable
 import torch
 from torch import nn
 
+from .modules import int8_weights_used
+
 _PATH_TYPES = [pathlib.PosixPath, pathlib.PurePosixPath, pathlib.WindowsPath, pathlib.PureWindowsPath]
 
 
@@ -52,7 +54,10 @@ class GraphedForward:
     call: clone it to keep it).  The inputs must keep the example's shapes,
     dtypes and device.  For inference only (the capture runs under
     ``torch.inference_mode``); the module's parameters may change in place
-    between calls, but not be replaced.  Each replay launches the same kernels
+    between calls, but not be replaced; a call that finds the weights of a
+    feed-forward that was captured on 8-bit integers changed raises
+    ``RuntimeError`` until ``quantize_feedforward()`` of its block is called again
+    (after ``quantize_feedforward(False)``, capture anew).  Each replay launches the same kernels
     as an eager forward, without the per-call host work.
     """
 
@@ -69,12 +74,14 @@ class GraphedForward:
                     module(*self.inputs)
             torch.cuda.current_stream().wait_stream(side)
             self.graph = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(self.graph):
+            with int8_weights_used() as self._int8_weights, torch.cuda.graph(self.graph):
                 self.output = module(*self.inputs)
 
     def __call__(self, *inputs: torch.Tensor) -> Any:
         if len(inputs) != len(self.inputs):
             raise ValueError(f"expected {len(self.inputs)} inputs, got {len(inputs)}")
+        if not all(weights.unchanged() for weights in self._int8_weights):
+            raise RuntimeError("the feed-forward's weights changed after quantize_feedforward(); call it again")
         for dst, src in zip(self.inputs, inputs):
             if src.shape != dst.shape or src.dtype != dst.dtype or src.device != dst.device:
                 raise ValueError("inputs must match the captured shapes, dtypes and device")

@@ -13,8 +13,9 @@ library; in the blocks the norms and the feed-forward run on its kernels too
 from __future__ import annotations
 
 import math
+from contextlib import contextmanager
 from dataclasses import dataclass
-from typing import NamedTuple
+from typing import Iterator, NamedTuple
 
 import torch
 import torch.nn as nn
@@ -898,6 +899,22 @@ class _HipFeedForwardInt8Function(torch.autograd.Function):
         return grad if wants[0] else None, dh, d_w1, d_b1, d_w2, d_b2
 
 
+# The 8-bit weights of the forwards that run, in each of these lists.
+_int8_uses: list[list[_Int8FeedForward]] = []
+
+
+@contextmanager
+def int8_weights_used() -> Iterator[list[_Int8FeedForward]]:
+    """Collects the 8-bit weights that forwards take inside of it."""
+
+    used: list[_Int8FeedForward] = []
+    _int8_uses.append(used)
+    try:
+        yield used
+    finally:
+        _int8_uses.pop()
+
+
 class _Int8FeedForward:
     """A feed-forward's two weights in 8 bits, and what tells whether they still
     stand for the parameters that they were made from."""
@@ -922,6 +939,21 @@ class _Int8FeedForward:
 
         versions = tuple(_version_of(w) for w in self.made_from)
         return None not in versions and versions == self.versions
+
+    def take(self, other: _Int8FeedForward) -> bool:
+        """The other's weights in place of these, in this memory, which captured
+        graphs read; False where the two differ in their layout."""
+
+        for mine, new in zip(self.rows, other.rows):
+            for a, b in zip(mine[:2], new[:2]):
+                if a.shape != b.shape or a.stride() != b.stride() or a.device != b.device:
+                    return False
+        with torch.inference_mode():   # these may have been made there
+            for mine, new in zip(self.rows, other.rows):
+                mine.values.copy_(new.values)
+                mine.scales.copy_(new.scales)
+        self.made_from, self.versions = other.made_from, other.versions
+        return True
 
     # A copied or loaded parameter counts its versions anew: what is kept of them
     # is whether they were the current ones.
@@ -989,9 +1021,13 @@ class DoubleAttentionBlock(nn.Module):
         (``quantize_int8_hip``); activations are quantized for each token in
         every forward.  Call it again after the weights change: a forward that
         finds them replaced or changed in place raises ``RuntimeError`` (writes
-        through ``.data`` and into a captured graph's weights are not seen;
-        weights made under ``torch.inference_mode`` have nothing that would show
-        a change, and are refused); ``enabled=False`` drops the 8-bit weights.  Forwards that autograd
+        through ``.data`` are not seen; weights made under
+        ``torch.inference_mode`` have nothing that would show a change, and are
+        refused).  The new 8-bit weights are written into the memory of the old
+        ones, so that graphs captured with these go on with them;
+        ``enabled=False`` drops the 8-bit weights, and a graph captured by other
+        means than ``GraphedForward``, which keeps them and looks for changed
+        weights, may not be replayed after it.  Forwards that autograd
         records, and those that do not run on the HIP kernels, use the full
         weights as before.
         """
@@ -1005,7 +1041,9 @@ class DoubleAttentionBlock(nn.Module):
         if first.weight.is_inference() or second.weight.is_inference():
             raise ValueError("quantize_feedforward: changes of inference tensors are not seen; make the model outside of "
                              "torch.inference_mode()")
-        self._int8_feedforward = _Int8FeedForward((first.weight, second.weight))
+        kept, new = self._int8_feedforward, _Int8FeedForward((first.weight, second.weight))
+        if kept is None or not kept.take(new):
+            self._int8_feedforward = new
 
     def _int8_weights(self) -> tuple | None:
         """The 8-bit weights, if the feed-forward runs on them."""
@@ -1021,6 +1059,9 @@ class DoubleAttentionBlock(nn.Module):
             or kept.rows[0].values.device != first.device
         ):
             raise RuntimeError("the feed-forward's weights changed after quantize_feedforward(); call it again")
+        for used in _int8_uses:
+            if kept not in used:
+                used.append(kept)
         return kept.rows
 
     def _int8_inference(self, x: Tensor, attended: Tensor) -> tuple | None:
