@@ -14,6 +14,8 @@ Three operators around one format (``QuantizedRows``: signed integers from
 
 As in ``hip_ops``, PyTorch supplies memory and the current stream, and nothing
 falls back to another implementation: a call the kernels do not cover raises.
+``add_rms_norm_hip`` is differentiable; the other calls refuse tensors whose
+gradients autograd would record.
 The kernels run on the inputs' device, whichever is current.
 """
 
@@ -192,6 +194,7 @@ def quantize_int8_hip(x: Tensor, group: int | None = None) -> QuantizedRows:
     """
 
     what = "quantize_int8_hip"
+    _no_grad(what, x)
     code = _check_input(what, x, _CODES)
     if group is not None and group != INT8_GROUP:
         raise NotImplementedError(f"{what}: a scale for each row (group None) or each {INT8_GROUP} columns")
@@ -210,6 +213,7 @@ def dequantize_int8_hip(rows: QuantizedRows, dtype: torch.dtype = torch.bfloat16
     """What the 8-bit rows stand for: ``values * scale``, rounded once to ``dtype``."""
 
     what = "dequantize_int8_hip"
+    _no_grad(what, rows[1])
     _check_quantized(what, rows)
     values, scales, group = rows
     code = dtype_code(dtype)
@@ -273,7 +277,7 @@ def linear_int8_hip(
         raise ValueError(f"{what}: rows of {shape[-1]} columns against a weight of {in_features}")
     *lead, _ = shape
     out_shape = (*lead, out_features)
-    _no_grad(what, x, bias, residual)
+    _no_grad(what, x, x_scales, w_scales, bias, residual)
     bias_ptr, bias_code = None, _lib.DA_F32
     if bias is not None:
         bias_code = _check_param(what, device, bias, out_features)
@@ -410,6 +414,7 @@ def add_rms_norm_backward_hip(
     """
 
     what = "add_rms_norm_backward_hip"
+    _no_grad(what, total, grad, grad_sum, weight)
     code = _check_input(what, total)
     _check_like(what, total, grad)
     shape, device = total.shape, total.device
@@ -468,6 +473,7 @@ def gelu_int8_backward_hip(kept: QuantizedRows, grad: Tensor, *, want_output: bo
     rows stand for; fp32, one rounding to grad's 16-bit type."""
 
     what = "gelu_int8_backward_hip"
+    _no_grad(what, grad, kept[1])
     code = _check_input(what, grad)
     shape, device = grad.shape, grad.device
     _check_quantized(what, kept, device)

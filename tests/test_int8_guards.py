@@ -169,3 +169,56 @@ def test_rows_in_each_others_gaps() -> None:
     assert torch.equal(scales, kept.scales) and torch.equal(store[:, 304:454].view(torch.int8), kept.values)
     assert torch.equal(store[:, 464:764].contiguous().view(torch.float16), da.dequantize_int8_hip(kept, torch.float16))
     assert torch.equal(store[:, :300].contiguous().view(torch.float16), data) and not store[:, 764:].any()
+
+
+def _calls_without_autograd(device):
+    """``(call, the tensors that a gradient could be asked of)`` for each operator
+    but the norm, which has a backward."""
+
+    x, r, g = (torch.randn(4, 128).bfloat16().to(device) for _ in range(3))
+    w, bias = torch.randn(128).to(device), torch.randn(6).to(device)
+    kept = lambda scales: da.QuantizedRows(torch.zeros(4, 128, dtype=torch.int8, device=device), scales)  # noqa: E731
+    weight = lambda scales: da.QuantizedRows(torch.zeros(6, 128, dtype=torch.int8, device=device), scales)  # noqa: E731
+    ones, six = torch.ones(4, 1, device=device), torch.ones(6, 1, device=device)
+    return {
+        "quantize": (lambda x: da.quantize_int8_hip(x), [x]),
+        "dequantize": (lambda scales: da.dequantize_int8_hip(kept(scales)), [ones]),
+        "linear": (lambda x, scales, bias, residual: da.linear_int8_hip(x, weight(scales), bias, residual=residual),
+                   [x, six, bias, torch.zeros(4, 6, dtype=torch.bfloat16, device=device)]),
+        "linear of 8-bit rows": (lambda scales: da.linear_int8_hip(kept(scales), weight(six)), [ones]),
+        "norm in 8 bits": (lambda x, r, w: da.add_rms_norm_int8_hip(x, r, w), [x, r, w]),
+        "norm backward": (lambda s, g, gs, w: da.add_rms_norm_backward_hip(s, g, gs, w), [x, g, r, w]),
+        "gelu": (lambda z: da.gelu_int8_hip(z), [x]),
+        "gelu backward": (lambda scales, g: da.gelu_int8_backward_hip(kept(scales)._replace(group=128), g), [ones, g]),
+    }
+
+
+@pytest.mark.gpu
+def test_tensors_that_require_grad_are_refused() -> None:
+    """No operator drops a gradient that autograd would have recorded."""
+
+    for name, (call, tensors) in _calls_without_autograd(_device()).items():
+        call(*tensors)
+        for i in range(len(tensors)):
+            asked = [t.detach().clone().requires_grad_(i == j) for j, t in enumerate(tensors)]
+            with pytest.raises(ValueError, match="no autograd"):
+                call(*asked)
+            with torch.no_grad():
+                call(*asked)
+
+
+def test_tensors_that_require_grad_are_refused_on_the_host() -> None:
+    x = torch.zeros(4, 128, dtype=torch.bfloat16)
+    scales = torch.ones(4, 1)
+    kept = da.QuantizedRows(torch.zeros(4, 128, dtype=torch.int8), scales)
+    trained, trained_scales = x.clone().requires_grad_(), scales.clone().requires_grad_()
+    for call in (lambda: da.quantize_int8_hip(trained), lambda: da.quantize_int8_hip(trained, 128),
+                 lambda: da.dequantize_int8_hip(kept._replace(scales=trained_scales)),
+                 lambda: da.add_rms_norm_backward_hip(x, trained, None, None),
+                 lambda: da.add_rms_norm_backward_hip(x, x, None, torch.ones(128, requires_grad=True)),
+                 lambda: da.gelu_int8_backward_hip(kept._replace(group=128), trained),
+                 lambda: da.gelu_int8_backward_hip(kept._replace(scales=trained_scales, group=128), x)):
+        with pytest.raises(ValueError, match="no autograd"):
+            call()
+        with torch.no_grad(), pytest.raises(ValueError, match="ROCm device"):
+            call()
