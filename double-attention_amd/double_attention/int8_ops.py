@@ -25,6 +25,7 @@ from typing import NamedTuple
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import _lib
 from .hip_ops import _stream, dtype_code
@@ -105,7 +106,17 @@ def _check_param(what: str, device: torch.device, t: Tensor, size: int) -> int:
     return code
 
 
+def _has_tangent(*tensors: Tensor | None) -> bool:
+    """Whether one of the tensors carries a forward-mode tangent (under torch.no_grad(), too)."""
+
+    return forward_ad._current_level >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors
+    )
+
+
 def _no_grad(what: str, *tensors: Tensor | None) -> None:
+    if _has_tangent(*tensors):
+        raise ValueError(f"{what} has no forward-mode derivative: detach its inputs")
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
@@ -374,10 +385,13 @@ def add_rms_norm_hip(
     itself without a residual) and its root-mean-square norm
     ``n = s / sqrt(mean(s^2) + eps) * weight`` over the last dimension (at most
     16384 wide), statistics in fp32 and one rounding; one launch.
-    Differentiable in x, the residual and the weight, through both outputs.
+    Differentiable in x, the residual and the weight, through both outputs (in
+    reverse mode; tensors with forward-mode tangents are refused).
     """
 
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight)):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight)) or _has_tangent(
+        x, residual, weight
+    ):   # which has no forward-mode derivative, and says so
         got = _AddRmsNormFunction.apply(x, residual, weight, eps)
         return (got, x) if residual is None else got
     out, _, _, total = _add_rms_norm("add_rms_norm_hip", x, residual, weight, eps, True, False)

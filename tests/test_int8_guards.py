@@ -222,3 +222,30 @@ def test_tensors_that_require_grad_are_refused_on_the_host() -> None:
             call()
         with torch.no_grad(), pytest.raises(ValueError, match="ROCm device"):
             call()
+
+
+@pytest.mark.gpu
+def test_tensors_with_tangents_are_refused() -> None:
+    """No operator drops a forward-mode tangent, whether autograd records or not."""
+
+    calls = _calls_without_autograd(_device())
+    norm, tensors = calls["norm in 8 bits"]
+    calls["norm"] = (da.add_rms_norm_hip, tensors)
+    with torch.autograd.forward_ad.dual_level():
+        for name, (call, tensors) in calls.items():
+            call(*tensors)
+            for i in range(len(tensors)):
+                dual = [torch.autograd.forward_ad.make_dual(t, t) if i == j else t for j, t in enumerate(tensors)]
+                for grad in (True, False):
+                    with torch.set_grad_enabled(grad), pytest.raises((ValueError, NotImplementedError), match="forward.mode"):
+                        call(*dual)
+
+
+def test_tensors_with_tangents_are_refused_on_the_host() -> None:
+    x = torch.zeros(4, 128, dtype=torch.bfloat16)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, x)
+        for call in (lambda: da.quantize_int8_hip(dual), lambda: da.add_rms_norm_int8_hip(x, dual),
+                     lambda: da.add_rms_norm_backward_hip(x, dual, None, None)):
+            with pytest.raises(ValueError, match="forward-mode"):
+                call()
