@@ -978,6 +978,10 @@ class DoubleAttentionBlock(nn.Module):
     feed-forward on 8-bit integers.
     """
 
+    # Blocks that were saved whole before they had these attributes have the defaults.
+    activation_checkpoint: str | None = None
+    _int8_feedforward: _Int8FeedForward | None = None   # set by quantize_feedforward
+
     def __init__(
         self,
         config: DoubleAttentionConfig,
@@ -1011,8 +1015,6 @@ class DoubleAttentionBlock(nn.Module):
             nn.Linear(feedforward_dim, config.model_dim),
             nn.Dropout(dropout),
         )
-        # Set by quantize_feedforward.
-        self._int8_feedforward: _Int8FeedForward | None = None
 
     def quantize_feedforward(self, enabled: bool = True) -> None:
         """Run the feed-forward on 8-bit integers in inference on the HIP kernels.

@@ -92,6 +92,37 @@ def test_inference_tensors_as_weights(monkeypatch) -> None:
             other._int8_weights()
 
 
+def _saved_before(block):
+    """The block as an older version saved it whole."""
+
+    state = block.__dict__.copy()
+    state.pop("activation_checkpoint")
+    state.pop("_int8_feedforward", None)
+    other = block.__class__.__new__(block.__class__)
+    other.__setstate__(state)
+    return other
+
+
+def test_block_that_was_saved_without_the_attributes(monkeypatch) -> None:
+    block = _host_block(monkeypatch)
+    bank = da.SharedDictionaryBank(8, 16)
+    x = torch.randn(2, 5, 32, generator=torch.Generator().manual_seed(1))
+    old = _saved_before(block)
+    assert torch.equal(old(x, bank), block(x, bank))
+    old.quantize_feedforward()
+    assert old._int8_weights() is not None and block._int8_weights() is None
+
+
+@pytest.mark.gpu
+def test_old_block_on_the_kernels() -> None:
+    block, bank = _block(torch.bfloat16)
+    old = _saved_before(block)
+    x = _randn(2, 33, 128, seed=1, dtype=torch.bfloat16)
+    with torch.no_grad():
+        assert torch.equal(old(x, bank), block(x, bank))
+    assert torch.equal(old(x, bank), block(x, bank))
+
+
 @pytest.mark.gpu
 def test_forward_of_a_copied_quantized_block() -> None:
     block, bank = _block(torch.bfloat16, norm="rms")
