@@ -645,15 +645,23 @@ static I8Plan plan_linear_int8(int64_t rows, int64_t K, int64_t N, bool quantize
   // (32 x 4096 -> 4096: 8.5 of the split K against 11.0 of the 64-tiles; 64 rows: 12.9 against 11.0.)
   if (rows <= kFewRows && (!quantize || K <= kFewCols)) return I8Plan::kFew;
   if (rows <= 32 && !quantize) return I8Plan::kFew32;
-  // 16-bit tokens are quantized again by every workgroup that multiplies them:
-  // as fast as a launch of its own for that, or nearly, while the workgroups
-  // are one round (4096 x 512 -> 512 7.6 against 8.6, 1024 x 512 -> 1536 7.4
-  // against 7.6, 64 x 512 -> 1536 6.3 against 6.3, 777 x 1000 -> 1111 9.8 against
-  // 9.2), and the call has one launch less, 3 us of the host's time.  Beyond, whole
-  // calls differ little either way (4096 x 512 -> 1536 16.0 against 15.8, 8192 x 512
-  // -> 1024 16.6 against 15.5, 32768 x 512 -> 512 29.9 against 26.5, but 16384 x 512
-  // -> 640 20.1 against 23.1), and with K over 512 it loses (4096 x 1024
-  // -> 1024 19 against 14).
+  // 16-bit tokens are quantized again by every workgroup that multiplies them,
+  // instead of once in a launch of its own.  While the workgroups are one round
+  // and K is at most 512, that is faster (both from a captured graph: 4096 x 512
+  // -> 512 6.8 against 8.2, 1024 x 512 -> 1536 6.7 against 7.3, 64 x 512 -> 1536 5.8
+  // against 6.0, 16384 x 512 -> 256 9.6 against 13.7).  With K up to 1024 it is
+  // as fast or up to a fifth slower on the GPU (777 x 1000 -> 1111 8.7 against 8.8,
+  // 300 x 1000 -> 300 8.3 against 7.7, 64 x 1024 -> 1024 7.8 against 7.2, 200 x 700
+  // -> 2000 8.6 against 7.1): taken for the host's 3 us of a launch, which bound
+  // such a call; a captured graph, which has no host to wait for, is the slower
+  // for it.  Over 1024 it loses (2500 x 1300 -> 3000 64 against 26).
+  // Beyond one round whole calls go either way: the tiles take 16384 x 512 -> 640 in
+  // 20.1 against 23.1, 16384 x 512 -> 512 with GELU 19.8 against 22.6, 32768 x 256
+  // -> 256 15.3 against 18.0 and 32768 x 384 -> 256 16.3 against 19.1, are alike at
+  // 4096 x 512 -> 1536 (16.0 and 15.8) and 16384 x 512 -> 768 (23.2 and 23.3), and
+  // lose at 32768 x 512 -> 512 (29.9 against 26.5), 65536 x 512 -> 512 (57.6 against
+  // 49.5), 16384 x 300 -> 512 (17.8 against 16.6) and, with K over 512, 4096 x 1024
+  // -> 1024 (19 against 14): the launch is taken there.
   // Between the two tiles: 64 x 512 -> 1536, 24 64-tiles, 6.3 against 6.8; 1024 x
   // 512 -> 1536, 384 of them, 9.2 against 7.4.
   if (quantize && K <= 1024 && tiles_of(rows, N, 64, 64) <= 256) return K <= 512 ? I8Plan::kToken64 : I8Plan::kToken64x1024;

@@ -208,8 +208,8 @@ __device__ __forceinline__ float wave_sum_dpp(float v) { return group_sum(row16_
 //     the scale is exact, amax = 127 scale: 254 for bf16, a power of two as a
 //     scale, where x * inverse is exact too; 127 j, j <= 16, for fp16, where
 //     eight rows of 1024 take the division's steps (fp32 rows take them all).
-// Checked against fp32 division for every pair of values up to 2^-11 of each
-// other.
+// The tests hold every pair of significands up to 2^-11 of each other against
+// fp32 division.  (The norm's rows are not such floats: rms_norm.hip.)
 template <typename T> inline constexpr bool kInt8Divides = true;        // all of fp32's rows
 template <> inline constexpr bool kInt8Divides<__bf16> = false;
 struct Int8Scale {

@@ -8,7 +8,10 @@
 // One pass over memory: NT threads hold a row in registers (CH chunks of
 // eight columns each).  The scale of the integers needs no second reduction:
 // max |n| = rstd max |s w|, so the sum of squares and the largest |s w| are
-// reduced together, and q = rint(s w (rstd / scale)).
+// reduced together, and q = rint(s w (rstd / scale)): one multiplication by a
+// rounded factor, so where n / scale is within its roundings (some 2^-15 of a
+// step) of a half of a step, either neighbour may come out.  Products s w of 16-bit
+// numbers do have exact halves of steps: max |s w| / 2 without weights.
 //
 // Backward at dy = dL/dn and ds = dL/ds (the gradient that reaches s past the
 // norm), with xh = s rstd and g = dy w:
@@ -152,7 +155,7 @@ __global__ __launch_bounds__(row_block<NT>()) void row_int8_kernel(RowInt8Args a
     }
     if (a.values == nullptr) return;
   }
-  // The norm's values are no 16-bit floats: one rounding of x * inverse.
+  // The norm's values are no 16-bit floats: one rounding of s w * inverse.
   const Int8Scale s = NORM ? int8_scale<float>(amax, rstd) : int8_scale<T>(amax);
   // A row whose scale is the floor may have an inverse beyond fp32.
   const float inverse = fminf(rstd * s.inverse, 3.4028234e38f);

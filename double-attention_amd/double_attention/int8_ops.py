@@ -402,8 +402,9 @@ def add_rms_norm_int8_hip(
     x: Tensor, residual: Tensor | None = None, weight: Tensor | None = None, eps: float = 1e-6
 ) -> tuple[QuantizedRows, Tensor]:
     """``add_rms_norm_hip`` with its norm in 8 bits, a scale for each row: the
-    fp32 norm is quantized without a rounding to 16 bits in between.  The sum
-    stays 16-bit.  For inference: no backward."""
+    fp32 norm is quantized without a rounding to 16 bits in between, by one
+    multiplication (a value within fp32's roundings of a half of a step may
+    become either neighbour).  The sum stays 16-bit.  For inference: no backward."""
 
     what = "add_rms_norm_int8_hip"
     _no_grad(what, x, residual, weight)

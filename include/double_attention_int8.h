@@ -21,7 +21,9 @@ extern "C" {
  * fp32 scale for the whole row (group 0) or for each 128 columns of it (group
  * 128, DA_INT8_GROUP; the last group may be shorter):
  *   scale = max(amax, 127 * 2^-126) / 127,  q = rint(x / scale) in [-127, 127]
- * with fp32's division and ties to even; scale is amax times fp32's 1 / 127.
+ * with fp32's division and ties to even; scale is amax times fp32's 1 / 127
+ * (da_add_rms_norm multiplies by rstd / scale instead: where n / scale is within
+ * fp32's roundings of a half, its q may be either neighbour).
  * A row (group) that holds an infinity or a NaN gets the scale NaN and zeros:
  * all of it then stands for NaN.  values: [rows] rows at a pitch ldv that is a
  * multiple of 16 (>= cols), 16-byte aligned; the bytes of a row's last chunk
