@@ -1023,7 +1023,7 @@ class DoubleAttentionBlock(nn.Module):
         (``quantize_int8_hip``); activations are quantized for each token in
         every forward.  Call it again after the weights change: a forward that
         finds them replaced or changed in place raises ``RuntimeError`` (writes
-        through ``.data`` are not seen; weights made under
+        through ``.data`` and by a captured graph are not seen; weights made under
         ``torch.inference_mode`` have nothing that would show a change, and are
         refused).  The new 8-bit weights are written into the memory of the old
         ones, so that graphs captured with these go on with them;
