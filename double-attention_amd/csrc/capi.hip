@@ -732,55 +732,52 @@ int validate_int8(const char* what, const char* name, const void* values, int64_
   return DA_OK;
 }
 
-// The memory of a tensor: `rows` spans of `cols` elements, `ld` elements apart.
-struct Rows {
-  const void* p;
-  int64_t rows, cols, ld, bytes;
-};
-Rows flat(const void* p, int64_t count, int64_t bytes) { return {p, 1, count, count, bytes}; }
-// 8-bit rows that a call writes: with the rest of the last chunk of 16.
-Rows written_int8(const void* p, int64_t rows, int64_t cols, int64_t ldv) { return {p, rows, da::round_up(cols, 16), ldv, 1}; }
-
-// Whether two tensors share a byte.  Rows of a between rows of b (columns of one
-// wider matrix) do not; where both have gaps and their pitches differ, their
-// ranges decide.
-bool overlap(const Rows& a, const Rows& b) {
+// The bytes of a tensor: `count` spans of `length`, `pitch` apart, up to `last`.
+struct Spans {
   typedef __int128 wide;
-  struct Spans {
-    wide first, count, length, pitch;
-  };
-  const auto spans = [](const Rows& r) {
-    Spans s{static_cast<wide>(reinterpret_cast<uintptr_t>(r.p)), r.rows, static_cast<wide>(r.cols) * r.bytes,
-            static_cast<wide>(r.ld) * r.bytes};
-    if (s.pitch == s.length) {
-      s.length *= s.count;
-      s.count = 1;
+  wide first, last, count, length, pitch;
+  // `rows` rows of `cols` elements of `bytes`, `ld` elements apart; nothing for a null pointer.
+  Spans(const void* p, int64_t rows, int64_t cols, int64_t ld, int64_t bytes)
+      : first(reinterpret_cast<uintptr_t>(p)), last(first), count(p ? rows : 0), length(static_cast<wide>(cols) * bytes),
+        pitch(static_cast<wide>(ld) * bytes) {
+    if (count > 0) last = first + (count - 1) * pitch + length;
+    if (count > 1 && pitch == length) {
+      length *= count;
+      count = 1;
     }
-    return s;
-  };
-  Spans x = spans(a), y = spans(b);
-  if (!a.p || !b.p || x.count < 1 || y.count < 1) return false;
-  if (x.first + (x.count - 1) * x.pitch + x.length <= y.first || y.first + (y.count - 1) * y.pitch + y.length <= x.first) return false;
+  }
+};
+Spans flat(const void* p, int64_t count, int64_t bytes) { return {p, 1, count, count, bytes}; }
+// 8-bit rows that a call writes: with the rest of the last chunk of 16.
+Spans written_int8(const void* p, int64_t rows, int64_t cols, int64_t ldv) { return {p, rows, da::round_up(cols, 16), ldv, 1}; }
+
+// Whether spans whose ranges meet share a byte.  Rows of x between rows of y
+// (columns of one wider matrix) do not; where both have gaps and their pitches
+// differ, their ranges decide.
+bool share_a_byte(Spans x, Spans y) {
+  typedef Spans::wide wide;
   // A single span has whichever pitch suits.
   if (x.count == 1) x.pitch = y.pitch;
   if (y.count == 1) y.pitch = x.pitch;
-  if (x.count == 1 && y.count == 1) return true;
-  if (x.pitch != y.pitch) return true;
+  if ((x.count == 1 && y.count == 1) || x.pitch != y.pitch) return true;
   // Spans i of x and j of y meet where -y.length < apart + k pitch < x.length with k = j - i.
   const auto floor_div = [](wide n, wide d) { return n / d - (n % d != 0 && n < 0 ? 1 : 0); };
   const wide apart = y.first - x.first, pitch = x.pitch;
   const wide least = floor_div(-y.length - apart, pitch) + 1, most = -floor_div(apart - x.length, pitch) - 1;
   return (least > -(x.count - 1) ? least : -(x.count - 1)) <= (most < y.count - 1 ? most : y.count - 1);
 }
+bool overlap(const Spans& x, const Spans& y) {
+  return x.count > 0 && y.count > 0 && x.first < y.last && y.first < x.last && share_a_byte(x, y);
+}
 
 // Workgroups read rows that others write without an order between them, and a
 // row's last columns in loads that begin before them: what a call writes stays
 // off what it reads, and off what else it writes.
-int validate_apart(const char* what, std::initializer_list<Rows> outputs, std::initializer_list<Rows> inputs) {
-  for (const Rows* out = outputs.begin(); out != outputs.end(); ++out) {
-    for (const Rows& in : inputs)
+int validate_apart(const char* what, std::initializer_list<Spans> outputs, std::initializer_list<Spans> inputs) {
+  for (const Spans* out = outputs.begin(); out != outputs.end(); ++out) {
+    for (const Spans& in : inputs)
       if (overlap(*out, in)) return fail(DA_ERR_INVALID_ARGUMENT, "%s: an output overlaps an input", what);
-    for (const Rows* other = out + 1; other != outputs.end(); ++other)
+    for (const Spans* other = out + 1; other != outputs.end(); ++other)
       if (overlap(*out, *other)) return fail(DA_ERR_INVALID_ARGUMENT, "%s: an output overlaps another output", what);
   }
   return DA_OK;

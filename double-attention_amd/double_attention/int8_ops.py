@@ -107,15 +107,14 @@ def _check_param(what: str, device: torch.device, t: Tensor, size: int) -> int:
 
 
 def _has_tangent(*tensors: Tensor | None) -> bool:
-    """Whether one of the tensors carries a forward-mode tangent (under torch.no_grad(), too)."""
+    """Whether one of the tensors carries a forward-mode tangent (under
+    torch.no_grad(), too).  There are tangents from level 0 on."""
 
-    return forward_ad._current_level >= 0 and any(
-        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors
-    )
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def _no_grad(what: str, *tensors: Tensor | None) -> None:
-    if _has_tangent(*tensors):
+    if forward_ad._current_level >= 0 and _has_tangent(*tensors):
         raise ValueError(f"{what} has no forward-mode derivative: detach its inputs")
     if torch.is_grad_enabled():
         for t in tensors:
@@ -389,8 +388,8 @@ def add_rms_norm_hip(
     reverse mode; tensors with forward-mode tangents are refused).
     """
 
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight)) or _has_tangent(
-        x, residual, weight
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight)) or (
+        forward_ad._current_level >= 0 and _has_tangent(x, residual, weight)
     ):   # which has no forward-mode derivative, and says so
         got = _AddRmsNormFunction.apply(x, residual, weight, eps)
         return (got, x) if residual is None else got
