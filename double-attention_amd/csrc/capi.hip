@@ -7,55 +7,24 @@
 // stream is untouched; launch failures are reported from hipGetLastError.
 #include <algorithm>
 #include <cmath>
-#include <cstdarg>
-#include <cstdio>
 #include <initializer_list>
 #include <mutex>
-#include <string>
 
 #include "../../include/double_attention_hip.h"
 #include "../../include/double_attention_int8.h"
+#include "da_capi.h"
 #include "da_launch.h"
 #include "dict_norm.h"
 #include "int8_rows.h"
 
+using namespace da::capi;
+
 namespace {
 
-thread_local std::string g_error;
-
-int fail(int code, const char* fmt, ...) {
-  char buf[512];
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(buf, sizeof(buf), fmt, ap);
-  va_end(ap);
-  g_error = buf;
-  return code;
-}
-
-bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) % bytes) == 0; }
 bool pow2_width(int64_t v) { return v == 64 || v == 128 || v == 256 || v == 512; }
 // The attention forward takes value (model) widths that are multiples of 64:
 // its value slices are 64, 128 or 256 features wide.
 constexpr int64_t kMaxValueDim = 4096;
-bool half_dtype(int d) { return d == DA_F16 || d == DA_BF16; }
-bool any_dtype(int d) { return d == DA_F32 || d == DA_F16 || d == DA_BF16; }
-
-int ok() {
-  g_error.clear();
-  return DA_OK;
-}
-
-int check_launch(const char* what) {
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return fail(DA_ERR_LAUNCH, "%s: launch failed: %s", what, hipGetErrorString(e));
-  g_error.clear();
-  return DA_OK;
-}
-
-constexpr int64_t kAlign = 256;
-int64_t align_up(int64_t v) { return (v + kAlign - 1) / kAlign * kAlign; }
-
 constexpr int kRouteFlagMask = DA_ROUTE_NORMALIZE_INPUT | DA_ROUTE_NORMALIZE_OUTPUT | DA_ROUTE_BETA_IS_LOG |
                                DA_ROUTE_UNIT_KEYS | DA_ROUTE_SILU_LOGITS | DA_ROUTE_STANDARDIZE |
                                DA_ROUTE_DIRECT_SILU;
@@ -127,7 +96,7 @@ extern "C" {
 static_assert(DA_OUT_SPLIT == da::kOutSplit, "split-output flag");
 static_assert(DA_ROUTE_BETA_IS_LOG_SCALE == da::kRouteBetaIsLogScale, "route flag");
 
-int da_abi_version(void) { return 20; }
+int da_abi_version(void) { return 21; }
 
 const char* da_last_error(void) { return g_error.c_str(); }
 
@@ -711,8 +680,6 @@ static_assert(DA_INT8_GROUP == da::kInt8Group && DA_I8 == da::kI8, "columns per 
 constexpr int64_t kInt8MaxElements = 1LL << 40;
 constexpr int64_t kInt8MaxPitch = 1 << 23;   // of 8-bit rows: 256 of them span less than 2^32 bytes
 
-int64_t element_bytes(int dtype) { return dtype == DA_F32 ? 4 : 2; }
-
 // Rows of a 16-bit or fp32 matrix.
 int validate_rows(const char* what, const char* name, const void* p, int64_t cols, int64_t ld, int dtype) {
   if (!p) return fail(DA_ERR_INVALID_ARGUMENT, "%s: %s is null", what, name);
@@ -729,57 +696,6 @@ int validate_int8(const char* what, const char* name, const void* values, int64_
     return fail(DA_ERR_ALIGNMENT, "%s: %s must be 16-byte aligned at a pitch of a multiple of 16", what, name);
   if (ldv < cols) return fail(DA_ERR_INVALID_ARGUMENT, "%s: %s has a pitch below its width", what, name);
   if (ldv > kInt8MaxPitch) return fail(DA_ERR_UNSUPPORTED, "%s: %s has a pitch over 2^23", what, name);
-  return DA_OK;
-}
-
-// The bytes of a tensor: `count` spans of `length`, `pitch` apart, up to `last`.
-struct Spans {
-  typedef __int128 wide;
-  wide first, last, count, length, pitch;
-  // `rows` rows of `cols` elements of `bytes`, `ld` elements apart; nothing for a null pointer.
-  Spans(const void* p, int64_t rows, int64_t cols, int64_t ld, int64_t bytes)
-      : first(reinterpret_cast<uintptr_t>(p)), last(first), count(p ? rows : 0), length(static_cast<wide>(cols) * bytes),
-        pitch(static_cast<wide>(ld) * bytes) {
-    if (count > 0) last = first + (count - 1) * pitch + length;
-    if (count > 1 && pitch == length) {
-      length *= count;
-      count = 1;
-    }
-  }
-};
-Spans flat(const void* p, int64_t count, int64_t bytes) { return {p, 1, count, count, bytes}; }
-// 8-bit rows that a call writes: with the rest of the last chunk of 16.
-Spans written_int8(const void* p, int64_t rows, int64_t cols, int64_t ldv) { return {p, rows, da::round_up(cols, 16), ldv, 1}; }
-
-// Whether spans whose ranges meet share a byte.  Rows of x between rows of y
-// (columns of one wider matrix) do not; where both have gaps and their pitches
-// differ, their ranges decide.
-bool share_a_byte(Spans x, Spans y) {
-  typedef Spans::wide wide;
-  // A single span has whichever pitch suits.
-  if (x.count == 1) x.pitch = y.pitch;
-  if (y.count == 1) y.pitch = x.pitch;
-  if ((x.count == 1 && y.count == 1) || x.pitch != y.pitch) return true;
-  // Spans i of x and j of y meet where -y.length < apart + k pitch < x.length with k = j - i.
-  const auto floor_div = [](wide n, wide d) { return n / d - (n % d != 0 && n < 0 ? 1 : 0); };
-  const wide apart = y.first - x.first, pitch = x.pitch;
-  const wide least = floor_div(-y.length - apart, pitch) + 1, most = -floor_div(apart - x.length, pitch) - 1;
-  return (least > -(x.count - 1) ? least : -(x.count - 1)) <= (most < y.count - 1 ? most : y.count - 1);
-}
-bool overlap(const Spans& x, const Spans& y) {
-  return x.count > 0 && y.count > 0 && x.first < y.last && y.first < x.last && share_a_byte(x, y);
-}
-
-// Workgroups read rows that others write without an order between them, and a
-// row's last columns in loads that begin before them: what a call writes stays
-// off what it reads, and off what else it writes.
-int validate_apart(const char* what, std::initializer_list<Spans> outputs, std::initializer_list<Spans> inputs) {
-  for (const Spans* out = outputs.begin(); out != outputs.end(); ++out) {
-    for (const Spans& in : inputs)
-      if (overlap(*out, in)) return fail(DA_ERR_INVALID_ARGUMENT, "%s: an output overlaps an input", what);
-    for (const Spans* other = out + 1; other != outputs.end(); ++other)
-      if (overlap(*out, *other)) return fail(DA_ERR_INVALID_ARGUMENT, "%s: an output overlaps another output", what);
-  }
   return DA_OK;
 }
 

@@ -4,7 +4,8 @@ Public names follow the reference package's API (reference
 ``src/double_attention/__init__.py:1-47``) for the attention path; the
 additions are ``backend="hip"`` in the config, ``HIP_AVAILABLE``, the gfx950
 operator functions ``dictionary_route_hip`` / ``routed_attention_hip``, and
-the 8-bit operators of the feed-forward (``int8_ops``).
+the 8-bit operators of the feed-forward (``int8_ops``) and the serving
+operators around a paged cache (``serving_ops``).
 """
 
 from . import _lib
@@ -32,6 +33,17 @@ from .modules import (
     SharedDictionaryBank,
 )
 from .ops import assemble_score_maps, dictionary_route_reference, routed_attention_reference
+from .serving_ops import (
+    PagedCache,
+    TokenLogProbs,
+    cache_append_hip,
+    cache_compact_hip,
+    cache_select_hip,
+    paged_attention_hip,
+    paged_attention_weights_hip,
+    paged_cache,
+    token_log_probs_hip,
+)
 from .triton_kernels import TRITON_AVAILABLE
 
 HIP_AVAILABLE = _lib.available()
@@ -45,14 +57,19 @@ __all__ = [
     "GraphedForward",
     "HIP_AVAILABLE",
     "INT8_GROUP",
+    "PagedCache",
     "QuantizedRows",
     "SharedDictionaryAttention",
     "SharedDictionaryBank",
     "TRITON_AVAILABLE",
+    "TokenLogProbs",
     "add_rms_norm_backward_hip",
     "add_rms_norm_hip",
     "add_rms_norm_int8_hip",
     "assemble_score_maps",
+    "cache_append_hip",
+    "cache_compact_hip",
+    "cache_select_hip",
     "dequantize_int8_hip",
     "dictionary_normalize_hip",
     "dictionary_route_hip",
@@ -64,7 +81,11 @@ __all__ = [
     "linear_int8_hip",
     "load_model_from_checkpoint",
     "load_training_checkpoint",
+    "paged_attention_hip",
+    "paged_attention_weights_hip",
+    "paged_cache",
     "quantize_int8_hip",
     "routed_attention_hip",
     "routed_attention_reference",
+    "token_log_probs_hip",
 ]

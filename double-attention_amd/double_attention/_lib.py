@@ -1,5 +1,5 @@
-"""ctypes binding of the gfx950 C ABI (``include/double_attention_hip.h`` and
-``include/double_attention_int8.h``).
+"""ctypes binding of the gfx950 C ABI (``include/double_attention_hip.h``,
+``include/double_attention_int8.h`` and ``include/double_attention_serving.h``).
 
 The library is built in-tree by ``double-attention_amd/build.py`` into
 ``double_attention/lib/libdouble_attention_hip.so``.  Loading needs no GPU
@@ -51,9 +51,10 @@ ERROR_NAMES = {
     -5: "workspace too small",
 }
 
-ABI_VERSION = 20
+ABI_VERSION = 21
 INT8_GROUP = 128
 NOALLOC_SCRATCH_BYTES = 128 << 20
+MAX_TOP = 64
 
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -143,6 +144,56 @@ class AttentionBackwardArgs(ctypes.Structure):
         ("grad_value_sum", _vp),
         ("grad_scores", _vp),
         ("grad_scores_ld", _i64),
+    ]
+
+
+class PagedCacheArgs(ctypes.Structure):
+    """Mirror of ``da_paged_cache``."""
+
+    _fields_ = [
+        ("keys", _vp),
+        ("key_page_stride", _i64),
+        ("values", _vp),
+        ("value_page_stride", _i64),
+        ("pages", _i64),
+        ("page_size", _i64),
+        ("key_width", _i64),
+        ("value_dim", _i64),
+        ("page_table", _vp),
+        ("ld_table", _i64),
+        ("table_pages", _i64),
+    ]
+
+
+class PagedAttentionArgs(ctypes.Structure):
+    """Mirror of ``da_paged_attention_args``."""
+
+    _fields_ = [
+        ("cache", PagedCacheArgs),
+        ("query", _vp),
+        ("ldq", _i64),
+        ("rows", _i64),
+        ("lengths", _vp),
+        ("offsets", _vp),
+        ("sequences", _i64),
+        ("scales", _vp),
+        ("scales_dtype", _i32),
+        ("scale_mult", _f32),
+        ("maps", _i64),
+        ("score_dim", _i64),
+        ("map_repeat", _i64),
+        ("causal", _i32),
+        ("mix", _vp),
+        ("qk_dtype", _i32),
+        ("v_dtype", _i32),
+        ("out", _vp),
+        ("weights_in", _vp),
+        ("weights_out", _vp),
+        ("ld_weights", _i64),
+        ("max_chunk", _i64),
+        ("max_length", _i64),
+        ("workspace", _vp),
+        ("workspace_bytes", _i64),
     ]
 
 
@@ -243,6 +294,25 @@ INT8_SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "da_gelu_int8_backward": (_i32, [_vp, _i64, _i64, _i64, _vp, _vp, _i64, _i32, _vp, _vp, _vp]),
 }
 
+_cache_p = ctypes.POINTER(PagedCacheArgs)
+# The serving operators, declared in include/double_attention_serving.h.
+SERVING_SIGNATURES: dict[str, tuple[object, list[object]]] = {
+    "da_cache_append": (_i32, [_cache_p, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp]),
+    "da_paged_attention_workspace_bytes": (_i64, [ctypes.POINTER(PagedAttentionArgs)]),
+    "da_paged_attention": (_i32, [ctypes.POINTER(PagedAttentionArgs), _vp]),
+    "da_cache_select": (_i32, [_vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp]),
+    "da_cache_compact": (_i32, [_cache_p, _cache_p, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _vp]),
+    "da_token_log_probs_workspace_bytes": (_i64, [_i64, _i64, _i64]),
+    "da_token_log_probs": (
+        _i32,
+        [_vp, _i64, _i64, _i64, _i32, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _vp],
+    ),
+    "da_token_log_probs_backward": (
+        _i32,
+        [_vp, _i64, _i64, _i64, _i32, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp],
+    ),
+}
+
 _lib: ctypes.CDLL | None = None
 _load_error: str | None = None
 
@@ -259,7 +329,7 @@ def _load() -> ctypes.CDLL:
             f"{path} does not exist; build it with `python double-attention_amd/build.py`"
         )
     lib = ctypes.CDLL(str(path))
-    for name, (restype, argtypes) in {**SIGNATURES, **INT8_SIGNATURES}.items():
+    for name, (restype, argtypes) in {**SIGNATURES, **INT8_SIGNATURES, **SERVING_SIGNATURES}.items():
         fn = getattr(lib, name)  # AttributeError if the symbol is missing
         fn.restype = restype
         fn.argtypes = argtypes
