@@ -21,10 +21,10 @@ constexpr int64_t kMaxStride = 1LL << 40;
 int validate_cache(const char* what, const da_paged_cache& c, int64_t sequences) {
   if (c.page_size < 32 || c.page_size % 32 || c.page_size > 4096)
     return fail(DA_ERR_UNSUPPORTED, "%s: page_size %lld must be a multiple of 32 in [32, 4096]", what, (long long)c.page_size);
-  if (c.key_width < 32 || c.key_width % 32 || c.key_width > 1024)
-    return fail(DA_ERR_UNSUPPORTED, "%s: key_width %lld must be a multiple of 32 in [32, 1024]", what, (long long)c.key_width);
-  if (c.value_dim < 16 || c.value_dim % 16 || c.value_dim > 4096)
-    return fail(DA_ERR_UNSUPPORTED, "%s: value_dim %lld must be a multiple of 16 in [16, 4096]", what, (long long)c.value_dim);
+  if (c.key_width < 64 || c.key_width % 64 || c.key_width > 1024)
+    return fail(DA_ERR_UNSUPPORTED, "%s: key_width %lld must be a multiple of 64 in [64, 1024]", what, (long long)c.key_width);
+  if (c.value_dim < 64 || c.value_dim % 64 || c.value_dim > 4096)
+    return fail(DA_ERR_UNSUPPORTED, "%s: value_dim %lld must be a multiple of 64 in [64, 4096]", what, (long long)c.value_dim);
   if (c.pages < 1 || c.pages > 0x7fffffff) return fail(DA_ERR_INVALID_ARGUMENT, "%s: the cache has no pages", what);
   if (sequences < 0 || sequences > kMaxSequences)
     return fail(DA_ERR_UNSUPPORTED, "%s: sequences must be in [0, %lld]", what, (long long)kMaxSequences);
@@ -42,7 +42,7 @@ int validate_cache(const char* what, const da_paged_cache& c, int64_t sequences)
 
 da::CacheView view(const da_paged_cache& c) {
   return {c.keys, c.key_page_stride, c.values, c.value_page_stride, static_cast<int>(c.pages), static_cast<int>(c.page_size / 32),
-          static_cast<int>(c.key_width), static_cast<int>(c.value_dim), c.page_table, c.ld_table, static_cast<int>(c.table_pages)};
+          c.page_size == 32 ? 0u : static_cast<uint32_t>((0xffffffffu + c.page_size / 32) / (c.page_size / 32)), static_cast<int>(c.key_width), static_cast<int>(c.value_dim), c.page_table, c.ld_table, static_cast<int>(c.table_pages)};
 }
 Spans pages_of(const void* p, const da_paged_cache& c, int64_t width, int64_t stride) {
   return {p, c.pages, c.page_size * width, stride, 2};
@@ -73,8 +73,8 @@ int attention_args(const da_paged_attention_args& a, da::PagedAttentionArgs& r) 
   if (!types_ok)
     return fail(DA_ERR_UNSUPPORTED, "%s: (qk_dtype, v_dtype) must be (F16,BF16), (F16,F16) or (BF16,BF16)", what);
   if (a.maps < 1 || a.maps > 64 || a.map_repeat < 1) return fail(DA_ERR_UNSUPPORTED, "%s: 1 to 64 maps", what);
-  if (a.score_dim < 32 || a.score_dim % 32 || a.score_dim > 512)
-    return fail(DA_ERR_UNSUPPORTED, "%s: score_dim %lld must be a multiple of 32 in [32, 512]", what, (long long)a.score_dim);
+  if (a.score_dim < 64 || a.score_dim % 64 || a.score_dim > 512)
+    return fail(DA_ERR_UNSUPPORTED, "%s: score_dim %lld must be a multiple of 64 in [64, 512]", what, (long long)a.score_dim);
   if (a.maps % a.map_repeat || a.maps / a.map_repeat * a.score_dim > a.cache.key_width)
     return fail(DA_ERR_INVALID_ARGUMENT, "%s: the maps' features do not fit the keys' %lld", what, (long long)a.cache.key_width);
   if (!any_dtype(a.scales_dtype) || !std::isfinite(a.scale_mult))

@@ -18,12 +18,31 @@ struct CacheView {
   int64_t value_page;
   int pages;
   int tiles;            // 32-token tiles of a page
+  uint32_t tiles_inv;   // ceil(2^32 / tiles), 0 for one tile
   int W;                // key features of a token (all branches)
   int D;
   const int32_t* table; // [sequences][ld_table]: the pages of each sequence, in order
   int64_t ld_table;
   int table_pages;      // entries of a row that are read
 };
+
+// Tile kt of a sequence: tile kt % tiles of the page in entry kt / tiles (exact
+// for kt below 2^25: the product's error is at most kt * tiles, tiles <= 128).
+__device__ __forceinline__ int entry_of(const CacheView& c, int kt) {
+  return c.tiles_inv == 0 ? kt : static_cast<int>(__umulhi(static_cast<uint32_t>(kt), c.tiles_inv));
+}
+// A number that no kernel writes, at a uniform address: a scalar load.
+template <typename T>
+__device__ __forceinline__ T load_constant(const T* p) {
+  return *(__attribute__((address_space(4))) const T*)(p);
+}
+// The page of tile kt of sequence b, or -1 where the table names none.
+__device__ __forceinline__ int page_of(const CacheView& c, int b, int kt) {
+  const int entry = entry_of(c, kt);
+  if (entry >= c.table_pages) return -1;
+  const int id = c.table[b * c.ld_table + entry];
+  return static_cast<unsigned>(id) < static_cast<unsigned>(c.pages) ? id : -1;
+}
 
 // Packed new tokens: those of sequence b are rows offsets[b] .. offsets[b+1],
 // and the last ones of its lengths[b] tokens.

@@ -30,18 +30,33 @@ namespace da {
 namespace {
 
 constexpr int kWaves = 4;
-constexpr int kKeyChunk = 8;          // 32-feature steps whose keys a wave holds
-constexpr int kMaxSplits = 1024;
+constexpr int kMaxSplits = 256;
+constexpr int kWantWorkgroups = 1024;
 constexpr float kNoScore = -3.0e38f;  // the running maximum before the first score
+
+// Division of numbers below 2^23 by a divisor up to 2^16, by a product (the
+// quotient of n and d is the whole part of n m / 2^40 with m = ceil(2^40 / d):
+// the excess n (m d - 2^40) / (2^40 d) stays below 1 / d).
+struct Divisor {
+  uint32_t d;
+  uint64_t m;
+  Divisor() = default;
+  explicit Divisor(int64_t n) : d(static_cast<uint32_t>(n)), m(((uint64_t{1} << 40) + d - 1) / d) {}
+  __device__ __forceinline__ uint32_t divide(uint32_t n) const { return static_cast<uint32_t>(n * m >> 40); }
+  __device__ __forceinline__ uint32_t remainder(uint32_t n) const { return n - divide(n) * d; }
+};
 
 struct Params {
   PagedAttentionArgs a;
   int n_ct;        // column tiles a workgroup index stands for (a stride, not a bound)
-  int n_slices;    // slices of the value features
-  int n_split;     // parts of the cached tokens
+  int n_split;     // parts of a sequence's tokens
+  int per;         // tiles of a part (the last one takes what is left)
   int units;       // B * n_split
-  float* part_o;   // [n_split][N * S][D], or nullptr: rows are finished here
-  float* part_m;   // [n_split][N * S]
+  int64_t rows;    // N * S
+  Divisor members; // workgroups of a unit
+  Divisor sequences, slices, maps, repeats;
+  float* part_o;   // [n_split][rows][D], or nullptr: rows are finished here
+  float* part_m;   // [n_split][rows]
   float* part_l;
 };
 
@@ -53,13 +68,14 @@ struct Sequence {
   int length;      // tokens, the new ones among them
   int cached;      // of these, those that the table has entries for
 };
+// b is the same in all lanes.
 __device__ __forceinline__ Sequence sequence_of(const NewTokens& t, const CacheView& c, int b) {
   Sequence s;
-  const int64_t first = min(max(static_cast<int64_t>(t.offsets[b]), int64_t{0}), t.N);
-  const int64_t last = min(max(static_cast<int64_t>(t.offsets[b + 1]), first), t.N);
+  const int64_t first = min(max(static_cast<int64_t>(load_constant(t.offsets + b)), int64_t{0}), t.N);
+  const int64_t last = min(max(static_cast<int64_t>(load_constant(t.offsets + b + 1)), first), t.N);
   s.n0 = first;
   s.rows = static_cast<int>(last - first);
-  s.length = max(t.lengths[b], 0);
+  s.length = max(load_constant(t.lengths + b), 0);
   s.cached = static_cast<int>(min(static_cast<int64_t>(s.length), static_cast<int64_t>(c.table_pages) * c.tiles * 32));
   return s;
 }
@@ -67,13 +83,15 @@ __device__ __forceinline__ Sequence sequence_of(const NewTokens& t, const CacheV
 __device__ __forceinline__ int visible_to(const Sequence& s, int i, bool causal) {
   return causal ? max(0, min(s.cached, s.length - s.rows + i + 1)) : s.cached;
 }
-// The page of tile kt of sequence b, or -1 where the table names none.
-__device__ __forceinline__ int page_of(const CacheView& c, int b, int kt) {
-  const int id = c.table[b * c.ld_table + kt / c.tiles];
-  return static_cast<unsigned>(id) < static_cast<unsigned>(c.pages) ? id : -1;
-}
+__device__ __forceinline__ int tile_of(const CacheView& c, int kt) { return kt - entry_of(c, kt) * c.tiles; }
 __device__ __forceinline__ float score_scale(const PagedAttentionArgs& a, int s) {
   return load_scalar(a.scales, a.scales_dtype, s) * a.scale_mult * kLog2e;
+}
+
+// Sixteen bytes at a uniform global address and a lane's offset.
+typedef __attribute__((address_space(1))) const char* global_ptr;
+__device__ __forceinline__ u32x4 load_at(const char* base, uint32_t lane_offset) {
+  return *reinterpret_cast<__attribute__((address_space(1))) const u32x4*>((global_ptr)(base) + lane_offset);
 }
 
 // Rows of no sequence (in front of the first and behind the last one) are zero.
@@ -91,250 +109,352 @@ __device__ void clear_other_rows(const PagedAttentionArgs& a, int64_t wg, int64_
 
 }  // namespace
 
-template <typename TQ, typename TV, int DB>
-__global__ __launch_bounds__(64 * kWaves) void paged_token_kernel(Params p) {
+// NK: groups of 64 key features that a wave holds (fewer features leave the rest
+// zero, more are taken in turn); DBW: 16-feature blocks of the values of a wave;
+// CT: column tiles; NW: waves; ONE: the columns are one map's tokens (many new
+// tokens; member index: slice, then map, then column tile), else (token, map)
+// pairs over all features; PB: buffers of the probabilities.
+//
+// A step takes NW tiles of 32 tokens.  Wave w forms tile w's scores of all
+// columns and leaves its probabilities in LDS; after a barrier every wave
+// multiplies them with its own DBW blocks of the values of all tiles.  A wave's
+// next keys and the next two tiles' values are on their way meanwhile.
+template <typename TQ, typename TV, int NK, int DBW, int CT, int NW, bool ONE, int PB, int OCC>
+__global__ __launch_bounds__(64 * NW, OCC) void paged_attention_kernel(Params p) {
   typedef typename Elem<TQ>::v8 q8;
   typedef typename Elem<TV>::v8 v8;
-  constexpr int DS = 16 * DB, OP = DS + 4;   // pitch of the outputs in LDS
+  constexpr int DS = 16 * DBW * NW;
+  constexpr int FW = 64 * NK;               // features of a pass
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const PagedAttentionArgs& a = p.a;
   const CacheView& cache = a.cache;
   const int lane = lane_id(), c = lane & 15, g = lane >> 4;
   const int wave = uniform_wave();
-  const int S = a.S, W = cache.W, D = cache.D;
-  if (p.part_o == nullptr) clear_other_rows<TV>(a, blockIdx.x, gridDim.x);
+  const int W = cache.W, D = cache.D;
 
   // Workgroups are dealt to the XCDs in turn.  Those that read the same tokens
-  // (a unit's column tiles and slices) go to one, for its L2.
-  const int members = p.n_ct * p.n_slices;
-  const int wg = static_cast<int>(blockIdx.x);
-  const int unit = wg / (kXcds * members) * kXcds + wg % kXcds;
+  // (a unit's column tiles, maps and slices) go to one, for its L2.  All
+  // sequences' first parts come first, so that the parts that have tiles are
+  // dealt evenly.
+  const uint32_t wg = blockIdx.x;
+  if (p.part_o == nullptr) clear_other_rows<TV>(a, wg, gridDim.x);
+  const uint32_t round = p.members.divide(wg / kXcds);
+  const int unit = static_cast<int>(round * kXcds + wg % kXcds);
   if (unit >= p.units) return;
-  const int member = wg / kXcds % members;
-  const int slice = member % p.n_slices;
-  const int b = unit / p.n_split, split = unit % p.n_split;
+  int member = static_cast<int>(wg / kXcds - round * p.members.d);
+  const int split = static_cast<int>(p.sequences.divide(unit)), b = unit - split * a.tokens.B;
   const Sequence seq = sequence_of(a.tokens, cache, b);
-  const int n_cols = seq.rows * S;
+  if (seq.rows == 0) return;
+  const int slice = static_cast<int>(p.slices.remainder(member));
+  member = static_cast<int>(p.slices.divide(member));
+  const int map = ONE ? static_cast<int>(p.maps.remainder(member)) : 0;
+  if (ONE) member = static_cast<int>(p.maps.divide(member));
+  const int n_cols = ONE ? seq.rows : seq.rows * a.S;
+  const int width = ONE ? a.RP : W, f0 = ONE ? static_cast<int>(p.repeats.divide(map)) * a.RP : 0;
+  const int passes = ONE ? 1 : (W + FW - 1) / FW;
+  const int QP = passes * FW + 8;           // pitch of the queries in LDS
+  const int d0 = slice * DS + wave * DBW * 16;
+  const int nb = max(0, min(DBW, (D - d0) / 16));   // blocks of this wave (the last slice may have fewer)
 
-  const int d0 = slice * DS;
-  const int nb = min(DB, (D - d0) / 16);       // 16-feature blocks of this slice
-  const int steps = (W + 32 * kKeyChunk - 1) / (32 * kKeyChunk);
-  const int qp = steps * 32 * kKeyChunk + 8;   // pitch of the queries in LDS
   TQ* qs = reinterpret_cast<TQ*>(lds);
-  float* os = reinterpret_cast<float*>(lds);
-  float* stats = reinterpret_cast<float*>(lds + max(16 * qp * 2, 16 * OP * 4));   // [2][kWaves][16]
+  char* ps = lds + 32 * CT * QP;                                  // [PB][NW][CT][64 lanes] 16 bytes
+  float* ms = reinterpret_cast<float*>(ps + PB * NW * CT * 1024); // [PB][NW][16 CT]
+  int* moved = reinterpret_cast<int*>(ms + PB * NW * 16 * CT);    // [PB][NW]
 
-  for (int ct = member / p.n_slices; ct * 16 < n_cols; ct += p.n_ct) {
-    const int col0 = ct * 16;
-    __syncthreads();   // the last tile's outputs have been read
-    for (int i = static_cast<int>(threadIdx.x); i < 2 * (qp - 8); i += 64 * kWaves) {
-      const int col = i / ((qp - 8) / 8), f = i % ((qp - 8) / 8) * 8;
-      const int token = (col0 + col) / S, from = (col0 + col) % S / a.repeat * a.RP;
-      u32x4 v = {0, 0, 0, 0};
-      if (col0 + col < n_cols && f >= from && f < from + a.RP)
-        v = load16B(static_cast<const TQ*>(a.q) + (seq.n0 + token) * a.ldq + f);
-      store16B(qs + col * qp + f, v);
-    }
-    __syncthreads();
-
-    // This lane's column; columns behind the last one count as seeing all.
-    const int mine = min(col0 + c, n_cols - 1);
-    const int vis = visible_to(seq, mine / S, a.causal);
-    const float sc = score_scale(a, mine % S);
-    const int limit = visible_to(seq, min(col0 + 15, n_cols - 1) / S, a.causal);
-    const int all_see = visible_to(seq, col0 / S, a.causal);
+  for (int ct0 = member; ct0 * 16 * CT < n_cols; ct0 += p.n_ct) {
+    const int col0 = ct0 * 16 * CT, n_used = min(16 * CT, n_cols - col0);
+    auto token_of = [&](int col) { return ONE ? col : static_cast<int>(p.maps.divide(col)); };
+    auto map_of = [&](int col) { return ONE ? map : static_cast<int>(p.maps.remainder(col)); };
+    auto row_of = [&](int col) { return ONE ? (seq.n0 + col0 + col) * a.S + map : seq.n0 * a.S + col0 + col; };
+    const int limit = visible_to(seq, token_of(col0 + n_used - 1), a.causal);
     const int n_kt = (limit + 31) / 32;
-    const int per = (n_kt + p.n_split - 1) / p.n_split;
-    const int kt0 = min(n_kt, split * per), kt1 = min(n_kt, kt0 + per);
-
-    f32x4 acc[DB];
-#pragma unroll
-    for (int i = 0; i < DB; ++i) acc[i] = zero4();
-    float m_run = kNoScore, l_part = 0.f;
-
-    q8 kf[kKeyChunk][2];
-    auto load_keys = [&](const TQ* base, int step) {
-#pragma unroll
-      for (int k = 0; k < kKeyChunk; ++k) {
-        const int f = min((step * kKeyChunk + k) * 32, W - 32);   // past the last: multiplied by zero
-        kf[k][0] = load8(base + f);
-        kf[k][1] = load8(base + f + 4 * W);
-      }
-    };
-    // Block h of the scores has token 8 (c / 4) + 4 h + c % 4 in row c.
-    const int key_lane = (8 * (c >> 2) + (c & 3)) * W + 8 * g;
-    auto key_base = [&](int page, int kt) {
-      return static_cast<const TQ*>(cache.keys) + max(page, 0) * cache.key_page +
-             static_cast<int64_t>(kt % cache.tiles) * 32 * W + key_lane;
-    };
-    int page = -1;
-    if (kt0 + wave < kt1) {
-      page = page_of(cache, b, kt0 + wave);
-      load_keys(key_base(page, kt0 + wave), 0);
+    const int kt0 = min(n_kt, split * p.per), kt1 = split == p.n_split - 1 ? n_kt : min(n_kt, kt0 + p.per);
+    if (split > 0 && kt0 == kt1) {   // nothing left for this part
+      if (slice == 0)
+        for (int i = static_cast<int>(threadIdx.x); i < n_used; i += 64 * NW) p.part_l[split * p.rows + row_of(i)] = 0.f;
+      continue;
     }
-    for (int kt = kt0 + wave; kt < kt1; kt += kWaves) {
-      const TV* vb = static_cast<const TV*>(cache.values) + max(page, 0) * cache.value_page +
-                     static_cast<int64_t>(kt % cache.tiles) * 32 * D + 32 * (d0 + c) + 8 * g;
-      v8 vf[DB];
-#pragma unroll
-      for (int i = 0; i < DB; ++i) vf[i] = load8(vb + 512 * min(i, nb - 1));
-      __builtin_amdgcn_sched_barrier(0);
-      f32x4 st[2] = {zero4(), zero4()};
-      for (int step = 0; step < steps; ++step) {
-        if (step > 0) load_keys(key_base(page, kt), step);
-#pragma unroll
-        for (int k = 0; k < kKeyChunk; ++k) {
-          const q8 qv = load8(qs + c * qp + (step * kKeyChunk + k) * 32 + 8 * g);
-          st[0] = Elem<TQ>::mma(kf[k][0], qv, st[0]);
-          st[1] = Elem<TQ>::mma(kf[k][1], qv, st[1]);
-        }
+
+    // A tile's page is in the lane of its place in the step: the next two steps'
+    // are on their way.
+    auto pages_at = [&](int base) { return lane < NW && base + lane < kt1 ? page_of(cache, b, base + lane) : -1; };
+    int pages = pages_at(kt0), pages_next = pages_at(kt0 + NW);
+
+    // Queries: sixteen threads to a column.
+    if (ct0 != member) lds_barrier();   // the last tiles' have been read
+    for (int col = static_cast<int>(threadIdx.x) >> 4; col < 16 * CT; col += 4 * NW) {
+      const bool used = col < n_used;
+      const int from = ONE ? 0 : static_cast<int>(p.repeats.divide(map_of(col0 + col))) * a.RP;
+      const TQ* src = static_cast<const TQ*>(a.q) + (seq.n0 + token_of(col0 + (used ? col : 0))) * a.ldq + f0;
+      for (int f = (static_cast<int>(threadIdx.x) & 15) * 8; f < passes * FW; f += 128) {
+        u32x4 v = {0, 0, 0, 0};
+        if (used && f >= from && f < from + a.RP) v = load16B(src + f);
+        store16B(qs + col * QP + f, v);
       }
-      const bool whole = page >= 0 && kt * 32 + 32 <= all_see;   // nothing to mask
+    }
+    // This lane's columns; those behind the last one count as it.
+    int vis[CT];
+    float sc[CT], m_run[CT], l_part[CT];
+#pragma unroll
+    for (int i = 0; i < CT; ++i) {
+      const int col = col0 + min(16 * i + c, n_used - 1);
+      vis[i] = visible_to(seq, token_of(col), a.causal);
+      sc[i] = score_scale(a, map_of(col));
+      m_run[i] = kNoScore;
+      l_part[i] = 0.f;
+    }
+
+    // Addresses are a uniform base and a lane's 32-bit offset.  Block h of the
+    // scores has token 8 (c / 4) + 4 h + c % 4 in row c.  Where there is no tile
+    // or page every lane reads one place, and nothing uses it.
+    const uint32_t key_lane = static_cast<uint32_t>(((8 * (c >> 2) + (c & 3)) * W + 8 * g) * 2);
+    const uint32_t value_lane = static_cast<uint32_t>((32 * c + 8 * g) * 2);
+    u32x4 kf[NK][4], vf[2][DBW];
+    auto load_keys = [&](int kt, int page, int pass) {
+      const char* base = uniform_ptr(static_cast<const char*>(cache.keys) +
+                                     (max(page, 0) * cache.key_page + static_cast<int64_t>(tile_of(cache, kt)) * 32 * W + f0) * 2);
+      const uint32_t at = page < 0 ? 0 : key_lane;
+#pragma unroll
+      for (int j = 0; j < NK; ++j) {   // a group past the last feature is multiplied by zero
+        const char* from = base + 128 * min(pass * NK + j, width / 64 - 1);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) kf[j][i] = load_at(from + (i & 1) * 8 * W, at + 64 * (i >> 1));
+      }
+    };
+    auto load_values = [&](u32x4 (&v)[DBW], int kt, int page) {
+      const char* base = uniform_ptr(static_cast<const char*>(cache.values) +
+                                     (max(page, 0) * cache.value_page + (static_cast<int64_t>(tile_of(cache, kt)) * D + (nb > 0 ? d0 : 0)) * 32) * 2);
+      const uint32_t at = page < 0 ? 0 : value_lane;
+#pragma unroll
+      for (int i = 0; i < DBW; ++i) v[i] = load_at(base + 1024 * max(0, min(i, nb - 1)), at);
+    };
+    load_keys(kt0 + wave, __builtin_amdgcn_readlane(pages, wave), 0);
+    load_values(vf[0], kt0, __builtin_amdgcn_readlane(pages, 0));
+    load_values(vf[1], kt0 + 1, __builtin_amdgcn_readlane(pages, 1));
+    f32x4 acc[CT][DBW];
+#pragma unroll
+    for (int i = 0; i < CT; ++i)
+#pragma unroll
+      for (int j = 0; j < DBW; ++j) acc[i][j] = zero4();
+    __builtin_amdgcn_sched_barrier(0);
+    lds_barrier();   // the queries are there
+
+    int buf = 0;
+    for (int base = kt0; base < kt1; base += NW) {
+      const int pages_after = pages_at(base + 2 * NW);
+      const int kt = base + wave, page = __builtin_amdgcn_readlane(pages, wave);
       const int live = page < 0 ? 0 : min(32, limit - kt * 32);
-      if (kt + kWaves < kt1) {
-        page = page_of(cache, b, kt + kWaves);
-        load_keys(key_base(page, kt + kWaves), 0);
+      char* mine = ps + (buf * NW + wave) * CT * 1024 + lane * 16;
+      bool any = false;
+      // Scores of this wave's tile, and its probabilities.
+      auto scores = [&](f32x4 (&st)[2], int i, int pass) {
+#pragma unroll
+        for (int j = 0; j < 2 * NK; ++j) {
+          const q8 qf = load8(qs + (16 * i + c) * QP + pass * FW + 32 * j + 8 * g);
+          st[0] = Elem<TQ>::mma(__builtin_bit_cast(q8, kf[j >> 1][2 * (j & 1)]), qf, st[0]);
+          st[1] = Elem<TQ>::mma(__builtin_bit_cast(q8, kf[j >> 1][2 * (j & 1) + 1]), qf, st[1]);
+        }
+      };
+#pragma unroll
+      for (int i = 0; i < CT; ++i) {
+        f32x4 st[2] = {zero4(), zero4()};
+        scores(st, i, 0);
+        if constexpr (!ONE && CT == 1) {
+          for (int pass = 1; pass < passes; ++pass) {
+            load_keys(kt, page, pass);
+            scores(st, i, pass);
+          }
+        }
+        const int seen = min(live, vis[i] - kt * 32) - 8 * g;   // of this lane's eight tokens
+        float mx = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float s = e < seen ? st[e >> 2][e & 3] * sc[i] : -INFINITY;
+          st[e >> 2][e & 3] = s;
+          mx = fmaxf(mx, s);
+        }
+        // The reference moves, to a whole number (so that what it scales stays
+        // exact), where a score exceeds it by more than kRescaleSlack.
+        float m = m_run[i];
+        if (__ballot(mx > m + kRescaleSlack)) {
+          const float tile_max = group_max(mx);
+          if (tile_max > m + kRescaleSlack) m = __builtin_ceilf(tile_max);
+          any = true;
+        }
+        float l = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float s = __builtin_amdgcn_exp2f(st[e >> 2][e & 3] - m);
+          st[e >> 2][e & 3] = s;
+          l += s;
+        }
+        if (any) l_part[i] *= __builtin_amdgcn_exp2f(m_run[i] - m);
+        l_part[i] += l;
+        // The probabilities are rounded to the values' type for the product, the
+        // sum is of the unrounded ones.
+        if (PB == 1 && i == 0 && base > kt0) lds_barrier();   // the last step's have been read
+        *reinterpret_cast<v8*>(mine + i * 1024) = pack_blocked<TV>(st[0], st[1]);
+        ms[(buf * NW + wave) * 16 * CT + 16 * i + c] = m;
+      }
+      if (lane == 0) moved[buf * NW + wave] = any;
+      __builtin_amdgcn_sched_barrier(0);
+      load_keys(kt + NW, __builtin_amdgcn_readlane(pages_next, wave), 0);
+      __builtin_amdgcn_sched_barrier(0);
+      lds_barrier();
+      int moves = 0;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) moves |= moved[buf * NW + w];
+      if (__builtin_amdgcn_readfirstlane(moves)) {
+        // To the largest of the waves' references: this wave's probabilities and
+        // sums, and what has been added up.
+#pragma unroll
+        for (int i = 0; i < CT; ++i) {
+          const float own = ms[(buf * NW + wave) * 16 * CT + 16 * i + c];
+          float m = own;
+#pragma unroll
+          for (int w = 0; w < NW; ++w) m = fmaxf(m, ms[(buf * NW + w) * 16 * CT + 16 * i + c]);
+          const float f = __builtin_amdgcn_exp2f(own - m), fa = __builtin_amdgcn_exp2f(m_run[i] - m);
+          m_run[i] = m;
+          l_part[i] *= f;
+#pragma unroll
+          for (int j = 0; j < DBW; ++j) acc[i][j] *= fa;
+          v8 pv = *reinterpret_cast<const v8*>(mine + i * 1024);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) pv[e] = static_cast<TV>(static_cast<float>(pv[e]) * f);
+          *reinterpret_cast<v8*>(mine + i * 1024) = pv;
+        }
+        lds_barrier();
+      }
+      const char* probs = ps + buf * NW * CT * 1024 + lane * 16;
+#pragma unroll
+      for (int t = 0; t < NW; ++t) {
+        const int page_t = __builtin_amdgcn_readlane(pages, t);
+        const int live_t = page_t < 0 ? 0 : min(32, limit - (base + t) * 32);
+        v8 vv[DBW];
+        if (live_t == 32) {
+#pragma unroll
+          for (int j = 0; j < DBW; ++j) vv[j] = __builtin_bit_cast(v8, vf[t & 1][j]);
+        } else {   // what lies behind the last token is not multiplied: it may hold anything
+          u32x4 keep;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            keep[e] = (8 * g + 2 * e < live_t ? 0xffffu : 0u) | (8 * g + 2 * e + 1 < live_t ? 0xffff0000u : 0u);
+#pragma unroll
+          for (int j = 0; j < DBW; ++j) vv[j] = __builtin_bit_cast(v8, vf[t & 1][j] & keep);
+        }
+#pragma unroll
+        for (int i = 0; i < CT; ++i) {
+          const v8 pv = *reinterpret_cast<const v8*>(probs + (t * CT + i) * 1024);
+#pragma unroll
+          for (int j = 0; j < DBW; ++j) acc[i][j] = Elem<TV>::mma(vv[j], pv, acc[i][j]);
+        }
+        const int next = t + 2 < NW ? __builtin_amdgcn_readlane(pages, t + 2 < NW ? t + 2 : 0)
+                                    : __builtin_amdgcn_readlane(pages_next, t + 2 < NW ? 0 : t + 2 - NW);
+        load_values(vf[t & 1], base + t + 2, next);
         __builtin_amdgcn_sched_barrier(0);
       }
-      float mx = -INFINITY;
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int t = 8 * g + 4 * h + e;
-          const float s = st[h][e] * sc;
-          st[h][e] = whole || (t < live && kt * 32 + t < vis) ? s : -INFINITY;
-          mx = fmaxf(mx, st[h][e]);
-        }
-      lazy_rescale<DB>(mx, 1.f, m_run, l_part, acc);
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          st[h][e] = __builtin_amdgcn_exp2f(st[h][e] - m_run);
-          l_part += st[h][e];
-        }
-      // The probabilities are rounded to the values' type for the product, the
-      // sum is of the unrounded ones.
-      const v8 pv = pack_blocked<TV>(st[0], st[1]);
-      if (live < 32) {   // what lies behind the last token is not multiplied
-#pragma unroll
-        for (int i = 0; i < DB; ++i)
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (8 * g + e >= live) vf[i][e] = static_cast<TV>(0.f);
-      }
-#pragma unroll
-      for (int i = 0; i < DB; ++i) acc[i] = Elem<TV>::mma(vf[i], pv, acc[i]);
+      pages = pages_next;
+      pages_next = pages_after;
+      if (PB == 2) buf ^= 1;
     }
 
-    // The waves' sums, to the largest maximum.
-    const float l_run = group_sum(l_part);
-    if (g == 0) {
-      stats[wave * 16 + c] = m_run;
-      stats[(kWaves + wave) * 16 + c] = l_run;
+    // The waves' sums of exponentials; the rest of a column is in one wave.
+    float* ls = reinterpret_cast<float*>(ps);
+    lds_barrier();   // the probabilities have been read
+#pragma unroll
+    for (int i = 0; i < CT; ++i) {
+      const float l = group_sum(l_part[i]);
+      if (g == 0) ls[wave * 16 * CT + 16 * i + c] = l;
     }
-    __syncthreads();   // and the queries have been read
-    float m_all = kNoScore, l_all = 0.f;
+    lds_barrier();
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) m_all = fmaxf(m_all, stats[w * 16 + c]);
+    for (int i = 0; i < CT; ++i) {
+      const int col = 16 * i + c;
+      if (col >= n_used) continue;
+      float l = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) l_all += stats[(kWaves + w) * 16 + c] * __builtin_amdgcn_exp2f(stats[w * 16 + c] - m_all);
-    const float factor = __builtin_amdgcn_exp2f(m_run - m_all);
-    const bool used = col0 + c < n_cols;
-    for (int w = 0; w < kWaves; ++w) {
-      if (wave == w && used) {
-#pragma unroll
-        for (int i = 0; i < DB; ++i) {
-          f32x4* dst = reinterpret_cast<f32x4*>(os + c * OP + 16 * i + 4 * g);
-          *dst = w == 0 ? acc[i] * factor : *dst + acc[i] * factor;
+      for (int w = 0; w < NW; ++w) l += ls[w * 16 * CT + col];
+      const int64_t row = row_of(col);
+      if (wave == 0 && g == 0 && slice == 0) {
+        if (p.part_o) {
+          p.part_m[split * p.rows + row] = m_run[i];
+          p.part_l[split * p.rows + row] = l;
+        } else if (a.lse2) {
+          a.lse2[row] = l == 0.f ? -INFINITY : m_run[i] + __builtin_amdgcn_logf(l);
         }
       }
-      __syncthreads();
-    }
-    const int64_t row0 = seq.n0 * S + col0;
-    const int n_used = min(16, n_cols - col0);
-    if (wave == 0 && g == 0 && used && slice == 0) {
       if (p.part_o) {
-        p.part_m[split * a.tokens.N * S + row0 + c] = m_all;
-        p.part_l[split * a.tokens.N * S + row0 + c] = l_all;
-      } else if (a.lse2) {
-        a.lse2[row0 + c] = l_all == 0.f ? -INFINITY : m_all + __builtin_amdgcn_logf(l_all);
-      }
-    }
-    if (wave == 0 && g == 0) stats[c] = l_all;
-    __syncthreads();
-    for (int i = static_cast<int>(threadIdx.x); i < n_used * 4 * DB; i += 64 * kWaves) {
-      const int col = i / (4 * DB), d = i % (4 * DB) * 4;
-      if (d >= 16 * nb) continue;
-      f32x4 o = *reinterpret_cast<const f32x4*>(os + col * OP + d);
-      if (p.part_o) {
-        *reinterpret_cast<f32x4*>(p.part_o + ((split * a.tokens.N * S + row0 + col) * D + d0 + d)) = o;
-      } else {
-        const float l = stats[col];
-        o *= l == 0.f ? 0.f : 1.f / l;
-        typename Elem<TV>::v4 r;
+        float* to = p.part_o + (split * p.rows + row) * D + d0 + 4 * g;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) r[e] = static_cast<TV>(o[e]);
-        *reinterpret_cast<typename Elem<TV>::v4*>(static_cast<TV*>(a.out) + (row0 + col) * D + d0 + d) = r;
+        for (int j = 0; j < DBW; ++j)
+          if (j < nb) *reinterpret_cast<f32x4*>(to + 16 * j) = acc[i][j];
+      } else {
+        const float f = l == 0.f ? 0.f : 1.f / l;
+        TV* to = static_cast<TV*>(a.out) + row * D + d0 + 4 * g;
+#pragma unroll
+        for (int j = 0; j < DBW; ++j) {
+          typename Elem<TV>::v4 r;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) r[e] = static_cast<TV>(acc[i][j][e] * f);
+          if (j < nb) *reinterpret_cast<typename Elem<TV>::v4*>(to + 16 * j) = r;
+        }
       }
     }
   }
 }
 
 // The parts of a row joined: out = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i,
-// summed over the maps by their weights where asked.  A workgroup takes 256
-// features of a row; its waves take the parts in turn.
-constexpr int kMergeWaves = 8;
+// summed over the maps by their weights where asked.  A workgroup takes 64
+// features of a row; a wave reads them of four parts at once.
+constexpr int kMergeWaves = 16;
 template <typename TV>
 __global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(Params p) {
-  __shared__ __attribute__((aligned(16))) float sums[kMergeWaves][256];
+  __shared__ __attribute__((aligned(16))) float sums[kMergeWaves][64];
   const PagedAttentionArgs& a = p.a;
   const int S = a.S, D = a.cache.D;
-  const int64_t rows = a.tokens.N * S;
-  const int64_t n = a.mix ? blockIdx.x : blockIdx.x / S;
-  const int s0 = a.mix ? 0 : static_cast<int>(blockIdx.x % S), s1 = a.mix ? S : s0 + 1;
-  const int lane = lane_id(), wave = uniform_wave();
-  const int d = static_cast<int>(blockIdx.y) * 256 + lane * 4;
-  const bool owned = n >= a.tokens.offsets[0] && n < a.tokens.offsets[a.tokens.B];
+  const uint32_t block = blockIdx.x;
+  const int64_t n = a.mix ? block : p.maps.divide(block);
+  const int s0 = a.mix ? 0 : static_cast<int>(p.maps.remainder(block)), s1 = a.mix ? S : s0 + 1;
+  const int lane = lane_id(), wave = uniform_wave(), waves = static_cast<int>(blockDim.x) / 64;
+  const int d = static_cast<int>(blockIdx.y) * 64 + (lane & 15) * 4;
+  const bool owned = n >= load_constant(a.tokens.offsets) && n < load_constant(a.tokens.offsets + a.tokens.B);
   f32x4 total = zero4();
-  for (int s = s0; s < s1; ++s) {
+  for (int s = s0; s < s1 && owned; ++s) {
     const int64_t row = n * S + s;
-    float m = -INFINITY;
-    if (owned)
-      for (int i = lane; i < p.n_split; i += 64)
-        if (p.part_l[i * rows + row] != 0.f) m = fmaxf(m, p.part_m[i * rows + row]);
+    // A part that saw nothing (l = 0) has written nothing else.
+    float m = -INFINITY, l = 0.f;
+    for (int i = lane; i < p.n_split; i += 64) {
+      const float li = p.part_l[i * p.rows + row], mi = p.part_m[i * p.rows + row];
+      if (li != 0.f) m = fmaxf(m, mi);
+    }
 #pragma unroll
     for (int x = 32; x >= 1; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
-    float l = 0.f;
     f32x4 o = zero4();
-    if (owned) {
-      for (int i = lane; i < p.n_split; i += 64) {
-        const float li = p.part_l[i * rows + row];
-        if (li != 0.f) l += li * __builtin_amdgcn_exp2f(p.part_m[i * rows + row] - m);
-      }
 #pragma unroll 4
-      for (int i = wave; i < p.n_split; i += kMergeWaves) {
-        // A part that saw nothing has written nothing.
-        const float li = p.part_l[i * rows + row], mi = p.part_m[i * rows + row];
-        f32x4 v = zero4();
-        if (li != 0.f && d < D) v = *reinterpret_cast<const f32x4*>(p.part_o + (i * rows + row) * D + d);
-        o += v * (li != 0.f ? __builtin_amdgcn_exp2f(mi - m) : 0.f);
-      }
+    for (int i = wave * 4 + (lane >> 4); i < p.n_split; i += waves * 4) {
+      const float li = p.part_l[i * p.rows + row], mi = p.part_m[i * p.rows + row];
+      if (li != 0.f && d < D) o += *reinterpret_cast<const f32x4*>(p.part_o + (i * p.rows + row) * D + d) * __builtin_amdgcn_exp2f(mi - m);
+    }
+    for (int i = lane; i < p.n_split; i += 64) {
+      const float li = p.part_l[i * p.rows + row], mi = p.part_m[i * p.rows + row];
+      if (li != 0.f) l += li * __builtin_amdgcn_exp2f(mi - m);
     }
     l = wave_sum(l);
     if (a.lse2 && blockIdx.y == 0 && threadIdx.x == 0) a.lse2[row] = l == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(l);
     total += o * (l == 0.f ? 0.f : (a.mix ? a.mix[s] : 1.f) / l);
   }
-  *reinterpret_cast<f32x4*>(&sums[wave][lane * 4]) = total;
-  __syncthreads();
-  const int t = static_cast<int>(threadIdx.x);
-  if (t < 256) {
-    float v = 0.f;
 #pragma unroll
-    for (int w = 0; w < kMergeWaves; ++w) v += sums[w][t];
-    const int64_t at = (a.mix ? n : n * S + s0) * D + static_cast<int64_t>(blockIdx.y) * 256 + t;
-    if (static_cast<int>(blockIdx.y) * 256 + t < D) static_cast<TV*>(a.out)[at] = static_cast<TV>(v);
+  for (int e = 0; e < 4; ++e) {
+    total[e] += __shfl_xor(total[e], 16);
+    total[e] += __shfl_xor(total[e], 32);
+  }
+  if (lane < 16) *reinterpret_cast<f32x4*>(&sums[wave][lane * 4]) = total;
+  __syncthreads();
+  const int t = static_cast<int>(threadIdx.x), at = static_cast<int>(blockIdx.y) * 64 + t;
+  if (t < 64 && at < D) {
+    float v = 0.f;
+    for (int w = 0; w < waves; ++w) v += sums[w][t];
+    static_cast<TV*>(a.out)[(a.mix ? n : n * S + s0) * D + at] = static_cast<TV>(v);
   }
 }
 
@@ -354,7 +474,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_weights_kernel(PagedAttenti
   const int page = kt * 32 < seq.cached ? page_of(cache, b, kt) : -1;
   if (page >= 0) {
     const TQ* kb = static_cast<const TQ*>(cache.keys) + page * cache.key_page +
-                   (static_cast<int64_t>(kt % cache.tiles) * 32 + 8 * (c >> 2) + (c & 3)) * W + 8 * g;
+                   (static_cast<int64_t>(tile_of(cache, kt)) * 32 + 8 * (c >> 2) + (c & 3)) * W + 8 * g;
     for (int s = 0; s < S; ++s) {
       const int from = s / a.repeat * RP;
       q8 kf[KS][2];
@@ -403,50 +523,69 @@ __global__ __launch_bounds__(64 * kWaves) void paged_weights_kernel(PagedAttenti
 
 namespace {
 
+// How a call is cut: one of the kernel's forms, and parts of the tokens.
 struct Plan {
-  int n_ct, n_slices, db, n_split;
+  bool one;        // columns of one map (ONE)
+  int ct, nw;      // column tiles and waves of a workgroup
+  int n_slices, dbw, members, n_ct, n_split, per;
   bool parts;
 };
 
 Plan plan(const PagedAttentionArgs& a) {
   Plan r;
-  const int64_t cols = static_cast<int64_t>(std::max(a.max_chunk, 1)) * a.S;
-  r.n_slices = (a.cache.D + 511) / 512;
-  r.n_ct = static_cast<int>(std::min<int64_t>((cols + 15) / 16, std::max(1, (1 << 20) / (a.tokens.B * r.n_slices))));
-  r.db = static_cast<int>(round_up((a.cache.D + r.n_slices - 1) / r.n_slices, 64) / 16);
-  // Workgroups for four rounds of the chip, each wave at least one tile.
+  r.one = false;
+  r.ct = 1;
+  r.nw = 4;
+  const int64_t cols = static_cast<int64_t>(std::max(a.max_chunk, 1)) * (r.one ? 1 : a.S);
+  const int most = 8 * 16 * r.nw;   // features of a workgroup
+  r.n_slices = (a.cache.D + most - 1) / most;
+  r.dbw = (a.cache.D + r.n_slices * 16 * r.nw - 1) / (r.n_slices * 16 * r.nw);
+  const int per_ct = r.n_slices * (r.one ? a.S : 1);
+  r.n_ct = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((cols + 16 * r.ct - 1) / (16 * r.ct), 16384 / (a.tokens.B * per_ct) + 1)));
+  r.members = r.n_ct * per_ct;
+  // Parts of whole steps, as many as make kWantWorkgroups where all sequences
+  // are as long as the longest.
   const int64_t tiles = (std::max(a.max_length, 1) + 31) / 32;
-  const int64_t wgs = static_cast<int64_t>(a.tokens.B) * r.n_ct * r.n_slices;
-  int64_t split = std::min<int64_t>((1024 + wgs - 1) / wgs, (tiles + kWaves - 1) / kWaves);
-  r.n_split = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(split, kMaxSplits)));
+  int64_t per = (a.tokens.B * r.members * tiles + kWantWorkgroups - 1) / kWantWorkgroups;
+  per = std::max(per, (tiles + kMaxSplits - 1) / kMaxSplits);
+  r.per = static_cast<int>(round_up(std::max<int64_t>(per, 1), r.nw));
+  r.n_split = static_cast<int>((tiles + r.per - 1) / r.per);
   r.parts = r.n_split > 1 || a.mix != nullptr;
   return r;
 }
 
-template <typename TQ, typename TV, int DB>
-void launch_token(const Params& p, hipStream_t stream) {
-  const int steps = (p.a.cache.W + 32 * kKeyChunk - 1) / (32 * kKeyChunk);
-  const size_t q_bytes = static_cast<size_t>(16) * (steps * 32 * kKeyChunk + 8) * 2;
-  const size_t lds = std::max(q_bytes, static_cast<size_t>(16) * (16 * DB + 4) * 4) + 2 * kWaves * 16 * 4;
+template <typename TQ, typename TV, int NK, int DBW, int CT, int NW, bool ONE, int PB, int OCC>
+void launch_kernel(const Params& p, hipStream_t stream) {
+  const int width = ONE ? p.a.RP : p.a.cache.W;
+  const int QP = static_cast<int>(round_up(width, 64 * NK)) + 8;
+  const size_t lds = static_cast<size_t>(32) * CT * QP + PB * NW * (CT * 1024 + CT * 64 + 4);
   const unsigned units = static_cast<unsigned>(round_up(p.units, kXcds));
-  hipLaunchKernelGGL((paged_token_kernel<TQ, TV, DB>), dim3(units * p.n_ct * p.n_slices), dim3(64 * kWaves), lds, stream, p);
+  hipLaunchKernelGGL((paged_attention_kernel<TQ, TV, NK, DBW, CT, NW, ONE, PB, OCC>), dim3(units * p.members.d), dim3(64 * NW), lds,
+                     stream, p);
+}
+
+template <typename TQ, typename TV, int DBW>
+void launch_width(const Params& p, hipStream_t stream) {
+  if (p.a.cache.W <= 256) launch_kernel<TQ, TV, 4, DBW, 1, 4, false, 2, 2>(p, stream);
+  else launch_kernel<TQ, TV, 8, DBW, 1, 4, false, 2, 2>(p, stream);
 }
 
 template <typename TQ, typename TV>
-void launch_typed(const Params& p, int db, hipStream_t stream) {
-  switch (db) {
-    case 4: launch_token<TQ, TV, 4>(p, stream); break;
-    case 8: launch_token<TQ, TV, 8>(p, stream); break;
-    case 12: launch_token<TQ, TV, 12>(p, stream); break;
-    case 16: launch_token<TQ, TV, 16>(p, stream); break;
-    case 20: launch_token<TQ, TV, 20>(p, stream); break;
-    case 24: launch_token<TQ, TV, 24>(p, stream); break;
-    case 28: launch_token<TQ, TV, 28>(p, stream); break;
-    default: launch_token<TQ, TV, 32>(p, stream); break;
+void launch_typed(const Params& p, const Plan& r, hipStream_t stream) {
+  switch (r.dbw) {
+    case 1: launch_width<TQ, TV, 1>(p, stream); break;
+    case 2: launch_width<TQ, TV, 2>(p, stream); break;
+    case 3: launch_width<TQ, TV, 3>(p, stream); break;
+    case 4: launch_width<TQ, TV, 4>(p, stream); break;
+    case 5: launch_width<TQ, TV, 5>(p, stream); break;
+    case 6: launch_width<TQ, TV, 6>(p, stream); break;
+    case 7: launch_width<TQ, TV, 7>(p, stream); break;
+    default: launch_width<TQ, TV, 8>(p, stream); break;
   }
   if (p.part_o) {
-    const dim3 grid(static_cast<unsigned>(p.a.tokens.N * (p.a.mix ? 1 : p.a.S)), static_cast<unsigned>((p.a.cache.D + 255) / 256));
-    hipLaunchKernelGGL((paged_merge_kernel<TV>), grid, dim3(64 * kMergeWaves), 0, stream, p);
+    const dim3 grid(static_cast<unsigned>(p.a.tokens.N * (p.a.mix ? 1 : p.a.S)), static_cast<unsigned>((p.a.cache.D + 63) / 64));
+    const int waves = std::max(1, std::min(kMergeWaves, (p.n_split + 15) / 16));
+    hipLaunchKernelGGL((paged_merge_kernel<TV>), grid, dim3(64 * waves), 0, stream, p);
   }
 }
 
@@ -459,16 +598,26 @@ int64_t paged_attention_workspace(const PagedAttentionArgs& a) {
 
 void launch_paged_attention(const PagedAttentionArgs& a, void* workspace, hipStream_t stream) {
   const Plan r = plan(a);
-  Params p{a, r.n_ct, r.n_slices, r.n_split, a.tokens.B * r.n_split, nullptr, nullptr, nullptr};
+  Params p{};
+  p.a = a;
+  p.n_ct = r.n_ct;
+  p.n_split = r.n_split;
+  p.per = r.per;
+  p.units = a.tokens.B * r.n_split;
+  p.rows = a.tokens.N * a.S;
+  p.members = Divisor(r.members);
+  p.sequences = Divisor(a.tokens.B);
+  p.slices = Divisor(r.n_slices);
+  p.maps = Divisor(a.S);
+  p.repeats = Divisor(a.repeat);
   if (r.parts) {
-    const int64_t rows = r.n_split * a.tokens.N * a.S;
     p.part_o = static_cast<float*>(workspace);
-    p.part_m = p.part_o + rows * a.cache.D;
-    p.part_l = p.part_m + rows;
+    p.part_m = p.part_o + r.n_split * p.rows * a.cache.D;
+    p.part_l = p.part_m + r.n_split * p.rows;
   }
-  if (a.qk_dtype == kBF16) launch_typed<__bf16, __bf16>(p, r.db, stream);
-  else if (a.v_dtype == kBF16) launch_typed<_Float16, __bf16>(p, r.db, stream);
-  else launch_typed<_Float16, _Float16>(p, r.db, stream);
+  if (a.qk_dtype == kBF16) launch_typed<__bf16, __bf16>(p, r, stream);
+  else if (a.v_dtype == kBF16) launch_typed<_Float16, __bf16>(p, r, stream);
+  else launch_typed<_Float16, _Float16>(p, r, stream);
 }
 
 template <typename TQ>

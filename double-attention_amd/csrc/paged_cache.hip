@@ -13,13 +13,6 @@ namespace {
 
 constexpr int kMoveThreads = 256;
 
-// Page of a tile of sequence b, or -1 where the table names none.
-__device__ __forceinline__ int page_at(const CacheView& c, int b, int kt) {
-  const int entry = kt / c.tiles;
-  if (entry >= c.table_pages) return -1;
-  const int id = c.table[b * c.ld_table + entry];
-  return static_cast<unsigned>(id) < static_cast<unsigned>(c.pages) ? id : -1;
-}
 __device__ __forceinline__ uint16_t* key_row(const CacheView& c, int page, int t) {
   return static_cast<uint16_t*>(c.keys) + page * c.key_page + static_cast<int64_t>(t) * c.W;
 }
@@ -66,7 +59,7 @@ __global__ __launch_bounds__(kMoveThreads) void cache_append_kernel(CacheAppendA
   const int64_t end = min(length, static_cast<int64_t>(cache.table_pages) * cache.tiles * 32);
   const int64_t row0 = first - (length - rows);   // row of position 0
   for (int64_t kt = begin / 32 + blockIdx.x; kt * 32 < end; kt += n_tiles) {
-    const int page = page_at(cache, b, static_cast<int>(kt));
+    const int page = page_of(cache, b, static_cast<int>(kt));
     if (page < 0) continue;
     const int tile = static_cast<int>(kt % cache.tiles);
     const int t0 = static_cast<int>(max(begin - kt * 32, int64_t{0})), t1 = static_cast<int>(min(end - kt * 32, int64_t{32}));
@@ -231,12 +224,12 @@ __global__ __launch_bounds__(kMoveThreads) void cache_compact_kernel(CacheCompac
     if (i < a.capacity_out) a.weights_out[b * a.ld_out + i] = t >= 0 && t < a.capacity_in ? a.weights_in[b * a.ld_in + t] : 0.f;
   }
   if (kt * 32 >= count) return;
-  const int page = page_at(a.to, b, kt);
+  const int page = page_of(a.to, b, kt);
   if (page < 0) return;
   if (tid < 32) {
     const int i = kt * 32 + tid;
     const int t = i < count ? a.kept[b * a.ld_kept + i] : -1;
-    const int from = t >= 0 ? page_at(a.from, b, t / 32) : -1;
+    const int from = t >= 0 ? page_of(a.from, b, t / 32) : -1;
     const int at = t % (a.from.tiles * 32);
     key_at[tid] = from < 0 ? -1 : from * a.from.key_page + static_cast<int64_t>(at) * W;
     value_at[tid] = from < 0 ? -1 : from * a.from.value_page + static_cast<int64_t>(at / 32) * 32 * D + at % 32;

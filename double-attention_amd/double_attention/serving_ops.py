@@ -96,10 +96,10 @@ def _check_sizes(what: str, pages: int, page_size: int, width: int, value_dim: i
         raise ValueError(f"{what}: a cache has at least one page")
     if page_size < CACHE_TILE or page_size % CACHE_TILE or page_size > MAX_PAGE_SIZE:
         raise NotImplementedError(f"{what}: page sizes are multiples of {CACHE_TILE} up to {MAX_PAGE_SIZE}, not {page_size}")
-    if width < 32 or width % 32 or width > MAX_KEY_WIDTH:
-        raise NotImplementedError(f"{what}: branches * routing_dim is a multiple of 32 up to {MAX_KEY_WIDTH}, not {width}")
-    if value_dim < 16 or value_dim % 16 or value_dim > MAX_VALUE_DIM:
-        raise NotImplementedError(f"{what}: value_dim is a multiple of 16 up to {MAX_VALUE_DIM}, not {value_dim}")
+    if width < 64 or width % 64 or width > MAX_KEY_WIDTH:
+        raise NotImplementedError(f"{what}: branches * routing_dim is a multiple of 64 up to {MAX_KEY_WIDTH}, not {width}")
+    if value_dim < 64 or value_dim % 64 or value_dim > MAX_VALUE_DIM:
+        raise NotImplementedError(f"{what}: value_dim is a multiple of 64 up to {MAX_VALUE_DIM}, not {value_dim}")
 
 
 def _check_cache(what: str, cache: PagedCache) -> torch.device:
@@ -227,8 +227,8 @@ def _paged_attention(what, query, cache, page_table, lengths, offsets, scales, w
     if maps > MAX_MAPS or max(maps, branches) % min(maps, branches):
         raise NotImplementedError(f"{what}: {maps} maps of {branches} branches (multiples of each other, at most {MAX_MAPS} maps)")
     score_dim, _, repeat, mult = routed_score_layout(branches, maps, routing_dim)
-    if score_dim % 32 or score_dim > 512:
-        raise NotImplementedError(f"{what}: score widths are multiples of 32 up to 512, not {score_dim}")
+    if score_dim % 64 or score_dim > 512:
+        raise NotImplementedError(f"{what}: score widths are multiples of 64 up to 512, not {score_dim}")
     for name, t in (("query", query), ("scales", scales), ("mix", mix), ("weights", weights), ("out", weights_out)):
         if t is not None and t.get_device() != device.index:
             raise ValueError(f"{what}: all tensors must be on {device}, got {name} on {t.device}")

@@ -23,8 +23,8 @@ extern "C" {
  *   value feature d  values[p * value_page_stride + (t / 32) * 32 * value_dim + 32 * d + t % 32]
  * (elements; values lie in tiles of 32 tokens, a feature's tokens side by
  * side).  key_width is branches * routing_dim.  page_size: a multiple of 32 up
- * to 4096.  key_width: a multiple of 32 up to 1024.  value_dim: a multiple of
- * 16 up to 4096.  table_pages * page_size: up to 2^28.  Both tensors 16-byte aligned, page strides multiples of 8.
+ * to 4096.  key_width: a multiple of 64 up to 1024.  value_dim: a multiple of
+ * 64 up to 4096.  table_pages * page_size: up to 2^28.  Both tensors 16-byte aligned, page strides multiples of 8.
  *
  * page_table: [sequences] rows of table_pages entries, ld_table apart: the pages
  * of each sequence in order.  An entry outside [0, pages) names no page: its
@@ -63,7 +63,7 @@ int da_cache_append(const da_paged_cache* cache, const void* key, int64_t ldk, c
  * over the tokens j of row n's sequence up to its own (causal) or all of them.
  * Map s has features [(s / map_repeat) * score_dim, + score_dim) of the rows of
  * query [rows, key_width] (pitch ldq, a multiple of 8) and of the keys;
- * score_dim is a multiple of 32 up to 512, at most 64 maps.
+ * score_dim is a multiple of 64 up to 512, at most 64 maps.
  * out: [rows, maps, value_dim], or with mix [maps] (fp32) its sum
  * over the maps with these weights, [rows, value_dim].  Rows that see nothing,
  * and rows of no sequence, are zero.  Scores, the softmax and sums are fp32;
