@@ -19,6 +19,7 @@
 // take every fourth tile of its part of the tokens and add up in LDS; parts
 // are joined by paged_merge_kernel.
 #include <algorithm>
+#include <type_traits>
 
 #include "da_common.h"
 #include "da_launch.h"
@@ -403,6 +404,314 @@ __global__ __launch_bounds__(64 * NW, OCC) void paged_attention_kernel(Params p)
   }
 }
 
+// Many new tokens.  A workgroup of eight waves takes 16 CT tokens of one map;
+// a step takes four tiles.  Wave w forms the scores of half a tile (16 tokens)
+// for all columns, with its keys in registers and the queries in LDS, and
+// leaves its probabilities in LDS; after a barrier every wave multiplies them
+// with its own DBW blocks of the values, straight from memory.  The scores are formed against the reference that all waves share, without a
+// look at their maximum first; where one exceeds it by more than kRescaleSlack
+// (in the first step always) a wave forms them again and raises its reference,
+// and the waves agree on the largest.
+constexpr int kChunkWaves = 8, kChunkTiles = 4;
+template <int NK, int CT>
+struct ChunkLds {   // bytes
+  static constexpr int QP = 64 * NK + 8;
+  static constexpr int PROBS = 32 * CT * QP;                              // [2][tiles][CT][64 lanes] 16 bytes
+  static constexpr int REFS = PROBS + 2 * kChunkTiles * CT * 1024;        // [16 CT] floats: the shared references
+  static constexpr int OWN = REFS + 64 * CT;                              // [waves][16 CT] floats
+  static constexpr int SEES = OWN + kChunkWaves * 64 * CT;                // [16 CT] ints: tokens that a column sees
+  static constexpr int MOVED = SEES + 64 * CT;                            // [2][waves] ints
+  static constexpr int BYTES = MOVED + 2 * kChunkWaves * 4;
+};
+
+template <typename TQ, typename TV, int NK, int DBW, int CT>
+__global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(Params p) {
+  typedef typename Elem<TQ>::v8 q8;
+  typedef typename Elem<TV>::v8 v8;
+  typedef typename Elem<TV>::v4 v4;
+  typedef ChunkLds<NK, CT> Lds;
+  constexpr int NW = kChunkWaves, TS = kChunkTiles, QP = Lds::QP;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const PagedAttentionArgs& a = p.a;
+  const CacheView& cache = a.cache;
+  const int lane = lane_id(), c = lane & 15, g = lane >> 4;
+  const int wave = uniform_wave();
+  const int W = cache.W, D = cache.D;
+
+  // As above; members are slices, then maps, then column tiles.
+  const uint32_t wg = blockIdx.x;
+  if (p.part_o == nullptr) clear_other_rows<TV>(a, wg, gridDim.x);
+  const uint32_t round = p.members.divide(wg / kXcds);
+  const int unit = static_cast<int>(round * kXcds + wg % kXcds);
+  if (unit >= p.units) return;
+  int member = static_cast<int>(wg / kXcds - round * p.members.d);
+  const int split = static_cast<int>(p.sequences.divide(unit)), b = unit - split * a.tokens.B;
+  const Sequence seq = sequence_of(a.tokens, cache, b);
+  const int slice = static_cast<int>(p.slices.remainder(member));
+  member = static_cast<int>(p.slices.divide(member));
+  const int map = static_cast<int>(p.maps.remainder(member)), f0 = static_cast<int>(p.repeats.divide(map)) * a.RP;
+  member = static_cast<int>(p.maps.divide(member));
+  const int d0 = (slice * NW + wave) * DBW * 16;
+  const int nb = max(0, min(DBW, (D - d0) / 16));   // blocks of this wave (the last slice may have fewer)
+  const int wt = wave >> 1, wh = wave & 1;          // this wave's tile of a step, and half of it
+  const float sc = score_scale(a, map);
+
+  TQ* qs = reinterpret_cast<TQ*>(lds);
+  float* refs = reinterpret_cast<float*>(lds + Lds::REFS);
+  float* own = reinterpret_cast<float*>(lds + Lds::OWN) + wave * 16 * CT;
+  int* sees = reinterpret_cast<int*>(lds + Lds::SEES);
+  int* moved = reinterpret_cast<int*>(lds + Lds::MOVED);
+
+  for (int ct0 = member; ct0 * 16 * CT < seq.rows; ct0 += p.n_ct) {
+    const int col0 = ct0 * 16 * CT, n_used = min(16 * CT, seq.rows - col0);
+    auto row_of = [&](int col) { return (seq.n0 + col0 + col) * a.S + map; };
+    const int limit = visible_to(seq, col0 + n_used - 1, a.causal), all_see = visible_to(seq, col0, a.causal);
+    const int n_kt = (limit + 31) / 32;
+    const int kt0 = min(n_kt, split * p.per), kt1 = split == p.n_split - 1 ? n_kt : min(n_kt, kt0 + p.per);
+    if (split > 0 && kt0 == kt1) {   // nothing left for this part
+      if (slice == 0)
+        for (int i = static_cast<int>(threadIdx.x); i < n_used; i += 64 * NW) p.part_l[split * p.rows + row_of(i)] = 0.f;
+      continue;
+    }
+
+    // A tile's page is in the lane of its place in the step.
+    auto pages_at = [&](int base) { return lane < TS && base + lane < kt1 ? page_of(cache, b, base + lane) : -1; };
+    int pages = pages_at(kt0), pages_next = pages_at(kt0 + TS);
+
+    // Queries: sixteen threads to a column, zero behind the last one.
+    if (ct0 != member) lds_barrier();   // the last tiles' have been read
+    for (int col = static_cast<int>(threadIdx.x) >> 4; col < 16 * CT; col += 4 * NW) {
+      const TQ* src = static_cast<const TQ*>(a.q) + (seq.n0 + col0 + (col < n_used ? col : 0)) * a.ldq + f0;
+      for (int f = (static_cast<int>(threadIdx.x) & 15) * 8; f < 64 * NK; f += 128) {
+        u32x4 v = {0, 0, 0, 0};
+        if (col < n_used && f < a.RP) v = load16B(src + f);
+        store16B(qs + col * QP + f, v);
+      }
+    }
+    for (int i = static_cast<int>(threadIdx.x); i < 16 * CT; i += 64 * NW) {
+      sees[i] = visible_to(seq, col0 + min(i, n_used - 1), a.causal);
+      refs[i] = kNoScore;
+    }
+
+    // Addresses as above.
+    const uint32_t key_lane = static_cast<uint32_t>(((8 * (c >> 2) + 4 * wh + (c & 3)) * W + 8 * g) * 2);
+    const uint32_t value_lane = static_cast<uint32_t>((32 * c + 8 * g) * 2);
+    u32x4 kf[2 * NK], vf[2][DBW];
+    auto load_keys = [&](int kt, int page) {
+      const char* base = uniform_ptr(static_cast<const char*>(cache.keys) +
+                                     (max(page, 0) * cache.key_page + static_cast<int64_t>(tile_of(cache, kt)) * 32 * W + f0) * 2);
+      const uint32_t at = page < 0 ? 0 : key_lane;
+#pragma unroll
+      for (int j = 0; j < NK; ++j) {   // a group past the last feature is multiplied by zero
+        const char* from = base + 128 * min(j, a.RP / 64 - 1);
+        kf[2 * j] = load_at(from, at);
+        kf[2 * j + 1] = load_at(from, at + 64);
+      }
+    };
+    auto load_values = [&](u32x4 (&v)[DBW], int kt, int page) {
+      const char* base = uniform_ptr(static_cast<const char*>(cache.values) +
+                                     (max(page, 0) * cache.value_page + (static_cast<int64_t>(tile_of(cache, kt)) * D + (nb > 0 ? d0 : 0)) * 32) * 2);
+      const uint32_t at = page < 0 ? 0 : value_lane;
+#pragma unroll
+      for (int i = 0; i < DBW; ++i) v[i] = load_at(base + 1024 * max(0, min(i, nb - 1)), at);
+    };
+    load_keys(kt0 + wt, __builtin_amdgcn_readlane(pages, wt));
+    load_values(vf[0], kt0, __builtin_amdgcn_readlane(pages, 0));
+    load_values(vf[1], kt0 + 1, __builtin_amdgcn_readlane(pages, 1));
+    f32x4 acc[CT][DBW];
+    float l_part[CT], l_step[CT];   // sums of this lane's probabilities, and of a step's
+#pragma unroll
+    for (int i = 0; i < CT; ++i)
+#pragma unroll
+      for (int j = 0; j < DBW; ++j) acc[i][j] = zero4();
+#pragma unroll
+    for (int i = 0; i < CT; ++i) l_part[i] = l_step[i] = 0.f;
+    __builtin_amdgcn_sched_barrier(0);
+    lds_barrier();   // the queries are there
+
+    int buf = 0;
+    for (int base = kt0; base < kt1; base += TS) {
+      const int pages_after = pages_at(base + 2 * TS);
+      const int kt = base + wt, page = __builtin_amdgcn_readlane(pages, wt);
+      const int live = page < 0 ? 0 : min(32, limit - kt * 32);
+      char* mine = lds + Lds::PROBS + (buf * TS + wt) * CT * 1024 + lane * 16 + 8 * wh;
+      const q8* qf = reinterpret_cast<const q8*>(qs + c * QP + 8 * g);
+      float over = -INFINITY;   // the largest exponent
+      // Probabilities of column tiles i and i + 1 for this wave's tokens.
+      // FIND: with a reference of their own maximum, rounded up to a whole number
+      // so that what it scales stays exact.
+      auto probabilities = [&](int i, auto masked, auto find) {
+        constexpr int PAIR = CT > 1 ? 2 : 1;
+        f32x4 st[PAIR];
+#pragma unroll
+        for (int u = 0; u < PAIR; ++u) st[u] = zero4();
+#pragma unroll
+        for (int j = 0; j < 2 * NK; ++j)
+#pragma unroll
+          for (int u = 0; u < PAIR; ++u)
+            st[u] = Elem<TQ>::mma(__builtin_bit_cast(q8, kf[j]), qf[(16 * (i + u) * QP + 32 * j) / 8], st[u]);
+#pragma unroll
+        for (int u = 0; u < PAIR; ++u) {
+          const int col = 16 * (i + u) + c;
+          float m = refs[col];
+          const int seen = masked ? min(live, sees[col] - kt * 32) - 8 * g - 4 * wh : 4;   // of this lane's four tokens
+          f32x4 x;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = masked && e >= seen ? -INFINITY : st[u][e] * sc;
+          if constexpr (find) {
+            const float mx = group_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
+            if (mx > m + kRescaleSlack) m = __builtin_ceilf(mx);
+            own[col] = m;
+          }
+          v4 pv;
+          float l = 0.f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[e] -= m;
+            if constexpr (!find) over = fmaxf(over, x[e]);
+            const float v = __builtin_amdgcn_exp2f(x[e]);
+            l += v;
+            pv[e] = static_cast<TV>(v);
+          }
+          l_step[i + u] = l;
+          *reinterpret_cast<v4*>(mine + (i + u) * 1024) = pv;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      };
+      constexpr std::true_type yes{};
+      constexpr std::false_type no{};
+      if (base > kt0) {
+        if (live == 32 && kt * 32 + 32 <= all_see) {
+#pragma unroll
+          for (int i = 0; i < CT; i += 2) probabilities(i, no, no);
+        } else {
+#pragma unroll
+          for (int i = 0; i < CT; i += 2) probabilities(i, yes, no);
+        }
+      }
+      const bool raises = base == kt0 || __ballot(over > kRescaleSlack);
+      if (raises) {
+#pragma unroll
+        for (int i = 0; i < CT; i += 2) probabilities(i, yes, yes);
+#pragma unroll
+        for (int i = 0; i < CT; ++i) l_part[i] *= __builtin_amdgcn_exp2f(refs[16 * i + c] - own[16 * i + c]);
+      }
+#pragma unroll
+      for (int i = 0; i < CT; ++i) l_part[i] += l_step[i];
+      if (lane == 0) moved[buf * NW + wave] = raises;
+      __builtin_amdgcn_sched_barrier(0);
+      load_keys(kt + TS, __builtin_amdgcn_readlane(pages_next, wt));
+      __builtin_amdgcn_sched_barrier(0);
+      lds_barrier();
+      int moves = 0;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) moves |= moved[buf * NW + w];
+      if (__builtin_amdgcn_readfirstlane(moves)) {
+        // To the largest of the waves' references: this wave's probabilities, and
+        // what has been added up.
+        if (!raises)
+          for (int i = lane; i < 16 * CT; i += 64) own[i] = refs[i];
+        lds_barrier();
+#pragma unroll
+        for (int i = 0; i < CT; ++i) {
+          const float* all = reinterpret_cast<const float*>(lds + Lds::OWN) + 16 * i + c;
+          float m = all[0];
+#pragma unroll
+          for (int w = 1; w < NW; ++w) m = fmaxf(m, all[w * 16 * CT]);
+          const float f = __builtin_amdgcn_exp2f(own[16 * i + c] - m), fa = __builtin_amdgcn_exp2f(refs[16 * i + c] - m);
+          l_part[i] *= f;
+#pragma unroll
+          for (int j = 0; j < DBW; ++j) acc[i][j] *= fa;
+          v4 pv = *reinterpret_cast<const v4*>(mine + i * 1024);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) pv[e] = static_cast<TV>(static_cast<float>(pv[e]) * f);
+          *reinterpret_cast<v4*>(mine + i * 1024) = pv;
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        lds_barrier();
+        for (int i = static_cast<int>(threadIdx.x); i < 16 * CT; i += 64 * NW) {
+          const float* all = reinterpret_cast<const float*>(lds + Lds::OWN) + i;
+          float m = all[0];
+          for (int w = 1; w < NW; ++w) m = fmaxf(m, all[w * 16 * CT]);
+          refs[i] = m;   // read again behind the next step's barrier, or by this step's next
+        }
+        lds_barrier();
+      }
+      const char* probs = lds + Lds::PROBS + buf * TS * CT * 1024 + lane * 16;
+#pragma unroll
+      for (int t = 0; t < TS; ++t) {
+        const int page_t = __builtin_amdgcn_readlane(pages, t);
+        const int live_t = page_t < 0 ? 0 : min(32, limit - (base + t) * 32);
+        u32x4(&v)[DBW] = vf[t & 1];
+        if (live_t < 32) {   // what lies behind the last token is not multiplied: it may hold anything
+          u32x4 keep;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            keep[e] = (8 * g + 2 * e < live_t ? 0xffffu : 0u) | (8 * g + 2 * e + 1 < live_t ? 0xffff0000u : 0u);
+#pragma unroll
+          for (int j = 0; j < DBW; ++j) v[j] &= keep;
+        }
+#pragma unroll
+        for (int i = 0; i < CT; ++i) {
+          const v8 pv = *reinterpret_cast<const v8*>(probs + (t * CT + i) * 1024);
+#pragma unroll
+          for (int j = 0; j < DBW; ++j) acc[i][j] = Elem<TV>::mma(__builtin_bit_cast(v8, v[j]), pv, acc[i][j]);
+        }
+        const int next = t + 2 < TS ? __builtin_amdgcn_readlane(pages, t + 2) : __builtin_amdgcn_readlane(pages_next, t + 2 - TS);
+        load_values(v, base + t + 2, next);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      pages = pages_next;
+      pages_next = pages_after;
+      buf ^= 1;
+    }
+
+    // The waves' sums of exponentials; the rest of a column is in one wave.
+    float* ls = reinterpret_cast<float*>(lds + Lds::OWN);
+    lds_barrier();
+#pragma unroll
+    for (int i = 0; i < CT; ++i) {
+      const float l = group_sum(l_part[i]);
+      if (g == 0) ls[wave * 16 * CT + 16 * i + c] = l;
+    }
+    lds_barrier();
+#pragma unroll
+    for (int i = 0; i < CT; ++i) {
+      const int col = 16 * i + c;
+      float l = 0.f;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) l += ls[w * 16 * CT + col];
+      const float m = refs[col];
+      const int64_t row = row_of(min(col, n_used - 1));
+      if (wave == 0 && g == 0 && slice == 0 && col < n_used) {
+        if (p.part_o) {
+          p.part_m[split * p.rows + row] = m;
+          p.part_l[split * p.rows + row] = l;
+        } else if (a.lse2) {
+          a.lse2[row] = l == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(l);
+        }
+      }
+      if (p.part_o) {
+        float* to = p.part_o + (split * p.rows + row) * D + d0 + 4 * g;
+#pragma unroll
+        for (int j = 0; j < DBW; ++j)
+          if (j < nb && col < n_used) *reinterpret_cast<f32x4*>(to + 16 * j) = acc[i][j];
+      } else {
+        const float f = l == 0.f ? 0.f : 1.f / l;
+        TV* to = static_cast<TV*>(a.out) + row * D + d0 + 4 * g;
+#pragma unroll
+        for (int j = 0; j < DBW; ++j) {
+          v4 r;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) r[e] = static_cast<TV>(acc[i][j][e] * f);
+          if (j < nb && col < n_used) *reinterpret_cast<v4*>(to + 16 * j) = r;
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+}
+
 // The parts of a row joined: out = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i,
 // summed over the maps by their weights where asked.  A workgroup takes 64
 // features of a row; a wave reads them of four parts at once.
@@ -533,11 +842,11 @@ struct Plan {
 
 Plan plan(const PagedAttentionArgs& a) {
   Plan r;
-  r.one = false;
-  r.ct = 1;
-  r.nw = 4;
+  r.one = a.max_chunk >= 32;
+  r.ct = r.one ? a.RP <= 256 ? 8 : 4 : 1;
+  r.nw = r.one ? 8 : 4;
   const int64_t cols = static_cast<int64_t>(std::max(a.max_chunk, 1)) * (r.one ? 1 : a.S);
-  const int most = 8 * 16 * r.nw;   // features of a workgroup
+  const int most = 512;   // features of a workgroup
   r.n_slices = (a.cache.D + most - 1) / most;
   r.dbw = (a.cache.D + r.n_slices * 16 * r.nw - 1) / (r.n_slices * 16 * r.nw);
   const int per_ct = r.n_slices * (r.one ? a.S : 1);
@@ -546,9 +855,10 @@ Plan plan(const PagedAttentionArgs& a) {
   // Parts of whole steps, as many as make kWantWorkgroups where all sequences
   // are as long as the longest.
   const int64_t tiles = (std::max(a.max_length, 1) + 31) / 32;
-  int64_t per = (a.tokens.B * r.members * tiles + kWantWorkgroups - 1) / kWantWorkgroups;
+  const int want = r.one ? 512 : kWantWorkgroups;
+  int64_t per = (a.tokens.B * r.members * tiles + want - 1) / want;
   per = std::max(per, (tiles + kMaxSplits - 1) / kMaxSplits);
-  r.per = static_cast<int>(round_up(std::max<int64_t>(per, 1), r.nw));
+  r.per = static_cast<int>(round_up(std::max<int64_t>(per, 1), 4));
   r.n_split = static_cast<int>((tiles + r.per - 1) / r.per);
   r.parts = r.n_split > 1 || a.mix != nullptr;
   return r;
@@ -564,6 +874,19 @@ void launch_kernel(const Params& p, hipStream_t stream) {
                      stream, p);
 }
 
+template <typename TQ, typename TV, int NK, int DBW, int CT>
+void launch_chunk_kernel(const Params& p, hipStream_t stream) {
+  const unsigned units = static_cast<unsigned>(round_up(p.units, kXcds));
+  hipLaunchKernelGGL((paged_chunk_kernel<TQ, TV, NK, DBW, CT>), dim3(units * p.members.d), dim3(64 * kChunkWaves), (ChunkLds<NK, CT>::BYTES),
+                     stream, p);
+}
+template <typename TQ, typename TV, int DBW>
+void launch_chunk(const Params& p, hipStream_t stream) {
+  if (p.a.RP <= 128) launch_chunk_kernel<TQ, TV, 2, DBW, 8>(p, stream);
+  else if (p.a.RP <= 256) launch_chunk_kernel<TQ, TV, 4, DBW, 8>(p, stream);
+  else launch_chunk_kernel<TQ, TV, 8, DBW, 4>(p, stream);
+}
+
 template <typename TQ, typename TV, int DBW>
 void launch_width(const Params& p, hipStream_t stream) {
   if (p.a.cache.W <= 256) launch_kernel<TQ, TV, 4, DBW, 1, 4, false, 2, 2>(p, stream);
@@ -572,7 +895,14 @@ void launch_width(const Params& p, hipStream_t stream) {
 
 template <typename TQ, typename TV>
 void launch_typed(const Params& p, const Plan& r, hipStream_t stream) {
-  switch (r.dbw) {
+  if (r.one) {
+    switch (r.dbw) {
+      case 1: launch_chunk<TQ, TV, 1>(p, stream); break;
+      case 2: launch_chunk<TQ, TV, 2>(p, stream); break;
+      case 3: launch_chunk<TQ, TV, 3>(p, stream); break;
+      default: launch_chunk<TQ, TV, 4>(p, stream); break;
+    }
+  } else switch (r.dbw) {
     case 1: launch_width<TQ, TV, 1>(p, stream); break;
     case 2: launch_width<TQ, TV, 2>(p, stream); break;
     case 3: launch_width<TQ, TV, 3>(p, stream); break;
