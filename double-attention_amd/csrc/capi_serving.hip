@@ -15,7 +15,7 @@ namespace {
 
 constexpr int64_t kMaxRows = 1 << 22;        // new tokens of a call
 constexpr int64_t kMaxSequences = 65535;     // a grid's second dimension
-constexpr int64_t kMaxTokens = 1 << 28;      // tokens of a sequence
+constexpr int64_t kMaxTokens = 1 << 27;      // tokens of a sequence
 constexpr int64_t kMaxStride = 1LL << 40;
 
 int validate_cache(const char* what, const da_paged_cache& c, int64_t sequences) {
@@ -29,7 +29,7 @@ int validate_cache(const char* what, const da_paged_cache& c, int64_t sequences)
   if (sequences < 0 || sequences > kMaxSequences)
     return fail(DA_ERR_UNSUPPORTED, "%s: sequences must be in [0, %lld]", what, (long long)kMaxSequences);
   if (c.table_pages < 0 || c.ld_table < c.table_pages || c.ld_table > kMaxStride || c.table_pages > kMaxTokens / c.page_size)
-    return fail(DA_ERR_INVALID_ARGUMENT, "%s: a page table's row has fewer entries than are read, or more than 2^28 tokens", what);
+    return fail(DA_ERR_INVALID_ARGUMENT, "%s: a page table's row has fewer entries than are read, or more than 2^27 tokens", what);
   if (!c.keys || !c.values || (sequences > 0 && c.table_pages > 0 && !c.page_table))
     return fail(DA_ERR_INVALID_ARGUMENT, "%s: null pointer in the cache", what);
   if (!aligned(c.keys, 16) || !aligned(c.values, 16) || !aligned(c.page_table, 4) || c.key_page_stride % 8 || c.value_page_stride % 8)
@@ -189,7 +189,7 @@ int da_cache_select(const float* weights, int64_t ld_weights, int64_t capacity, 
                     int64_t keep, int64_t recent, int32_t* kept, int32_t* counts, da_stream_t stream) {
   const char* what = "cache select";
   if (sequences < 0 || sequences > kMaxSequences || capacity < 0 || capacity > kMaxTokens)
-    return fail(DA_ERR_UNSUPPORTED, "%s: sequences must be in [0, %lld], rows up to 2^28 tokens", what, (long long)kMaxSequences);
+    return fail(DA_ERR_UNSUPPORTED, "%s: sequences must be in [0, %lld], rows up to 2^27 tokens", what, (long long)kMaxSequences);
   if (keep < 0 || keep > kMaxTokens || recent < 0 || recent > keep)
     return fail(DA_ERR_INVALID_ARGUMENT, "%s: needs 0 <= recent <= keep", what);
   if (sequences == 0) return ok();

@@ -767,25 +767,49 @@ __global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(Params p)
   }
 }
 
-// Attention weights of the cached tokens: a wave takes 32 tokens of a sequence,
-// holds a map's keys in registers and goes through the new tokens, 16 at a
-// time; S^T = K Q^T as above, p = 2^(score - lse2), summed over the columns.
+// Attention weights of the cached tokens: p = 2^(score - lse2), summed over the
+// columns.  A wave takes 32 tokens of a sequence, holds a map's keys in registers
+// and goes through the new tokens, 16 at a time, the next ones' queries on their
+// way; S^T = K Q^T as above.  With many new tokens `share` waves of a workgroup
+// take the same tokens and a part of the maps and new tokens each.
 template <typename TQ, int KS>
-__global__ __launch_bounds__(64 * kWaves) void paged_weights_kernel(PagedAttentionArgs a) {
+__global__ __launch_bounds__(64 * kWaves) void paged_weights_kernel(PagedAttentionArgs a, int share) {
   typedef typename Elem<TQ>::v8 q8;
+  __shared__ float sums[kWaves][32];
   const CacheView& cache = a.cache;
   const int lane = lane_id(), c = lane & 15, g = lane >> 4;
-  const int kt = static_cast<int>(blockIdx.x) * kWaves + uniform_wave(), b = static_cast<int>(blockIdx.y);
-  if (kt * 32 >= a.capacity) return;
+  const int wave = uniform_wave(), part = wave % share;
+  const int kt = (static_cast<int>(blockIdx.x) * kWaves + wave) / share, b = static_cast<int>(blockIdx.y);
   const Sequence seq = sequence_of(a.tokens, cache, b);
   const int S = a.S, W = cache.W, RP = a.RP;
   f32x4 sum[2] = {zero4(), zero4()};
   const int page = kt * 32 < seq.cached ? page_of(cache, b, kt) : -1;
-  if (page >= 0) {
+  // The first sixteen new tokens that see one of these tokens, and how many
+  // sixteens follow, over all maps.
+  const int first = a.causal ? max(0, kt * 32 - (seq.length - seq.rows)) / 16 : 0;
+  const int blocks = max(0, (seq.rows + 15) / 16 - first);
+  if (page >= 0 && blocks > 0) {
     const TQ* kb = static_cast<const TQ*>(cache.keys) + page * cache.key_page +
                    (static_cast<int64_t>(tile_of(cache, kt)) * 32 + 8 * (c >> 2) + (c & 3)) * W + 8 * g;
-    for (int s = 0; s < S; ++s) {
-      const int from = s / a.repeat * RP;
+    const int64_t total = static_cast<int64_t>(S) * blocks;
+    int64_t at = total * part / share;
+    const int64_t end = total * (part + 1) / share;
+    q8 qf[KS];
+    float lse2 = 0.f;
+    int vis = 0;
+    auto load_queries = [&](int s, int i0) {
+      const int i = min(i0 + c, seq.rows - 1);
+      const TQ* qb = static_cast<const TQ*>(a.q) + (seq.n0 + i) * a.ldq + s / a.repeat * RP + 8 * g;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) qf[k] = load8(qb + min(32 * k, RP - 32));
+      lse2 = a.lse2[(seq.n0 + i) * S + s];
+      vis = i0 + c < seq.rows ? visible_to(seq, i, a.causal) : 0;
+    };
+    while (at < end) {
+      const int s = static_cast<int>(at / blocks), from = s / a.repeat * RP;
+      const int r0 = static_cast<int>(at - static_cast<int64_t>(s) * blocks);
+      const int r1 = static_cast<int>(min(static_cast<int64_t>(blocks), r0 + (end - at)));
+      at += r1 - r0;
       q8 kf[KS][2];
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
@@ -793,26 +817,26 @@ __global__ __launch_bounds__(64 * kWaves) void paged_weights_kernel(PagedAttenti
         kf[k][1] = load8(kb + from + min(32 * k, RP - 32) + 4 * W);
       }
       const float sc = score_scale(a, s);
-      // The first new token that sees one of these tokens.
-      const int first = a.causal ? max(0, kt * 32 - (seq.length - seq.rows)) / 16 : 0;
-      for (int i0 = first * 16; i0 < seq.rows; i0 += 16) {
-        const int i = min(i0 + c, seq.rows - 1);
-        const TQ* qb = static_cast<const TQ*>(a.q) + (seq.n0 + i) * a.ldq + from + 8 * g;
+      load_queries(s, (first + r0) * 16);
+      for (int r = r0; r < r1; ++r) {
         f32x4 st[2] = {zero4(), zero4()};
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
-          if (32 * k >= RP) break;
-          const q8 qv = load8(qb + 32 * k);
-          st[0] = Elem<TQ>::mma(kf[k][0], qv, st[0]);
-          st[1] = Elem<TQ>::mma(kf[k][1], qv, st[1]);
+          if (32 * k < RP) {
+            st[0] = Elem<TQ>::mma(kf[k][0], qf[k], st[0]);
+            st[1] = Elem<TQ>::mma(kf[k][1], qf[k], st[1]);
+          }
         }
-        const int vis = i0 + c < seq.rows ? visible_to(seq, i, a.causal) : 0;
-        const float lse2 = a.lse2[(seq.n0 + i) * S + s];
+        const float l = lse2;
+        const int seen = vis - kt * 32 - 8 * g;
+        if (r + 1 < r1) load_queries(s, (first + r + 1) * 16);
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (kt * 32 + 8 * g + 4 * h + e < vis) sum[h][e] += __builtin_amdgcn_exp2f(st[h][e] * sc - lse2);
+          for (int e = 0; e < 4; ++e) {
+            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(st[h][e], sc, -l));
+            sum[h][e] += 4 * h + e < seen ? x : 0.f;
+          }
       }
     }
   }
@@ -822,12 +846,15 @@ __global__ __launch_bounds__(64 * kWaves) void paged_weights_kernel(PagedAttenti
     for (int e = 0; e < 4; ++e) {
 #pragma unroll
       for (int x = 8; x >= 1; x >>= 1) sum[h][e] += __shfl_xor(sum[h][e], x);
-      const int t = kt * 32 + 8 * g + 4 * h + e;
-      if (c == 0 && t < a.capacity) {
-        const float before = a.weights_in && t < seq.length - seq.rows && t < seq.cached ? a.weights_in[b * a.ld_weights + t] : 0.f;
-        a.weights_out[b * a.ld_weights + t] = t < seq.cached ? before + sum[h][e] : 0.f;
-      }
+      if (c == 0) sums[wave][8 * g + 4 * h + e] = sum[h][e];
     }
+  __syncthreads();
+  const int t = kt * 32 + lane;
+  if (part == 0 && lane < 32 && t < a.capacity) {
+    float v = a.weights_in && t < seq.length - seq.rows && t < seq.cached ? a.weights_in[b * a.ld_weights + t] : 0.f;
+    for (int w = 0; w < share; ++w) v += sums[wave + w][lane];
+    a.weights_out[b * a.ld_weights + t] = t < seq.cached ? v : 0.f;
+  }
 }
 
 namespace {
@@ -962,11 +989,14 @@ void launch_paged_attention(const PagedAttentionArgs& a, void* workspace, hipStr
 
 template <typename TQ>
 static void launch_weights_typed(const PagedAttentionArgs& a, hipStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(((a.capacity + 31) / 32 + kWaves - 1) / kWaves), static_cast<unsigned>(a.tokens.B));
+  const int64_t blocks = static_cast<int64_t>(a.S) * ((std::max(a.max_chunk, 1) + 15) / 16);
+  const int share = blocks >= 4 ? 4 : blocks >= 2 ? 2 : 1;
+  const dim3 grid(static_cast<unsigned>((static_cast<int64_t>((a.capacity + 31) / 32) * share + kWaves - 1) / kWaves),
+                  static_cast<unsigned>(a.tokens.B));
   const dim3 block(64 * kWaves);
-  if (a.RP <= 128) hipLaunchKernelGGL((paged_weights_kernel<TQ, 4>), grid, block, 0, stream, a);
-  else if (a.RP <= 256) hipLaunchKernelGGL((paged_weights_kernel<TQ, 8>), grid, block, 0, stream, a);
-  else hipLaunchKernelGGL((paged_weights_kernel<TQ, 16>), grid, block, 0, stream, a);
+  if (a.RP <= 128) hipLaunchKernelGGL((paged_weights_kernel<TQ, 4>), grid, block, 0, stream, a, share);
+  else if (a.RP <= 256) hipLaunchKernelGGL((paged_weights_kernel<TQ, 8>), grid, block, 0, stream, a, share);
+  else hipLaunchKernelGGL((paged_weights_kernel<TQ, 16>), grid, block, 0, stream, a, share);
 }
 
 void launch_paged_weights(const PagedAttentionArgs& a, hipStream_t stream) {

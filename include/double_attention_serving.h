@@ -24,7 +24,7 @@ extern "C" {
  * (elements; values lie in tiles of 32 tokens, a feature's tokens side by
  * side).  key_width is branches * routing_dim.  page_size: a multiple of 32 up
  * to 4096.  key_width: a multiple of 64 up to 1024.  value_dim: a multiple of
- * 64 up to 4096.  table_pages * page_size: up to 2^28.  Both tensors 16-byte aligned, page strides multiples of 8.
+ * 64 up to 4096.  table_pages * page_size: up to 2^27.  Both tensors 16-byte aligned, page strides multiples of 8.
  *
  * page_table: [sequences] rows of table_pages entries, ld_table apart: the pages
  * of each sequence in order.  An entry outside [0, pages) names no page: its

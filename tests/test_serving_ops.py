@@ -845,7 +845,7 @@ BAD_CACHES = [
     (dict(pages=0), -1, "no pages"), (dict(table_pages=5), -1, "fewer entries"), (dict(keys=0), -1, "null"), (dict(values=0), -1, "null"),
     (dict(page_table=0), -1, "null"), (dict(keys=PTR + 8), -3, "aligned"), (dict(key_page_stride=64 * 64 + 4), -3, "multiples of 8"),
     (dict(key_page_stride=64 * 32), -1, "at least a page"), (dict(value_page_stride=64 * 64), -1, "at least a page"),
-    (dict(table_pages=1 << 30, ld_table=1 << 30), -1, "2\\^28"),
+    (dict(table_pages=1 << 30, ld_table=1 << 30), -1, "2\\^27"),
 ]
 
 
