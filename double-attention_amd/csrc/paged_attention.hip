@@ -408,20 +408,21 @@ __global__ __launch_bounds__(64 * NW, OCC) void paged_attention_kernel(Params p)
 // a step takes four tiles.  Wave w forms the scores of half a tile (16 tokens)
 // for all columns, with its keys in registers and the queries in LDS, and
 // leaves its probabilities in LDS; after a barrier every wave multiplies them
-// with its own DBW blocks of the values, straight from memory.  The scores are formed against the reference that all waves share, without a
-// look at their maximum first; where one exceeds it by more than kRescaleSlack
-// (in the first step always) a wave forms them again and raises its reference,
-// and the waves agree on the largest.
+// with its own DBW blocks of the values, straight from memory.
+// Where a score exceeds the reference that all waves share by more than
+// kRescaleSlack a wave raises its own, and the waves agree on the largest behind
+// the barrier.
 constexpr int kChunkWaves = 8, kChunkTiles = 4;
 template <int NK, int CT>
 struct ChunkLds {   // bytes
   static constexpr int QP = 64 * NK + 8;
-  static constexpr int PROBS = 32 * CT * QP;                              // [2][tiles][CT][64 lanes] 16 bytes
-  static constexpr int REFS = PROBS + 2 * kChunkTiles * CT * 1024;        // [16 CT] floats: the shared references
-  static constexpr int OWN = REFS + 64 * CT;                              // [waves][16 CT] floats
-  static constexpr int SEES = OWN + kChunkWaves * 64 * CT;                // [16 CT] ints: tokens that a column sees
-  static constexpr int MOVED = SEES + 64 * CT;                            // [2][waves] ints
-  static constexpr int BYTES = MOVED + 2 * kChunkWaves * 4;
+  static constexpr int REFS = 0;                                    // [16 CT] floats: the shared references
+  static constexpr int SEES = 64 * CT;                              // [16 CT] ints: tokens that a column sees
+  static constexpr int OWN = 2 * 64 * CT;                           // [waves][16 CT] floats: the waves' references
+  static constexpr int MOVED = OWN + kChunkWaves * 64 * CT;         // [2][waves] ints
+  static constexpr int QUERIES = MOVED + 2 * kChunkWaves * 4;       // [16 CT] rows of QP
+  static constexpr int PROBS = QUERIES + 32 * CT * QP;              // [2][tiles][CT][64 lanes] 16 bytes
+  static constexpr int BYTES = PROBS + 2 * kChunkTiles * CT * 1024;
 };
 
 template <typename TQ, typename TV, int NK, int DBW, int CT>
@@ -456,7 +457,7 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(Params
   const int wt = wave >> 1, wh = wave & 1;          // this wave's tile of a step, and half of it
   const float sc = score_scale(a, map);
 
-  TQ* qs = reinterpret_cast<TQ*>(lds);
+  TQ* qs = reinterpret_cast<TQ*>(lds + Lds::QUERIES);
   float* refs = reinterpret_cast<float*>(lds + Lds::REFS);
   float* own = reinterpret_cast<float*>(lds + Lds::OWN) + wave * 16 * CT;
   int* sees = reinterpret_cast<int*>(lds + Lds::SEES);
@@ -492,6 +493,7 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(Params
       sees[i] = visible_to(seq, col0 + min(i, n_used - 1), a.causal);
       refs[i] = kNoScore;
     }
+    for (int i = lane; i < 16 * CT; i += 64) own[i] = kNoScore;
 
     // Addresses as above.
     const uint32_t key_lane = static_cast<uint32_t>(((8 * (c >> 2) + 4 * wh + (c & 3)) * W + 8 * g) * 2);
@@ -519,13 +521,13 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(Params
     load_values(vf[0], kt0, __builtin_amdgcn_readlane(pages, 0));
     load_values(vf[1], kt0 + 1, __builtin_amdgcn_readlane(pages, 1));
     f32x4 acc[CT][DBW];
-    float l_part[CT], l_step[CT];   // sums of this lane's probabilities, and of a step's
+    float l_part[CT];   // sums of this lane's probabilities
 #pragma unroll
     for (int i = 0; i < CT; ++i)
 #pragma unroll
       for (int j = 0; j < DBW; ++j) acc[i][j] = zero4();
 #pragma unroll
-    for (int i = 0; i < CT; ++i) l_part[i] = l_step[i] = 0.f;
+    for (int i = 0; i < CT; ++i) l_part[i] = 0.f;
     __builtin_amdgcn_sched_barrier(0);
     lds_barrier();   // the queries are there
 
@@ -536,12 +538,10 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(Params
       const int live = page < 0 ? 0 : min(32, limit - kt * 32);
       char* mine = lds + Lds::PROBS + (buf * TS + wt) * CT * 1024 + lane * 16 + 8 * wh;
       const q8* qf = reinterpret_cast<const q8*>(qs + c * QP + 8 * g);
-      float over = -INFINITY;   // the largest exponent
+      bool raises = false;
       // Probabilities of column tiles i and i + 1 for this wave's tokens.
-      // FIND: with a reference of their own maximum, rounded up to a whole number
-      // so that what it scales stays exact.
-      auto probabilities = [&](int i, auto masked, auto find) {
-        constexpr int PAIR = CT > 1 ? 2 : 1;
+      auto probabilities = [&](int i, auto masked) {
+        constexpr int PAIR = 2, READS = PAIR * 2 * NK, AHEAD = 4;
         f32x4 st[PAIR];
 #pragma unroll
         for (int u = 0; u < PAIR; ++u) st[u] = zero4();
@@ -550,6 +550,15 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(Params
 #pragma unroll
           for (int u = 0; u < PAIR; ++u)
             st[u] = Elem<TQ>::mma(__builtin_bit_cast(q8, kf[j]), qf[(16 * (i + u) * QP + 32 * j) / 8], st[u]);
+        // Four fragments stay in flight ahead of their MFMAs (left to itself the
+        // compiler reads one, waits, and multiplies).
+        __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+#pragma unroll
+        for (int n = 0; n < READS - AHEAD; ++n) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
 #pragma unroll
         for (int u = 0; u < PAIR; ++u) {
           const int col = 16 * (i + u) + c;
@@ -558,46 +567,36 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(Params
           f32x4 x;
 #pragma unroll
           for (int e = 0; e < 4; ++e) x[e] = masked && e >= seen ? -INFINITY : st[u][e] * sc;
-          if constexpr (find) {
-            const float mx = group_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
-            if (mx > m + kRescaleSlack) m = __builtin_ceilf(mx);
+          const float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+          // The reference moves, to a whole number (so that what it scales stays
+          // exact), where a score exceeds it by more than kRescaleSlack.
+          if (__ballot(mx > m + kRescaleSlack)) {
+            const float before = m, most = group_max(mx);
+            if (most > m + kRescaleSlack) m = __builtin_ceilf(most);
             own[col] = m;
+            l_part[i + u] *= __builtin_amdgcn_exp2f(before - m);
+            raises = true;
           }
           v4 pv;
-          float l = 0.f;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            x[e] -= m;
-            if constexpr (!find) over = fmaxf(over, x[e]);
-            const float v = __builtin_amdgcn_exp2f(x[e]);
-            l += v;
+            const float v = __builtin_amdgcn_exp2f(x[e] - m);
+            l_part[i + u] += v;
             pv[e] = static_cast<TV>(v);
           }
-          l_step[i + u] = l;
           *reinterpret_cast<v4*>(mine + (i + u) * 1024) = pv;
         }
         __builtin_amdgcn_sched_barrier(0);
       };
       constexpr std::true_type yes{};
       constexpr std::false_type no{};
-      if (base > kt0) {
-        if (live == 32 && kt * 32 + 32 <= all_see) {
+      if (live == 32 && kt * 32 + 32 <= all_see) {
 #pragma unroll
-          for (int i = 0; i < CT; i += 2) probabilities(i, no, no);
-        } else {
+        for (int i = 0; i < CT; i += 2) probabilities(i, no);
+      } else {
 #pragma unroll
-          for (int i = 0; i < CT; i += 2) probabilities(i, yes, no);
-        }
+        for (int i = 0; i < CT; i += 2) probabilities(i, yes);
       }
-      const bool raises = base == kt0 || __ballot(over > kRescaleSlack);
-      if (raises) {
-#pragma unroll
-        for (int i = 0; i < CT; i += 2) probabilities(i, yes, yes);
-#pragma unroll
-        for (int i = 0; i < CT; ++i) l_part[i] *= __builtin_amdgcn_exp2f(refs[16 * i + c] - own[16 * i + c]);
-      }
-#pragma unroll
-      for (int i = 0; i < CT; ++i) l_part[i] += l_step[i];
       if (lane == 0) moved[buf * NW + wave] = raises;
       __builtin_amdgcn_sched_barrier(0);
       load_keys(kt + TS, __builtin_amdgcn_readlane(pages_next, wt));
@@ -609,9 +608,6 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(Params
       if (__builtin_amdgcn_readfirstlane(moves)) {
         // To the largest of the waves' references: this wave's probabilities, and
         // what has been added up.
-        if (!raises)
-          for (int i = lane; i < 16 * CT; i += 64) own[i] = refs[i];
-        lds_barrier();
 #pragma unroll
         for (int i = 0; i < CT; ++i) {
           const float* all = reinterpret_cast<const float*>(lds + Lds::OWN) + 16 * i + c;
@@ -630,10 +626,11 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(Params
         }
         lds_barrier();
         for (int i = static_cast<int>(threadIdx.x); i < 16 * CT; i += 64 * NW) {
-          const float* all = reinterpret_cast<const float*>(lds + Lds::OWN) + i;
+          float* all = reinterpret_cast<float*>(lds + Lds::OWN) + i;
           float m = all[0];
           for (int w = 1; w < NW; ++w) m = fmaxf(m, all[w * 16 * CT]);
-          refs[i] = m;   // read again behind the next step's barrier, or by this step's next
+          refs[i] = m;
+          for (int w = 0; w < NW; ++w) all[w * 16 * CT] = m;
         }
         lds_barrier();
       }
@@ -657,6 +654,13 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(Params
 #pragma unroll
           for (int j = 0; j < DBW; ++j) acc[i][j] = Elem<TV>::mma(__builtin_bit_cast(v8, v[j]), pv, acc[i][j]);
         }
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+#pragma unroll
+        for (int i = 0; i < CT - 2; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, DBW, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, 2 * DBW, 0);
         const int next = t + 2 < TS ? __builtin_amdgcn_readlane(pages, t + 2) : __builtin_amdgcn_readlane(pages_next, t + 2 - TS);
         load_values(v, base + t + 2, next);
         __builtin_amdgcn_sched_barrier(0);
