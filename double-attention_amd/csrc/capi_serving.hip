@@ -17,6 +17,7 @@ constexpr int64_t kMaxRows = 1 << 22;        // new tokens of a call
 constexpr int64_t kMaxSequences = 65535;     // a grid's second dimension
 constexpr int64_t kMaxTokens = 1 << 27;      // tokens of a sequence
 constexpr int64_t kMaxStride = 1LL << 40;
+constexpr int64_t kMaxQueryPitch = 1 << 22;  // 128 rows span less than 2^32 bytes
 
 int validate_cache(const char* what, const da_paged_cache& c, int64_t sequences) {
   if (c.page_size < 32 || c.page_size % 32 || c.page_size > 4096)
@@ -153,6 +154,7 @@ int da_paged_attention(const da_paged_attention_args* args, da_stream_t stream) 
   const int64_t capacity = a.cache.table_pages * a.cache.page_size;
   if (a.rows > 0) {
     if ((rc = validate_rows16(what, "query", a.query, a.cache.key_width, a.ldq))) return rc;
+    if (a.ldq > kMaxQueryPitch) return fail(DA_ERR_UNSUPPORTED, "%s: a pitch of the queries above 2^22", what);
     if (!a.scales || !aligned(a.scales, static_cast<int>(element_bytes(a.scales_dtype))) || !aligned(a.mix, 4))
       return fail(DA_ERR_INVALID_ARGUMENT, "%s: the scales are null, or scales or mix not aligned", what);
     if (!a.out || !aligned(a.out, 16)) return fail(DA_ERR_ALIGNMENT, "%s: out must be 16-byte aligned", what);

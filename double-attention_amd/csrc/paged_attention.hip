@@ -89,6 +89,13 @@ __device__ __forceinline__ float score_scale(const PagedAttentionArgs& a, int s)
   return load_scalar(a.scales, a.scales_dtype, s) * a.scale_mult * kLog2e;
 }
 
+// A number that the compiler takes for a new one: what is worked out from it
+// stays where it is used, and out of registers elsewhere.
+__device__ __forceinline__ int opaque(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 // Sixteen bytes at a uniform global address and a lane's offset.
 typedef __attribute__((address_space(1))) const char* global_ptr;
 __device__ __forceinline__ u32x4 load_at(const char* base, uint32_t lane_offset) {
@@ -129,7 +136,6 @@ __global__ __launch_bounds__(64 * NW, OCC) void paged_attention_kernel(Params p)
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const PagedAttentionArgs& a = p.a;
   const CacheView& cache = a.cache;
-  const int lane = lane_id(), c = lane & 15, g = lane >> 4;
   const int wave = uniform_wave();
   const int W = cache.W, D = cache.D;
 
@@ -163,6 +169,10 @@ __global__ __launch_bounds__(64 * NW, OCC) void paged_attention_kernel(Params p)
   int* moved = reinterpret_cast<int*>(ms + PB * NW * 16 * CT);    // [PB][NW]
 
   for (int ct0 = member; ct0 * 16 * CT < n_cols; ct0 += p.n_ct) {
+    // Nearly always the only round: what depends on the lane is worked out in it,
+    // rather than in front of it and kept in registers that there are not.
+    const int tid = opaque(static_cast<int>(threadIdx.x));
+    const int lane = tid & 63, c = lane & 15, g = lane >> 4;
     const int col0 = ct0 * 16 * CT, n_used = min(16 * CT, n_cols - col0);
     auto token_of = [&](int col) { return ONE ? col : static_cast<int>(p.maps.divide(col)); };
     auto map_of = [&](int col) { return ONE ? map : static_cast<int>(p.maps.remainder(col)); };
@@ -172,7 +182,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void paged_attention_kernel(Params p)
     const int kt0 = min(n_kt, split * p.per), kt1 = split == p.n_split - 1 ? n_kt : min(n_kt, kt0 + p.per);
     if (split > 0 && kt0 == kt1) {   // nothing left for this part
       if (slice == 0)
-        for (int i = static_cast<int>(threadIdx.x); i < n_used; i += 64 * NW) p.part_l[split * p.rows + row_of(i)] = 0.f;
+        for (int i = tid; i < n_used; i += 64 * NW) p.part_l[split * p.rows + row_of(i)] = 0.f;
       continue;
     }
 
@@ -183,11 +193,11 @@ __global__ __launch_bounds__(64 * NW, OCC) void paged_attention_kernel(Params p)
 
     // Queries: sixteen threads to a column.
     if (ct0 != member) lds_barrier();   // the last tiles' have been read
-    for (int col = static_cast<int>(threadIdx.x) >> 4; col < 16 * CT; col += 4 * NW) {
+    for (int col = tid >> 4; col < 16 * CT; col += 4 * NW) {
       const bool used = col < n_used;
       const int from = ONE ? 0 : static_cast<int>(p.repeats.divide(map_of(col0 + col))) * a.RP;
       const TQ* src = static_cast<const TQ*>(a.q) + (seq.n0 + token_of(col0 + (used ? col : 0))) * a.ldq + f0;
-      for (int f = (static_cast<int>(threadIdx.x) & 15) * 8; f < passes * FW; f += 128) {
+      for (int f = (tid & 15) * 8; f < passes * FW; f += 128) {
         u32x4 v = {0, 0, 0, 0};
         if (used && f >= from && f < from + a.RP) v = load16B(src + f);
         store16B(qs + col * QP + f, v);
@@ -415,13 +425,12 @@ __global__ __launch_bounds__(64 * NW, OCC) void paged_attention_kernel(Params p)
 constexpr int kChunkWaves = 8, kChunkTiles = 4;
 template <int NK, int CT>
 struct ChunkLds {   // bytes
-  static constexpr int QP = 64 * NK + 8;
   static constexpr int REFS = 0;                                    // [16 CT] floats: the shared references
   static constexpr int SEES = 64 * CT;                              // [16 CT] ints: tokens that a column sees
   static constexpr int OWN = 2 * 64 * CT;                           // [waves][16 CT] floats: the waves' references
   static constexpr int MOVED = OWN + kChunkWaves * 64 * CT;         // [2][waves] ints
-  static constexpr int QUERIES = MOVED + 2 * kChunkWaves * 4;       // [16 CT] rows of QP
-  static constexpr int PROBS = QUERIES + 32 * CT * QP;              // [2][tiles][CT][64 lanes] 16 bytes
+  static constexpr int QUERIES = MOVED + 2 * kChunkWaves * 4;       // [CT][2 NK][64 lanes] 16 bytes
+  static constexpr int PROBS = QUERIES + 2 * NK * CT * 1024;        // [2][tiles][CT][64 lanes] 16 bytes
   static constexpr int BYTES = PROBS + 2 * kChunkTiles * CT * 1024;
 };
 
@@ -431,11 +440,10 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(Params
   typedef typename Elem<TV>::v8 v8;
   typedef typename Elem<TV>::v4 v4;
   typedef ChunkLds<NK, CT> Lds;
-  constexpr int NW = kChunkWaves, TS = kChunkTiles, QP = Lds::QP;
+  constexpr int NW = kChunkWaves, TS = kChunkTiles;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const PagedAttentionArgs& a = p.a;
   const CacheView& cache = a.cache;
-  const int lane = lane_id(), c = lane & 15, g = lane >> 4;
   const int wave = uniform_wave();
   const int W = cache.W, D = cache.D;
 
@@ -457,13 +465,15 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(Params
   const int wt = wave >> 1, wh = wave & 1;          // this wave's tile of a step, and half of it
   const float sc = score_scale(a, map);
 
-  TQ* qs = reinterpret_cast<TQ*>(lds + Lds::QUERIES);
   float* refs = reinterpret_cast<float*>(lds + Lds::REFS);
   float* own = reinterpret_cast<float*>(lds + Lds::OWN) + wave * 16 * CT;
   int* sees = reinterpret_cast<int*>(lds + Lds::SEES);
   int* moved = reinterpret_cast<int*>(lds + Lds::MOVED);
 
   for (int ct0 = member; ct0 * 16 * CT < seq.rows; ct0 += p.n_ct) {
+    const int tid = opaque(static_cast<int>(threadIdx.x));   // as above
+    const int lane = tid & 63, c = lane & 15, g = lane >> 4;
+    const q8* qs = reinterpret_cast<const q8*>(lds + Lds::QUERIES) + lane;
     const int col0 = ct0 * 16 * CT, n_used = min(16 * CT, seq.rows - col0);
     auto row_of = [&](int col) { return (seq.n0 + col0 + col) * a.S + map; };
     const int limit = visible_to(seq, col0 + n_used - 1, a.causal), all_see = visible_to(seq, col0, a.causal);
@@ -471,7 +481,7 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(Params
     const int kt0 = min(n_kt, split * p.per), kt1 = split == p.n_split - 1 ? n_kt : min(n_kt, kt0 + p.per);
     if (split > 0 && kt0 == kt1) {   // nothing left for this part
       if (slice == 0)
-        for (int i = static_cast<int>(threadIdx.x); i < n_used; i += 64 * NW) p.part_l[split * p.rows + row_of(i)] = 0.f;
+        for (int i = tid; i < n_used; i += 64 * NW) p.part_l[split * p.rows + row_of(i)] = 0.f;
       continue;
     }
 
@@ -479,17 +489,20 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(Params
     auto pages_at = [&](int base) { return lane < TS && base + lane < kt1 ? page_of(cache, b, base + lane) : -1; };
     int pages = pages_at(kt0), pages_next = pages_at(kt0 + TS);
 
-    // Queries: sixteen threads to a column, zero behind the last one.
+    // Queries, as the fragments that the products read; zero behind the last
+    // column and feature.  Thread t has the chunks t, t + 512, ... of the columns.
     if (ct0 != member) lds_barrier();   // the last tiles' have been read
-    for (int col = static_cast<int>(threadIdx.x) >> 4; col < 16 * CT; col += 4 * NW) {
-      const TQ* src = static_cast<const TQ*>(a.q) + (seq.n0 + col0 + (col < n_used ? col : 0)) * a.ldq + f0;
-      for (int f = (static_cast<int>(threadIdx.x) & 15) * 8; f < 64 * NK; f += 128) {
-        u32x4 v = {0, 0, 0, 0};
-        if (col < n_used && f < a.RP) v = load16B(src + f);
-        store16B(qs + col * QP + f, v);
-      }
+    constexpr int CHUNKS = 8 * NK, COLS = 64 * NW / CHUNKS, LOADS = 16 * CT / COLS;
+    const int q_col = tid / CHUNKS, q_f = tid % CHUNKS * 8;
+    const uint32_t q_lane = static_cast<uint32_t>((q_col * static_cast<int>(a.ldq) + q_f) * 2);
+    u32x4 qv[LOADS];
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const char* rows = uniform_ptr(static_cast<const char*>(a.q) + ((seq.n0 + col0 + min(i * COLS, n_used - 1)) * a.ldq + f0) * 2);
+      const bool there = i * COLS + q_col < n_used && q_f < a.RP;
+      qv[i] = load_at(rows, there ? q_lane : 0);
     }
-    for (int i = static_cast<int>(threadIdx.x); i < 16 * CT; i += 64 * NW) {
+    for (int i = tid; i < 16 * CT; i += 64 * NW) {
       sees[i] = visible_to(seq, col0 + min(i, n_used - 1), a.causal);
       refs[i] = kNoScore;
     }
@@ -520,6 +533,12 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(Params
     load_keys(kt0 + wt, __builtin_amdgcn_readlane(pages, wt));
     load_values(vf[0], kt0, __builtin_amdgcn_readlane(pages, 0));
     load_values(vf[1], kt0 + 1, __builtin_amdgcn_readlane(pages, 1));
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int col = i * COLS + q_col;
+      if (col >= n_used || q_f >= a.RP) qv[i] = u32x4{0, 0, 0, 0};
+      store16B(lds + Lds::QUERIES + ((col / 16 * 2 * NK + q_f / 32) * 64 + q_f % 32 * 2 + col % 16) * 16, qv[i]);
+    }
     f32x4 acc[CT][DBW];
     float l_part[CT];   // sums of this lane's probabilities
 #pragma unroll
@@ -537,7 +556,6 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(Params
       const int kt = base + wt, page = __builtin_amdgcn_readlane(pages, wt);
       const int live = page < 0 ? 0 : min(32, limit - kt * 32);
       char* mine = lds + Lds::PROBS + (buf * TS + wt) * CT * 1024 + lane * 16 + 8 * wh;
-      const q8* qf = reinterpret_cast<const q8*>(qs + c * QP + 8 * g);
       bool raises = false;
       // Probabilities of column tiles i and i + 1 for this wave's tokens.
       auto probabilities = [&](int i, auto masked) {
@@ -549,7 +567,7 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(Params
         for (int j = 0; j < 2 * NK; ++j)
 #pragma unroll
           for (int u = 0; u < PAIR; ++u)
-            st[u] = Elem<TQ>::mma(__builtin_bit_cast(q8, kf[j]), qf[(16 * (i + u) * QP + 32 * j) / 8], st[u]);
+            st[u] = Elem<TQ>::mma(__builtin_bit_cast(q8, kf[j]), qs[((i + u) * 2 * NK + j) * 64], st[u]);
         // Four fragments stay in flight ahead of their MFMAs (left to itself the
         // compiler reads one, waits, and multiplies).
         __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
@@ -563,7 +581,7 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(Params
         for (int u = 0; u < PAIR; ++u) {
           const int col = 16 * (i + u) + c;
           float m = refs[col];
-          const int seen = masked ? min(live, sees[col] - kt * 32) - 8 * g - 4 * wh : 4;   // of this lane's four tokens
+          const int seen = masked ? min(live, sees[col] - kt * 32) - (opaque(tid) & 48) / 2 - 4 * wh : 4;   // of this lane's four tokens
           f32x4 x;
 #pragma unroll
           for (int e = 0; e < 4; ++e) x[e] = masked && e >= seen ? -INFINITY : st[u][e] * sc;
@@ -608,6 +626,7 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(Params
       if (__builtin_amdgcn_readfirstlane(moves)) {
         // To the largest of the waves' references: this wave's probabilities, and
         // what has been added up.
+        const int c = opaque(tid) & 15;
 #pragma unroll
         for (int i = 0; i < CT; ++i) {
           const float* all = reinterpret_cast<const float*>(lds + Lds::OWN) + 16 * i + c;
@@ -625,7 +644,7 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(Params
           __builtin_amdgcn_sched_barrier(0);
         }
         lds_barrier();
-        for (int i = static_cast<int>(threadIdx.x); i < 16 * CT; i += 64 * NW) {
+        for (int i = tid; i < 16 * CT; i += 64 * NW) {
           float* all = reinterpret_cast<float*>(lds + Lds::OWN) + i;
           float m = all[0];
           for (int w = 1; w < NW; ++w) m = fmaxf(m, all[w * 16 * CT]);
@@ -641,6 +660,7 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(Params
         const int live_t = page_t < 0 ? 0 : min(32, limit - (base + t) * 32);
         u32x4(&v)[DBW] = vf[t & 1];
         if (live_t < 32) {   // what lies behind the last token is not multiplied: it may hold anything
+          const int g = (opaque(tid) & 63) >> 4;
           u32x4 keep;
 #pragma unroll
           for (int e = 0; e < 4; ++e)

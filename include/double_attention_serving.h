@@ -62,7 +62,7 @@ int da_cache_append(const da_paged_cache* cache, const void* key, int64_t ldk, c
  *   out[n, s] = sum_j softmax_j(scales[s] scale_mult <q_{n,s}, k_{j,s}>) v_j
  * over the tokens j of row n's sequence up to its own (causal) or all of them.
  * Map s has features [(s / map_repeat) * score_dim, + score_dim) of the rows of
- * query [rows, key_width] (pitch ldq, a multiple of 8) and of the keys;
+ * query [rows, key_width] (pitch ldq, a multiple of 8 up to 2^22) and of the keys;
  * score_dim is a multiple of 64 up to 512, at most 64 maps.
  * out: [rows, maps, value_dim], or with mix [maps] (fp32) its sum
  * over the maps with these weights, [rows, value_dim].  Rows that see nothing,
