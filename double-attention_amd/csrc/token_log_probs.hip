@@ -27,7 +27,8 @@ constexpr int kThreads = 64 * kWaves;
 constexpr float kSlack = 8.f;
 constexpr float kLowest = -3.402823466e38f;
 // Differences below this have no weight in 32 bits (e^-200 = 0).
-constexpr float kNoWeight = -200.f;
+constexpr float kNoWeight = -200.f, kNoWeight2 = -300.f;   // (base 2)
+constexpr float kLn2 = 0.6931471805599453f;
 typedef unsigned long long Key;
 
 struct Sums {
@@ -147,8 +148,13 @@ template <typename T, bool TOP>
 __global__ __launch_bounds__(kThreads) void token_log_probs_kernel(Params p) {
   __shared__ Sums wave_sums[kWaves];
   __shared__ Key wave_keys[TOP ? kWaves * kMaxTop : 1];
+  __shared__ volatile float wave_floors[kWaves];   // the waves' lists' last values, as far as they are known
   const TokenLogProbsArgs& a = p.a;
   const int lane = lane_id(), wave = wave_id(), tid = static_cast<int>(threadIdx.x);
+  if constexpr (TOP) {
+    if (tid < kWaves) wave_floors[tid] = -INFINITY;
+    __syncthreads();
+  }
   const int64_t row = blockIdx.x / p.parts;
   const int part = static_cast<int>(blockIdx.x % p.parts);
   const T* x = static_cast<const T*>(a.logits) + row * a.ldx;
@@ -156,63 +162,103 @@ __global__ __launch_bounds__(kThreads) void token_log_probs_kernel(Params p) {
   const int per = (shape.chunks + p.parts - 1) / p.parts;
   const int c1 = min(shape.chunks, (part + 1) * per);
 
+  // In this loop t is in units of log 2.  The difference to m is taken first: a
+  // rounded m log2(e) would shift all terms where the logits are far from zero.
   Sums v{kLowest, 0.f, 0.f};
+  // What the list still takes: more than its last value, or until it is full
+  // what reaches `bound`.
   TopList list{0, 0, a.top};
-  float floor = -INFINITY;
-  auto add = [&](float value, float m) {
-    const float d = value - m;
-    const float e = fast_exp(d);
+  float bound = -INFINITY, floor = -INFINITY;
+  auto add = [&](float value) {
+    const float d = (value - v.m) * kLog2e;
+    const float e = __builtin_amdgcn_exp2f(d);
     v.s += e;
-    v.t += e * fmaxf(d, kNoWeight);
+    v.t += e * fmaxf(d, kNoWeight2);
   };
   auto raise = [&](float largest) {   // the reference to this chunk's largest value
     if (largest > v.m + kSlack || (v.s == 0.f && largest > v.m)) {
       const float d = fmaxf(v.m - largest, kNoWeight), f = fast_exp(d);
-      v.t = (v.t + v.s * d) * f;
+      v.t = (v.t + v.s * d * kLog2e) * f;
       v.s *= f;
       v.m = largest;
     }
+  };
+  auto offer = [&](float value, int j, bool valid) {
+    list.offer(valid && value >= bound ? key_of(value, j) : 0);
+    floor = list.floor();
   };
   auto one = [&](int j, bool valid) {   // at most one element a lane
     const float value = valid ? static_cast<float>(x[j]) : 0.f;
     if (valid) {
       raise(value);
-      add(value, v.m);
+      add(value);
     }
-    if constexpr (TOP) {
-      list.offer(valid ? key_of(value, j) : 0);
-      floor = list.floor();
-    }
+    if constexpr (TOP) offer(value, j, valid);
   };
   if (part == 0 && wave == 0 && shape.head) one(lane, lane < shape.head);
   const T* body = x + shape.head;
   constexpr int U = 4;
-  for (int base = part * per + wave * 64; base < c1; base += kThreads * U) {
-    Chunk<T> ch[U];
+  Chunk<T> ch[U];
+  auto fetch = [&](int base) {
 #pragma unroll
     for (int u = 0; u < U; ++u) ch[u].load(body + static_cast<int64_t>(min(base + u * kThreads + lane, c1 - 1)) * 8);
+  };
+  const int first = part * per + wave * 64;
+  if (first < c1) fetch(first);
+  for (int base = first; base < c1; base += kThreads * U) {
+    Chunk<T> now[U];
+    float largest[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      now[u] = ch[u];
+      const bool valid = base + u * kThreads + lane < c1;
+      largest[u] = now[u][0];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) largest[u] = fmaxf(largest[u], now[u][e]);
+      if (!valid) largest[u] = -INFINITY;
+    }
+    if (base + kThreads * U < c1) fetch(base + kThreads * U);
+    if constexpr (TOP) {
+      if (base == first) {
+        // The top-th largest of the lanes' maxima: as many values reach it.
+        float mine = fmaxf(fmaxf(largest[0], largest[1]), fmaxf(largest[2], largest[3]));
+        mine = mine == mine ? mine : -INFINITY;
+        int rank = 0;
+        for (int i = 0; i < 64; ++i) {
+          const float other = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(mine), i));
+          rank += other > mine || (other == mine && i < lane);
+        }
+        bound = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(mine), __builtin_ctzll(__ballot(rank == a.top - 1))));
+      } else {
+        // No less than what the other waves' lists end with (equal values may
+        // come in front of theirs).
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) bound = fmaxf(bound, wave_floors[w]);
+      }
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int c = base + u * kThreads + lane;
       const bool valid = c < c1;
-      float largest = ch[u][0];
-#pragma unroll
-      for (int e = 1; e < 8; ++e) largest = fmaxf(largest, ch[u][e]);
       if (valid) {
-        raise(largest);
+        raise(largest[u]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) add(ch[u][e], v.m);
+        for (int e = 0; e < 8; ++e) add(now[u][e]);
       }
       if constexpr (TOP) {
-        if (__ballot(valid && (largest > floor || list.last == 0))) {
+        if (__ballot(valid && largest[u] >= bound && (largest[u] > floor || list.last == 0))) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) list.offer(valid ? key_of(ch[u][e], shape.head + 8 * c + e) : 0);
-          floor = list.floor();
+          for (int e = 0; e < 8; ++e) offer(now[u][e], shape.head + 8 * c + e, valid);
+          if (lane == 0) wave_floors[wave] = floor;
         }
       }
     }
   }
-  if (part == p.parts - 1 && wave == 0 && shape.tail) one(a.V - shape.tail + lane, lane < shape.tail);
+  if (part == p.parts - 1 && wave == 0 && shape.tail) {
+    bound = -INFINITY;
+    one(a.V - shape.tail + lane, lane < shape.tail);
+  }
+  v.t *= kLn2;
 
   v = join_wave(v);
   if (lane == 0) wave_sums[wave] = v;
