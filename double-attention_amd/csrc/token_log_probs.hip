@@ -77,7 +77,10 @@ struct TopList {
   int top;
   __device__ __forceinline__ void insert(Key k) {   // k: the same in all lanes, larger than last
     const int at = __popcll(__ballot(mine > k));
-    const Key up = __shfl_up(mine, 1);
+    // The lane in front's key (wave_shr:1 of both halves).
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<uint32_t>(mine), 0x138, 0xf, 0xf, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<uint32_t>(mine >> 32), 0x138, 0xf, 0xf, false);
+    const Key up = static_cast<Key>(hi) << 32 | lo;
     const int lane = lane_id();
     mine = lane < at ? mine : lane == at ? k : up;
     last = read_lane(mine, top - 1);
@@ -184,8 +187,12 @@ __global__ __launch_bounds__(kThreads) void token_log_probs_kernel(Params p) {
     }
   };
   auto offer = [&](float value, int j, bool valid) {
-    list.offer(valid && value >= bound ? key_of(value, j) : 0);
-    floor = list.floor();
+    // (An equal value may be of an earlier token than the list's last one.)
+    const bool wanted = valid && value >= bound && value >= floor;
+    if (__ballot(wanted)) {
+      list.offer(wanted ? key_of(value, j) : 0);
+      floor = list.floor();
+    }
   };
   auto one = [&](int j, bool valid) {   // at most one element a lane
     const float value = valid ? static_cast<float>(x[j]) : 0.f;
@@ -229,11 +236,6 @@ __global__ __launch_bounds__(kThreads) void token_log_probs_kernel(Params p) {
           rank += other > mine || (other == mine && i < lane);
         }
         bound = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(mine), __builtin_ctzll(__ballot(rank == a.top - 1))));
-      } else {
-        // No less than what the other waves' lists end with (equal values may
-        // come in front of theirs).
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) bound = fmaxf(bound, wave_floors[w]);
       }
     }
 #pragma unroll
@@ -247,6 +249,10 @@ __global__ __launch_bounds__(kThreads) void token_log_probs_kernel(Params p) {
       }
       if constexpr (TOP) {
         if (__ballot(valid && largest[u] >= bound && (largest[u] > floor || list.last == 0))) {
+          // No less than what the other waves' lists end with (equal values may
+          // come in front of theirs).
+#pragma unroll
+          for (int w = 0; w < kWaves; ++w) bound = fmaxf(bound, wave_floors[w]);
 #pragma unroll
           for (int e = 0; e < 8; ++e) offer(now[u][e], shape.head + 8 * c + e, valid);
           if (lane == 0) wave_floors[wave] = floor;
