@@ -107,50 +107,66 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 constexpr int kSelectThreads = 1024;
 constexpr int kSelectWaves = kSelectThreads / 64;
 constexpr int kDigit = 256;
+constexpr int kCopies = 4;   // of the bins
 
 }  // namespace
 
 // The `need` largest of a sequence's older tokens by the digits of their keys
 // from the highest: four counts of 256 bins find the key of the last one that
-// stays and how many of its equals do (the first ones).  Each wave then takes
-// a contiguous part of the tokens and writes the kept ones in order.
-__global__ __launch_bounds__(kSelectThreads) void cache_select_kernel(CacheSelectArgs a) {
-  __shared__ int bins[kDigit];
+// stays and how many of its equals do (the first ones).  Each wave has a
+// contiguous part of the tokens, read once where they fit its registers (32768
+// in all), and writes its kept ones in order.  The first digits of most weights
+// are alike, so the lanes of a wave share four copies of the bins: atomics of
+// one address wait for each other.  Bound by its passes on one CU: 1001 tokens of
+// each sequence 7 us, 32768 of them 22 us (46 us with one copy and the weights read
+// again at each pass).
+template <int KEYS>
+__device__ void select_older(const float* w, int32_t* kept, int older, int need, int rounds) {
+  __shared__ int copies[kCopies * (kDigit + 1)];
   __shared__ int picked[2];
   __shared__ int counts[2][kSelectWaves];
-  const int b = static_cast<int>(blockIdx.x), tid = static_cast<int>(threadIdx.x);
-  const int lane = lane_id(), wave = wave_id();
-  const int length = min(max(a.lengths[b], 0), a.capacity);
-  const int count = min(length, a.keep);
-  const int recent = min(a.recent, count);
-  const int older = length - recent;            // tokens to choose from
-  int need = count - recent;
-  const float* w = a.weights + b * a.ld_weights;
-  int32_t* kept = a.kept + static_cast<int64_t>(b) * a.keep;
-  if (tid == 0) a.counts[b] = count;
-  for (int i = tid; i < recent; i += kSelectThreads) kept[need + i] = older + i;
-  for (int i = count + tid; i < a.keep; i += kSelectThreads) kept[i] = -1;
-  if (need == older) {   // all stay
-    for (int i = tid; i < need; i += kSelectThreads) kept[i] = i;
-    return;
+  const int tid = static_cast<int>(threadIdx.x), lane = lane_id(), wave = wave_id();
+  const int i0 = wave * rounds * 64, i1 = min(older, i0 + rounds * 64);
+  uint32_t keys[KEYS > 0 ? KEYS : 1];
+  if constexpr (KEYS > 0) {
+#pragma unroll
+    for (int j = 0; j < KEYS; ++j)   // all in flight
+      if (j < rounds) keys[j] = __float_as_uint(w[min(i0 + j * 64 + lane, older - 1)]);
+#pragma unroll
+    for (int j = 0; j < KEYS; ++j)
+      if (j < rounds) keys[j] = weight_key(__uint_as_float(keys[j]));
   }
-  if (need == 0) return;
+  // f(first token of the round, this lane's key, whether it has one)
+  auto each = [&](auto f) {
+    if constexpr (KEYS > 0) {
+#pragma unroll
+      for (int j = 0; j < KEYS; ++j)
+        if (j < rounds) f(i0 + j * 64, keys[j], i0 + j * 64 + lane < i1);
+    } else {
+      for (int i = i0; i < i1; i += 64) f(i, i + lane < i1 ? weight_key(w[i + lane]) : 0, i + lane < i1);
+    }
+  };
   uint32_t prefix = 0, mask = 0;
   int equals = need;   // of the tokens with the key's digits so far, those that stay
   for (int shift = 24; shift >= 0; shift -= 8) {
-    if (tid < kDigit) bins[tid] = 0;
+    for (int i = tid; i < kCopies * (kDigit + 1); i += kSelectThreads) copies[i] = 0;
     __syncthreads();
-    for (int i = tid; i < older; i += kSelectThreads) {
-      const uint32_t key = weight_key(w[i]);
-      if ((key & mask) == prefix) atomicAdd(&bins[key >> shift & 255], 1);
-    }
+    int* mine = copies + (lane & (kCopies - 1)) * (kDigit + 1);
+    each([&](int, uint32_t key, bool there) {
+      if (there && (key & mask) == prefix) atomicAdd(&mine[key >> shift & 255], 1);
+    });
     __syncthreads();
     if (wave == 0) {
       // Lane l has bins 255 - 4 l down to 252 - 4 l; the sum in front of them
       // tells which lane's bins reach the number that stays.
       int n[4], own = 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) own += n[e] = bins[255 - 4 * lane - e];
+      for (int e = 0; e < 4; ++e) {
+        n[e] = 0;
+#pragma unroll
+        for (int c = 0; c < kCopies; ++c) n[e] += copies[c * (kDigit + 1) + 255 - 4 * lane - e];
+        own += n[e];
+      }
       int before = own;
 #pragma unroll
       for (int x = 1; x < 64; x <<= 1) {
@@ -159,10 +175,14 @@ __global__ __launch_bounds__(kSelectThreads) void cache_select_kernel(CacheSelec
       }
       before -= own;
       if (before < equals && before + own >= equals) {
-        int e = 0;
-        while (before + n[e] < equals) before += n[e++];
-        picked[0] = 255 - 4 * lane - e;
-        picked[1] = equals - before;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (before < equals && before + n[e] >= equals) {
+            picked[0] = 255 - 4 * lane - e;
+            picked[1] = equals - before;
+          }
+          before += n[e];
+        }
       }
     }
     __syncthreads();
@@ -171,14 +191,11 @@ __global__ __launch_bounds__(kSelectThreads) void cache_select_kernel(CacheSelec
     equals = picked[1];
   }
   // Above the key: all stay; at the key: the first `equals`.
-  const int part = (older + kSelectThreads - 1) / kSelectThreads * 64;   // tokens of a wave
-  const int i0 = min(older, wave * part), i1 = min(older, i0 + part);
   int above = 0, at = 0;
-  for (int i = i0 + lane; i < i1; i += 64) {
-    const uint32_t key = weight_key(w[i]);
-    above += key > prefix;
-    at += key == prefix;
-  }
+  each([&](int, uint32_t key, bool there) {
+    above += there && key > prefix;
+    at += there && key == prefix;
+  });
 #pragma unroll
   for (int x = 32; x >= 1; x >>= 1) {
     above += __shfl_xor(above, x);
@@ -195,30 +212,58 @@ __global__ __launch_bounds__(kSelectThreads) void cache_select_kernel(CacheSelec
     seen += counts[1][v];
   }
   put += min(seen, equals);
-  for (int i = i0; i < i1; i += 64) {
-    const uint32_t key = i + lane < i1 ? weight_key(w[i + lane]) : 0;
-    const bool equal = i + lane < i1 && key == prefix;
+  const uint64_t below = (uint64_t{1} << lane) - 1;
+  each([&](int i, uint32_t key, bool there) {
+    const bool equal = there && key == prefix;
     const uint64_t ties = __ballot(equal);
-    const uint64_t below = (uint64_t{1} << lane) - 1;
-    const bool stays = i + lane < i1 && (key > prefix || (equal && seen + __popcll(ties & below) < equals));
+    const bool stays = there && (key > prefix || (equal && seen + __popcll(ties & below) < equals));
     const uint64_t all = __ballot(stays);
     if (stays) kept[put + __popcll(all & below)] = i + lane;
     put += __popcll(all);
     seen += __popcll(ties);
+  });
+}
+
+__global__ __launch_bounds__(kSelectThreads) void cache_select_kernel(CacheSelectArgs a) {
+  const int b = static_cast<int>(blockIdx.x), tid = static_cast<int>(threadIdx.x);
+  const int length = min(max(a.lengths[b], 0), a.capacity);
+  const int count = min(length, a.keep);
+  const int recent = min(a.recent, count);
+  const int older = length - recent;            // tokens to choose from
+  const int need = count - recent;
+  const float* w = a.weights + b * a.ld_weights;
+  int32_t* kept = a.kept + static_cast<int64_t>(b) * a.keep;
+  if (tid == 0) a.counts[b] = count;
+  for (int i = tid; i < recent; i += kSelectThreads) kept[need + i] = older + i;
+  for (int i = count + tid; i < a.keep; i += kSelectThreads) kept[i] = -1;
+  if (need == older) {   // all stay
+    for (int i = tid; i < need; i += kSelectThreads) kept[i] = i;
+    return;
   }
+  if (need == 0) return;
+  // Up to 4096 and 32768 tokens in registers, longer rows read again at each pass.
+  const int rounds = (older + kSelectThreads - 1) / kSelectThreads;   // of 64 tokens of a wave
+  if (rounds <= 4) select_older<4>(w, kept, older, need, rounds);
+  else if (rounds <= 32) select_older<32>(w, kept, older, need, rounds);
+  else select_older<0>(w, kept, older, need, rounds);
 }
 
 void launch_cache_select(const CacheSelectArgs& a, hipStream_t stream) {
   hipLaunchKernelGGL(cache_select_kernel, dim3(static_cast<unsigned>(a.B)), dim3(kSelectThreads), 0, stream, a);
 }
 
-// A workgroup takes 32 kept tokens of a sequence: a tile of the new pages.
+// A workgroup takes 32 kept tokens of a sequence, a tile of the new pages, and a
+// part (blockIdx.z) of their features.  The tokens' values lie 64 bytes apart in
+// their tiles, a feature's 32 side by side, so that most of the old tiles' lines
+// are read: bound by bytes (8192 of 32768 tokens of four sequences, keys of 256
+// and values of 512 features: 200 MB in 40 us).
 __global__ __launch_bounds__(kMoveThreads) void cache_compact_kernel(CacheCompactArgs a) {
   __shared__ int64_t key_at[32], value_at[32];   // where the tokens come from, or -1
   const int b = static_cast<int>(blockIdx.y), kt = static_cast<int>(blockIdx.x), tid = static_cast<int>(threadIdx.x);
   const int count = min(max(a.counts[b], 0), a.keep);
   const int D = a.to.D, W = a.to.W;
-  if (a.weights_out && tid < 32) {
+  const int nz = static_cast<int>(gridDim.z), z = static_cast<int>(blockIdx.z);
+  if (a.weights_out && tid < 32 && z == 0) {
     const int i = kt * 32 + tid;
     const int t = i < count ? a.kept[b * a.ld_kept + i] : -1;
     if (i < a.capacity_out) a.weights_out[b * a.ld_out + i] = t >= 0 && t < a.capacity_in ? a.weights_in[b * a.ld_in + t] : 0.f;
@@ -239,12 +284,12 @@ __global__ __launch_bounds__(kMoveThreads) void cache_compact_kernel(CacheCompac
   const uint16_t* keys = static_cast<const uint16_t*>(a.from.keys);
   const uint16_t* values = static_cast<const uint16_t*>(a.from.values);
   const int chunks = W / 8;
-  for (int i = tid; i < 32 * chunks; i += kMoveThreads) {
+  for (int i = z * kMoveThreads + tid; i < 32 * chunks; i += nz * kMoveThreads) {
     const int t = i / chunks, f = i % chunks * 8;
     if (key_at[t] >= 0) store16B(key_row(a.to, page, tile * 32 + t) + f, load16B(keys + key_at[t] + f));
   }
   uint16_t* out = value_tile(a.to, page, tile);
-  for (int i = tid; i < 4 * D; i += kMoveThreads) {
+  for (int i = z * kMoveThreads + tid; i < 4 * D; i += nz * kMoveThreads) {
     const int tg = (i & 3) * 8, d = i >> 2;
     u16x8 v;
     unsigned mask = 0;
@@ -271,7 +316,13 @@ void launch_cache_compact(const CacheCompactArgs& a, hipStream_t stream) {
   // The new weights are written to the end of their rows.
   const int tokens = std::max(a.keep, a.weights_out ? a.capacity_out : 0);
   if (tokens == 0) return;
-  hipLaunchKernelGGL(cache_compact_kernel, dim3(static_cast<unsigned>((tokens + 31) / 32), static_cast<unsigned>(a.B)),
+  // A tile's features in parts while its workgroups do not fill the chip (128
+  // tiles of 512 features: 14 us whole, 7 us in four; 1024 tiles of them: 40 and
+  // 45 us), 128 features and two rounds of a thread's loads in each.
+  const int64_t tiles = (tokens + 31) / 32;
+  const int64_t fill = 1024 / std::max<int64_t>(1, tiles * a.B);
+  const unsigned parts = static_cast<unsigned>(std::min<int64_t>(std::max<int64_t>(1, fill), std::max(1, a.to.D / 128)));
+  hipLaunchKernelGGL(cache_compact_kernel, dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(a.B), parts),
                      dim3(kMoveThreads), 0, stream, a);
 }
 

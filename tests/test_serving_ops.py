@@ -437,6 +437,19 @@ def test_cache_select(keep, recent) -> None:
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("length", [1024, 1025, 4096, 4097, 32768, 32769])
+def test_cache_select_where_rows_stop_to_fit_registers(length) -> None:
+    g = torch.Generator().manual_seed(length)
+    weights = torch.rand(3, length, generator=g) ** 8
+    weights[1] = (weights[1] * 20).floor()
+    lengths = [length, length, length - 1]
+    keep = length // 3
+    expected = plain_select(weights, lengths, keep, 0)
+    got = da.cache_select_hip(weights.to(_device()), torch.tensor(lengths, dtype=torch.int32, device="cuda"), keep, 0)
+    assert torch.equal(got[0].cpu(), expected[0]) and torch.equal(got[1].cpu(), expected[1])
+
+
+@pytest.mark.gpu
 def test_cache_select_long() -> None:
     device = _device()
     weights = torch.rand(2, 140000, generator=torch.Generator().manual_seed(5)).to(device)
