@@ -5,7 +5,8 @@ Public names follow the reference package's API (reference
 additions are ``backend="hip"`` in the config, ``HIP_AVAILABLE``, the gfx950
 operator functions ``dictionary_route_hip`` / ``routed_attention_hip``, and
 the 8-bit operators of the feed-forward (``int8_ops``) and the serving
-operators around a paged cache (``serving_ops``).
+operators around a paged cache (``serving_ops``; ``serving`` has the
+sequences that a language model continues with them).
 """
 
 from . import _lib
@@ -33,6 +34,7 @@ from .modules import (
     SharedDictionaryBank,
 )
 from .ops import assemble_score_maps, dictionary_route_reference, routed_attention_reference
+from .serving import CachedSequences
 from .serving_ops import (
     PagedCache,
     TokenLogProbs,
@@ -49,6 +51,7 @@ from .triton_kernels import TRITON_AVAILABLE
 HIP_AVAILABLE = _lib.available()
 
 __all__ = [
+    "CachedSequences",
     "DoubleAttentionAux",
     "DoubleAttentionBlock",
     "DoubleAttentionConfig",

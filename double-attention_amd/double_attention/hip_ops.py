@@ -1487,12 +1487,14 @@ def linear_hip(
     *,
     activation: str | None = None,
     residual: Tensor | None = None,
+    out: Tensor | None = None,
 ) -> Tensor:
     """``act(x @ weight.T (+ bias)) (+ residual)`` with the library's MFMA GEMM.
 
     ``activation`` is None or ``"gelu"`` (exact, ``nn.GELU()``); ``residual``
     has the output's shape and is added to the rounded result, as the
-    unfused ``residual + linear(x)`` does.
+    unfused ``residual + linear(x)`` does.  ``out`` (contiguous, 16-byte
+    aligned) takes the result.
     """
 
     _require_cuda(x, weight)
@@ -1503,7 +1505,11 @@ def linear_hip(
         raise ValueError(f"unsupported activation {activation!r}")
     rows = _aligned(x.reshape(-1, x.shape[-1]))
     w = _aligned(weight.detach())
-    out = torch.empty(*x.shape[:-1], weight.shape[0], dtype=x.dtype, device=x.device)
+    shape = (*x.shape[:-1], weight.shape[0])
+    if out is None:
+        out = torch.empty(shape, dtype=x.dtype, device=x.device)
+    elif out.shape != shape or out.dtype != x.dtype or out.device != x.device or not out.is_contiguous() or out.data_ptr() % 16:
+        raise ValueError("out must have the output's shape, dtype and device, contiguous and 16-byte aligned")
     b = None if bias is None else bias.detach().contiguous()
     res = None
     if residual is not None:

@@ -15,7 +15,7 @@ from __future__ import annotations
 import math
 from contextlib import contextmanager
 from dataclasses import dataclass
-from typing import Iterator, NamedTuple
+from typing import TYPE_CHECKING, Iterator, NamedTuple, Sequence
 
 import torch
 import torch.nn as nn
@@ -30,6 +30,9 @@ from .ops import (
     routed_attention_reference,
     score_scale_from_log,
 )
+
+if TYPE_CHECKING:
+    from .serving_ops import PagedCache, TokenLogProbs
 
 # Reference switch (modules.py:22): one GEMM over cat(Wq, Wk) instead of two.
 FUSED_QUERY_KEY_PROJECTION = True
@@ -317,6 +320,50 @@ class SharedDictionaryAttention(nn.Module):
         layout = hip_ops.route_layout(*normalized_dictionary, key_dtype)
         return hip_ops.shared_dictionary_attention_hip(self, x, layout, dtype, residual=residual,
                                                        want_routed=want_routed)
+
+    def _hip_cached_call(
+        self,
+        x: Tensor,
+        normalized_dictionary: tuple[Tensor, Tensor],
+        dtype: torch.dtype,
+        residual: Tensor,
+        tokens: CachedTokens,
+        layer: int,
+    ) -> Tensor:
+        """``residual`` plus the attention of new tokens ``x`` ``[N, model_dim]``,
+        whose routed keys and values go into the layer's cache first."""
+
+        from . import hip_ops, serving_ops
+
+        cfg = self.config
+        count = x.shape[0]
+        wq, wk, wv, wo, bv, log_beta, log_scales, mix, _ = hip_ops._module_operands(self, dtype)
+        rows = torch.empty(2, count, cfg.total_qk_width, dtype=dtype, device=x.device)
+        hip_ops.linear_hip(x, wq, out=rows[0])
+        hip_ops.linear_hip(x, wk, out=rows[1])
+        value = hip_ops.linear_hip(x, wv, bv)
+        # fp16 rows, as the whole forward has them.
+        routed = hip_ops._route_forward(
+            rows.view(-1, cfg.routing_dim),
+            hip_ops.route_layout(*normalized_dictionary, hip_ops.route_key_dtype(cfg.normalize_routing_input, dtype)),
+            log_beta, cfg.eps, cfg.normalize_routing_input, cfg.normalize_routing_output, hip_ops.RouteVariant.of_config(cfg),
+            out_dtype=torch.float16, beta_is_log=True,
+        ).view(2, count, cfg.qk_branches, cfg.routing_dim)
+        cache, where = tokens.caches[layer], (tokens.page_table, tokens.lengths, tokens.offsets)
+        serving_ops.cache_append_hip(cache, routed[1], value, *where, max_chunk=tokens.max_chunk)
+        factors = None
+        if mix is not None:
+            # The weights rounded to the map dtype, the sum in fp32 (as _combine).
+            factors = torch.softmax(mix, dim=0).to(dtype).float()
+        arguments = (routed[0], cache, *where, score_scale_from_log(log_scales))
+        hints = {"mix": factors, "max_chunk": tokens.max_chunk, "max_length": tokens.max_length}
+        if tokens.weights is None:
+            maps = serving_ops.paged_attention_hip(*arguments, **hints)
+        else:
+            weights = tokens.weights[layer]
+            maps, _ = serving_ops.paged_attention_weights_hip(*arguments, weights=weights, out=weights, **hints)
+        mixed = maps.reshape(count, -1)   # one map, their weighted sum, or all side by side
+        return residual + mixed if wo is None else hip_ops.linear_hip(mixed, wo, residual=residual)
 
     def _hip_inference_dtype(self, x: Tensor, bank: SharedDictionaryBank) -> torch.dtype | None:
         """The compute dtype when a forward of ``x`` would run the HIP kernels
@@ -1120,6 +1167,19 @@ class DoubleAttentionBlock(nn.Module):
         x = x.contiguous()
         hidden = _hip_norm(self.attention_norm, x)
         x = attention._hip_call(hidden, bank, normalized_dictionary, dtype, residual=x, want_routed=False).output
+        return self._hip_feedforward(x, bank, normalized_dictionary, dtype)
+
+    def _hip_feedforward(
+        self,
+        x: Tensor,
+        bank: SharedDictionaryBank,
+        normalized_dictionary: tuple[Tensor, Tensor] | None,
+        dtype: torch.dtype,
+    ) -> Tensor:
+        """``x + FFN(norm(x))`` on the HIP kernels, without autograd."""
+
+        from . import hip_ops
+
         norm2 = self.feedforward_norm
         weights = self._int8_weights()
         if weights is not None:
@@ -1131,11 +1191,26 @@ class DoubleAttentionBlock(nn.Module):
                 normalized = _hip_norm(norm2, x)
             return self._feedforward_int8(x, normalized, weights)
         normalized_x = _hip_norm(norm2, x)
-        if attention.config.q_dictionary_feedforward:
+        if self.attention.config.q_dictionary_feedforward:
             return self._q_dictionary_feedforward_hip(x, normalized_x, bank, normalized_dictionary, dtype)
         first, second = self.feedforward[0], self.feedforward[2]
         expanded = hip_ops.linear_hip(normalized_x, first.weight, first.bias, activation="gelu")
         return hip_ops.linear_hip(expanded, second.weight, second.bias, residual=x)
+
+    def _hip_cached_block(
+        self,
+        x: Tensor,
+        bank: SharedDictionaryBank,
+        normalized_dictionary: tuple[Tensor, Tensor],
+        dtype: torch.dtype,
+        tokens: CachedTokens,
+        layer: int,
+    ) -> Tensor:
+        """The block for new tokens ``[N, model_dim]`` of cached sequences."""
+
+        hidden = _hip_norm(self.attention_norm, x)
+        x = self.attention._hip_cached_call(hidden, normalized_dictionary, dtype, x, tokens, layer)
+        return self._hip_feedforward(x, bank, normalized_dictionary, dtype)
 
     def _q_dictionary_feedforward_hip(
         self,
@@ -1302,6 +1377,18 @@ class DoubleAttentionStack(nn.Module):
         return x
 
 
+class CachedTokens(NamedTuple):
+    """Where the new tokens of ``DoubleAttentionLM.cached_forward`` lie; see there."""
+
+    caches: Sequence[PagedCache]
+    page_table: Tensor
+    lengths: Tensor
+    offsets: Tensor
+    weights: Tensor | None = None
+    max_chunk: int | None = None
+    max_length: int | None = None
+
+
 class DoubleAttentionLM(nn.Module):
     """Causal LM over a ``DoubleAttentionStack`` (``modules.py:415-460``)."""
 
@@ -1372,3 +1459,109 @@ class DoubleAttentionLM(nn.Module):
                 raise ValueError("targets must match token_ids shape")
             loss = F.cross_entropy(logits.flatten(0, 1), targets.flatten())
         return logits, loss
+
+    # ---- serving ----------------------------------------------------------
+
+    def paged_caches(self, pages: int, page_size: int = 64) -> tuple[PagedCache, ...]:
+        """An empty ``PagedCache`` for each layer, on the model's device: the
+        routed rows in fp16, the values in the model's type."""
+
+        from .serving_ops import paged_cache
+
+        cfg, weight = self.stack.config, self.token_embedding.weight
+        dtype = torch.float16 if weight.dtype == torch.float16 else torch.bfloat16
+        return tuple(
+            paged_cache(pages, page_size, cfg.qk_branches, cfg.routing_dim, cfg.model_dim, dtype=dtype, device=weight.device)
+            for _ in self.stack.blocks
+        )
+
+    @torch.no_grad()
+    def cached_forward(
+        self,
+        token_ids: Tensor,
+        positions: Tensor,
+        caches: Sequence[PagedCache],
+        page_table: Tensor,
+        lengths: Tensor,
+        offsets: Tensor,
+        *,
+        weights: Tensor | None = None,
+        rows: Tensor | None = None,
+        max_chunk: int | None = None,
+        max_length: int | None = None,
+    ) -> Tensor:
+        """Logits ``[N, vocab]`` of new tokens that continue cached sequences.
+
+        ``token_ids`` ``[N]`` are the new tokens of all sequences, packed: those
+        of sequence b are ``offsets[b]`` to ``offsets[b + 1]``, at the
+        ``positions`` ``[N]`` of the position table.  ``caches`` (one for each
+        layer, ``paged_caches``) hold the tokens in front of them and take
+        theirs; ``page_table`` (one for all layers), ``lengths`` (with the new
+        tokens) and ``offsets`` are int32 tensors on the device, as for
+        ``cache_append_hip`` and ``paged_attention_hip``.  ``weights`` (fp32
+        ``[layers, sequences, entries * page_size]``, contiguous) gathers in place
+        the attention that every cached token received, for
+        ``cache_select_hip``.  ``rows``: the places of the tokens whose logits are
+        wanted (default: all).  ``max_chunk`` and ``max_length`` are the largest
+        numbers of new and of all tokens of a sequence, where the program knows
+        them.
+
+        For causal models in fp16 or bf16 on the HIP kernels, in evaluation;
+        without gradients.  Nothing is read on the host, so that a step can be
+        captured in a graph and replayed; token ids and positions are then the
+        caller's to keep inside their tables, those of rows of no sequence, too.
+        ``CachedSequences`` keeps the pages and lengths for a program.
+        """
+
+        if token_ids.ndim != 1 or positions.shape != token_ids.shape:
+            raise ValueError("cached_forward: token_ids and positions must have shape [N]")
+        if len(caches) != len(self.stack.blocks):
+            raise ValueError(f"cached_forward: expected {len(self.stack.blocks)} caches, got {len(caches)}")
+        dtype = self._cached_dtype()
+        if weights is not None and (weights.ndim != 3 or weights.shape[0] != len(caches) or not weights.is_contiguous()):
+            raise ValueError("cached_forward: weights must be contiguous [layers, sequences, entries * page_size]")
+        tokens = CachedTokens(caches, page_table, lengths, offsets, weights, max_chunk, max_length)
+        x = self.token_embedding(token_ids) + self.position_embedding(positions)
+        stack = self.stack
+        dictionaries = stack._normalize_banks(x)
+        if token_ids.shape[0]:
+            for index, block in enumerate(stack.blocks):
+                bank = min(index // stack.dictionary_group_size, len(stack.banks) - 1)
+                x = block._hip_cached_block(x, stack.banks[bank], dictionaries[bank], dtype, tokens, index)
+        if rows is not None:
+            x = x.index_select(0, rows)
+        return self.lm_head(self._final_norm(x))
+
+    def _cached_dtype(self) -> torch.dtype:
+        """The type that ``cached_forward`` computes in; raises where it does not run."""
+
+        from . import hip_ops
+
+        cfg, weight = self.stack.config, self.token_embedding.weight
+        if not cfg.causal:
+            raise ValueError("cached_forward: tokens of a model without causal attention depend on later ones")
+        if weight.dtype not in (torch.float16, torch.bfloat16) or cfg.backend == "torch":
+            raise NotImplementedError("cached_forward runs fp16 and bf16 models on the HIP kernels")
+        if torch.is_autocast_enabled("cuda"):
+            raise NotImplementedError("cached_forward runs in the model's own type, not under autocast")
+        hip_ops.check_module_supported(cfg)
+        resolve_backend("hip", (_Spec(weight.is_cuda, weight.dtype),))  # type: ignore[arg-type]
+        for block in self.stack.blocks:
+            if block.attention.query.weight.dtype != weight.dtype:
+                raise NotImplementedError("cached_forward: the embeddings and the attention must share a type")
+            if block.training and any(isinstance(m, nn.Dropout) and m.p > 0 for m in block.feedforward):
+                raise RuntimeError("cached_forward: dropout is active; call eval() first")
+        return weight.dtype
+
+    def token_log_probs(self, token_ids: Tensor, *, top: int = 0, entropy: bool = False) -> TokenLogProbs:
+        """Log probabilities ``[B, T - 1]`` that the model gives each next token
+        of ``token_ids`` ``[B, T]``, on request with the entropies and the
+        ``top`` most probable tokens (``token_log_probs_hip``; differentiable)."""
+
+        from .serving_ops import TokenLogProbs, token_log_probs_hip
+
+        logits, _ = self(token_ids)
+        # The last position has no next token; its row is left out as ignored.
+        following = torch.cat((token_ids[:, 1:], token_ids.new_full((token_ids.shape[0], 1), -100)), dim=1)
+        result = token_log_probs_hip(logits, following, top=top, entropy=entropy)
+        return TokenLogProbs(*(None if t is None else t[:, :-1] for t in result))
