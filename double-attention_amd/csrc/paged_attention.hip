@@ -3,21 +3,21 @@
 // over the tokens j of row n's sequence up to its own position, for each score
 // map s; all maps share the values.
 //
-// Columns.  A sequence's (new token, map) pairs are the columns of its score
-// matrix, tokens outermost, 16 to a tile.  A tile's queries are laid over all
-// W key features, zero outside of their map's: one product K Q^T then serves
-// every map, and keys and values are read once for all maps of few tokens.
-//
-// paged_token_kernel: a wave takes 32 cached tokens at a time,
+// Both kernels take 32 cached tokens (a tile) at a time,
 //   S^T[token, column] = K Q^T     (keys straight from memory, queries in LDS)
 //   O^T[feature, column] += V^T P^T (values straight from memory: their tiles
 //                                    hold a feature's tokens side by side, so a
 //                                    wave's load is one contiguous KiB)
 // with the running maximum and sum of each column in 32 bits.  The key rows go
 // to the MFMA's rows in such an order that the score accumulators are the next
-// product's operand as they stand (da_common.h).  A workgroup's four waves
-// take every fourth tile of its part of the tokens and add up in LDS; parts
-// are joined by paged_merge_kernel.
+// product's operand as they stand (da_common.h).  A sequence's tokens are split
+// over workgroups where there are few columns; paged_merge_kernel joins the parts.
+//
+// Columns are 16 to a tile.  paged_token_kernel, for few new tokens: a sequence's
+// (new token, map) pairs, tokens outermost.  A tile's queries are laid over all
+// W key features, zero outside of their map's: one product K Q^T then serves
+// every map, and keys and values are read once for all maps.  paged_chunk_kernel,
+// for many: one map's tokens, with that map's features alone.
 #include <algorithm>
 #include <type_traits>
 
@@ -118,19 +118,24 @@ __device__ void clear_other_rows(const PagedAttentionArgs& a, int64_t wg, int64_
 }  // namespace
 
 // NK: groups of 64 key features that a wave holds (fewer features leave the rest
-// zero, more are taken in turn); DBW: 16-feature blocks of the values of a wave;
-// CT: column tiles; NW: waves; ONE: the columns are one map's tokens (many new
-// tokens; member index: slice, then map, then column tile), else (token, map)
-// pairs over all features; PB: buffers of the probabilities.
+// zero, more are taken in turn); DBW: 16-feature blocks of the values of a wave.
+// The 16 columns are (token, map) pairs over all features.
 //
-// A step takes NW tiles of 32 tokens.  Wave w forms tile w's scores of all
-// columns and leaves its probabilities in LDS; after a barrier every wave
-// multiplies them with its own DBW blocks of the values of all tiles.  A wave's
-// next keys and the next two tiles' values are on their way meanwhile.
-template <typename TQ, typename TV, int NK, int DBW, int CT, int NW, bool ONE, int PB, int OCC>
-__global__ __launch_bounds__(64 * NW, OCC) void paged_attention_kernel(Params p) {
+// A step takes four tiles.  Wave w forms tile w's scores and leaves its
+// probabilities in LDS; after a barrier every wave multiplies them with its own
+// DBW blocks of the values of all tiles.  A wave's next keys and the next two
+// tiles' values are on their way meanwhile, and the probabilities have two buffers,
+// so that a step has one barrier.
+//
+// Bound by the cache's bytes: 64 sequences of 4096 tokens (keys of 256, values of
+// 512 features, 400 MB) 51 us with the merge, one of 131072 tokens (201 MB) 41 us.
+// Waves that held whole tiles, each with all features, had a register file too
+// small for their loads in flight: 78 us for the former.
+template <typename TQ, typename TV, int NK, int DBW>
+__global__ __launch_bounds__(64 * kWaves, 2) void paged_token_kernel(Params p) {
   typedef typename Elem<TQ>::v8 q8;
   typedef typename Elem<TV>::v8 v8;
+  constexpr int NW = kWaves;
   constexpr int DS = 16 * DBW * NW;
   constexpr int FW = 64 * NK;               // features of a pass
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -154,35 +159,32 @@ __global__ __launch_bounds__(64 * NW, OCC) void paged_attention_kernel(Params p)
   if (seq.rows == 0) return;
   const int slice = static_cast<int>(p.slices.remainder(member));
   member = static_cast<int>(p.slices.divide(member));
-  const int map = ONE ? static_cast<int>(p.maps.remainder(member)) : 0;
-  if (ONE) member = static_cast<int>(p.maps.divide(member));
-  const int n_cols = ONE ? seq.rows : seq.rows * a.S;
-  const int width = ONE ? a.RP : W, f0 = ONE ? static_cast<int>(p.repeats.divide(map)) * a.RP : 0;
-  const int passes = ONE ? 1 : (W + FW - 1) / FW;
+  const int n_cols = seq.rows * a.S;
+  const int passes = (W + FW - 1) / FW;
   const int QP = passes * FW + 8;           // pitch of the queries in LDS
   const int d0 = slice * DS + wave * DBW * 16;
   const int nb = max(0, min(DBW, (D - d0) / 16));   // blocks of this wave (the last slice may have fewer)
 
   TQ* qs = reinterpret_cast<TQ*>(lds);
-  char* ps = lds + 32 * CT * QP;                                  // [PB][NW][CT][64 lanes] 16 bytes
-  float* ms = reinterpret_cast<float*>(ps + PB * NW * CT * 1024); // [PB][NW][16 CT]
-  int* moved = reinterpret_cast<int*>(ms + PB * NW * 16 * CT);    // [PB][NW]
+  char* ps = lds + 32 * QP;                           // [2][NW][64 lanes] 16 bytes
+  float* ms = reinterpret_cast<float*>(ps + 2 * NW * 1024); // [2][NW][16]
+  int* moved = reinterpret_cast<int*>(ms + 2 * NW * 16);    // [2][NW]
 
-  for (int ct0 = member; ct0 * 16 * CT < n_cols; ct0 += p.n_ct) {
+  for (int ct0 = member; ct0 * 16 < n_cols; ct0 += p.n_ct) {
     // Nearly always the only round: what depends on the lane is worked out in it,
     // rather than in front of it and kept in registers that there are not.
     const int tid = opaque(static_cast<int>(threadIdx.x));
     const int lane = tid & 63, c = lane & 15, g = lane >> 4;
-    const int col0 = ct0 * 16 * CT, n_used = min(16 * CT, n_cols - col0);
-    auto token_of = [&](int col) { return ONE ? col : static_cast<int>(p.maps.divide(col)); };
-    auto map_of = [&](int col) { return ONE ? map : static_cast<int>(p.maps.remainder(col)); };
-    auto row_of = [&](int col) { return ONE ? (seq.n0 + col0 + col) * a.S + map : seq.n0 * a.S + col0 + col; };
+    const int col0 = ct0 * 16, n_used = min(16, n_cols - col0);
+    auto token_of = [&](int col) { return static_cast<int>(p.maps.divide(col)); };
+    auto map_of = [&](int col) { return static_cast<int>(p.maps.remainder(col)); };
+    const int64_t row0 = seq.n0 * a.S + col0;
     const int limit = visible_to(seq, token_of(col0 + n_used - 1), a.causal);
     const int n_kt = (limit + 31) / 32;
     const int kt0 = min(n_kt, split * p.per), kt1 = split == p.n_split - 1 ? n_kt : min(n_kt, kt0 + p.per);
     if (split > 0 && kt0 == kt1) {   // nothing left for this part
       if (slice == 0)
-        for (int i = tid; i < n_used; i += 64 * NW) p.part_l[split * p.rows + row_of(i)] = 0.f;
+        for (int i = tid; i < n_used; i += 64 * NW) p.part_l[split * p.rows + row0 + i] = 0.f;
       continue;
     }
 
@@ -193,27 +195,21 @@ __global__ __launch_bounds__(64 * NW, OCC) void paged_attention_kernel(Params p)
 
     // Queries: sixteen threads to a column.
     if (ct0 != member) lds_barrier();   // the last tiles' have been read
-    for (int col = tid >> 4; col < 16 * CT; col += 4 * NW) {
+    for (int col = tid >> 4; col < 16; col += 4 * NW) {
       const bool used = col < n_used;
-      const int from = ONE ? 0 : static_cast<int>(p.repeats.divide(map_of(col0 + col))) * a.RP;
-      const TQ* src = static_cast<const TQ*>(a.q) + (seq.n0 + token_of(col0 + (used ? col : 0))) * a.ldq + f0;
+      const int from = static_cast<int>(p.repeats.divide(map_of(col0 + col))) * a.RP;
+      const TQ* src = static_cast<const TQ*>(a.q) + (seq.n0 + token_of(col0 + (used ? col : 0))) * a.ldq;
       for (int f = (tid & 15) * 8; f < passes * FW; f += 128) {
         u32x4 v = {0, 0, 0, 0};
         if (used && f >= from && f < from + a.RP) v = load16B(src + f);
         store16B(qs + col * QP + f, v);
       }
     }
-    // This lane's columns; those behind the last one count as it.
-    int vis[CT];
-    float sc[CT], m_run[CT], l_part[CT];
-#pragma unroll
-    for (int i = 0; i < CT; ++i) {
-      const int col = col0 + min(16 * i + c, n_used - 1);
-      vis[i] = visible_to(seq, token_of(col), a.causal);
-      sc[i] = score_scale(a, map_of(col));
-      m_run[i] = kNoScore;
-      l_part[i] = 0.f;
-    }
+    // This lane's column; those behind the last one count as it.
+    const int own_col = col0 + min(c, n_used - 1);
+    const int vis = visible_to(seq, token_of(own_col), a.causal);
+    const float sc = score_scale(a, map_of(own_col));
+    float m_run = kNoScore, l_part = 0.f;
 
     // Addresses are a uniform base and a lane's 32-bit offset.  Block h of the
     // scores has token 8 (c / 4) + 4 h + c % 4 in row c.  Where there is no tile
@@ -223,11 +219,11 @@ __global__ __launch_bounds__(64 * NW, OCC) void paged_attention_kernel(Params p)
     u32x4 kf[NK][4], vf[2][DBW];
     auto load_keys = [&](int kt, int page, int pass) {
       const char* base = uniform_ptr(static_cast<const char*>(cache.keys) +
-                                     (max(page, 0) * cache.key_page + static_cast<int64_t>(tile_of(cache, kt)) * 32 * W + f0) * 2);
+                                     (max(page, 0) * cache.key_page + static_cast<int64_t>(tile_of(cache, kt)) * 32 * W) * 2);
       const uint32_t at = page < 0 ? 0 : key_lane;
 #pragma unroll
       for (int j = 0; j < NK; ++j) {   // a group past the last feature is multiplied by zero
-        const char* from = base + 128 * min(pass * NK + j, width / 64 - 1);
+        const char* from = base + 128 * min(pass * NK + j, W / 64 - 1);
 #pragma unroll
         for (int i = 0; i < 4; ++i) kf[j][i] = load_at(from + (i & 1) * 8 * W, at + 64 * (i >> 1));
       }
@@ -242,11 +238,9 @@ __global__ __launch_bounds__(64 * NW, OCC) void paged_attention_kernel(Params p)
     load_keys(kt0 + wave, __builtin_amdgcn_readlane(pages, wave), 0);
     load_values(vf[0], kt0, __builtin_amdgcn_readlane(pages, 0));
     load_values(vf[1], kt0 + 1, __builtin_amdgcn_readlane(pages, 1));
-    f32x4 acc[CT][DBW];
+    f32x4 acc[DBW];
 #pragma unroll
-    for (int i = 0; i < CT; ++i)
-#pragma unroll
-      for (int j = 0; j < DBW; ++j) acc[i][j] = zero4();
+    for (int j = 0; j < DBW; ++j) acc[j] = zero4();
     __builtin_amdgcn_sched_barrier(0);
     lds_barrier();   // the queries are there
 
@@ -255,58 +249,52 @@ __global__ __launch_bounds__(64 * NW, OCC) void paged_attention_kernel(Params p)
       const int pages_after = pages_at(base + 2 * NW);
       const int kt = base + wave, page = __builtin_amdgcn_readlane(pages, wave);
       const int live = page < 0 ? 0 : min(32, limit - kt * 32);
-      char* mine = ps + (buf * NW + wave) * CT * 1024 + lane * 16;
+      char* mine = ps + (buf * NW + wave) * 1024 + lane * 16;
       bool any = false;
       // Scores of this wave's tile, and its probabilities.
-      auto scores = [&](f32x4 (&st)[2], int i, int pass) {
+      f32x4 st[2] = {zero4(), zero4()};
+      auto scores = [&](int pass) {
 #pragma unroll
         for (int j = 0; j < 2 * NK; ++j) {
-          const q8 qf = load8(qs + (16 * i + c) * QP + pass * FW + 32 * j + 8 * g);
+          const q8 qf = load8(qs + c * QP + pass * FW + 32 * j + 8 * g);
           st[0] = Elem<TQ>::mma(__builtin_bit_cast(q8, kf[j >> 1][2 * (j & 1)]), qf, st[0]);
           st[1] = Elem<TQ>::mma(__builtin_bit_cast(q8, kf[j >> 1][2 * (j & 1) + 1]), qf, st[1]);
         }
       };
-#pragma unroll
-      for (int i = 0; i < CT; ++i) {
-        f32x4 st[2] = {zero4(), zero4()};
-        scores(st, i, 0);
-        if constexpr (!ONE && CT == 1) {
-          for (int pass = 1; pass < passes; ++pass) {
-            load_keys(kt, page, pass);
-            scores(st, i, pass);
-          }
-        }
-        const int seen = min(live, vis[i] - kt * 32) - 8 * g;   // of this lane's eight tokens
-        float mx = -INFINITY;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float s = e < seen ? st[e >> 2][e & 3] * sc[i] : -INFINITY;
-          st[e >> 2][e & 3] = s;
-          mx = fmaxf(mx, s);
-        }
-        // The reference moves, to a whole number (so that what it scales stays
-        // exact), where a score exceeds it by more than kRescaleSlack.
-        float m = m_run[i];
-        if (__ballot(mx > m + kRescaleSlack)) {
-          const float tile_max = group_max(mx);
-          if (tile_max > m + kRescaleSlack) m = __builtin_ceilf(tile_max);
-          any = true;
-        }
-        float l = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float s = __builtin_amdgcn_exp2f(st[e >> 2][e & 3] - m);
-          st[e >> 2][e & 3] = s;
-          l += s;
-        }
-        if (any) l_part[i] *= __builtin_amdgcn_exp2f(m_run[i] - m);
-        l_part[i] += l;
-        // The probabilities are rounded to the values' type for the product, the
-        // sum is of the unrounded ones.
-        if (PB == 1 && i == 0 && base > kt0) lds_barrier();   // the last step's have been read
-        *reinterpret_cast<v8*>(mine + i * 1024) = pack_blocked<TV>(st[0], st[1]);
-        ms[(buf * NW + wave) * 16 * CT + 16 * i + c] = m;
+      scores(0);
+      for (int pass = 1; pass < passes; ++pass) {
+        load_keys(kt, page, pass);
+        scores(pass);
       }
+      const int seen = min(live, vis - kt * 32) - 8 * g;   // of this lane's eight tokens
+      float mx = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float s = e < seen ? st[e >> 2][e & 3] * sc : -INFINITY;
+        st[e >> 2][e & 3] = s;
+        mx = fmaxf(mx, s);
+      }
+      // The reference moves, to a whole number (so that what it scales stays
+      // exact), where a score exceeds it by more than kRescaleSlack.
+      float m = m_run;
+      if (__ballot(mx > m + kRescaleSlack)) {
+        const float tile_max = group_max(mx);
+        if (tile_max > m + kRescaleSlack) m = __builtin_ceilf(tile_max);
+        any = true;
+      }
+      float l = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float s = __builtin_amdgcn_exp2f(st[e >> 2][e & 3] - m);
+        st[e >> 2][e & 3] = s;
+        l += s;
+      }
+      if (any) l_part *= __builtin_amdgcn_exp2f(m_run - m);
+      l_part += l;
+      // The probabilities are rounded to the values' type for the product, the
+      // sum is of the unrounded ones.
+      *reinterpret_cast<v8*>(mine) = pack_blocked<TV>(st[0], st[1]);
+      ms[(buf * NW + wave) * 16 + c] = m;
       if (lane == 0) moved[buf * NW + wave] = any;
       __builtin_amdgcn_sched_barrier(0);
       load_keys(kt + NW, __builtin_amdgcn_readlane(pages_next, wave), 0);
@@ -318,25 +306,22 @@ __global__ __launch_bounds__(64 * NW, OCC) void paged_attention_kernel(Params p)
       if (__builtin_amdgcn_readfirstlane(moves)) {
         // To the largest of the waves' references: this wave's probabilities and
         // sums, and what has been added up.
+        const float own = ms[(buf * NW + wave) * 16 + c];
+        float m = own;
 #pragma unroll
-        for (int i = 0; i < CT; ++i) {
-          const float own = ms[(buf * NW + wave) * 16 * CT + 16 * i + c];
-          float m = own;
+        for (int w = 0; w < NW; ++w) m = fmaxf(m, ms[(buf * NW + w) * 16 + c]);
+        const float f = __builtin_amdgcn_exp2f(own - m), fa = __builtin_amdgcn_exp2f(m_run - m);
+        m_run = m;
+        l_part *= f;
 #pragma unroll
-          for (int w = 0; w < NW; ++w) m = fmaxf(m, ms[(buf * NW + w) * 16 * CT + 16 * i + c]);
-          const float f = __builtin_amdgcn_exp2f(own - m), fa = __builtin_amdgcn_exp2f(m_run[i] - m);
-          m_run[i] = m;
-          l_part[i] *= f;
+        for (int j = 0; j < DBW; ++j) acc[j] *= fa;
+        v8 pv = *reinterpret_cast<const v8*>(mine);
 #pragma unroll
-          for (int j = 0; j < DBW; ++j) acc[i][j] *= fa;
-          v8 pv = *reinterpret_cast<const v8*>(mine + i * 1024);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) pv[e] = static_cast<TV>(static_cast<float>(pv[e]) * f);
-          *reinterpret_cast<v8*>(mine + i * 1024) = pv;
-        }
+        for (int e = 0; e < 8; ++e) pv[e] = static_cast<TV>(static_cast<float>(pv[e]) * f);
+        *reinterpret_cast<v8*>(mine) = pv;
         lds_barrier();
       }
-      const char* probs = ps + buf * NW * CT * 1024 + lane * 16;
+      const char* probs = ps + buf * NW * 1024 + lane * 16;
 #pragma unroll
       for (int t = 0; t < NW; ++t) {
         const int page_t = __builtin_amdgcn_readlane(pages, t);
@@ -353,12 +338,9 @@ __global__ __launch_bounds__(64 * NW, OCC) void paged_attention_kernel(Params p)
 #pragma unroll
           for (int j = 0; j < DBW; ++j) vv[j] = __builtin_bit_cast(v8, vf[t & 1][j] & keep);
         }
+        const v8 pv = *reinterpret_cast<const v8*>(probs + t * 1024);
 #pragma unroll
-        for (int i = 0; i < CT; ++i) {
-          const v8 pv = *reinterpret_cast<const v8*>(probs + (t * CT + i) * 1024);
-#pragma unroll
-          for (int j = 0; j < DBW; ++j) acc[i][j] = Elem<TV>::mma(vv[j], pv, acc[i][j]);
-        }
+        for (int j = 0; j < DBW; ++j) acc[j] = Elem<TV>::mma(vv[j], pv, acc[j]);
         const int next = t + 2 < NW ? __builtin_amdgcn_readlane(pages, t + 2 < NW ? t + 2 : 0)
                                     : __builtin_amdgcn_readlane(pages_next, t + 2 < NW ? 0 : t + 2 - NW);
         load_values(vf[t & 1], base + t + 2, next);
@@ -366,49 +348,42 @@ __global__ __launch_bounds__(64 * NW, OCC) void paged_attention_kernel(Params p)
       }
       pages = pages_next;
       pages_next = pages_after;
-      if (PB == 2) buf ^= 1;
+      buf ^= 1;
     }
 
     // The waves' sums of exponentials; the rest of a column is in one wave.
     float* ls = reinterpret_cast<float*>(ps);
     lds_barrier();   // the probabilities have been read
-#pragma unroll
-    for (int i = 0; i < CT; ++i) {
-      const float l = group_sum(l_part[i]);
-      if (g == 0) ls[wave * 16 * CT + 16 * i + c] = l;
-    }
+    l_part = group_sum(l_part);
+    if (g == 0) ls[wave * 16 + c] = l_part;
     lds_barrier();
+    if (c >= n_used) continue;
+    float l = 0.f;
 #pragma unroll
-    for (int i = 0; i < CT; ++i) {
-      const int col = 16 * i + c;
-      if (col >= n_used) continue;
-      float l = 0.f;
-#pragma unroll
-      for (int w = 0; w < NW; ++w) l += ls[w * 16 * CT + col];
-      const int64_t row = row_of(col);
-      if (wave == 0 && g == 0 && slice == 0) {
-        if (p.part_o) {
-          p.part_m[split * p.rows + row] = m_run[i];
-          p.part_l[split * p.rows + row] = l;
-        } else if (a.lse2) {
-          a.lse2[row] = l == 0.f ? -INFINITY : m_run[i] + __builtin_amdgcn_logf(l);
-        }
-      }
+    for (int w = 0; w < NW; ++w) l += ls[w * 16 + c];
+    const int64_t row = row0 + c;
+    if (wave == 0 && g == 0 && slice == 0) {
       if (p.part_o) {
-        float* to = p.part_o + (split * p.rows + row) * D + d0 + 4 * g;
+        p.part_m[split * p.rows + row] = m_run;
+        p.part_l[split * p.rows + row] = l;
+      } else if (a.lse2) {
+        a.lse2[row] = l == 0.f ? -INFINITY : m_run + __builtin_amdgcn_logf(l);
+      }
+    }
+    if (p.part_o) {
+      float* to = p.part_o + (split * p.rows + row) * D + d0 + 4 * g;
 #pragma unroll
-        for (int j = 0; j < DBW; ++j)
-          if (j < nb) *reinterpret_cast<f32x4*>(to + 16 * j) = acc[i][j];
-      } else {
-        const float f = l == 0.f ? 0.f : 1.f / l;
-        TV* to = static_cast<TV*>(a.out) + row * D + d0 + 4 * g;
+      for (int j = 0; j < DBW; ++j)
+        if (j < nb) *reinterpret_cast<f32x4*>(to + 16 * j) = acc[j];
+    } else {
+      const float f = l == 0.f ? 0.f : 1.f / l;
+      TV* to = static_cast<TV*>(a.out) + row * D + d0 + 4 * g;
 #pragma unroll
-        for (int j = 0; j < DBW; ++j) {
-          typename Elem<TV>::v4 r;
+      for (int j = 0; j < DBW; ++j) {
+        typename Elem<TV>::v4 r;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) r[e] = static_cast<TV>(acc[i][j][e] * f);
-          if (j < nb) *reinterpret_cast<typename Elem<TV>::v4*>(to + 16 * j) = r;
-        }
+        for (int e = 0; e < 4; ++e) r[e] = static_cast<TV>(acc[j][e] * f);
+        if (j < nb) *reinterpret_cast<typename Elem<TV>::v4*>(to + 16 * j) = r;
       }
     }
   }
@@ -925,14 +900,12 @@ Plan plan(const PagedAttentionArgs& a) {
   return r;
 }
 
-template <typename TQ, typename TV, int NK, int DBW, int CT, int NW, bool ONE, int PB, int OCC>
-void launch_kernel(const Params& p, hipStream_t stream) {
-  const int width = ONE ? p.a.RP : p.a.cache.W;
-  const int QP = static_cast<int>(round_up(width, 64 * NK)) + 8;
-  const size_t lds = static_cast<size_t>(32) * CT * QP + PB * NW * (CT * 1024 + CT * 64 + 4);
+template <typename TQ, typename TV, int NK, int DBW>
+void launch_token_kernel(const Params& p, hipStream_t stream) {
+  const int QP = static_cast<int>(round_up(p.a.cache.W, 64 * NK)) + 8;
+  const size_t lds = static_cast<size_t>(32) * QP + 2 * kWaves * (1024 + 64 + 4);
   const unsigned units = static_cast<unsigned>(round_up(p.units, kXcds));
-  hipLaunchKernelGGL((paged_attention_kernel<TQ, TV, NK, DBW, CT, NW, ONE, PB, OCC>), dim3(units * p.members.d), dim3(64 * NW), lds,
-                     stream, p);
+  hipLaunchKernelGGL((paged_token_kernel<TQ, TV, NK, DBW>), dim3(units * p.members.d), dim3(64 * kWaves), lds, stream, p);
 }
 
 template <typename TQ, typename TV, int NK, int DBW, int CT>
@@ -949,9 +922,9 @@ void launch_chunk(const Params& p, hipStream_t stream) {
 }
 
 template <typename TQ, typename TV, int DBW>
-void launch_width(const Params& p, hipStream_t stream) {
-  if (p.a.cache.W <= 256) launch_kernel<TQ, TV, 4, DBW, 1, 4, false, 2, 2>(p, stream);
-  else launch_kernel<TQ, TV, 8, DBW, 1, 4, false, 2, 2>(p, stream);
+void launch_token(const Params& p, hipStream_t stream) {
+  if (p.a.cache.W <= 256) launch_token_kernel<TQ, TV, 4, DBW>(p, stream);
+  else launch_token_kernel<TQ, TV, 8, DBW>(p, stream);
 }
 
 template <typename TQ, typename TV>
@@ -964,14 +937,14 @@ void launch_typed(const Params& p, const Plan& r, hipStream_t stream) {
       default: launch_chunk<TQ, TV, 4>(p, stream); break;
     }
   } else switch (r.dbw) {
-    case 1: launch_width<TQ, TV, 1>(p, stream); break;
-    case 2: launch_width<TQ, TV, 2>(p, stream); break;
-    case 3: launch_width<TQ, TV, 3>(p, stream); break;
-    case 4: launch_width<TQ, TV, 4>(p, stream); break;
-    case 5: launch_width<TQ, TV, 5>(p, stream); break;
-    case 6: launch_width<TQ, TV, 6>(p, stream); break;
-    case 7: launch_width<TQ, TV, 7>(p, stream); break;
-    default: launch_width<TQ, TV, 8>(p, stream); break;
+    case 1: launch_token<TQ, TV, 1>(p, stream); break;
+    case 2: launch_token<TQ, TV, 2>(p, stream); break;
+    case 3: launch_token<TQ, TV, 3>(p, stream); break;
+    case 4: launch_token<TQ, TV, 4>(p, stream); break;
+    case 5: launch_token<TQ, TV, 5>(p, stream); break;
+    case 6: launch_token<TQ, TV, 6>(p, stream); break;
+    case 7: launch_token<TQ, TV, 7>(p, stream); break;
+    default: launch_token<TQ, TV, 8>(p, stream); break;
   }
   if (p.part_o) {
     const dim3 grid(static_cast<unsigned>(p.a.tokens.N * (p.a.mix ? 1 : p.a.S)), static_cast<unsigned>((p.a.cache.D + 63) / 64));
