@@ -31,6 +31,7 @@ namespace da {
 namespace {
 
 constexpr int kWaves = 4;
+constexpr int kTokenGroups = 4;       // of 64 key features, at a time
 constexpr int kMaxSplits = 256;
 constexpr int kWantWorkgroups = 1024, kChunkWorkgroups = 256;
 constexpr float kNoScore = -3.0e38f;  // the running maximum before the first score
@@ -118,8 +119,10 @@ __device__ void clear_other_rows(const PagedAttentionArgs& a, int64_t wg, int64_
 }  // namespace
 
 // NK: groups of 64 key features that a wave holds (fewer features leave the rest
-// zero, more are taken in turn); DBW: 16-feature blocks of the values of a wave.
-// The 16 columns are (token, map) pairs over all features.
+// zero, more are taken in turn: eight groups at once spill with 512 value
+// features, and 32 sequences of 4096 tokens with 512 key features take 71 us
+// instead of 58); DBW: 16-feature blocks of the values of a wave.  The 16 columns
+// are (token, map) pairs over all features.
 //
 // A step takes four tiles.  Wave w forms tile w's scores and leaves its
 // probabilities in LDS; after a barrier every wave multiplies them with its own
@@ -131,11 +134,11 @@ __device__ void clear_other_rows(const PagedAttentionArgs& a, int64_t wg, int64_
 // 512 features, 400 MB) 51 us with the merge, one of 131072 tokens (201 MB) 41 us.
 // Waves that held whole tiles, each with all features, had a register file too
 // small for their loads in flight: 78 us for the former.
-template <typename TQ, typename TV, int NK, int DBW>
+template <typename TQ, typename TV, int DBW>
 __global__ __launch_bounds__(64 * kWaves, 2) void paged_token_kernel(Params p) {
   typedef typename Elem<TQ>::v8 q8;
   typedef typename Elem<TV>::v8 v8;
-  constexpr int NW = kWaves;
+  constexpr int NW = kWaves, NK = kTokenGroups;
   constexpr int DS = 16 * DBW * NW;
   constexpr int FW = 64 * NK;               // features of a pass
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -900,12 +903,12 @@ Plan plan(const PagedAttentionArgs& a) {
   return r;
 }
 
-template <typename TQ, typename TV, int NK, int DBW>
-void launch_token_kernel(const Params& p, hipStream_t stream) {
-  const int QP = static_cast<int>(round_up(p.a.cache.W, 64 * NK)) + 8;
+template <typename TQ, typename TV, int DBW>
+void launch_token(const Params& p, hipStream_t stream) {
+  const int QP = static_cast<int>(round_up(p.a.cache.W, 64 * kTokenGroups)) + 8;
   const size_t lds = static_cast<size_t>(32) * QP + 2 * kWaves * (1024 + 64 + 4);
   const unsigned units = static_cast<unsigned>(round_up(p.units, kXcds));
-  hipLaunchKernelGGL((paged_token_kernel<TQ, TV, NK, DBW>), dim3(units * p.members.d), dim3(64 * kWaves), lds, stream, p);
+  hipLaunchKernelGGL((paged_token_kernel<TQ, TV, DBW>), dim3(units * p.members.d), dim3(64 * kWaves), lds, stream, p);
 }
 
 template <typename TQ, typename TV, int NK, int DBW, int CT>
@@ -919,12 +922,6 @@ void launch_chunk(const Params& p, hipStream_t stream) {
   if (p.a.RP <= 128) launch_chunk_kernel<TQ, TV, 2, DBW, 8>(p, stream);
   else if (p.a.RP <= 256) launch_chunk_kernel<TQ, TV, 4, DBW, 8>(p, stream);
   else launch_chunk_kernel<TQ, TV, 8, DBW, 4>(p, stream);
-}
-
-template <typename TQ, typename TV, int DBW>
-void launch_token(const Params& p, hipStream_t stream) {
-  if (p.a.cache.W <= 256) launch_token_kernel<TQ, TV, 4, DBW>(p, stream);
-  else launch_token_kernel<TQ, TV, 8, DBW>(p, stream);
 }
 
 template <typename TQ, typename TV>
