@@ -120,7 +120,7 @@ __device__ void clear_other_rows(const PagedAttentionArgs& a, int64_t wg, int64_
 
 // NK: groups of 64 key features that a wave holds (fewer features leave the rest
 // zero, more are taken in turn: eight groups at once spill with 512 value
-// features, and 32 sequences of 4096 tokens with 512 key features take 71 us
+// features, and 32 sequences of up to 4096 tokens with 512 key features take 71 us
 // instead of 58); DBW: 16-feature blocks of the values of a wave.  The 16 columns
 // are (token, map) pairs over all features.
 //
@@ -130,10 +130,10 @@ __device__ void clear_other_rows(const PagedAttentionArgs& a, int64_t wg, int64_
 // tiles' values are on their way meanwhile, and the probabilities have two buffers,
 // so that a step has one barrier.
 //
-// Bound by the cache's bytes: 64 sequences of 4096 tokens (keys of 256, values of
-// 512 features, 400 MB) 51 us with the merge, one of 131072 tokens (201 MB) 41 us.
+// Bound by the cache's bytes: 64 sequences of up to 4096 tokens (keys of 256, values of
+// 512 features, 254 MB) 51 us with the merge, one of 131072 tokens (201 MB) 41 us.
 // Waves that held whole tiles, each with all features, had a register file too
-// small for their loads in flight: 78 us for the former.
+// small for their loads in flight: 85 us for the former.
 template <typename TQ, typename TV, int DBW>
 __global__ __launch_bounds__(64 * kWaves, 2) void paged_token_kernel(Params p) {
   typedef typename Elem<TQ>::v8 q8;

@@ -337,7 +337,7 @@ class SharedDictionaryAttention(nn.Module):
 
         cfg = self.config
         count = x.shape[0]
-        wq, wk, wv, wo, bv, log_beta, log_scales, mix, _ = hip_ops._module_operands(self, dtype)
+        wq, wk, wv, wo, bv, log_beta, _, _, _ = hip_ops._module_operands(self, dtype)
         rows = torch.empty(2, count, cfg.total_qk_width, dtype=dtype, device=x.device)
         hip_ops.linear_hip(x, wq, out=rows[0])
         hip_ops.linear_hip(x, wk, out=rows[1])
@@ -351,12 +351,9 @@ class SharedDictionaryAttention(nn.Module):
         ).view(2, count, cfg.qk_branches, cfg.routing_dim)
         cache, where = tokens.caches[layer], (tokens.page_table, tokens.lengths, tokens.offsets)
         serving_ops.cache_append_hip(cache, routed[1], value, *where, max_chunk=tokens.max_chunk)
-        factors = None
-        if mix is not None:
-            # The weights rounded to the map dtype, the sum in fp32 (as _combine).
-            factors = torch.softmax(mix, dim=0).to(dtype).float()
-        arguments = (routed[0], cache, *where, score_scale_from_log(log_scales))
-        hints = {"mix": factors, "max_chunk": tokens.max_chunk, "max_length": tokens.max_length}
+        arguments = (routed[0], cache, *where, tokens.scales[layer])
+        mix = None if tokens.mixes is None else tokens.mixes[layer]
+        hints = {"mix": mix, "max_chunk": tokens.max_chunk, "max_length": tokens.max_length}
         if tokens.weights is None:
             maps = serving_ops.paged_attention_hip(*arguments, **hints)
         else:
@@ -1378,15 +1375,18 @@ class DoubleAttentionStack(nn.Module):
 
 
 class CachedTokens(NamedTuple):
-    """Where the new tokens of ``DoubleAttentionLM.cached_forward`` lie; see there."""
+    """Where the new tokens of ``DoubleAttentionLM.cached_forward`` lie (see there),
+    and the layers' temperatures and map weights."""
 
     caches: Sequence[PagedCache]
     page_table: Tensor
     lengths: Tensor
     offsets: Tensor
-    weights: Tensor | None = None
-    max_chunk: int | None = None
-    max_length: int | None = None
+    weights: Tensor | None
+    max_chunk: int | None
+    max_length: int | None
+    scales: Tensor          # fp32 [layers, maps]
+    mixes: Tensor | None    # fp32 [layers, maps]
 
 
 class DoubleAttentionLM(nn.Module):
@@ -1520,9 +1520,16 @@ class DoubleAttentionLM(nn.Module):
         dtype = self._cached_dtype()
         if weights is not None and (weights.ndim != 3 or weights.shape[0] != len(caches) or not weights.is_contiguous()):
             raise ValueError("cached_forward: weights must be contiguous [layers, sequences, entries * page_size]")
-        tokens = CachedTokens(caches, page_table, lengths, offsets, weights, max_chunk, max_length)
         x = self.token_embedding(token_ids) + self.position_embedding(positions)
         stack = self.stack
+        # All layers' at once: fewer launches.  fp32 temperatures, as the fused
+        # forward forms them; weights rounded to the map dtype, as by _combine.
+        attentions = [block.attention for block in stack.blocks]
+        scales = score_scale_from_log(torch.stack([a.log_score_scales for a in attentions]).float())
+        mixes = None
+        if attentions[0].map_mix_logits is not None:
+            mixes = torch.softmax(torch.stack([a.map_mix_logits for a in attentions]), dim=1).to(dtype).float()
+        tokens = CachedTokens(caches, page_table, lengths, offsets, weights, max_chunk, max_length, scales, mixes)
         dictionaries = stack._normalize_banks(x)
         if token_ids.shape[0]:
             for index, block in enumerate(stack.blocks):
