@@ -114,6 +114,7 @@ class CachedSequences:
         self.positions = [at + n for at, n in zip(self.positions, counts)]
         return logits
 
+    @torch.inference_mode()   # the tensors may have been made there
     def evict(self, keep: int, recent: int = 0) -> None:
         """Cuts every sequence of more than ``keep`` tokens, in each layer by itself,
         to its last ``recent`` tokens and those of the others that gathered the

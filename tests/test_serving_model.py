@@ -236,6 +236,26 @@ def test_eviction_of_a_model_s_sequences() -> None:
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("made_in,used_in", [(True, False), (False, True), (True, True)])
+def test_sequences_in_inference_mode(made_in, used_in) -> None:
+    model = model_of().cuda()
+    expected = None
+    for made, used in ((False, False), (made_in, used_in)):
+        with torch.inference_mode(made):
+            s = da.CachedSequences(model, 2, 8, page_size=32, gather_weights=True)
+        with torch.inference_mode(used):
+            s.extend(torch.cat(ids(40, 9)), [40, 9])
+            s.evict(20, 4)
+            s.extend(torch.cat(ids(1, 2, seed=1)), [1, 2])
+            s.release(1)
+            logits = s.extend(torch.cat(ids(3, 5, seed=2)), [3, 5])
+        assert s.lengths == [24, 5] and s.positions == [44, 5]
+        if expected is None:
+            expected = logits
+    assert torch.equal(logits, expected)
+
+
+@pytest.mark.gpu
 def test_decoding_step_as_a_graph() -> None:
     model = model_of("two-branches").cuda()
     page, sequences, steps = 32, 3, 5
