@@ -42,8 +42,10 @@ int validate_cache(const char* what, const da_paged_cache& c, int64_t sequences)
 }
 
 da::CacheView view(const da_paged_cache& c) {
-  return {c.keys, c.key_page_stride, c.values, c.value_page_stride, static_cast<int>(c.pages), static_cast<int>(c.page_size / 32),
-          c.page_size == 32 ? 0u : static_cast<uint32_t>((0xffffffffu + c.page_size / 32) / (c.page_size / 32)), static_cast<int>(c.key_width), static_cast<int>(c.value_dim), c.page_table, c.ld_table, static_cast<int>(c.table_pages)};
+  const int64_t tiles = c.page_size / 32;
+  const uint32_t inverse = tiles == 1 ? 0u : static_cast<uint32_t>((0xffffffffu + tiles) / tiles);
+  return {c.keys, c.key_page_stride, c.values, c.value_page_stride, static_cast<int>(c.pages), static_cast<int>(tiles), inverse,
+          static_cast<int>(c.key_width), static_cast<int>(c.value_dim), c.page_table, c.ld_table, static_cast<int>(c.table_pages)};
 }
 Spans pages_of(const void* p, const da_paged_cache& c, int64_t width, int64_t stride) {
   return {p, c.pages, c.page_size * width, stride, 2};
