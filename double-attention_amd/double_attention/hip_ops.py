@@ -1494,7 +1494,7 @@ def linear_hip(
     ``activation`` is None or ``"gelu"`` (exact, ``nn.GELU()``); ``residual``
     has the output's shape and is added to the rounded result, as the
     unfused ``residual + linear(x)`` does.  ``out`` (contiguous, 16-byte
-    aligned) takes the result.
+    aligned, apart from the inputs) takes the result.
     """
 
     _require_cuda(x, weight)
@@ -1506,6 +1506,7 @@ def linear_hip(
     rows = _aligned(x.reshape(-1, x.shape[-1]))
     w = _aligned(weight.detach())
     shape = (*x.shape[:-1], weight.shape[0])
+    given = out is not None
     if out is None:
         out = torch.empty(shape, dtype=x.dtype, device=x.device)
     elif out.shape != shape or out.dtype != x.dtype or out.device != x.device or not out.is_contiguous() or out.data_ptr() % 16:
@@ -1516,6 +1517,11 @@ def linear_hip(
         if residual.shape != out.shape or residual.dtype != x.dtype:
             raise ValueError("residual must match the output's shape and dtype")
         res = _aligned(residual.detach())
+    if given:   # workgroups read rows that others write
+        first, last = out.data_ptr(), out.data_ptr() + out.numel() * out.element_size()
+        for t in (rows, w, b, res):
+            if t is not None and t.data_ptr() < last and first < t.data_ptr() + t.numel() * t.element_size():
+                raise ValueError("out must not overlap the inputs")
     lib = _lib.get()
     bias_code = dtype_code(b.dtype) if b is not None else _lib.DA_F32
     if activation is None and res is None:

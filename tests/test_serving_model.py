@@ -314,6 +314,27 @@ def test_decoding_step_as_a_graph() -> None:
         assert torch.equal(weights, eager_weights)
 
 
+@pytest.mark.gpu
+def test_linear_into_a_given_tensor() -> None:
+    from double_attention.hip_ops import linear_hip
+
+    g = torch.Generator().manual_seed(0)
+    x, w = (torch.randn(128, 128, generator=g).cuda().bfloat16() for _ in range(2))
+    both = torch.zeros(3, 128, 128, dtype=torch.bfloat16, device="cuda")
+    assert linear_hip(x, w, out=both[1]).data_ptr() == both[1].data_ptr()
+    assert torch.equal(both[1], linear_hip(x, w)) and not both[::2].any()
+    assert torch.equal(linear_hip(x, w, activation="gelu", residual=x, out=both[0]), linear_hip(x, w, activation="gelu", residual=x))
+    wide = torch.empty(128, 256, dtype=torch.bfloat16, device="cuda")
+    for out in (both, both[0].float(), wide[:, :128], both.flatten()[4:4 + 128 * 128].view(128, 128), both[0].cpu()):
+        with pytest.raises(ValueError, match="out must have"):
+            linear_hip(x, w, out=out)
+    for out in (x, w):
+        with pytest.raises(ValueError, match="overlap"):
+            linear_hip(x, w, out=out)
+    with pytest.raises(ValueError, match="overlap"):
+        linear_hip(x, w, residual=both[2], out=both[2])
+
+
 # ---- log probabilities of next tokens --------------------------------------
 
 
