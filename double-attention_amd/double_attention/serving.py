@@ -25,9 +25,10 @@ class CachedSequences:
     token's attention is gathered, and ``evict`` cuts sequences to the tokens
     that got most of it; their positions go on as if nothing had been cut.
 
-    Lengths and pages are kept on the host, so nothing waits for the device.
-    A refused call changes nothing.  Use one stream: pages that were freed are
-    written anew by later calls.
+    Lengths and pages are kept on the host; nothing is read back from the
+    device (its small tables are copied there in each call, which waits for what
+    the stream still does).  A refused call changes nothing.  Use one
+    stream: pages that were freed are written anew by later calls.
     """
 
     def __init__(

@@ -256,6 +256,21 @@ def test_sequences_in_inference_mode(made_in, used_in) -> None:
 
 
 @pytest.mark.gpu
+def test_sequences_that_wait_or_start_anew() -> None:
+    model = model_of().cuda()
+    s = da.CachedSequences(model, 2, 8, page_size=32, gather_weights=True)
+    s.extend(torch.cat(ids(40, 33)), [40, 33])
+    before = s.weights.clone()
+    s.extend(ids(3, seed=1)[0], [3, 0])
+    assert torch.equal(s.weights[:, 1], before[:, 1]) and not torch.equal(s.weights[:, 0], before[:, 0])
+    s.release(0)
+    alone = da.CachedSequences(model, 2, 8, page_size=32, gather_weights=True)
+    alone.extend(torch.cat(ids(0, 33)), [0, 33])
+    again = [t.extend(ids(35, seed=2)[0], [35, 0]) for t in (s, alone)]
+    assert torch.equal(*again) and torch.equal(s.weights[:, 0], alone.weights[:, 0])
+
+
+@pytest.mark.gpu
 def test_decoding_step_as_a_graph() -> None:
     model = model_of("two-branches").cuda()
     page, sequences, steps = 32, 3, 5
