@@ -96,7 +96,7 @@ extern "C" {
 static_assert(DA_OUT_SPLIT == da::kOutSplit, "split-output flag");
 static_assert(DA_ROUTE_BETA_IS_LOG_SCALE == da::kRouteBetaIsLogScale, "route flag");
 
-int da_abi_version(void) { return 21; }
+int da_abi_version(void) { return 22; }
 
 const char* da_last_error(void) { return g_error.c_str(); }
 

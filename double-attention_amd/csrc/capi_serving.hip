@@ -277,7 +277,7 @@ int da_token_log_probs(const void* logits, int64_t rows, int64_t vocab, int64_t 
     if (!aligned(workspace, 16)) return fail(DA_ERR_ALIGNMENT, "%s: the workspace must be 16-byte aligned", what);
   }
   if ((rc = validate_apart(what,
-                           {flat(log_probs, rows, 4), flat(entropy, rows, 4), flat(lse, rows, 4), flat(top ? top_log_probs : nullptr, rows * top, 4),
+                           {flat(log_probs, rows, 4), flat(entropy, rows, 4), flat(lse, 2 * rows, 4), flat(top ? top_log_probs : nullptr, rows * top, 4),
                             flat(top ? top_tokens : nullptr, rows * top, 8), flat(need ? workspace : nullptr, need, 1)},
                            {{logits, rows, vocab, ldx, element_bytes(dtype)}, flat(tokens, rows, 8)})))
     return rc;
@@ -315,7 +315,7 @@ int da_token_log_probs_backward(const void* logits, int64_t rows, int64_t vocab,
       !aligned(grad_entropy, 4) || !aligned(grad_top, 4))
     return fail(DA_ERR_ALIGNMENT, "%s: tensors must be aligned to their elements", what);
   if ((rc = validate_apart(what, {{grad, rows, vocab, ldg, element_bytes(dtype)}},
-                           {{logits, rows, vocab, ldx, element_bytes(dtype)}, flat(tokens, rows, 8), flat(lse, rows, 4),
+                           {{logits, rows, vocab, ldx, element_bytes(dtype)}, flat(tokens, rows, 8), flat(lse, 2 * rows, 4),
                             flat(entropy, rows, 4), flat(grad_top ? top_tokens : nullptr, rows * top, 8), flat(grad_log_probs, rows, 4),
                             flat(grad_entropy, rows, 4), flat(grad_top, rows * top, 4)})))
     return rc;

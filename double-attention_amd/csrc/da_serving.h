@@ -135,7 +135,7 @@ struct TokenLogProbsArgs {
   int64_t ignore;
   float* log_probs;     // [rows]
   float* entropy;       // [rows]
-  float* lse;           // [rows] or nullptr
+  float* lse;           // [rows][2]: a reference m and log sum e^(x - m), or nullptr
   int top;
   float* top_log_probs; // [rows][top]
   int64_t* top_tokens;  // [rows][top]

@@ -13,7 +13,9 @@
 // TB/s) where the last level of cache still has most of them, 77 us after the
 // gradient of others; their gradient in 86 us (6.1 TB/s).
 // Backward: dx_j = -p_j (G + g_H (log p_j + H)) + what is given for j itself,
-// with G the sum of the gradients at log probabilities of the row.
+// with G the sum of the gradients at log probabilities of the row.  It gets m and
+// log s apart: their rounded sum would shift every log p_j of a row whose logits
+// are far from zero (by 2^-7 at 10^5), and be m where that is the lowest value.
 #include <algorithm>
 #include <type_traits>
 
@@ -140,7 +142,10 @@ __device__ void finish_row(const TokenLogProbsArgs& a, int64_t row, Sums v, floa
   if (token == a.ignore) lp = 0.f;
   a.log_probs[row] = lp;
   if (a.entropy) a.entropy[row] = log_s - v.t / v.s;
-  if (a.lse) a.lse[row] = v.m + log_s;
+  if (a.lse) {
+    a.lse[2 * row] = v.m;
+    a.lse[2 * row + 1] = log_s;
+  }
 }
 template <typename T>
 __device__ __forceinline__ float token_logit(const TokenLogProbsArgs& a, int64_t row) {
@@ -398,7 +403,7 @@ __global__ __launch_bounds__(kThreads) void token_log_probs_backward_kernel(Toke
   const T* x = static_cast<const T*>(a.logits) + row * a.ldx;
   T* out = static_cast<T*>(a.grad) + row * a.ldg;
   const int64_t token = a.tokens[row];
-  const float lse = a.lse[row];
+  const float m = a.lse[2 * row], log_s = a.lse[2 * row + 1];
   const float g_h = a.g_entropy ? a.g_entropy[row] : 0.f, h = a.entropy ? a.entropy[row] : 0.f;
   float g_token = a.g_log_probs && token != a.ignore ? a.g_log_probs[row] : 0.f;
   if (token != a.ignore && (token < 0 || token >= a.V)) g_token = __builtin_nanf("");
@@ -408,7 +413,7 @@ __global__ __launch_bounds__(kThreads) void token_log_probs_backward_kernel(Toke
   // g_H H + G, once.
   const float base = g_all + g_h * h;
   auto at = [&](float value) {
-    const float lp = value - lse;
+    const float lp = (value - m) - log_s;
     return -fast_exp(lp) * (base + g_h * fmaxf(lp, kNoWeight));
   };
   const RowShape<T> shape(x, a.V);

@@ -51,7 +51,7 @@ ERROR_NAMES = {
     -5: "workspace too small",
 }
 
-ABI_VERSION = 21
+ABI_VERSION = 22
 INT8_GROUP = 128
 NOALLOC_SCRATCH_BYTES = 128 << 20
 MAX_TOP = 64

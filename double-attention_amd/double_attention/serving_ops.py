@@ -440,7 +440,7 @@ def _token_log_probs(logits: Tensor, tokens: Tensor, top: int, entropy: bool, ig
 
     log_probs = new()
     entropies = new() if entropy else None
-    lse = new() if want_lse else None
+    lse = new(2) if want_lse else None
     top_log_probs, top_tokens = (new(top), new(top, dtype=_INT64)) if top else (None, None)
     lib = _lib.get()
     nbytes = lib.da_token_log_probs_workspace_bytes(count, vocab, top)

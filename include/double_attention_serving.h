@@ -138,7 +138,8 @@ int da_cache_compact(const da_paged_cache* from, const da_paged_cache* to, int64
  * Of logits [rows, vocab] (any dtype, pitch ldx, aligned to their elements):
  *   log_probs[r] = log softmax(logits[r])[tokens[r]]   (0 at ignore_index, NaN for other tokens outside [0, vocab))
  *   entropy[r]   = -sum_j p_j log p_j                  (NULL: not wanted)
- *   lse[r]       = log sum_j exp(logits[r, j])         (NULL: not wanted; the backward's)
+ *   lse[r]       = (m, log sum_j exp(logits[r, j] - m)) with some m near the row's largest logit: two floats, whose
+ *                  sum is the log-sum-exp                (NULL: not wanted; the backward's)
  *   top_tokens[r], top_log_probs[r]: the `top` most probable tokens in order,
  *                  equal ones the lowest first (top <= 64, top <= vocab; a NaN is never among them: -1 and NaN stand for what is missing).
  * Rows with a NaN or +infinity, and rows of -infinity throughout, have NaN log
@@ -152,7 +153,7 @@ int da_token_log_probs(const void* logits, int64_t rows, int64_t vocab, int64_t 
 
 /*
  * Its gradient at the logits, rounded once to their type, from the gradients at
- * log_probs, entropy and top_log_probs (each NULL: zero), lse, and the entropy
+ * log_probs, entropy and top_log_probs (each NULL: zero), and the lse, entropy
  * and top_tokens that the forward gave.  grad: [rows, vocab] at pitch ldg, off
  * the logits.
  */
