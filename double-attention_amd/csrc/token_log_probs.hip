@@ -15,7 +15,7 @@
 // Backward: dx_j = -p_j (G + g_H (log p_j + H)) + what is given for j itself,
 // with G the sum of the gradients at log probabilities of the row.  It gets m and
 // log s apart: their rounded sum would shift every log p_j of a row whose logits
-// are far from zero (by 2^-7 at 10^5), and be m where that is the lowest value.
+// are far from zero (by up to 2^-8 at 10^5), and be m where that is the lowest value.
 #include <algorithm>
 #include <type_traits>
 
