@@ -357,8 +357,9 @@ class SharedDictionaryAttention(nn.Module):
         if tokens.weights is None:
             maps = serving_ops.paged_attention_hip(*arguments, **hints)
         else:
-            weights = tokens.weights[layer]
-            maps, _ = serving_ops.paged_attention_weights_hip(*arguments, weights=weights, out=weights, **hints)
+            maps, _ = serving_ops.paged_attention_weights_hip(
+                *arguments, weights=tokens.weights[layer], out=tokens.weights_out[layer], **hints
+            )
         mixed = maps.reshape(count, -1)   # one map, their weighted sum, or all side by side
         return residual + mixed if wo is None else hip_ops.linear_hip(mixed, wo, residual=residual)
 
@@ -1383,6 +1384,7 @@ class CachedTokens(NamedTuple):
     lengths: Tensor
     offsets: Tensor
     weights: Tensor | None
+    weights_out: Tensor | None
     max_chunk: int | None
     max_length: int | None
     scales: Tensor          # fp32 [layers, maps]
@@ -1486,6 +1488,7 @@ class DoubleAttentionLM(nn.Module):
         offsets: Tensor,
         *,
         weights: Tensor | None = None,
+        weights_out: Tensor | None = None,
         rows: Tensor | None = None,
         max_chunk: int | None = None,
         max_length: int | None = None,
@@ -1499,12 +1502,13 @@ class DoubleAttentionLM(nn.Module):
         theirs; ``page_table`` (one for all layers), ``lengths`` (with the new
         tokens) and ``offsets`` are int32 tensors on the device, as for
         ``cache_append_hip`` and ``paged_attention_hip``.  ``weights`` (fp32
-        ``[layers, sequences, entries * page_size]``, contiguous) gathers in place
-        the attention that every cached token received, for
-        ``cache_select_hip``.  ``rows``: the places of the tokens whose logits are
-        wanted (default: all).  ``max_chunk`` and ``max_length`` are the largest
-        numbers of new and of all tokens of a sequence, where the program knows
-        them.
+        ``[layers, sequences, entries * page_size]``, contiguous) gathers the
+        attention that every cached token received, for ``cache_select_hip``: in
+        place, or ``weights_out`` (of the same shape) takes the sums and
+        ``weights`` stays, so that a call that raised can be made again.
+        ``rows``: the places of the tokens whose logits are wanted (default: all).
+        ``max_chunk`` and ``max_length`` are the largest numbers of new and of all
+        tokens of a sequence, where the program knows them.
 
         For causal models in fp16 or bf16 on the HIP kernels, in evaluation;
         without gradients.  Nothing is read on the host, so that a step can be
@@ -1520,6 +1524,10 @@ class DoubleAttentionLM(nn.Module):
         dtype = self._cached_dtype()
         if weights is not None and (weights.ndim != 3 or weights.shape[0] != len(caches) or not weights.is_contiguous()):
             raise ValueError("cached_forward: weights must be contiguous [layers, sequences, entries * page_size]")
+        if weights_out is None:
+            weights_out = weights
+        elif weights is None or weights_out.shape != weights.shape or not weights_out.is_contiguous():
+            raise ValueError("cached_forward: weights_out must be contiguous, of the shape of weights")
         x = self.token_embedding(token_ids) + self.position_embedding(positions)
         stack = self.stack
         # All layers' at once: fewer launches.  fp32 temperatures, as the fused
@@ -1529,12 +1537,15 @@ class DoubleAttentionLM(nn.Module):
         mixes = None
         if attentions[0].map_mix_logits is not None:
             mixes = torch.softmax(torch.stack([a.map_mix_logits for a in attentions]), dim=1).to(dtype).float()
-        tokens = CachedTokens(caches, page_table, lengths, offsets, weights, max_chunk, max_length, scales, mixes)
+        tokens = CachedTokens(caches, page_table, lengths, offsets, weights, weights_out, max_chunk, max_length, scales, mixes)
         dictionaries = stack._normalize_banks(x)
         if token_ids.shape[0]:
             for index, block in enumerate(stack.blocks):
                 bank = min(index // stack.dictionary_group_size, len(stack.banks) - 1)
                 x = block._hip_cached_block(x, stack.banks[bank], dictionaries[bank], dtype, tokens, index)
+        elif weights_out is not weights:
+            with torch.inference_mode():   # the tensors may have been made there
+                weights_out.copy_(weights)
         if rows is not None:
             x = x.index_select(0, rows)
         return self.lm_head(self._final_norm(x))

@@ -7,7 +7,7 @@ and the weights that cached tokens gathered.
 
 from __future__ import annotations
 
-from typing import Sequence
+from typing import Iterator, Sequence
 
 import torch
 from torch import Tensor
@@ -27,8 +27,10 @@ class CachedSequences:
 
     Lengths and pages are kept on the host; nothing is read back from the
     device (its small tables are copied there in each call, which waits for what
-    the stream still does).  A refused call changes nothing.  Use one
-    stream: pages that were freed are written anew by later calls.
+    the stream still does).  A call that raises changes nothing: pages, lengths
+    and gathered weights (of which there are two buffers) are the new ones when
+    all of its work has been enqueued.  Use one stream: pages that were freed are
+    written anew by later calls.
     """
 
     def __init__(
@@ -45,11 +47,12 @@ class CachedSequences:
         self._pages: list[list[int]] = [[] for _ in range(sequences)]
         self._free = list(range(pages - 1, -1, -1))
         self._device = self.caches[0].keys.device
-        self.weights = None
+        self.weights = self._next_weights = None
         if gather_weights:
             self.weights = torch.zeros(
                 len(self.caches), sequences, self.entries * page_size, dtype=torch.float32, device=self._device
             )
+            self._next_weights = torch.empty_like(self.weights)
 
     @property
     def free_pages(self) -> int:
@@ -66,6 +69,9 @@ class CachedSequences:
 
     def _count(self, tokens: int) -> int:
         return -(-tokens // self.page_size)
+
+    def _last_free(self, pages: int) -> Iterator[int]:
+        return reversed(self._free[len(self._free) - pages:])
 
     def extend(self, token_ids: Tensor, counts: Sequence[int], *, last_only: bool = False) -> Tensor:
         """Continues sequence b by ``counts[b]`` tokens (0: not at all).
@@ -95,9 +101,8 @@ class CachedSequences:
                 raise RuntimeError(f"extend: sequence {b} does not fit {self.entries} pages")
         if sum(need) > len(self._free):
             raise RuntimeError(f"extend: needs {sum(need)} more pages, {len(self._free)} are free")
-        self.model._cached_dtype()   # refuses before pages change hands
-        for own, n in zip(self._pages, need):
-            own.extend(self._free.pop() for _ in range(n))
+        taken = self._last_free(sum(need))
+        pages = [[*own, *(next(taken) for _ in range(n))] if n else own for own, n in zip(self._pages, need)]
         offsets = [0]
         for n in counts:
             offsets.append(offsets[-1] + n)
@@ -107,12 +112,15 @@ class CachedSequences:
         last = [end - 1 for end, n in zip(offsets[1:], counts) if n]
         logits = self.model.cached_forward(
             token_ids.to(self._device), torch.tensor(positions, dtype=torch.int64).to(self._device), self.caches,
-            self._table(self._pages), numbers[:sequences], numbers[sequences:], weights=self.weights,
+            self._table(pages), numbers[:sequences], numbers[sequences:], weights=self.weights, weights_out=self._next_weights,
             rows=torch.tensor(last, dtype=torch.int64).to(self._device) if last_only else None,
             max_chunk=max(1, *counts), max_length=max(1, *lengths),
         )
-        self.lengths = lengths
+        # Nothing below raises.
+        del self._free[len(self._free) - sum(need):]
+        self._pages, self.lengths = pages, lengths
         self.positions = [at + n for at, n in zip(self.positions, counts)]
+        self.weights, self._next_weights = self._next_weights, self.weights
         return logits
 
     @torch.inference_mode()   # the tensors may have been made there
@@ -133,18 +141,22 @@ class CachedSequences:
         if each * len(cut) > len(self._free):
             raise RuntimeError(f"evict: needs {each * len(cut)} free pages, {len(self._free)} are free")
         # Pages of the sequences that stay whole are not named: nothing of theirs moves.
+        taken = self._last_free(each * len(cut))
         moved_to: list[list[int]] = [[] for _ in self._pages]
         for b in cut:
-            moved_to[b] = [self._free.pop() for _ in range(each)]
+            moved_to[b] = [next(taken) for _ in range(each)]
         table, new_table = self._table(self._pages), self._table(moved_to)
         lengths = torch.tensor(self.lengths, dtype=torch.int32).to(self._device)
-        for cache, weights in zip(self.caches, self.weights):
+        for cache, weights, out in zip(self.caches, self.weights, self._next_weights):
             kept, counts = cache_select_hip(weights, lengths, keep, recent)
-            weights.copy_(cache_compact_hip(cache, table, kept, counts, cache, new_table, weights=weights))
+            out.copy_(cache_compact_hip(cache, table, kept, counts, cache, new_table, weights=weights))
+        # Nothing below raises.
+        del self._free[len(self._free) - each * len(cut):]
         for b in cut:
             self._free.extend(reversed(self._pages[b]))
             self._pages[b] = moved_to[b]
             self.lengths[b] = keep
+        self.weights, self._next_weights = self._next_weights, self.weights
 
     def release(self, sequence: int) -> None:
         """Frees a sequence's pages; it starts anew, empty."""
