@@ -103,6 +103,37 @@ __device__ __forceinline__ u32x4 load_at(const char* base, uint32_t lane_offset)
   return *reinterpret_cast<__attribute__((address_space(1))) const u32x4*>((global_ptr)(base) + lane_offset);
 }
 
+// A product multiplies every token of a tile with every column, those that do
+// not see the token with zero: there an infinity or a NaN among the values is
+// taken out, and the features' first such tokens are kept in LDS (`first`, this
+// lane's feature).  Columns that see one are NaN in that feature at the end.
+constexpr int kNoToken = 0x7fffffff;
+// Bit 15 of each half where that is an infinity or a NaN.
+template <typename TV>
+__device__ __forceinline__ uint32_t non_finite(uint32_t halves) {
+  constexpr uint32_t exponents = std::is_same<TV, __bf16>::value ? 0x7f807f80u : 0x7c007c00u;
+  constexpr uint32_t step = std::is_same<TV, __bf16>::value ? 0x00800080u : 0x04000400u;
+  return ((halves & exponents) + step) & 0x80008000u;
+}
+// v: eight tokens of a feature from `token` on.  True where any lane had one.
+template <typename TV>
+__device__ __forceinline__ bool take_out(u32x4& v, int* first, int token) {
+  uint32_t any = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) any |= non_finite<TV>(v[e]);
+  if (__ballot(any != 0) == 0) return false;
+  int at = kNoToken;
+#pragma unroll
+  for (int e = 3; e >= 0; --e) {
+    const uint32_t bits = non_finite<TV>(v[e]);
+    if (bits >> 31) at = token + 2 * e + 1;
+    if (bits & 0x8000u) at = token + 2 * e;
+    v[e] &= ~((bits >> 15) * 0xffffu);
+  }
+  if (at != kNoToken) atomicMin(first, at);
+  return true;
+}
+
 // Rows of no sequence (in front of the first and behind the last one) are zero.
 template <typename TV>
 __device__ void clear_other_rows(const PagedAttentionArgs& a, int64_t wg, int64_t n_wg) {
@@ -172,6 +203,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_token_kernel(Params p) {
   char* ps = lds + 32 * QP;                           // [2][NW][64 lanes] 16 bytes
   float* ms = reinterpret_cast<float*>(ps + 2 * NW * 1024); // [2][NW][16]
   int* moved = reinterpret_cast<int*>(ms + 2 * NW * 16);    // [2][NW]
+  int* firsts = moved + 2 * NW + wave * DBW * 16;           // [NW][DBW][16], this wave's features
 
   for (int ct0 = member; ct0 * 16 < n_cols; ct0 += p.n_ct) {
     // Nearly always the only round: what depends on the lane is worked out in it,
@@ -182,7 +214,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_token_kernel(Params p) {
     auto token_of = [&](int col) { return static_cast<int>(p.maps.divide(col)); };
     auto map_of = [&](int col) { return static_cast<int>(p.maps.remainder(col)); };
     const int64_t row0 = seq.n0 * a.S + col0;
-    const int limit = visible_to(seq, token_of(col0 + n_used - 1), a.causal);
+    const int limit = visible_to(seq, token_of(col0 + n_used - 1), a.causal), all_see = visible_to(seq, token_of(col0), a.causal);
     const int n_kt = (limit + 31) / 32;
     const int kt0 = min(n_kt, split * p.per), kt1 = split == p.n_split - 1 ? n_kt : min(n_kt, kt0 + p.per);
     if (split > 0 && kt0 == kt1) {   // nothing left for this part
@@ -213,6 +245,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_token_kernel(Params p) {
     const int vis = visible_to(seq, token_of(own_col), a.causal);
     const float sc = score_scale(a, map_of(own_col));
     float m_run = kNoScore, l_part = 0.f;
+    for (int i = lane; i < DBW * 16; i += 64) firsts[i] = kNoToken;
+    bool taken = false;   // some value was taken out
 
     // Addresses are a uniform base and a lane's 32-bit offset.  Block h of the
     // scores has token 8 (c / 4) + 4 h + c % 4 in row c.  Where there is no tile
@@ -327,19 +361,24 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_token_kernel(Params p) {
       const char* probs = ps + buf * NW * 1024 + lane * 16;
 #pragma unroll
       for (int t = 0; t < NW; ++t) {
-        const int page_t = __builtin_amdgcn_readlane(pages, t);
-        const int live_t = page_t < 0 ? 0 : min(32, limit - (base + t) * 32);
+        const int page_t = __builtin_amdgcn_readlane(pages, t), at = (base + t) * 32;
         v8 vv[DBW];
-        if (live_t == 32) {
+        if (page_t >= 0 && at + 32 <= all_see) {
 #pragma unroll
           for (int j = 0; j < DBW; ++j) vv[j] = __builtin_bit_cast(v8, vf[t & 1][j]);
         } else {   // what lies behind the last token is not multiplied: it may hold anything
+          const int live_t = page_t < 0 ? 0 : min(32, limit - at);
+          const int c = opaque(tid) & 15, g = (opaque(tid) & 63) >> 4;
           u32x4 keep;
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             keep[e] = (8 * g + 2 * e < live_t ? 0xffffu : 0u) | (8 * g + 2 * e + 1 < live_t ? 0xffff0000u : 0u);
 #pragma unroll
-          for (int j = 0; j < DBW; ++j) vv[j] = __builtin_bit_cast(v8, vf[t & 1][j] & keep);
+          for (int j = 0; j < DBW; ++j) {
+            u32x4 v = vf[t & 1][j] & keep;
+            if (at + live_t > all_see) taken |= take_out<TV>(v, firsts + 16 * j + c, at + 8 * g);
+            vv[j] = __builtin_bit_cast(v8, v);
+          }
         }
         const v8 pv = *reinterpret_cast<const v8*>(probs + t * 1024);
 #pragma unroll
@@ -365,6 +404,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_token_kernel(Params p) {
 #pragma unroll
     for (int w = 0; w < NW; ++w) l += ls[w * 16 + c];
     const int64_t row = row0 + c;
+    if (taken) {
+#pragma unroll
+      for (int j = 0; j < DBW; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (vis > firsts[16 * j + 4 * g + e]) acc[j][e] = __builtin_nanf("");
+    }
     if (wave == 0 && g == 0 && slice == 0) {
       if (p.part_o) {
         p.part_m[split * p.rows + row] = m_run;
@@ -409,7 +455,8 @@ struct ChunkLds {   // bytes
   static constexpr int MOVED = OWN + kChunkWaves * 64 * CT;         // [2][waves] ints
   static constexpr int QUERIES = MOVED + 2 * kChunkWaves * 4;       // [CT][2 NK][64 lanes] 16 bytes
   static constexpr int PROBS = QUERIES + 2 * NK * CT * 1024;        // [2][tiles][CT][64 lanes] 16 bytes
-  static constexpr int BYTES = PROBS + 2 * kChunkTiles * CT * 1024;
+  static constexpr int FIRSTS = PROBS + 2 * kChunkTiles * CT * 1024; // [waves][4 blocks][16] ints: see take_out
+  static constexpr int BYTES = FIRSTS + kChunkWaves * 4 * 64;
 };
 
 template <typename TQ, typename TV, int NK, int DBW, int CT>
@@ -447,6 +494,7 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(Params
   float* own = reinterpret_cast<float*>(lds + Lds::OWN) + wave * 16 * CT;
   int* sees = reinterpret_cast<int*>(lds + Lds::SEES);
   int* moved = reinterpret_cast<int*>(lds + Lds::MOVED);
+  int* firsts = reinterpret_cast<int*>(lds + Lds::FIRSTS) + wave * DBW * 16;
 
   for (int ct0 = member; ct0 * 16 * CT < seq.rows; ct0 += p.n_ct) {
     const int tid = opaque(static_cast<int>(threadIdx.x));   // as above
@@ -485,6 +533,8 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(Params
       refs[i] = kNoScore;
     }
     for (int i = lane; i < 16 * CT; i += 64) own[i] = kNoScore;
+    for (int i = lane; i < 16 * DBW; i += 64) firsts[i] = kNoToken;
+    bool taken = false;   // some value was taken out
 
     // Addresses as above.
     const uint32_t key_lane = static_cast<uint32_t>(((8 * (c >> 2) + 4 * wh + (c & 3)) * W + 8 * g) * 2);
@@ -635,7 +685,7 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(Params
 #pragma unroll
       for (int t = 0; t < TS; ++t) {
         const int page_t = __builtin_amdgcn_readlane(pages, t);
-        const int live_t = page_t < 0 ? 0 : min(32, limit - (base + t) * 32);
+        const int at = (base + t) * 32, live_t = page_t < 0 ? 0 : min(32, limit - at);
         u32x4(&v)[DBW] = vf[t & 1];
         if (live_t < 32) {   // what lies behind the last token is not multiplied: it may hold anything
           const int g = (opaque(tid) & 63) >> 4;
@@ -645,6 +695,11 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(Params
             keep[e] = (8 * g + 2 * e < live_t ? 0xffffu : 0u) | (8 * g + 2 * e + 1 < live_t ? 0xffff0000u : 0u);
 #pragma unroll
           for (int j = 0; j < DBW; ++j) v[j] &= keep;
+        }
+        if (live_t > 0 && at + live_t > all_see) {
+          const int c = opaque(tid) & 15, g = (opaque(tid) & 63) >> 4;
+#pragma unroll
+          for (int j = 0; j < DBW; ++j) taken |= take_out<TV>(v[j], firsts + 16 * j + c, at + 8 * g);
         }
 #pragma unroll
         for (int i = 0; i < CT; ++i) {
@@ -685,6 +740,13 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(Params
       for (int w = 0; w < NW; ++w) l += ls[w * 16 * CT + col];
       const float m = refs[col];
       const int64_t row = row_of(min(col, n_used - 1));
+      if (taken) {
+#pragma unroll
+        for (int j = 0; j < DBW; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            acc[i][j][e] = sees[col] > firsts[16 * j + 4 * g + e] ? __builtin_nanf("") : acc[i][j][e];
+      }
       if (wave == 0 && g == 0 && slice == 0 && col < n_used) {
         if (p.part_o) {
           p.part_m[split * p.rows + row] = m;
@@ -906,7 +968,7 @@ Plan plan(const PagedAttentionArgs& a) {
 template <typename TQ, typename TV, int DBW>
 void launch_token(const Params& p, hipStream_t stream) {
   const int QP = static_cast<int>(round_up(p.a.cache.W, 64 * kTokenGroups)) + 8;
-  const size_t lds = static_cast<size_t>(32) * QP + 2 * kWaves * (1024 + 64 + 4);
+  const size_t lds = static_cast<size_t>(32) * QP + 2 * kWaves * (1024 + 64 + 4) + kWaves * DBW * 64;
   const unsigned units = static_cast<unsigned>(round_up(p.units, kXcds));
   hipLaunchKernelGGL((paged_token_kernel<TQ, TV, DBW>), dim3(units * p.members.d), dim3(64 * kWaves), lds, stream, p);
 }

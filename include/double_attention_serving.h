@@ -68,9 +68,9 @@ int da_cache_append(const da_paged_cache* cache, const void* key, int64_t ldk, c
  * over the maps with these weights, [rows, value_dim].  Rows that see nothing,
  * and rows of no sequence, are zero.  Scores, the softmax and sums are fp32;
  * probabilities are rounded to v_dtype for the product with the values, and the
- * result once.  Where a row sees a token whose value holds an infinity or a
- * NaN, the 15 rows and maps next to it that see any of that token's tile of 32
- * may have NaN too; what lies behind a sequence's last token reaches nothing.
+ * result once.  A value that is an infinity or a NaN makes its feature one in the
+ * rows that see its token, and in no other; what lies behind a sequence's last
+ * token reaches nothing.
  * Types: (qk_dtype, v_dtype) in (F16, BF16), (F16, F16), (BF16, BF16).
  *
  * weights_out (NULL: none) [sequences] rows of table_pages * page_size fp32, ld_weights apart:

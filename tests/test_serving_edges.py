@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import double_attention as da
-from test_serving_ops import F32, close, half_step, score_tolerance
+from test_serving_ops import F32, TYPES, Setup, close, half_step, scales_of, score_tolerance
 
 # ---- the gradient of log probabilities ---------------------------------------
 
@@ -72,3 +72,43 @@ def test_gradient_of_special_rows(vocab, dtype) -> None:
     x[7] = low / 2
     tokens = torch.randint(0, 3, (8,), generator=torch.Generator().manual_seed(1)).cuda()
     check_gradient(x.to(dtype).cuda(), tokens, 2)
+
+
+# ---- infinities and NaN in the cache -----------------------------------------
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("lengths,chunks,layout,value_dim,mixed", [
+    pytest.param([90, 40], [40, 3], (1, 1, 64), 64, False, id="few"),
+    pytest.param([700, 40], [20, 1], (2, 2, 128), 320, True, id="few-in-parts"),
+    pytest.param([700, 40], [20, 1], (1, 2, 64), 1088, False, id="few-in-slices"),
+    pytest.param([640, 40], [600, 1], (1, 1, 64), 192, False, id="chunk"),
+    pytest.param([2000, 40], [530, 1], (2, 2, 192), 576, True, id="chunk-in-parts"),
+    pytest.param([700, 40], [640, 40], (1, 1, 512), 64, False, id="chunk-of-wide-keys"),
+])
+def test_a_value_reaches_the_rows_that_see_it(lengths, chunks, layout, value_dim, mixed, types, bad) -> None:
+    branches, maps, routing_dim = layout
+    s = Setup(lengths, chunks, branches, routing_dim, value_dim, 32, types)
+    scales = scales_of(maps)
+    mix = torch.softmax(torch.arange(maps, dtype=torch.float32), 0) if mixed else None
+    expected, tolerance, weights, w_tolerance = s.exact(scales, True, mix)
+    length, new = lengths[0], chunks[0]
+    # New tokens at and off the tiles' borders, an old one, and the last one.
+    for position in sorted({length - new - 1, length - new + 1, (length - new) // 32 * 32 + 32, length - 9, length - 1} & set(range(length))):
+        feature = (position * 7) % value_dim
+        at = (int(s.table[0, position // 32]), 0, feature, position % 32)
+        held = s.cache.values[at].clone()
+        s.cache.values[at] = bad
+        got, gathered = da.paged_attention_weights_hip(*s.where(), scales.cuda(), mix=None if mix is None else mix.cuda(),
+                                                       max_chunk=max(chunks))
+        s.cache.values[at] = held
+        got = got.cpu()
+        seen = torch.zeros(s.total, dtype=torch.bool)
+        seen[max(0, position - (length - new)):new] = True
+        assert not got[seen][..., feature].isfinite().any()
+        there = torch.zeros_like(got, dtype=torch.bool)
+        there[seen, ..., feature] = True
+        close(torch.where(there, 0, got), torch.where(there, 0.0, expected), tolerance)
+        close(gathered.cpu(), weights, w_tolerance)
