@@ -304,12 +304,44 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_token_kernel(Params p) {
         scores(pass);
       }
       const int seen = min(live, vis - kt * 32) - 8 * g;   // of this lane's eight tokens
-      float mx = -INFINITY;
+      float mx, sum;
+      auto scaled = [&] {
+        mx = -INFINITY;
+        sum = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float s = e < seen ? st[e >> 2][e & 3] * sc : -INFINITY;
-        st[e >> 2][e & 3] = s;
-        mx = fmaxf(mx, s);
+        for (int e = 0; e < 8; ++e) {
+          const float s = e < seen ? st[e >> 2][e & 3] * sc : -INFINITY;
+          st[e >> 2][e & 3] = s;
+          mx = fmaxf(mx, s);
+          sum += s;
+        }
+      };
+      scaled();
+      if (__ballot(sum != sum)) {
+        // An infinity or a NaN among another map's features makes a score NaN, times
+        // this map's zeros there: each map's features alone, and each lane's own sum.
+        const char* base = uniform_ptr(static_cast<const char*>(cache.keys) +
+                                       (max(page, 0) * cache.key_page + static_cast<int64_t>(tile_of(cache, kt)) * 32 * W) * 2);
+        const int c = opaque(tid) & 15, g = (opaque(tid) & 63) >> 4;
+        const int own = static_cast<int>(p.repeats.divide(map_of(col0 + min(c, n_used - 1))));
+        f32x4 mine[2] = {zero4(), zero4()};
+#pragma nounroll
+        for (int r = 0; r < a.S / a.repeat; ++r) {
+          f32x4 part[2] = {zero4(), zero4()};
+#pragma nounroll
+          for (int f = r * a.RP; f < (r + 1) * a.RP; f += 32) {
+            const q8 qf = load8(qs + c * QP + f + 8 * g);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) part[h] = Elem<TQ>::mma(__builtin_bit_cast(q8, load_at(base + 2 * f + h * 8 * W, key_lane)), qf, part[h]);
+          }
+          if (r == own) {
+            mine[0] = part[0];
+            mine[1] = part[1];
+          }
+        }
+        st[0] = mine[0];
+        st[1] = mine[1];
+        scaled();
       }
       // The reference moves, to a whole number (so that what it scales stays
       // exact), where a score exceeds it by more than kRescaleSlack.

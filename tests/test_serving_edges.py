@@ -112,3 +112,38 @@ def test_a_value_reaches_the_rows_that_see_it(lengths, chunks, layout, value_dim
         there[seen, ..., feature] = True
         close(torch.where(there, 0, got), torch.where(there, 0.0, expected), tolerance)
         close(gathered.cpu(), weights, w_tolerance)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("lengths,chunks,layout", [
+    pytest.param([90, 40], [40, 3], (2, 2, 64), id="few"),
+    pytest.param([90, 40], [9, 3], (4, 4, 128), id="few-of-512"),
+    pytest.param([300, 40], [9, 3], (4, 2, 192), id="few-of-768"),
+    pytest.param([90, 40], [3, 1], (2, 4, 64), id="few-shared"),
+    pytest.param([640, 40], [600, 1], (2, 2, 64), id="chunk"),
+])
+def test_a_key_reaches_the_rows_and_maps_that_see_it(lengths, chunks, layout, types) -> None:
+    branches, maps, routing_dim = layout
+    s = Setup(lengths, chunks, branches, routing_dim, 128, 32, types)
+    scales = scales_of(maps)
+    expected, tolerance, weights, w_tolerance = s.exact(scales)
+    length, new = lengths[0], chunks[0]
+    for bad in (math.nan, math.inf, -math.inf):
+        for position in (length - new + 1, length - 1):
+            branch = branches - 1
+            at = (int(s.table[0, position // 32]), position % 32, branch, 5)
+            held = s.cache.keys[at].clone()
+            s.cache.keys[at] = bad
+            got, gathered = da.paged_attention_weights_hip(*s.where(), scales.cuda(), max_chunk=max(chunks))
+            s.cache.keys[at] = held
+            got = got.cpu()
+            seen = torch.zeros(s.total, dtype=torch.bool)
+            seen[position - (length - new):new] = True
+            touched = torch.arange(maps) * branches // maps
+            touched = (touched <= branch) & (branch < touched + max(1, branches // maps))
+            there = (seen[:, None] & touched)[..., None].expand_as(got)
+            if math.isnan(bad):
+                assert got[there].isnan().all()
+            close(torch.where(there, 0, got), torch.where(there, 0.0, expected), tolerance)
+            close(gathered[1:].cpu(), weights[1:], w_tolerance[1:])
