@@ -34,7 +34,19 @@ constexpr int kWaves = 4;
 constexpr int kTokenGroups = 4;       // of 64 key features, at a time
 constexpr int kMaxSplits = 256;
 constexpr int kWantWorkgroups = 1024, kChunkWorkgroups = 256;
-constexpr float kNoScore = -3.0e38f;  // the running maximum before the first score
+constexpr float kNoScore = -3.0e38f;  // the running reference before the first score
+
+// A running reference is a whole number (log2); it moves where a score exceeds it
+// by more than SLACK, to BELOW under that rounded up.  Probabilities beside it are
+// rounded to the values' type, relative to their size in bf16, but by up to 2^-25 in
+// fp16, below 2^-14: there the reference stays low, so that the largest ones are
+// between 2^6 and 2^15.  At BELOW 0, 131072 tokens of 2^-25.1 beside one of 1 were all
+// lost (0.4% of the sum); now what the rounding adds up to is below 2^-31 a token.
+template <typename TV>
+struct Reference {
+  static constexpr bool wide = std::is_same<TV, __bf16>::value;
+  static constexpr float BELOW = wide ? 0.f : 7.f, SLACK = wide ? kRescaleSlack : 15.f;
+};
 
 // Division of numbers below 2^23 by a divisor up to 2^16, by a product (the
 // quotient of n and d is the whole part of n m / 2^40 with m = ceil(2^40 / d):
@@ -343,12 +355,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_token_kernel(Params p) {
         st[1] = mine[1];
         scaled();
       }
-      // The reference moves, to a whole number (so that what it scales stays
-      // exact), where a score exceeds it by more than kRescaleSlack.
+      // What a moving reference scales stays exact (but for fp16 probabilities that
+      // fall below 2^-14).
       float m = m_run;
-      if (__ballot(mx > m + kRescaleSlack)) {
+      if (__ballot(mx > m + Reference<TV>::SLACK)) {
         const float tile_max = group_max(mx);
-        if (tile_max > m + kRescaleSlack) m = __builtin_ceilf(tile_max);
+        if (tile_max > m + Reference<TV>::SLACK) m = __builtin_ceilf(tile_max) - Reference<TV>::BELOW;
         any = true;
       }
       float l = 0.f;
@@ -475,9 +487,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_token_kernel(Params p) {
 // for all columns, with its keys in registers and the queries in LDS, and
 // leaves its probabilities in LDS; after a barrier every wave multiplies them
 // with its own DBW blocks of the values, straight from memory.
-// Where a score exceeds the reference that all waves share by more than
-// kRescaleSlack a wave raises its own, and the waves agree on the largest behind
-// the barrier.
+// Where a score exceeds the reference that all waves share by too much a wave
+// raises its own, and the waves agree on the largest behind the barrier.
 constexpr int kChunkWaves = 8, kChunkTiles = 4;
 template <int NK, int CT>
 struct ChunkLds {   // bytes
@@ -646,11 +657,9 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(Params
 #pragma unroll
           for (int e = 0; e < 4; ++e) x[e] = masked && e >= seen ? -INFINITY : st[u][e] * sc;
           const float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-          // The reference moves, to a whole number (so that what it scales stays
-          // exact), where a score exceeds it by more than kRescaleSlack.
-          if (__ballot(mx > m + kRescaleSlack)) {
+          if (__ballot(mx > m + Reference<TV>::SLACK)) {   // as above
             const float before = m, most = group_max(mx);
-            if (most > m + kRescaleSlack) m = __builtin_ceilf(most);
+            if (most > m + Reference<TV>::SLACK) m = __builtin_ceilf(most) - Reference<TV>::BELOW;
             own[col] = m;
             l_part[i + u] *= __builtin_amdgcn_exp2f(before - m);
             raises = true;

@@ -147,3 +147,40 @@ def test_a_key_reaches_the_rows_and_maps_that_see_it(lengths, chunks, layout, ty
                 assert got[there].isnan().all()
             close(torch.where(there, 0, got), torch.where(there, 0.0, expected), tolerance)
             close(gathered[1:].cpu(), weights[1:], w_tolerance[1:])
+
+
+# ---- probabilities at the lower end of fp16 ----------------------------------
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("below", [23.4, 24.6, 25.1, 27.0])
+@pytest.mark.parametrize("chunk,length", [(1, 131072), (600, 16384)])
+def test_a_long_flat_tail_beside_one_token_in_fp16(chunk, length, below) -> None:
+    """One token of probability near one and value zero, and all others 2^-below
+    of it with value one: what the tail has together is not lost or rounded up."""
+
+    device = torch.device("cuda")
+    # A scale of below / log2(e): the first key is the query, the others are half of
+    # it beside a query of length two.
+    keys = torch.zeros(length // 64, 64, 1, 64, dtype=torch.float16, device=device)
+    keys[..., 0] = 0.5
+    keys[0, 0, 0, 0] = 1.0
+    values = torch.ones(length // 64, 2, 64, 32, dtype=torch.float16, device=device)
+    values[0, 0, :, 0] = 0.0
+    query = torch.zeros(chunk, 1, 64, dtype=torch.float16, device=device)
+    query[..., 0] = 2.0
+    table = torch.arange(length // 64, dtype=torch.int32, device=device)[None]
+    lengths = torch.tensor([length], dtype=torch.int32, device=device)
+    offsets = torch.tensor([0, chunk], dtype=torch.int32, device=device)
+    scale = torch.tensor([below * math.log(2.0)])
+    # One part for all tokens (a part has a reference of its own).
+    got = da.paged_attention_hip(query, da.PagedCache(keys, values), table, lengths, offsets, scale.to(device), max_chunk=chunk, max_length=1)
+    each = math.exp(-float(scale.double()))
+    tail = each * (torch.arange(length - chunk, length, dtype=torch.float64))
+    expected = (tail / (1 + tail))[:, None, None].expand(chunk, 1, 64)
+    # A probability is off by half a step of fp16, or by 2^-25 where it is below
+    # the normal range; the reference lies more than 6 below the largest score, so
+    # that its probability is more than 2^6 beside that.  Scores of up to 54 (log2)
+    # are off by three roundings each.
+    tolerance = expected * (2 * half_step(torch.float16) + 2.0 ** -17) + length * 2.0 ** -25 / 2 ** 6 + 2.0 ** -25
+    close(got.cpu(), expected, tolerance)
