@@ -976,13 +976,15 @@ Plan plan(const PagedAttentionArgs& a) {
   Plan r;
   // Measured over 2000 cached tokens (us, columns of one map / all maps): 32
   // sequences of 64 tokens 59 / 56, of 128 73 / 90; on two maps 32 tokens 68 /
-  // 91, on four 130 / 141; one sequence of 128 tokens 37 / 20.
-  r.one = a.max_chunk >= 32 && a.max_chunk * a.S >= 64 && a.tokens.N * a.S >= 512;
+  // 91, on four 130 / 141; one sequence of 128 tokens 37 / 20.  A launch has fewer
+  // than 2^32 threads.
+  const int most = 512;   // features of a workgroup
+  r.n_slices = (a.cache.D + most - 1) / most;
+  r.one = a.max_chunk >= 32 && a.max_chunk * a.S >= 64 && a.tokens.N * a.S >= 512 &&
+          static_cast<int64_t>(a.tokens.B) * r.n_slices * a.S < (1 << 22);
   r.ct = r.one ? a.RP <= 256 ? 8 : 4 : 1;
   r.nw = r.one ? 8 : 4;
   const int64_t cols = static_cast<int64_t>(std::max(a.max_chunk, 1)) * (r.one ? 1 : a.S);
-  const int most = 512;   // features of a workgroup
-  r.n_slices = (a.cache.D + most - 1) / most;
   r.dbw = (a.cache.D + r.n_slices * 16 * r.nw - 1) / (r.n_slices * 16 * r.nw);
   const int per_ct = r.n_slices * (r.one ? a.S : 1);
   r.n_ct = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((cols + 16 * r.ct - 1) / (16 * r.ct), 16384 / (a.tokens.B * per_ct) + 1)));

@@ -184,3 +184,26 @@ def test_a_long_flat_tail_beside_one_token_in_fp16(chunk, length, below) -> None
     # are off by three roundings each.
     tolerance = expected * (2 * half_step(torch.float16) + 2.0 ** -17) + length * 2.0 ** -25 / 2 ** 6 + 2.0 ** -25
     close(got.cpu(), expected, tolerance)
+
+
+# ---- launches --------------------------------------------------------------------
+
+
+@pytest.mark.gpu
+def test_many_sequences_of_many_maps_and_wide_values() -> None:
+    """One token of each of 16384 sequences, 64 maps, 4096 value features, without a
+    word on the chunks: workgroups for a chunk of each would be 2^32 threads."""
+
+    if torch.cuda.mem_get_info()[0] < 20 << 30:
+        pytest.skip("needs 20 GiB")
+    sequences, maps, page = 16384, 64, 32
+    g = torch.Generator().manual_seed(0)
+    cache = da.PagedCache(torch.randn(2, page, 1, 64, generator=g).half().cuda() / 8, torch.randn(2, 1, 4096, 32, generator=g).bfloat16().cuda())
+    table = (torch.arange(sequences, dtype=torch.int32) % 2)[:, None].cuda()
+    lengths = torch.full((sequences,), page, dtype=torch.int32, device="cuda")
+    offsets = torch.arange(sequences + 1, dtype=torch.int32, device="cuda")
+    query = torch.randn(2, 1, 64, generator=g).half().cuda().repeat(sequences // 2, 1, 1)
+    scales = scales_of(maps, 1.0).cuda()
+    got = da.paged_attention_hip(query, cache, table, lengths, offsets, scales)
+    two = da.paged_attention_hip(query[:2], cache, table[:2], lengths[:2], offsets[:3], scales)
+    assert bool(two.any()) and torch.equal(got.view(sequences // 2, 2, maps, 4096), two.expand(sequences // 2, 2, maps, 4096))
