@@ -121,7 +121,7 @@ def _check_cache(what: str, cache: PagedCache) -> torch.device:
     if not (keys.is_contiguous() and values.is_contiguous()) and (
         keys.stride()[1:] != (branches * routing_dim, routing_dim, 1)
         or values.stride()[1:] != (value_shape[2] * CACHE_TILE, CACHE_TILE, 1)
-    ):
+    ) and not (keys[0].is_contiguous() and values[0].is_contiguous()):   # (dimensions of size one have any stride)
         raise ValueError(f"{what}: a cache's pages are contiguous")
     return keys.device
 

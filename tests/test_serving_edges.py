@@ -207,3 +207,22 @@ def test_many_sequences_of_many_maps_and_wide_values() -> None:
     got = da.paged_attention_hip(query, cache, table, lengths, offsets, scales)
     two = da.paged_attention_hip(query[:2], cache, table[:2], lengths[:2], offsets[:3], scales)
     assert bool(two.any()) and torch.equal(got.view(sequences // 2, 2, maps, 4096), two.expand(sequences // 2, 2, maps, 4096))
+
+
+# ---- views ----------------------------------------------------------------------
+
+
+@pytest.mark.gpu
+def test_pages_of_one_branch_or_tile_with_any_stride_there() -> None:
+    """The stride of a dimension of size one says nothing about the memory."""
+
+    s = Setup([70, 33], [3, 1], 1, 64, 128, 32)
+    pages = s.cache.keys.shape[0]
+    keys = torch.full((pages, 3, 1, 32, 64), math.nan, dtype=torch.float16, device="cuda").transpose(2, 3)[:, 1]
+    values = torch.full((pages, 2, 128, 1, 32), math.nan, dtype=torch.bfloat16, device="cuda").transpose(2, 3)[:, 0]
+    keys.copy_(s.cache.keys)
+    values.copy_(s.cache.values)
+    assert keys.stride()[1:] == (64, 2048, 1) and values.stride()[1:] == (32, 32, 1)
+    expected, tolerance, _, _ = s.exact(scales_of(1))
+    got = da.paged_attention_hip(s.query, da.PagedCache(keys, values), *s.where()[2:], scales_of(1).cuda())
+    close(got.cpu(), expected, tolerance)
