@@ -13,7 +13,7 @@ import torch
 from torch import Tensor
 
 from .modules import DoubleAttentionLM
-from .serving_ops import cache_compact_hip, cache_select_hip
+from .serving_ops import PagedCache, cache_compact_hip, cache_select_hip
 
 
 class CachedSequences:
@@ -127,8 +127,9 @@ class CachedSequences:
     def evict(self, keep: int, recent: int = 0) -> None:
         """Cuts every sequence of more than ``keep`` tokens, in each layer by itself,
         to its last ``recent`` tokens and those of the others that gathered the
-        largest weights.  Their pages are freed after the kept tokens have moved
-        into free ones, which must be there."""
+        largest weights.  The kept tokens move into free pages, of as many
+        sequences at a time as those take, whose own pages become free; where
+        none are left for one sequence, through temporary memory."""
 
         if self.weights is None:
             raise RuntimeError("evict: the sequences were made without gather_weights")
@@ -138,23 +139,39 @@ class CachedSequences:
         if not cut:
             return
         each = self._count(keep)
-        if each * len(cut) > len(self._free):
-            raise RuntimeError(f"evict: needs {each * len(cut)} free pages, {len(self._free)} are free")
-        # Pages of the sequences that stay whole are not named: nothing of theirs moves.
-        taken = self._last_free(each * len(cut))
-        moved_to: list[list[int]] = [[] for _ in self._pages]
-        for b in cut:
-            moved_to[b] = [next(taken) for _ in range(each)]
-        table, new_table = self._table(self._pages), self._table(moved_to)
+        # The rounds' page tables: before, after, and of the temporary pages.  Pages
+        # of the sequences that stay in a round are not named: nothing of theirs moves.
+        pages, free, rounds = list(self._pages), list(self._free), []
+        waiting = cut
+        while waiting:
+            fit = len(free) // each
+            group, waiting = waiting[:max(1, fit)], waiting[max(1, fit):]
+            after: list[list[int]] = [[] for _ in pages]
+            for b in group:
+                after[b] = [free.pop() for _ in range(each)] if fit else pages[b][:each]
+            through = None if fit else self._table([list(range(len(row))) for row in after])
+            rounds.append((self._table(pages), self._table(after), through))
+            for b in group:
+                free.extend(reversed(pages[b] if fit else pages[b][each:]))
+                pages[b] = after[b]
         lengths = torch.tensor(self.lengths, dtype=torch.int32).to(self._device)
-        for cache, weights, out in zip(self.caches, self.weights, self._next_weights):
-            kept, counts = cache_select_hip(weights, lengths, keep, recent)
-            out.copy_(cache_compact_hip(cache, table, kept, counts, cache, new_table, weights=weights))
-        # Nothing below raises.
-        del self._free[len(self._free) - each * len(cut):]
+        chosen = [cache_select_hip(weights, lengths, keep, recent) for weights in self.weights]
+        if any(through is not None for *_, through in rounds):
+            temporary = [PagedCache(*(t.new_empty(each, *t.shape[1:]) for t in cache)) for cache in self.caches]
+            in_order = torch.arange(keep, dtype=torch.int32, device=self._device).repeat(len(pages), 1)
+        for n, (table, new_table, through) in enumerate(rounds):
+            for layer, (cache, (kept, counts)) in enumerate(zip(self.caches, chosen)):
+                out, to = (cache, new_table) if through is None else (temporary[layer], through)
+                if n == 0:   # the last that needs memory; no page of a sequence has been written yet
+                    moved = cache_compact_hip(cache, table, kept, counts, out, to, weights=self.weights[layer])
+                    self._next_weights[layer].copy_(moved)
+                else:
+                    cache_compact_hip(cache, table, kept, counts, out, to)
+            if through is not None:
+                for cache, held, (_, counts) in zip(self.caches, temporary, chosen):
+                    cache_compact_hip(held, through, in_order, counts, cache, new_table)
+        self._pages, self._free = pages, free
         for b in cut:
-            self._free.extend(reversed(self._pages[b]))
-            self._pages[b] = moved_to[b]
             self.lengths[b] = keep
         self.weights, self._next_weights = self._next_weights, self.weights
 

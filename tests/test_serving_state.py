@@ -117,9 +117,10 @@ def filled(sequences, pages, counts, monkeypatch, gather=True):
     return s
 
 
+@pytest.mark.parametrize("pages", [14, 8])
 @pytest.mark.parametrize("fails", [0, 1, 2, 3])
-def test_an_eviction_that_raises_changes_nothing(fails, monkeypatch) -> None:
-    s = filled(3, 14, [100, 20, 70], monkeypatch)
+def test_an_eviction_that_raises_changes_nothing(fails, pages, monkeypatch) -> None:
+    s = filled(3, pages, [100, 20, 70], monkeypatch)
     before = state_of(s)
     rows = [[[t.clone() for t in c.rows(s.pages(b), n)] for b, n in enumerate(s.lengths)] for c in s.caches]
     calls = iter(range(100))
@@ -142,7 +143,7 @@ def test_an_eviction_that_raises_changes_nothing(fails, monkeypatch) -> None:
         for b, n in enumerate(s.lengths):
             assert all(torch.equal(*pair) for pair in zip(cache.rows(s.pages(b), n), of_layer[b]))
     s.evict(40, 8)
-    assert s.lengths == [40, 20, 40] and sorted(sum(s._pages, s._free)) == list(range(14))
+    assert s.lengths == [40, 20, 40] and sorted(sum(s._pages, s._free)) == list(range(pages))
 
 
 def test_refusals_of_a_second_buffer_of_weights() -> None:
@@ -177,3 +178,60 @@ def test_a_failed_forward_can_be_made_again(monkeypatch) -> None:
     weights = s.weights.clone()
     s.extend(chunk[:0], [0, 0])   # no new token: nothing gathered
     assert torch.equal(s.weights, weights)
+
+
+def check_eviction(s, keep, recent, select) -> None:
+    """The pages hold what ``select`` chose before, and every page has one owner."""
+
+    lengths, pages = list(s.lengths), len(sum(s._pages, s._free))
+    rows = [[[t.clone() for t in c.rows(s.pages(b), n)] for b, n in enumerate(lengths)] for c in s.caches]
+    weights = s.weights.clone()
+    on_device = torch.tensor(lengths, dtype=torch.int32, device=weights.device)
+    chosen = [select(w.contiguous(), on_device, keep, recent) for w in weights]
+    positions = list(s.positions)
+    s.evict(keep, recent)
+    assert s.lengths == [min(n, keep) for n in lengths] and s.positions == positions
+    assert sorted(sum(s._pages, s._free)) == list(range(pages))
+    assert [len(p) for p in s._pages] == [-(-n // s.page_size) for n in s.lengths]
+    for layer, cache in enumerate(s.caches):
+        kept, counts = chosen[layer]
+        for b, n in enumerate(s.lengths):
+            assert int(counts[b]) == n
+            stays = kept[b, :n].long()
+            got = cache.rows(s.pages(b), n)
+            assert all(torch.equal(t, before[stays]) for t, before in zip(got, rows[layer][b]))
+            expected = torch.zeros_like(weights[layer, b])
+            expected[:n] = weights[layer, b][stays]
+            assert torch.equal(s.weights[layer, b], expected)
+
+
+# 12 pages for sequences of 4, 1, 3 and 4 pages, cut to two pages each: none free,
+# one too few for a sequence, for two and for all at once; and a page that a cut
+# sequence keeps all of.
+@pytest.mark.parametrize("pages,keep,recent", [(12, 40, 8), (13, 40, 8), (14, 40, 0), (17, 40, 40), (20, 40, 8), (12, 96, 3), (12, 64, 1),
+                                               (12, 1, 0), (13, 33, 2), (12, 127, 0)])
+def test_pools_without_room_are_cut(pages, keep, recent, monkeypatch) -> None:
+    check_eviction(filled(4, pages, [100, 20, 70, 128], monkeypatch), keep, recent, plain_select)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pages", [12, 13, 16])
+def test_pools_without_room_are_cut_on_the_device(pages) -> None:
+    model = model_of("two-maps").cuda()
+    s = da.CachedSequences(model, 4, pages, page_size=32, gather_weights=True)
+    s.extend(torch.cat(ids(100, 20, 70, 127)), [100, 20, 70, 127])
+    s.extend(torch.cat(ids(0, 1, 0, 1, seed=1)), [0, 1, 0, 1])
+    check_eviction(s, 40, 8, da.cache_select_hip)
+    other = da.CachedSequences(model, 4, pages, page_size=32, gather_weights=True)
+    other._pages, other._free = [list(p) for p in s._pages], list(s._free)
+    other.lengths, other.positions, other.weights = list(s.lengths), list(s.positions), s.weights.clone()
+    for mine, theirs in zip(other.caches, s.caches):
+        mine.keys.copy_(theirs.keys)
+        mine.values.copy_(theirs.values)
+    # What was left behind in the pages reaches nothing.
+    for cache in other.caches:
+        for p in other._free:
+            cache.keys[p] = float("nan")
+            cache.values[p] = float("nan")
+    tokens = torch.cat(ids(3, 1, 0, 2, seed=2))
+    assert torch.equal(s.extend(tokens, [3, 1, 0, 2]), other.extend(tokens, [3, 1, 0, 2]))
