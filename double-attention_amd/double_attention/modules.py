@@ -1528,6 +1528,8 @@ class DoubleAttentionLM(nn.Module):
             weights_out = weights
         elif weights is None or weights_out.shape != weights.shape or not weights_out.is_contiguous():
             raise ValueError("cached_forward: weights_out must be contiguous, of the shape of weights")
+        elif 0 < abs(weights_out.data_ptr() - weights.data_ptr()) < weights.numel() * weights.element_size():
+            raise ValueError("cached_forward: weights_out must be weights, or apart from them")   # a layer's reach the next
         x = self.token_embedding(token_ids) + self.position_embedding(positions)
         stack = self.stack
         # All layers' at once: fewer launches.  fp32 temperatures, as the fused

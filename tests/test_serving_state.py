@@ -151,7 +151,9 @@ def test_refusals_of_a_second_buffer_of_weights() -> None:
     token, ends = torch.zeros(1, dtype=torch.int64), torch.tensor([0, 1], dtype=torch.int32)
     where = (token, token, model.paged_caches(2, 32), torch.zeros(1, 1, dtype=torch.int32), ends[1:], ends)
     weights = torch.zeros(2, 1, 32)
-    for first, second in ((None, weights), (weights, weights[:1]), (weights, torch.zeros(2, 1, 64)[..., ::2])):
+    both = torch.zeros(3, 1, 32)
+    for first, second in ((None, weights), (weights, weights[:1]), (weights, torch.zeros(2, 1, 64)[..., ::2]), (both[:2], both[1:]),
+                          (both[1:], both[:2])):
         with pytest.raises(ValueError, match="weights_out"):
             model.cached_forward(*where, weights=first, weights_out=second)
 
