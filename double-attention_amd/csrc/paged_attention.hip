@@ -174,7 +174,7 @@ __device__ void clear_other_rows(const PagedAttentionArgs& a, int64_t wg, int64_
 // so that a step has one barrier.
 //
 // Bound by the cache's bytes: 64 sequences of up to 4096 tokens (keys of 256, values of
-// 512 features, 254 MB) 51 us with the merge, one of 131072 tokens (201 MB) 41 us.
+// 512 features, 254 MB) 54 us with the merge, one of 131072 tokens (201 MB) 42 us.
 // Waves that held whole tiles, each with all features, had a register file too
 // small for their loads in flight: 85 us for the former.
 template <typename TQ, typename TV, int DBW>
@@ -966,7 +966,7 @@ namespace {
 
 // How a call is cut: one of the kernel's forms, and parts of the tokens.
 struct Plan {
-  bool one;        // columns of one map (ONE)
+  bool one;        // columns of one map: paged_chunk_kernel
   int ct, nw;      // column tiles and waves of a workgroup
   int n_slices, dbw, members, n_ct, n_split, per;
   bool parts;
@@ -974,10 +974,10 @@ struct Plan {
 
 Plan plan(const PagedAttentionArgs& a) {
   Plan r;
-  // Measured over 2000 cached tokens (us, columns of one map / all maps): 32
-  // sequences of 64 tokens 59 / 56, of 128 73 / 90; on two maps 32 tokens 68 /
-  // 91, on four 130 / 141; one sequence of 128 tokens 37 / 20.  A launch has fewer
-  // than 2^32 threads.
+  // Measured (us, columns of one map / all maps): 32 sequences over 2000 cached
+  // tokens, 32 new ones 50 / 49, 64 58 / 63, 128 69 / 97; on two maps 32 72 / 79, on
+  // four 96 / 125; one sequence, 256 new ones 39 / 25 over 2000 cached and 170 / 146
+  // over 65536, 512 43 / 33 and 188 / 258.  A launch has fewer than 2^32 threads.
   const int most = 512;   // features of a workgroup
   r.n_slices = (a.cache.D + most - 1) / most;
   r.one = a.max_chunk >= 32 && a.max_chunk * a.S >= 64 && a.tokens.N * a.S >= 512 &&

@@ -301,10 +301,13 @@ def paged_attention_hip(
     maps, D]`` of the values' type, or with ``mix`` (fp32 ``[maps]``) the maps'
     sum with these weights, ``[N, D]``.  Rows of no sequence, and rows that see
     nothing, are zero.  Scores, softmax and sums are fp32; probabilities are
-    rounded to the values' type for their product, the result once.
+    rounded to the values' type for their product, the result once.  An
+    infinity or a NaN in a value reaches the rows that see its token, one in a
+    key the maps that read it, too.
     ``max_chunk`` and ``max_length``: the largest numbers of new and of all
     tokens of a sequence, where the program knows them (they choose the launch,
-    not the result).
+    not the result; without the first a call is launched as if all rows were one
+    sequence's, and single tokens of 64 sequences take 73 us instead of 40).
     """
 
     return _paged_attention("paged_attention_hip", query, cache, page_table, lengths, offsets, scales, None, False, mix, causal,

@@ -36,7 +36,8 @@ extern "C" {
  * front of the first and behind the last one belong to no sequence).  A new
  * token whose position would be negative sees nothing and is not written.
  * max_chunk and max_length are what the host knows of the new tokens and the
- * tokens of a sequence (0: nothing); they choose the launch, not the result.
+ * tokens of a sequence (0: nothing, and all rows may be one sequence's); they
+ * choose the launch, not the result.
  */
 typedef struct {
   void* keys;
@@ -69,9 +70,9 @@ int da_cache_append(const da_paged_cache* cache, const void* key, int64_t ldk, c
  * and rows of no sequence, are zero.  Scores, the softmax and sums are fp32;
  * probabilities are rounded to v_dtype for the product with the values, and the
  * result once.  A value that is an infinity or a NaN makes its feature one in the
- * rows that see its token, and in no other; a key feature that is one may make
- * the rows NaN that see its token, in the maps that read it, and their weights;
- * what lies behind a sequence's last token reaches nothing.
+ * rows that see its token, and in no other.  A key feature that is one may make
+ * the rows NaN that see its token, in the maps that read it, and the weights of
+ * what those rows see.  What lies behind a sequence's last token reaches nothing.
  * Types: (qk_dtype, v_dtype) in (F16, BF16), (F16, F16), (BF16, BF16).
  *
  * weights_out (NULL: none) [sequences] rows of table_pages * page_size fp32, ld_weights apart:
