@@ -186,6 +186,44 @@ def test_a_long_flat_tail_beside_one_token_in_fp16(chunk, length, below) -> None
     close(got.cpu(), expected, tolerance)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("chunk", [1, 40, 600])
+@pytest.mark.parametrize("step", [0.3, 7.9, 8.1, 14.9, 15.1, 40.0])
+def test_scores_that_rise_from_tile_to_tile(step, chunk, types) -> None:
+    """Scores that stay just below and go just above what moves a reference, up and
+    down along the sequence: nothing overflows the probabilities' type."""
+
+    device, length, page = torch.device("cuda"), 1000, 32
+    g = torch.Generator().manual_seed(0)
+    tile = torch.arange(length) // 32
+    level = torch.where(tile < 20, tile, 40 - tile) / 32 + torch.rand(length, generator=g) / 512
+    keys = torch.zeros(page, page, 1, 64, dtype=types[0])
+    keys.view(-1, 64)[:length, 0] = level.to(types[0])
+    values = torch.randn(page * page, 64, generator=g).to(types[1])
+    query = torch.zeros(chunk, 1, 64, dtype=types[0], device=device)
+    query[..., 0] = 2.0
+    scale = torch.tensor([step * 16 * math.log(2.0)])   # two times 1/32 of it: `step` in log2
+    cache = da.PagedCache(keys.to(device), values.view(page, 1, 32, 64).transpose(2, 3).contiguous().to(device))
+    table = torch.arange(page, dtype=torch.int32, device=device)[None]
+    lengths = torch.tensor([length], dtype=torch.int32, device=device)
+    offsets = torch.tensor([0, chunk], dtype=torch.int32, device=device)
+    scores = (2 * keys.view(-1, 64)[:length, 0].double() * scale.double()).expand(chunk, length)
+    seen = torch.arange(length)[None] <= torch.arange(length - chunk, length)[:, None]
+    p = torch.softmax(scores.masked_fill(~seen, -math.inf), -1)
+    v = values[:length].double()
+    half = half_step(types[1])
+    # A score is one exact product, times a scale of three roundings, and the
+    # difference to the reference; scores reach 20 steps.
+    delta = 8 * F32 * (20 * step + 1)
+    tolerance = (half + 2 * delta + 16 * F32) * (p @ v.abs()) + half * (p @ v).abs() + 2.0 ** -25
+    if types[1] is torch.float16:
+        tolerance = tolerance + length * 2.0 ** -25 / 2 ** 6 * 5
+    for max_length in (None, 1):
+        got = da.paged_attention_hip(query, cache, table, lengths, offsets, scale.to(device), max_chunk=chunk, max_length=max_length)
+        close(got[:, 0].cpu(), p @ v, tolerance)
+
+
 # ---- launches --------------------------------------------------------------------
 
 
